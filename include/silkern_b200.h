@@ -52,6 +52,10 @@ extern "C" {
 #define SILKERN_E_ALIAS 6        /* an output overlaps an input or another output */
 #define SILKERN_E_GEOMETRY 7     /* explicit launch geometry rejected */
 #define SILKERN_E_SCRATCH 8      /* batch x tiles exceeds SILKERN_NOALLOC_MAX_TILES */
+#define SILKERN_E_CACHE 9        /* unsupported cache geometry, stride or alignment */
+#define SILKERN_E_HEADS 10       /* heads not a positive multiple of the cache's heads */
+#define SILKERN_E_TYPE 11        /* element type is neither SILKERN_BF16 nor SILKERN_F16 */
+#define SILKERN_E_ATTEND 12      /* window, sinks or softmax scale out of range */
 
 #define SILKERN_STATUS_BAD_REQUEST 1
 /* Status bit of the converter entry points (OR-ed into *status): a row split
@@ -290,6 +294,134 @@ int silkern_topk_localize_explicit_v2(const float* logits, int64_t logits_stride
                                       int32_t dcp_interleave, int32_t compact_valid_to_front,
                                       int32_t candidate_capacity, int32_t stage_table,
                                       int32_t cta_threads, int32_t* status, void* stream);
+
+/*
+ * The 8-bit paged cache. A page (block) holds block_size consecutive
+ * rank-local tokens; slot = block * block_size + offset is what the converter
+ * emits. Keys and values are e4m3 codes, and every (block, head) pair has one
+ * float32 scale for its keys and one for its values: the stored value is
+ * scale * code. k is (num_blocks, block_size, kv_heads, key_dim) with strides
+ * in bytes, multiples of 16, for the first three dimensions and 1 for the
+ * last; v likewise with value_dim; k_scale and v_scale are contiguous
+ * (num_blocks, kv_heads). A latent cache has one head, key_dim 576, v and
+ * v_scale NULL and value_dim 512: the first 512 columns of a key are its
+ * value, and k_scale is the scale of both. Scales lie in [2^-100, 2^100], or
+ * are 0 (every value of the pair is 0) or NaN (every use gives NaN); codes of
+ * visible tokens are finite (neither 0x7f nor 0xff). num_blocks * block_size
+ * is below 2^31 and block_size at most 65536. Addresses of k and v are multiples
+ * of 16.
+ */
+typedef struct silkern_cache_v1 {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t kv_heads;
+  int32_t key_dim;
+  int32_t value_dim;
+  int64_t k_block, k_token, k_head;
+  int64_t v_block, v_token, v_head;
+} silkern_cache_v1;
+
+/* Element types of queries, new tokens and outputs. */
+#define SILKERN_BF16 0
+#define SILKERN_F16 1
+
+/* Status bits of the cache entry points (OR-ed into *status, with
+ * SILKERN_STATUS_BAD_REQUEST and SILKERN_STATUS_BAD_LENGTH): a slot past the
+ * cache, or a token whose page is outside its table row or the cache. Such a
+ * token is left out. */
+#define SILKERN_STATUS_BAD_SLOT 8
+/* Status bit of the attention entry points: a wait inside the kernel ran out
+ * of its bound. The outputs of the work items concerned are not valid. It
+ * does not occur in a working launch. */
+#define SILKERN_STATUS_WAIT_TIMEOUT 16
+
+/*
+ * Append tokens to the 8-bit cache. Sequence b (of `sequences`) has the new
+ * tokens [cu_tokens[b], cu_tokens[b + 1]) of keys (tokens, kv_heads, key_dim)
+ * and values (tokens, kv_heads, value_dim; NULL for a latent cache), at the
+ * positions starts[b], starts[b] + 1, ... of the request req_ids[b]; the
+ * positions that this rank owns are stored through block_table, the others
+ * are skipped. keys and values have unit column stride and strides in
+ * elements for tokens and heads.
+ *
+ * Scales are powers of two. With m the largest magnitude among the call's
+ * tokens in one (page, head), the scale becomes max(old, w), w the smallest
+ * power of two with 448 w >= m (within [2^-100, 2^100]; 0 where m is 0). A
+ * page whose first token is among the call's is new: old counts as 0.
+ * Otherwise, where the scale grows, the codes that the page holds are
+ * rescaled (exact for a power of two, but for codes that become subnormal).
+ * An infinity or NaN among a page's new values makes that scale NaN until the
+ * page is new again. A page takes tokens from one sequence of the call at
+ * most (a page shared by several requests is copied before one of them
+ * appends to it). Nothing else is written.
+ */
+int silkern_append_quantized_v1(const silkern_cache_v1* cache, const void* keys, int64_t key_token,
+                                int64_t key_head, const void* values, int64_t value_token,
+                                int64_t value_head, int32_t type, int64_t tokens,
+                                const int32_t* cu_tokens, const int32_t* starts,
+                                const int32_t* req_ids, int64_t sequences,
+                                const int32_t* block_table, int64_t table_rows,
+                                int64_t table_width, int32_t dcp_size, int32_t dcp_rank,
+                                int32_t dcp_interleave, int32_t* status, void* stream);
+
+/*
+ * Attention of each query row over its selected slots:
+ *   out[r][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(softmax_scale * q[r][h] . k_j)
+ *   lse[r][h] = log(sum_j p_j)
+ * over j in [0, counts[r]) (counts may be NULL: the whole width) with
+ * slots[r][j] >= 0; a row without such a j gets out 0 and lse -inf. q is
+ * (rows, heads, key_dim) and out (rows, heads, value_dim), both of `type`,
+ * with unit column stride, strides in elements for rows and heads (q's are
+ * multiples of 8 and its address of 16); lse is float32 (rows, heads),
+ * contiguous; slots has row stride slots_row. Query head h reads cache head
+ * h / (heads / kv_heads). key_dim is 64 or 128 with value_dim the same, or
+ * the cache is latent. A count outside [0, width] is clamped and flagged with
+ * SILKERN_STATUS_BAD_LENGTH.
+ */
+int silkern_attend_selected_v1(const silkern_cache_v1* cache, const void* q, int64_t q_row,
+                               int64_t q_head, int32_t type, int64_t rows, int32_t heads,
+                               const int32_t* slots, int64_t slots_row, int64_t width,
+                               const int32_t* counts, void* out, int64_t out_row, int64_t out_head,
+                               float* lse, float softmax_scale, int32_t* status, void* stream);
+
+/*
+ * Attention through the block table. Sequence b has the queries
+ * [cu_tokens[b], cu_tokens[b + 1]) of q, the last tokens of the request
+ * req_ids[b], whose length is lengths[b] with them; the query at position t
+ * sees the positions [max(0, t + 1 - window), t] and the first `sinks`
+ * positions up to t (window 0: every position up to t), as far as this rank
+ * owns them. Rows of q at and past cu_tokens[sequences] are not touched in
+ * out and lse. Outputs, types and layouts as for silkern_attend_selected_v1.
+ * A length below the number of queries is flagged with
+ * SILKERN_STATUS_BAD_LENGTH; queries at negative positions see nothing.
+ */
+int silkern_attend_window_v1(const silkern_cache_v1* cache, const void* q, int64_t q_row,
+                             int64_t q_head, int32_t type, int64_t rows, int32_t heads,
+                             const int32_t* cu_tokens, const int32_t* lengths,
+                             const int32_t* req_ids, int64_t sequences,
+                             const int32_t* block_table, int64_t table_rows, int64_t table_width,
+                             int64_t window, int64_t sinks, int32_t dcp_size, int32_t dcp_rank,
+                             int32_t dcp_interleave, void* out, int64_t out_row, int64_t out_head,
+                             float* lse, float softmax_scale, int32_t* status, void* stream);
+
+/*
+ * Join the partial results of `ranks` context-parallel ranks:
+ *   lse[r][h] = log(sum_i exp(lses[i][r][h]))
+ *   out[r][h] = sum_i exp(lses[i][r][h] - lse[r][h]) outs[i][r][h]
+ * outs is (ranks, rows, heads, dim) with unit column stride and strides in
+ * elements, lses float32 (ranks, rows, heads) contiguous, out (rows, heads,
+ * dim) of the same type with strides, lse float32 (rows, heads) contiguous or
+ * NULL. A partial result whose lse is -inf is not read; where all are, out
+ * is 0 and lse -inf. The ranks are added in order.
+ */
+int silkern_merge_partials_v1(const void* outs, int64_t outs_rank, int64_t outs_row,
+                              int64_t outs_head, const float* lses, int32_t type, int64_t ranks,
+                              int64_t rows, int64_t heads, int64_t dim, void* out, int64_t out_row,
+                              int64_t out_head, float* lse, void* stream);
 
 /* Static text for a return code (positive SILKERN_E*, 0, or -cudaError_t). */
 const char* silkern_status_string_v1(int code);

@@ -23,6 +23,12 @@ raise :class:`LocalizationError` if it is missing.
 
 from __future__ import annotations
 
+from silkern_b200.attention import (
+    append_quantized,
+    attend_selected,
+    attend_window,
+    merge_partials,
+)
 from silkern_b200.contract import (
     DEFAULT_TILE_SIZE,
     MAX_ROW_WIDTH,
@@ -54,11 +60,15 @@ __all__ = [
     "ConformanceReport",
     "LocalizationError",
     "ReplayGateReport",
+    "append_quantized",
+    "attend_selected",
+    "attend_window",
     "conformance",
     "exact_stable_compact_reference",
     "localize_hierarchical",
     "localize_reference",
     "localize_rowwise",
+    "merge_partials",
     "topk_localize",
     "replay_gate",
     "workspace_shapes",

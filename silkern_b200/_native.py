@@ -21,6 +21,31 @@ _i64 = ctypes.c_int64
 _u32 = ctypes.c_uint32
 _ptr = ctypes.c_void_p
 
+_f32 = ctypes.c_float
+
+
+class Cache(ctypes.Structure):
+    """``silkern_cache_v1``: the 8-bit paged cache."""
+
+    _fields_ = [
+        ("k", _ptr),
+        ("v", _ptr),
+        ("k_scale", _ptr),
+        ("v_scale", _ptr),
+        ("num_blocks", _i64),
+        ("block_size", _i32),
+        ("kv_heads", _i32),
+        ("key_dim", _i32),
+        ("value_dim", _i32),
+        ("k_block", _i64),
+        ("k_token", _i64),
+        ("k_head", _i64),
+        ("v_block", _i64),
+        ("v_token", _i64),
+        ("v_head", _i64),
+    ]
+
+
 #: name -> (restype, argtypes) for every symbol the header declares.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "silkern_localize_rowwise_v1": (
@@ -65,6 +90,25 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i32, _i32, _i32,
          _i32, _i32, _i32, _i32, _i32, _i32, _ptr, _ptr],
+    ),
+    "silkern_append_quantized_v1": (
+        _i32,
+        [_ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _i32, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _i64,
+         _i64, _i32, _i32, _i32, _ptr, _ptr],
+    ),
+    "silkern_attend_selected_v1": (
+        _i32,
+        [_ptr, _ptr, _i64, _i64, _i32, _i64, _i32, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr,
+         _f32, _ptr, _ptr],
+    ),
+    "silkern_attend_window_v1": (
+        _i32,
+        [_ptr, _ptr, _i64, _i64, _i32, _i64, _i32, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _i64, _i64,
+         _i64, _i32, _i32, _i32, _ptr, _i64, _i64, _ptr, _f32, _ptr, _ptr],
+    ),
+    "silkern_merge_partials_v1": (
+        _i32,
+        [_ptr, _i64, _i64, _i64, _ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr],
     ),
     "silkern_status_string_v1": (ctypes.c_char_p, [ctypes.c_int]),
     "silkern_abi_version_v1": (ctypes.c_int, []),

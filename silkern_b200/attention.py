@@ -1,0 +1,411 @@
+"""Attention over an 8-bit paged cache, past the localized selection.
+
+The converter says which physical slots of a rank's cache a query row selected;
+the operators here keep that cache and attend to it:
+
+``append_quantized``
+    Store new tokens as e4m3 codes, one float32 scale for each page and head.
+``attend_selected``
+    Attention of each query row over its slots, as
+    :func:`silkern_b200.localize_rowwise` and :func:`silkern_b200.topk_localize`
+    emit them: padding (-1) anywhere, any order, counts optional.
+``attend_window``
+    Attention through the block table over a sliding window and a few first
+    tokens that stay visible, or over the whole context; one query for each
+    sequence or pieces of prompts.
+``merge_partials``
+    Each rank's output and log-sum-exp over its own tokens, joined.
+
+The cache is a pair of ``torch.float8_e4m3fn`` tensors (num_blocks, block_size,
+kv_heads, dim), dim 64 or 128, with scales float32 (num_blocks, kv_heads). A
+latent cache is one such tensor with one head and dim 576, whose first 512
+columns are the values too: pass ``None`` for its values and value scales. A
+page's tokens are consecutive rank-local tokens, owned as the converter's
+contract says (silkern/contract.py:8-36).
+
+Every buffer is the caller's; nothing is allocated and nothing synchronises, so
+calls can be captured in a CUDA graph. They run on the current stream of the
+buffers' device. Each raises :class:`LocalizationError` before launch on an
+unsupported binding or geometry.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+from silkern_b200 import _native
+from silkern_b200.contract import _validate_dcp_config
+from silkern_b200.errors import LocalizationError
+from silkern_b200.kernels import _check_status, _device_scope, _is_int
+
+#: Dimensions of a latent cache: keys, and the leading part that is the value.
+LATENT_KEY_DIM = 576
+LATENT_VALUE_DIM = 512
+#: Status bits (OR-ed into ``status``) besides SILKERN_STATUS_BAD_REQUEST (1)
+#: and STATUS_BAD_LENGTH (2): a slot or page outside the cache, left out; and a
+#: wait inside a kernel that ran out of its bound.
+STATUS_BAD_SLOT = 8
+STATUS_WAIT_TIMEOUT = 16
+
+_INT32_MAX = 2**31 - 1
+_TYPES: dict = {}
+
+
+def _type_code(torch, dtype):
+    if not _TYPES:
+        _TYPES.update({torch.bfloat16: 0, torch.float16: 1})
+    code = _TYPES.get(dtype)
+    if code is None:
+        raise LocalizationError("queries, new tokens and outputs must be bfloat16 or float16")
+    return code
+
+
+def _on_device(torch, tensors, what: str):
+    """The device that every given tensor is on."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise LocalizationError(f"all {what} buffers must be torch tensors")
+        if not t.is_cuda:
+            raise LocalizationError(f"all {what} buffers must be CUDA tensors")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise LocalizationError(f"all {what} buffers must be on the same device")
+    return device
+
+
+def _check_ints(torch, tensors, names: str) -> None:
+    for t in tensors:
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise LocalizationError(f"{names} must be contiguous int32 tensors")
+
+
+def _cache(torch, k_cache, v_cache, k_scale, v_scale) -> _native.Cache:
+    """The checked ``silkern_cache_v1`` of a cache's tensors."""
+    if (v_cache is None) != (v_scale is None):
+        raise LocalizationError("v_cache and v_scale are both given or both None")
+    if k_cache.ndim != 4 or (v_cache is not None and v_cache.ndim != 4):
+        raise LocalizationError("caches must be (num_blocks, block_size, kv_heads, dim)")
+    blocks, block_size, kv_heads, dim = k_cache.shape
+    if blocks < 1 or block_size < 1 or kv_heads < 1:
+        raise LocalizationError("cache dimensions must be positive")
+    if block_size > 65536 or blocks * block_size > _INT32_MAX:
+        raise LocalizationError("block_size is at most 65536 and num_blocks * block_size below 2**31")
+    if v_cache is None:
+        if kv_heads != 1 or dim != LATENT_KEY_DIM:
+            raise LocalizationError(
+                f"a cache without values is latent: one head and dim {LATENT_KEY_DIM}")
+    elif dim not in (64, 128) or v_cache.shape != k_cache.shape:
+        raise LocalizationError("k_cache and v_cache must have the same shape, dim 64 or 128")
+    strides = []
+    for cache, scale in ((k_cache, k_scale), (v_cache, v_scale)):
+        if cache is None:
+            strides += (0, 0, 0)
+            continue
+        if cache.dtype != torch.float8_e4m3fn:
+            raise LocalizationError("caches must use float8_e4m3fn")
+        if scale.dtype != torch.float32 or scale.shape != (blocks, kv_heads) or not scale.is_contiguous():
+            raise LocalizationError("scales must be contiguous float32 (num_blocks, kv_heads)")
+        sb, st, sh, sd = cache.stride()
+        if sd != 1 or sb % 16 or st % 16 or sh % 16 or cache.data_ptr() % 16:
+            raise LocalizationError(
+                "caches need unit column stride, other strides that are multiples of 16 and 16-byte alignment")
+        strides += (sb, st, sh)
+    return _native.Cache(
+        k_cache.data_ptr(), None if v_cache is None else v_cache.data_ptr(), k_scale.data_ptr(),
+        None if v_scale is None else v_scale.data_ptr(), blocks, block_size, kv_heads, dim,
+        LATENT_VALUE_DIM if v_cache is None else dim, *strides)
+
+
+def _check_separate(outputs, others) -> None:
+    """No output shares storage with another output or with an input."""
+    taken = {t.untyped_storage().data_ptr() for t in others if t is not None}
+    for t in outputs:
+        if t is None:
+            continue
+        storage = t.untyped_storage().data_ptr()
+        if storage in taken:
+            raise LocalizationError("outputs must not share storage with inputs or with each other")
+        taken.add(storage)
+
+
+def _check_table(block_table) -> None:
+    if block_table.ndim != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+        raise LocalizationError("block_table must be 2D and non-empty")
+
+
+def _check_owner(block_size, dcp_size, dcp_rank, dcp_interleave) -> None:
+    _validate_dcp_config(dcp_size, dcp_rank, dcp_interleave)
+    if block_size % dcp_interleave:
+        raise LocalizationError("the cache's block_size must be divisible by dcp_interleave")
+    if dcp_size * dcp_interleave > _INT32_MAX:
+        raise LocalizationError("dcp_size * dcp_interleave must be below 2**31")
+
+
+def _check_queries(torch, q, k_cache, out, lse, softmax_scale) -> tuple[int, int]:
+    """Checks of an attention call's queries and results: (rows, type code)."""
+    code = _type_code(torch, q.dtype)
+    if q.ndim != 3 or q.shape[2] != k_cache.shape[3]:
+        raise LocalizationError("q must be (rows, heads, key_dim) with the cache's key_dim")
+    rows, heads, dim = q.shape
+    if rows < 1 or heads < 1 or heads > 65535 or heads % k_cache.shape[2]:
+        raise LocalizationError("q needs at least one row, and heads in a positive multiple of the cache's heads")
+    value_dim = LATENT_VALUE_DIM if dim == LATENT_KEY_DIM else dim
+    if out.dtype != q.dtype or out.shape != (rows, heads, value_dim) or out.stride(2) != 1:
+        raise LocalizationError(f"out must be (rows, heads, {value_dim}) of q's type with unit column stride")
+    if lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous():
+        raise LocalizationError("lse must be contiguous float32 (rows, heads)")
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        raise LocalizationError(
+            "q needs unit column stride, other strides that are multiples of 8 and 16-byte alignment")
+    if not math.isfinite(softmax_scale):
+        raise LocalizationError("softmax_scale must be finite")
+    return rows, code
+
+
+def append_quantized(
+    keys,
+    values,
+    k_cache,
+    v_cache,
+    k_scale,
+    v_scale,
+    cu_tokens,
+    starts,
+    req_ids,
+    block_table,
+    *,
+    dcp_size: int = 1,
+    dcp_rank: int = 0,
+    dcp_interleave: int = 1,
+    status=None,
+) -> None:
+    """Store the new tokens of each sequence in the 8-bit cache.
+
+    ``keys`` is (tokens, kv_heads, key_dim) in bfloat16 or float16, ``values``
+    (tokens, kv_heads, value_dim) of the same type, or ``None`` for a latent
+    cache; both have unit column stride. Sequence ``b`` has the tokens
+    ``cu_tokens[b]:cu_tokens[b + 1]`` (int32, one more element than sequences),
+    at the positions from ``starts[b]`` on of the request ``req_ids[b]``. The
+    positions of this rank go through ``block_table[req_ids[b]]`` into their
+    pages; others are skipped.
+
+    Scales are powers of two: with ``m`` the largest magnitude among the call's
+    tokens in one page and head, the scale becomes the larger of what it was
+    and the smallest power of two ``w`` with ``448 w >= m`` (within 2**-100 and
+    2**100). A page whose first token is among the call's is new: its old scale
+    does not count, so pages need no clearing before they are used again.
+    Where the scale of a page grows, the codes that it holds are rescaled. An
+    infinity or NaN among a page's new values makes the scale NaN, and so
+    everything read from that page and head, until the page is new again.
+
+    A page takes tokens from one sequence of a call at most: copy a page that
+    several requests share before one of them appends to it. ``status`` gets 1
+    for a request id outside the table, 2 for a position outside the int32
+    range, 8 for a token whose page is outside its table row or the cache; such
+    tokens are not stored.
+    """
+    import torch
+
+    device = _on_device(
+        torch, (keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table),
+        "append")
+    code = _type_code(torch, keys.dtype)
+    _check_ints(torch, (cu_tokens, starts, req_ids, block_table), "cu_tokens, starts, req_ids and block_table")
+    cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
+    if (values is None) != (v_cache is None):
+        raise LocalizationError("values are given exactly when the cache has values")
+    tokens = keys.shape[0] if keys.ndim == 3 else 0
+    for new in (keys, values):
+        if new is not None and (new.dtype != keys.dtype or tuple(new.shape) != (tokens, cache.kv_heads, cache.key_dim)
+                                or tokens < 1 or new.stride(2) != 1):
+            raise LocalizationError(
+                "keys and values must be (tokens, kv_heads, dim) of one type with unit column stride")
+    sequences = starts.shape[0] if starts.ndim == 1 else 0
+    if sequences < 1 or cu_tokens.shape != (sequences + 1,) or req_ids.shape != (sequences,):
+        raise LocalizationError("starts and req_ids need one element per sequence, cu_tokens one more")
+    _check_table(block_table)
+    _check_owner(cache.block_size, dcp_size, dcp_rank, dcp_interleave)
+    _check_separate((k_scale, v_scale), (keys, values, cu_tokens, starts, req_ids, block_table, k_cache, v_cache))
+    inputs = {t.untyped_storage().data_ptr() for t in (keys, values, cu_tokens, starts, req_ids, block_table)
+              if t is not None}
+    if any(t is not None and t.untyped_storage().data_ptr() in inputs for t in (k_cache, v_cache)):
+        raise LocalizationError("caches must not share storage with inputs")
+    status_ptr = _check_status(torch, status, device)
+
+    lib = _native.load()
+    with _device_scope(torch, device):
+        rc = lib.silkern_append_quantized_v1(
+            ctypes.addressof(cache), keys.data_ptr(), keys.stride(0), keys.stride(1),
+            None if values is None else values.data_ptr(),
+            0 if values is None else values.stride(0), 0 if values is None else values.stride(1),
+            code, tokens, cu_tokens.data_ptr(), starts.data_ptr(), req_ids.data_ptr(), sequences,
+            block_table.data_ptr(), block_table.shape[0], block_table.shape[1],
+            int(dcp_size), int(dcp_rank), int(dcp_interleave), status_ptr,
+            torch.cuda.current_stream(device).cuda_stream)
+    _native.check(rc, "append_quantized")
+
+
+def attend_selected(
+    q,
+    slots,
+    k_cache,
+    v_cache,
+    k_scale,
+    v_scale,
+    out,
+    lse,
+    *,
+    softmax_scale: float,
+    counts=None,
+    status=None,
+) -> None:
+    """Attention of each query row over the cache slots selected for it.
+
+    ``q`` is (rows, heads, key_dim) in bfloat16 or float16, its address and
+    strides multiples of 16 bytes; ``out`` (rows, heads, value_dim) of the same
+    type, ``lse`` float32 (rows, heads). Query head ``h`` reads cache head
+    ``h // (heads // kv_heads)``. ``slots`` is int32 (rows, width) with unit
+    column stride: what the converter writes. Negative slots are padding and
+    may stand anywhere; with ``counts`` (int32, (rows,)) only the first
+    ``counts[r]`` columns of row ``r`` are looked at, which is right for
+    compacted rows. A slot that is listed twice counts twice.
+
+    ``lse`` is the natural log of the sum of ``exp(softmax_scale * q . k)``, for
+    :func:`merge_partials`. A row without a slot gets output 0 and lse -inf.
+    ``status`` gets 2 for a count outside the row (clamped) and 8 for a slot
+    past the cache (left out).
+    """
+    import torch
+
+    device = _on_device(torch, (q, slots, k_cache, v_cache, k_scale, v_scale, out, lse, counts), "attention")
+    _check_ints(torch, (counts,), "counts")
+    cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
+    rows, code = _check_queries(torch, q, k_cache, out, lse, softmax_scale)
+    if slots.dtype != torch.int32 or slots.ndim != 2 or slots.shape[0] != rows or slots.shape[1] < 1:
+        raise LocalizationError("slots must be int32 with one non-empty row for each row of q")
+    if slots.stride(1) != 1:
+        raise LocalizationError("slots must have unit column stride")
+    if counts is not None and counts.shape != (rows,):
+        raise LocalizationError("counts must contain one element per row")
+    _check_separate((out, lse), (q, slots, counts, k_cache, v_cache, k_scale, v_scale))
+    status_ptr = _check_status(torch, status, device)
+
+    lib = _native.load()
+    with _device_scope(torch, device):
+        rc = lib.silkern_attend_selected_v1(
+            ctypes.addressof(cache), q.data_ptr(), q.stride(0), q.stride(1), code, rows, q.shape[1],
+            slots.data_ptr(), slots.stride(0), slots.shape[1], None if counts is None else counts.data_ptr(),
+            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), softmax_scale, status_ptr,
+            torch.cuda.current_stream(device).cuda_stream)
+    _native.check(rc, "attend_selected")
+
+
+def attend_window(
+    q,
+    cu_tokens,
+    lengths,
+    req_ids,
+    block_table,
+    k_cache,
+    v_cache,
+    k_scale,
+    v_scale,
+    out,
+    lse,
+    *,
+    softmax_scale: float,
+    window: int = 0,
+    sinks: int = 0,
+    dcp_size: int = 1,
+    dcp_rank: int = 0,
+    dcp_interleave: int = 1,
+    status=None,
+) -> None:
+    """Attention through the block table, over a window and the first tokens.
+
+    Sequence ``b`` has the queries ``cu_tokens[b]:cu_tokens[b + 1]`` of ``q``
+    (int32, one more element than sequences): the last tokens of the request
+    ``req_ids[b]``, which is ``lengths[b]`` tokens long with them. The query at
+    position ``t`` sees the positions ``max(0, t + 1 - window)`` to ``t`` and
+    the first ``sinks`` positions up to ``t``; with ``window`` 0 it sees all up
+    to ``t``. Of these it attends to the ones that this rank owns. Queries at
+    one position of each sequence (decode) and pieces of prompts take the same
+    call; rows of ``q`` at and past ``cu_tokens[-1]`` are left as they were in
+    ``out`` and ``lse``.
+
+    Layouts, types and results are those of :func:`attend_selected`. A query
+    that sees none of this rank's tokens gets output 0 and lse -inf. ``status``
+    gets 1 for a request id outside the table (its queries see nothing), 2 for
+    a length below the number of queries (those at negative positions see
+    nothing) and 8 for a visible token whose page is outside the table row or
+    the cache (left out).
+    """
+    import torch
+
+    device = _on_device(
+        torch, (q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale, out, lse),
+        "attention")
+    _check_ints(torch, (cu_tokens, lengths, req_ids, block_table), "cu_tokens, lengths, req_ids and block_table")
+    cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
+    rows, code = _check_queries(torch, q, k_cache, out, lse, softmax_scale)
+    sequences = lengths.shape[0] if lengths.ndim == 1 else 0
+    if sequences < 1 or cu_tokens.shape != (sequences + 1,) or req_ids.shape != (sequences,):
+        raise LocalizationError("lengths and req_ids need one element per sequence, cu_tokens one more")
+    _check_table(block_table)
+    _check_owner(cache.block_size, dcp_size, dcp_rank, dcp_interleave)
+    if not _is_int(window) or not 0 <= window <= _INT32_MAX or not _is_int(sinks) or not 0 <= sinks <= _INT32_MAX:
+        raise LocalizationError("window and sinks must be non-negative int32 integers")
+    _check_separate((out, lse), (q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale))
+    status_ptr = _check_status(torch, status, device)
+
+    lib = _native.load()
+    with _device_scope(torch, device):
+        rc = lib.silkern_attend_window_v1(
+            ctypes.addressof(cache), q.data_ptr(), q.stride(0), q.stride(1), code, rows, q.shape[1],
+            cu_tokens.data_ptr(), lengths.data_ptr(), req_ids.data_ptr(), sequences, block_table.data_ptr(),
+            block_table.shape[0], block_table.shape[1], int(window), int(sinks), int(dcp_size), int(dcp_rank),
+            int(dcp_interleave), out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), softmax_scale,
+            status_ptr, torch.cuda.current_stream(device).cuda_stream)
+    _native.check(rc, "attend_window")
+
+
+def merge_partials(outs, lses, out, lse=None) -> None:
+    """Join the ranks' partial attention results into the whole one.
+
+    ``outs`` is (ranks, rows, heads, dim) in bfloat16 or float16 with unit
+    column stride, ``lses`` contiguous float32 (ranks, rows, heads): each rank's
+    :func:`attend_selected` or :func:`attend_window` over its own tokens.
+    ``out`` (rows, heads, dim) becomes the average of the partial outputs
+    weighted by ``exp(lses)``, ``lse`` (optional, float32 (rows, heads)) the log
+    of the weights' sum. A partial result with lse -inf is not read; where every
+    rank's is, out is 0 and lse -inf. The ranks are added in order.
+    """
+    import torch
+
+    device = _on_device(torch, (outs, lses, out, lse), "merge")
+    code = _type_code(torch, outs.dtype)
+    if outs.ndim != 4 or min(outs.shape) < 1:
+        raise LocalizationError("outs must be a non-empty (ranks, rows, heads, dim)")
+    ranks, rows, heads, dim = outs.shape
+    if out.dtype != outs.dtype or out.shape != (rows, heads, dim):
+        raise LocalizationError("out must be (rows, heads, dim) of the type of outs")
+    if outs.stride(3) != 1 or out.stride(2) != 1:
+        raise LocalizationError("outs and out must have unit column stride")
+    if lses.dtype != torch.float32 or lses.shape != (ranks, rows, heads) or not lses.is_contiguous():
+        raise LocalizationError("lses must be contiguous float32 (ranks, rows, heads)")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous()):
+        raise LocalizationError("lse must be contiguous float32 (rows, heads)")
+    _check_separate((out, lse), (outs, lses))
+
+    lib = _native.load()
+    with _device_scope(torch, device):
+        rc = lib.silkern_merge_partials_v1(
+            outs.data_ptr(), outs.stride(0), outs.stride(1), outs.stride(2), lses.data_ptr(), code, ranks, rows,
+            heads, dim, out.data_ptr(), out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(),
+            torch.cuda.current_stream(device).cuda_stream)
+    _native.check(rc, "merge_partials")

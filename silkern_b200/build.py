@@ -22,10 +22,14 @@ SOURCES = [
     os.path.join(CSRC, "localize.cu"),
     os.path.join(CSRC, "topk_localize.cu"),
     os.path.join(CSRC, "atomic_baseline.cu"),
+    os.path.join(CSRC, "cache_ops.cu"),
+    os.path.join(CSRC, "attend.cu"),
 ]
 DEPENDS = SOURCES + [
     os.path.join(CSRC, "fastdiv.cuh"),
     os.path.join(CSRC, "ptx.cuh"),
+    os.path.join(CSRC, "host.cuh"),
+    os.path.join(CSRC, "paged.cuh"),
     os.path.join(INCLUDE, "silkern_b200.h"),
 ]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -65,6 +69,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         "-Xcompiler",
         "-fPIC",
         "-shared",
+        "--threads",
+        "0",
         "-I",
         INCLUDE,
         "-o",

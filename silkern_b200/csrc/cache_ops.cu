@@ -1,0 +1,401 @@
+// The cache's own operators: appending tokens in 8 bits, joining the ranks'
+// partial results, and the argument checks of the attention entry points.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cmath>
+
+#include "host.cuh"
+#include "paged.cuh"
+#include "ptx.cuh"
+#include "silkern_b200.h"
+
+namespace silkern {
+
+int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t stream);
+
+namespace {
+
+// ---------------------------------------------------------------- append
+
+struct AppendArgs {
+  PagedCache cache;
+  const void* keys;
+  const void* values;
+  int64_t key_token, key_head, value_token, value_head;  // elements
+  int32_t key_dim, value_dim;
+  int32_t tokens, sequences;
+  const int32_t* cu_tokens;
+  const int32_t* starts;
+  const int32_t* req_ids;
+  const int32_t* table;
+  int64_t table_rows;
+  uint32_t table_width;
+  FastDiv page_tokens;  // by block_size * dcp_size: positions from page to page
+  Ownership own;
+  int32_t* status;
+};
+
+constexpr int kAppendThreads = 128;
+
+// The scale that a largest magnitude asks for: the smallest power of two w
+// with 448 w >= m, from the bits of m (448 = 0.875 * 2^9, so with m = f 2^e,
+// f in [0.5, 1), w = 2^(e - 9), or twice that where f > 0.875).
+__device__ __forceinline__ float scale_for(float m) {
+  if (m == 0.f) return 0.f;
+  int e;
+  const float f = frexpf(m, &e);
+  const int p = e - 9 + (f > 0.875f ? 1 : 0);
+  return ldexpf(1.f, min(max(p, -100), 100));
+}
+
+__device__ __forceinline__ uint8_t to_e4m3(float x) {
+  return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float from_e4m3(uint8_t code) {
+  __nv_fp8_e4m3 x;
+  x.__x = code;
+  return static_cast<float>(x);
+}
+
+// One CTA for each (page that a sequence's tokens touch, head, keys or
+// values). Sequence b owns the items from cu[b] / page_tokens + 2 b on: n new
+// tokens touch at most n / page_tokens + 2 pages of a rank.
+template <typename T>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+  __shared__ uint32_t most_shared[kAppendThreads / 32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t item = blockIdx.x;
+  const uint32_t head = blockIdx.y;
+  const bool is_value = blockIdx.z != 0;
+  int32_t low = 0, high = a.sequences;
+  while (high - low > 1) {
+    const int32_t step = (high - low + 31) / 32;
+    const int32_t b = low + lane * step;
+    bool before = false;
+    if (b < high) {
+      const int32_t cu = min(max(__ldg(a.cu_tokens + b), 0), a.tokens);
+      before = static_cast<int64_t>(fastdiv(cu, a.page_tokens)) + 2 * static_cast<int64_t>(b) <= item;
+    }
+    const uint32_t hits = __ballot_sync(kAllLanes, before);
+    const int32_t last = hits == 0 ? 0 : 31 - __clz(hits);
+    low += last * step;
+    high = min(high, low + step);
+  }
+  const int32_t begin = min(max(__ldg(a.cu_tokens + low), 0), a.tokens);
+  const int32_t end = min(max(__ldg(a.cu_tokens + low + 1), begin), a.tokens);
+  const int64_t page_index = item - (static_cast<int64_t>(fastdiv(begin, a.page_tokens)) + 2 * static_cast<int64_t>(low));
+  if (page_index < 0 || begin == end) return;
+  const int32_t start = __ldg(a.starts + low);
+  const int32_t req = __ldg(a.req_ids + low);
+  const int64_t stop = static_cast<int64_t>(start) + (end - begin);
+  if (start < 0 || stop > 0x7fffffff) {
+    if (page_index == 0 && threadIdx.x == 0) flag_status(a.status, SILKERN_STATUS_BAD_LENGTH);
+    return;
+  }
+  if (req < 0 || req >= a.table_rows) {
+    if (page_index == 0 && threadIdx.x == 0) flag_status(a.status, SILKERN_STATUS_BAD_REQUEST);
+    return;
+  }
+  // This rank's new tokens are the local tokens [first, last).
+  const uint32_t first = a.own.owned_before(start), last = a.own.owned_before(static_cast<uint32_t>(stop));
+  if (first == last) return;
+  const uint32_t block_size = a.cache.block.divisor;
+  const uint32_t page = fastdiv(first, a.cache.block) + static_cast<uint32_t>(page_index);
+  const uint64_t page_first = static_cast<uint64_t>(page) * block_size;
+  if (page_first >= last) return;
+  const uint32_t lo = page_first > first ? static_cast<uint32_t>(page_first) : first;
+  const uint32_t hi = page_first + block_size < last ? static_cast<uint32_t>(page_first) + block_size : last;
+  const int32_t block = page < a.table_width ? __ldg(a.table + static_cast<int64_t>(req) * a.table_width + page) : -1;
+  if (static_cast<uint32_t>(block) >= a.cache.num_blocks) {
+    if (threadIdx.x == 0) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
+    return;
+  }
+  const int32_t dim = is_value ? a.value_dim : a.key_dim;
+  const int64_t src_token = is_value ? a.value_token : a.key_token;
+  const T* src = static_cast<const T*>(is_value ? a.values : a.keys) + head * (is_value ? a.value_head : a.key_head);
+  const int64_t dst_token = is_value ? a.cache.v_token : a.cache.k_token;
+  uint8_t* dst = const_cast<uint8_t*>(is_value ? a.cache.v : a.cache.k) +
+                 block * (is_value ? a.cache.v_block : a.cache.k_block) +
+                 head * (is_value ? a.cache.v_head : a.cache.k_head);
+  float* scale = const_cast<float*>(is_value ? a.cache.v_scale : a.cache.k_scale) +
+                 static_cast<int64_t>(block) * a.cache.kv_heads + head;
+  const int32_t count = static_cast<int32_t>(hi - lo), total = count * dim;
+  // The largest magnitude by its bits: NaN > infinity > finite.
+  uint32_t most = 0;
+  for (int32_t i = threadIdx.x; i < total; i += kAppendThreads) {
+    const int32_t t = i / dim, d = i - t * dim;
+    const int64_t row = begin + static_cast<int64_t>(a.own.position(lo + t)) - start;
+    most = max(most, __float_as_uint(static_cast<float>(src[row * src_token + d])) & 0x7fffffffu);
+  }
+  most = __reduce_max_sync(kAllLanes, most);
+  if (lane == 0) most_shared[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, most_shared[w]);
+  const bool fresh = lo == page_first;
+  const float old = fresh ? 0.f : *scale;
+  const float want = most >= 0x7f800000u ? NAN : scale_for(__uint_as_float(most));
+  const float use = want != want || old != old ? NAN : fmaxf(old, want);
+  __syncthreads();  // every thread has read the old scale
+  if (threadIdx.x == 0) *scale = use;
+  const bool live = use > 0.f;  // false for 0 and NaN
+  for (int32_t i = threadIdx.x; i < total; i += kAppendThreads) {
+    const int32_t t = i / dim, d = i - t * dim;
+    const int64_t row = begin + static_cast<int64_t>(a.own.position(lo + t)) - start;
+    const float x = static_cast<float>(src[row * src_token + d]);
+    dst[static_cast<int64_t>(lo - page_first + t) * dst_token + d] = live ? to_e4m3(__fdiv_rn(x, use)) : 0;
+  }
+  if (!fresh && live && use > old) {
+    const uint32_t skip = lo - static_cast<uint32_t>(page_first);
+    const float ratio = __fdiv_rn(old, use);
+    for (int32_t i = threadIdx.x; i < (static_cast<int32_t>(block_size) - count) * dim; i += kAppendThreads) {
+      int32_t t = i / dim;
+      const int32_t d = i - t * dim;
+      if (static_cast<uint32_t>(t) >= skip) t += count;
+      uint8_t* p = dst + t * dst_token + d;
+      *p = to_e4m3(from_e4m3(*p) * ratio);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- merge
+
+struct MergeArgs {
+  const void* outs;
+  const float* lses;
+  void* out;
+  float* lse;
+  int64_t outs_rank, outs_row, outs_head, out_row, out_head;
+  int64_t pairs;  // rows * heads
+  int32_t ranks, heads, dim;
+};
+
+constexpr int kMergeWarps = 8;
+
+// One warp for each (row, head).
+template <typename T>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ MergeArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t pair = static_cast<int64_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+  if (pair >= a.pairs) return;
+  const int64_t row = pair / a.heads;
+  const int64_t head = pair - row * a.heads;
+  float top = -INFINITY;
+  for (int i = 0; i < a.ranks; ++i) top = fmaxf(top, a.lses[i * a.pairs + pair]);
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = 0.f;
+  for (int i = 0; i < a.ranks; ++i) total += expf(a.lses[i * a.pairs + pair] - base);
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const T* src = static_cast<const T*>(a.outs) + row * a.outs_row + head * a.outs_head;
+  T* dst = static_cast<T*>(a.out) + row * a.out_row + head * a.out_head;
+  for (int d = lane; d < a.dim; d += 32) {
+    float x = 0.f;
+    for (int i = 0; i < a.ranks; ++i) {
+      const float l = a.lses[i * a.pairs + pair];
+      if (l != -INFINITY) x += expf(l - base) * inv * static_cast<float>(src[i * a.outs_rank + d]);
+    }
+    dst[d] = static_cast<T>(x);
+  }
+  if (a.lse != nullptr && lane == 0) a.lse[pair] = top + logf(total);
+}
+
+// ---------------------------------------------------------------- checks
+
+int check_cache(const silkern_cache_v1* c, PagedCache* out) {
+  if (c == nullptr || c->k == nullptr || c->k_scale == nullptr) return SILKERN_E_NULL;
+  const bool latent = c->key_dim == 576;
+  if (!latent && (c->v == nullptr || c->v_scale == nullptr)) return SILKERN_E_NULL;
+  if (latent ? (c->value_dim != 512 || c->kv_heads != 1 || c->v != nullptr || c->v_scale != nullptr)
+             : ((c->key_dim != 64 && c->key_dim != 128) || c->value_dim != c->key_dim)) {
+    return SILKERN_E_CACHE;
+  }
+  if (c->kv_heads < 1 || c->kv_heads > 65535 || c->num_blocks < 1) return SILKERN_E_CACHE;
+  if (c->block_size < 1 || c->block_size > 65536) return SILKERN_E_BLOCK_SIZE;
+  if (c->num_blocks > 0x7fffffff / c->block_size) return SILKERN_E_CACHE;
+  const int64_t strides[6] = {c->k_block, c->k_token, c->k_head, latent ? 0 : c->v_block,
+                              latent ? 0 : c->v_token, latent ? 0 : c->v_head};
+  for (const int64_t s : strides) {
+    if (s < 0 || s % 16 != 0) return SILKERN_E_CACHE;
+  }
+  if (reinterpret_cast<uintptr_t>(c->k) % 16 != 0 || reinterpret_cast<uintptr_t>(c->v) % 16 != 0) {
+    return SILKERN_E_CACHE;
+  }
+  out->k = static_cast<const uint8_t*>(c->k);
+  out->v = latent ? out->k : static_cast<const uint8_t*>(c->v);
+  out->k_scale = c->k_scale;
+  out->v_scale = latent ? c->k_scale : c->v_scale;
+  out->k_block = c->k_block;
+  out->k_token = c->k_token;
+  out->k_head = c->k_head;
+  out->v_block = latent ? c->k_block : c->v_block;
+  out->v_token = latent ? c->k_token : c->v_token;
+  out->v_head = latent ? c->k_head : c->v_head;
+  out->num_blocks = static_cast<uint32_t>(c->num_blocks);
+  out->kv_heads = static_cast<uint32_t>(c->kv_heads);
+  out->block = make_fastdiv(static_cast<uint32_t>(c->block_size));
+  return SILKERN_OK;
+}
+
+int check_owner(int32_t block_size, int32_t dcp_size, int32_t dcp_rank, int32_t interleave, Ownership* out) {
+  if (dcp_size < 1 || dcp_rank < 0 || dcp_rank >= dcp_size || interleave < 1) return SILKERN_E_DCP;
+  if (static_cast<int64_t>(dcp_size) * interleave > 0x7fffffff) return SILKERN_E_DCP;
+  if (block_size % interleave != 0) return SILKERN_E_BLOCK_SIZE;
+  out->group = make_fastdiv(static_cast<uint32_t>(dcp_size) * static_cast<uint32_t>(interleave));
+  out->interleave = make_fastdiv(static_cast<uint32_t>(interleave));
+  out->rank_first = static_cast<uint32_t>(dcp_rank) * static_cast<uint32_t>(interleave);
+  return SILKERN_OK;
+}
+
+int check_queries(const silkern_cache_v1* c, const void* q, int64_t q_row, int64_t q_head, int32_t type,
+                  int64_t rows, int32_t heads, void* out, int64_t out_row, int64_t out_head, float* lse,
+                  float softmax_scale, AttendArgs* a) {
+  if (q == nullptr || out == nullptr || lse == nullptr) return SILKERN_E_NULL;
+  if (type != SILKERN_BF16 && type != SILKERN_F16) return SILKERN_E_TYPE;
+  if (rows < 1 || rows > 0x7fffffff) return SILKERN_E_SHAPE;
+  if (heads < 1 || heads > 65535 || heads % c->kv_heads != 0) return SILKERN_E_HEADS;
+  if (q_row % 8 != 0 || q_head % 8 != 0 || reinterpret_cast<uintptr_t>(q) % 16 != 0) return SILKERN_E_CACHE;
+  if (!std::isfinite(softmax_scale)) return SILKERN_E_ATTEND;
+  a->q = q;
+  a->q_row = q_row;
+  a->q_head = q_head;
+  a->out = out;
+  a->out_row = out_row;
+  a->out_head = out_head;
+  a->lse = lse;
+  a->scale_log2 = softmax_scale * 1.4426950408889634f;
+  a->rows = static_cast<int32_t>(rows);
+  a->heads = heads;
+  a->heads_per_kv = heads / c->kv_heads;
+  a->one = make_fastdiv(1);
+  return SILKERN_OK;
+}
+
+}  // namespace
+}  // namespace silkern
+
+using namespace silkern;
+
+extern "C" int silkern_append_quantized_v1(const silkern_cache_v1* cache, const void* keys, int64_t key_token,
+                                           int64_t key_head, const void* values, int64_t value_token,
+                                           int64_t value_head, int32_t type, int64_t tokens,
+                                           const int32_t* cu_tokens, const int32_t* starts,
+                                           const int32_t* req_ids, int64_t sequences,
+                                           const int32_t* block_table, int64_t table_rows,
+                                           int64_t table_width, int32_t dcp_size, int32_t dcp_rank,
+                                           int32_t dcp_interleave, int32_t* status, void* stream) {
+  AppendArgs a{};
+  int rc = check_cache(cache, &a.cache);
+  if (rc != SILKERN_OK) return rc;
+  const bool latent = cache->key_dim == 576;
+  if (!keys || (!latent && !values) || !cu_tokens || !starts || !req_ids || !block_table) return SILKERN_E_NULL;
+  if (latent && values != nullptr) return SILKERN_E_CACHE;
+  if (type != SILKERN_BF16 && type != SILKERN_F16) return SILKERN_E_TYPE;
+  if (tokens < 1 || tokens > 0x7fffffff || sequences < 1 || sequences > 0x3fffffff || table_rows < 1 ||
+      table_width < 1 || table_width > 0x7fffffff) {
+    return SILKERN_E_SHAPE;
+  }
+  rc = check_owner(cache->block_size, dcp_size, dcp_rank, dcp_interleave, &a.own);
+  if (rc != SILKERN_OK) return rc;
+  a.keys = keys;
+  a.values = values;
+  a.key_token = key_token;
+  a.key_head = key_head;
+  a.value_token = value_token;
+  a.value_head = value_head;
+  a.key_dim = cache->key_dim;
+  a.value_dim = cache->value_dim;
+  a.tokens = static_cast<int32_t>(tokens);
+  a.sequences = static_cast<int32_t>(sequences);
+  a.cu_tokens = cu_tokens;
+  a.starts = starts;
+  a.req_ids = req_ids;
+  a.table = block_table;
+  a.table_rows = table_rows;
+  a.table_width = static_cast<uint32_t>(table_width);
+  const int64_t page_tokens = static_cast<int64_t>(cache->block_size) * dcp_size;
+  a.page_tokens = make_fastdiv(static_cast<uint32_t>(page_tokens > 0x7fffffff ? 0x7fffffff : page_tokens));
+  a.status = status;
+  const int64_t items = tokens / a.page_tokens.divisor + 2 * sequences;
+  if (items > 0x7fffffff) return SILKERN_E_SHAPE;
+  void (*fn)(AppendArgs) = type == SILKERN_BF16 ? append_kernel<__nv_bfloat16> : append_kernel<__half>;
+  return launch_pdl_grid(fn, dim3(static_cast<unsigned>(items), static_cast<unsigned>(cache->kv_heads), latent ? 1 : 2),
+                         kAppendThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
+}
+
+extern "C" int silkern_attend_selected_v1(const silkern_cache_v1* cache, const void* q, int64_t q_row, int64_t q_head,
+                                          int32_t type, int64_t rows, int32_t heads, const int32_t* slots,
+                                          int64_t slots_row, int64_t width, const int32_t* counts, void* out,
+                                          int64_t out_row, int64_t out_head, float* lse, float softmax_scale,
+                                          int32_t* status, void* stream) {
+  AttendArgs a{};
+  int rc = check_cache(cache, &a.cache);
+  if (rc != SILKERN_OK) return rc;
+  if (slots == nullptr) return SILKERN_E_NULL;
+  rc = check_queries(cache, q, q_row, q_head, type, rows, heads, out, out_row, out_head, lse, softmax_scale, &a);
+  if (rc != SILKERN_OK) return rc;
+  if (width < 1 || width > 0x7fffffff - 1024) return SILKERN_E_SHAPE;
+  a.slots = slots;
+  a.slots_row = slots_row;
+  a.width = static_cast<int32_t>(width);
+  a.counts = counts;
+  a.total_slots = static_cast<uint32_t>(cache->num_blocks * cache->block_size);
+  a.status = status;
+  return launch_attend(a, cache->key_dim, type, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int silkern_attend_window_v1(const silkern_cache_v1* cache, const void* q, int64_t q_row, int64_t q_head,
+                                        int32_t type, int64_t rows, int32_t heads, const int32_t* cu_tokens,
+                                        const int32_t* lengths, const int32_t* req_ids, int64_t sequences,
+                                        const int32_t* block_table, int64_t table_rows, int64_t table_width,
+                                        int64_t window, int64_t sinks, int32_t dcp_size, int32_t dcp_rank,
+                                        int32_t dcp_interleave, void* out, int64_t out_row, int64_t out_head,
+                                        float* lse, float softmax_scale, int32_t* status, void* stream) {
+  AttendArgs a{};
+  int rc = check_cache(cache, &a.cache);
+  if (rc != SILKERN_OK) return rc;
+  if (!cu_tokens || !lengths || !req_ids || !block_table) return SILKERN_E_NULL;
+  rc = check_queries(cache, q, q_row, q_head, type, rows, heads, out, out_row, out_head, lse, softmax_scale, &a);
+  if (rc != SILKERN_OK) return rc;
+  if (sequences < 1 || rows + sequences > 0x7fffffff || table_rows < 1 || table_width < 1 ||
+      table_width > 0x7fffffff) {
+    return SILKERN_E_SHAPE;
+  }
+  if (window < 0 || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff) return SILKERN_E_ATTEND;
+  rc = check_owner(cache->block_size, dcp_size, dcp_rank, dcp_interleave, &a.own);
+  if (rc != SILKERN_OK) return rc;
+  a.cu_tokens = cu_tokens;
+  a.lengths = lengths;
+  a.req_ids = req_ids;
+  a.sequences = static_cast<int32_t>(sequences);
+  a.table = block_table;
+  a.table_rows = table_rows;
+  a.table_width = static_cast<uint32_t>(table_width);
+  a.window = static_cast<uint32_t>(window);
+  a.sinks = static_cast<uint32_t>(sinks);
+  a.status = status;
+  return launch_attend(a, cache->key_dim, type, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int silkern_merge_partials_v1(const void* outs, int64_t outs_rank, int64_t outs_row, int64_t outs_head,
+                                         const float* lses, int32_t type, int64_t ranks, int64_t rows, int64_t heads,
+                                         int64_t dim, void* out, int64_t out_row, int64_t out_head, float* lse,
+                                         void* stream) {
+  if (outs == nullptr || lses == nullptr || out == nullptr) return SILKERN_E_NULL;
+  if (type != SILKERN_BF16 && type != SILKERN_F16) return SILKERN_E_TYPE;
+  if (ranks < 1 || ranks > 0x7fffffff || rows < 1 || heads < 1 || heads > 0x7fffffff || dim < 1 ||
+      dim > 0x7fffffff || rows > (int64_t{1} << 31) * kMergeWarps / heads - kMergeWarps) {
+    return SILKERN_E_SHAPE;
+  }
+  MergeArgs a{outs, lses, out, lse, outs_rank, outs_row, outs_head, out_row, out_head, rows * heads,
+              static_cast<int32_t>(ranks), static_cast<int32_t>(heads), static_cast<int32_t>(dim)};
+  void (*fn)(MergeArgs) = type == SILKERN_BF16 ? merge_kernel<__nv_bfloat16> : merge_kernel<__half>;
+  const int64_t ctas = (a.pairs + kMergeWarps - 1) / kMergeWarps;
+  if (ctas > 0x7fffffff) return SILKERN_E_SHAPE;
+  return launch_pdl(fn, static_cast<unsigned>(ctas), kMergeWarps * 32, 0, 1, static_cast<cudaStream_t>(stream), a);
+}

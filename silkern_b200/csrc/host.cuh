@@ -1,0 +1,71 @@
+// Host-side helpers of the entry points over the 8-bit paged cache.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <mutex>
+#include <utility>
+#include <vector>
+
+#include "silkern_b200.h"
+
+namespace silkern {
+
+// Launch `fn` under programmatic dependent launch, `cluster` CTAs to a
+// thread-block cluster. 0 or -(cudaError_t).
+template <typename... P, typename... A>
+int launch_pdl_grid(void (*fn)(P...), dim3 grid, unsigned threads, size_t smem, unsigned cluster,
+                    cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = cluster;
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  cfg.attrs = attrs;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, fn, args...);
+  if (err != cudaSuccess) {
+    (void)cudaGetLastError();
+    return -static_cast<int>(err);
+  }
+  return SILKERN_OK;
+}
+
+template <typename... P, typename... A>
+int launch_pdl(void (*fn)(P...), unsigned grid, unsigned threads, size_t smem, unsigned cluster,
+               cudaStream_t stream, A&&... args) {
+  return launch_pdl_grid(fn, dim3(grid, 1, 1), threads, smem, cluster, stream, args...);
+}
+
+// Let `kernel` use `bytes` of dynamic shared memory on the current device. The
+// driver is asked once for each kernel and device.
+inline int allow_shared_memory(const void* kernel, int bytes) {
+  static std::mutex mutex;
+  static std::vector<std::pair<const void*, int>> granted;
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err == cudaSuccess) {
+    std::lock_guard<std::mutex> lock(mutex);
+    for (const auto& g : granted) {
+      if (g.first == kernel && g.second == device) return SILKERN_OK;
+    }
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err == cudaSuccess) granted.emplace_back(kernel, device);
+  }
+  if (err == cudaSuccess) return SILKERN_OK;
+  (void)cudaGetLastError();
+  return -static_cast<int>(err);
+}
+
+}  // namespace silkern

@@ -1287,6 +1287,10 @@ extern "C" const char* silkern_status_string_v1(int code) {
     case SILKERN_E_GEOMETRY: return "explicit launch geometry rejected";
     case SILKERN_E_SCRATCH:
       return "batch x tiles exceeds the allocation-free entry point's static workspace";
+    case SILKERN_E_CACHE: return "unsupported cache geometry, stride or alignment";
+    case SILKERN_E_HEADS: return "heads must be a positive multiple of the cache's heads";
+    case SILKERN_E_TYPE: return "element type must be bfloat16 or float16";
+    case SILKERN_E_ATTEND: return "window, sinks or softmax scale out of range";
     default: break;
   }
   if (code < 0) return cudaGetErrorString(static_cast<cudaError_t>(-code));
