@@ -68,16 +68,19 @@ def append(keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, 
 
 
 def attend_row(q, slot, k_cache, v_cache, k_scale, v_scale, softmax_scale):
-    """One query row (heads, dim) over its int64 slots: (out, lse, spread).
+    """One query row (heads, dim) over its int64 slots: (out, lse, spread, near).
 
     ``spread`` (heads, value_dim) is the weighted mean of the values'
     magnitudes: an error of relative size u in each weight moves ``out`` by at
-    most ``u * spread``."""
+    most ``u * spread``. ``near`` is the same with each weight replaced by the
+    largest among its neighbours, up to 127 places away: an error of u times
+    the largest weight of a weight's run of 128 moves ``out`` by at most
+    ``u * near``."""
     heads, kv_heads = q.shape[0], k_cache.shape[2]
     value_dim = 512 if v_cache is None else v_cache.shape[3]
     if slot.numel() == 0:
         zero = torch.zeros((heads, value_dim), dtype=torch.float64, device=q.device)
-        return zero, torch.full((heads,), -math.inf, dtype=torch.float64, device=q.device), zero
+        return zero, torch.full((heads,), -math.inf, dtype=torch.float64, device=q.device), zero, zero
     block, offset = slot // k_cache.shape[1], slot % k_cache.shape[1]
     k = k_cache[block, offset].float().double() * k_scale[block].double()[:, :, None]
     v = k[:, :, :value_dim] if v_cache is None else (
@@ -88,7 +91,9 @@ def attend_row(q, slot, k_cache, v_cache, k_scale, v_scale, softmax_scale):
     weight = torch.exp(score - lse[..., None])
     out = torch.einsum("hgn,nhd->hgd", weight, v)
     spread = torch.einsum("hgn,nhd->hgd", weight, v.abs())
-    return out.reshape(heads, value_dim), lse.reshape(heads), spread.reshape(heads, value_dim)
+    around = torch.nn.functional.max_pool1d(weight, 255, stride=1, padding=127)
+    near = torch.einsum("hgn,nhd->hgd", around, v.abs())
+    return out.reshape(heads, value_dim), lse.reshape(heads), spread.reshape(heads, value_dim), near.reshape(heads, value_dim)
 
 
 def attend_selected(q, slots, k_cache, v_cache, k_scale, v_scale, *, softmax_scale, counts=None):
@@ -105,7 +110,7 @@ def attend_selected(q, slots, k_cache, v_cache, k_scale, v_scale, *, softmax_sca
 
 def attend_window(q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale, *,
                   softmax_scale, window=0, sinks=0, dcp_size=1, dcp_rank=0, dcp_interleave=1):
-    """(out, lse, spread) of the rows below cu_tokens[-1]."""
+    """(out, lse, spread, near) of the rows below cu_tokens[-1]."""
     rows = []
     block_size = k_cache.shape[1]
     cu, length, req = (t.tolist() for t in (cu_tokens, lengths, req_ids))

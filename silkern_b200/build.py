@@ -24,12 +24,18 @@ SOURCES = [
     os.path.join(CSRC, "atomic_baseline.cu"),
     os.path.join(CSRC, "cache_ops.cu"),
     os.path.join(CSRC, "attend.cu"),
+    os.path.join(CSRC, "attend_dim64.cu"),
+    os.path.join(CSRC, "attend_dim128.cu"),
+    os.path.join(CSRC, "attend_latent.cu"),
 ]
 DEPENDS = SOURCES + [
     os.path.join(CSRC, "fastdiv.cuh"),
     os.path.join(CSRC, "ptx.cuh"),
     os.path.join(CSRC, "host.cuh"),
     os.path.join(CSRC, "paged.cuh"),
+    os.path.join(CSRC, "tcgen05.cuh"),
+    os.path.join(CSRC, "attend_plan.cuh"),
+    os.path.join(CSRC, "attend_kernel.cuh"),
     os.path.join(INCLUDE, "silkern_b200.h"),
 ]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

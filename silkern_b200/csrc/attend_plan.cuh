@@ -1,0 +1,25 @@
+// How one attention call is laid over the GPU, and the launchers of the
+// kernel for each cache shape (one translation unit each).
+#pragma once
+
+#include "paged.cuh"
+
+namespace silkern {
+
+struct AttendPlan {
+  FastDiv per;     // queries of one sequence that share a CTA
+  int32_t blocks;  // column blocks of one (item, cache head)
+};
+
+struct AttendLaunch {
+  int columns;  // 16, 32 or 64 (query, head) pairs to a CTA
+  bool half;    // fp16 queries
+  unsigned grid, cluster;
+  cudaStream_t stream;
+};
+
+int launch_dim64(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);
+int launch_dim128(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);
+int launch_latent(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);
+
+}  // namespace silkern

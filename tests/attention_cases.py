@@ -41,18 +41,22 @@ def score_error(q, k_cache, k_scale, softmax_scale):
 
 
 def assert_attention(out, lse, want, q, k_cache, k_scale, softmax_scale):
-    """out within half a step of the output's type, plus what a weight's error makes.
+    """out within half a step of the output's type, plus what the weights' errors make.
 
-    A weight is a float32 exponential rounded to at least 8 (bf16) or 11
-    (fp16) bits, so its relative error is at most half a step of the type, plus
-    the score's own error (twice: in the weight and in the sum), plus 2**-14 of
-    the largest weight of its tile for those that are far below it, of which a
-    tile has 128: together 2**-7 of one weight's share, and never more than
-    2**-9 of the spread where scores are spread over a tile."""
-    ref_out, ref_lse, spread = want
+    A weight enters the product as x = 2^(u - R + 5), with the tile's largest x
+    in [2, 2^8.5], in parts of 8 bits. A first e4m3 part leaves at most
+    max(2^-4 2^e, 2^-10) for x in [2^e, 2^(e + 1)); an e5m2 part leaves of a
+    remainder r at most half a step of r's binade, which is 2^-3 of the
+    binade's start, or 2^-17 below 2^-14. So two parts (bf16) leave at most
+    max(2^-8 x, 2^-14), with 2^-11 x more from their way through fp16, and
+    three (fp16) max(2^-12 x, 2^-17): relative errors of 2^-8 + 2^-11 and 2^-12
+    in each weight, and 2^-15 and 2^-18 of the largest weight of its tile. The
+    score's own error counts twice, in the weight and in the sum."""
+    ref_out, ref_lse, spread, near = want
     u = HALF_STEP[out.dtype]
+    relative, floor = {torch.bfloat16: (2.0**-8 + 2.0**-11, 2.0**-15), torch.float16: (2.0**-12, 2.0**-18)}[out.dtype]
     ds = score_error(q, k_cache, k_scale, softmax_scale)
-    bound = u * ref_out.abs() + (u + 2 * ds + 2.0**-13) * spread + 1e-30
+    bound = u * ref_out.abs() + (relative + 2 * ds) * spread + floor * near + 1e-30
     error = (out.double() - ref_out).abs()
     bad = ~(error <= bound)
     assert not bool(bad.any()), f"{int(bad.sum())} outputs off, worst {float((error / bound).nan_to_num(9e9).max()):.3g} bounds"

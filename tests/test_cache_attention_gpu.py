@@ -555,8 +555,8 @@ def test_a_decode_step_over_ranks_is_attention_over_the_whole_selection(latent) 
     graph.replay()
     torch.cuda.synchronize()
     cache, _, slots, _ = alone
-    want, want_lse, spread = oracle.attend_selected(q, slots, *cache, softmax_scale=scale)
-    assert_attention(whole, whole_lse, (want, want_lse, spread), q, cache[0], cache[2], scale)
+    want, want_lse, spread, near = oracle.attend_selected(q, slots, *cache, softmax_scale=scale)
+    assert_attention(whole, whole_lse, (want, want_lse, spread, near), q, cache[0], cache[2], scale)
     # A rank's pages hold other tokens, so scales differ, and with them only codes that are subnormal in
     # one of the two (below 2**-6 of a code range that starts at 224): 2**-10 of a scale of at most 2**-5,
     # on both keys and values. Each partial output adds a rounding of its own.
