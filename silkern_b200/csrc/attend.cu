@@ -31,7 +31,7 @@ int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t strea
   // A latent cache's fp16 queries have three parts: 64 columns of them do not
   // fit the shared memory beside the keys.
   const int widest = latent && half ? 32 : 64;
-  const int columns = want <= 16 ? 16 : want <= 32 || widest == 32 ? 32 : 64;
+  const int columns = want <= 16 ? 16 : want <= 32 || widest == 32 || (latent && group <= 32) ? 32 : 64;
   const int32_t per = a.slots != nullptr || group >= columns ? 1 : columns / group;
   AttendPlan plan;
   plan.per = make_fastdiv(static_cast<uint32_t>(per));
@@ -48,12 +48,12 @@ int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t strea
     if (seen < keys) keys = seen;
   }
   const int64_t tiles = (keys + 127) / 128;
-  // Few work items: a cluster of up to 8 CTAs takes the tiles of each, as
+  // Few work items: a cluster of up to 16 CTAs takes the tiles of each, as
   // long as the CTAs still find an SM each and a tile each.
   const int64_t ctas = busy * a.cache.kv_heads * plan.blocks;
   const int64_t room = static_cast<int64_t>(multiprocessors()) * (!latent && columns == 16 ? 2 : 1);
   unsigned cluster = 1;
-  while (cluster < 8 && ctas * cluster * 2 <= room && tiles >= cluster * 2) cluster *= 2;
+  while (cluster < 16 && ctas * cluster * 2 <= room && tiles >= cluster * 2) cluster *= 2;
   const int64_t grid = items * a.cache.kv_heads * plan.blocks * cluster;
   if (grid > 0x7fffffff) return SILKERN_E_SHAPE;
   AttendLaunch l{columns, half, static_cast<unsigned>(grid), cluster, stream};

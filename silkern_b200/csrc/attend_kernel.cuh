@@ -71,24 +71,36 @@ struct Config {
   static constexpr int kGroups = NH >= 32 ? 2 : 1;               // softmax warpgroups, by columns
   static constexpr int kCols = NH / kGroups;                     // columns of a softmax thread
   static constexpr int kSoftmax = kGroups * 128;
-  static constexpr int kThreads = kSoftmax + 128 + 32;
+  // Two CTAs to an SM where a column block is narrow: each hides the other's
+  // start, end and softmax. With 4 + 2 + 1 warps (registers are given out for
+  // eight) both have 128 registers a thread. Otherwise one CTA, with all of
+  // shared memory.
+  static constexpr int kPerSm = !kIsLatent && NH == 16 ? 2 : 1;
+  static constexpr int kLoaders = kPerSm == 2 ? 2 : 4;           // gathering warps
+  static constexpr int kThreads = kSoftmax + kLoaders * 32 + 32;
   static constexpr int kQBytes = T * NH * kKeyDim;
   static constexpr int kPBytes = T * NH * kTile;
-  static constexpr int kMisc = 3072;
+  // Columns of several queries see different keys. 64 columns of a latent
+  // cache are one query's, so that its shared memory need not hold positions.
+  static constexpr bool kSeveral = !(kIsLatent && NH == 64);
+  static constexpr int kNoteBytes = kTile * ((kIsLatent ? 4 : 8) + (kSeveral ? 4 : 0)) + 16;  // a tile's scales, positions
+  static constexpr int kMisc = 20 * NH + (kSeveral ? 8 * NH : 0) + 256;
   static constexpr int kColumnsUsed = kValues * NH + 2 * T * NH;
   static constexpr int kColumns = kColumnsUsed <= 128 ? 128 : kColumnsUsed <= 256 ? 256 : 512;
   static_assert(kColumnsUsed <= 512, "TMEM");
-  // Two CTAs to an SM where a column block is narrow: each hides the other's
-  // start, end and softmax. Otherwise one, with all of shared memory.
-  static constexpr int kPerSm = !kIsLatent && NH == 16 ? 2 : 1;
   static constexpr int kSmemMax = smem_for_columns(512 / kPerSm);
   static constexpr int kFixed = kQBytes + kPBytes + kMisc;
-  static constexpr int kStages = kIsLatent ? 2 : (kSmemMax - kFixed) / kStageBytes < 8 ? (kSmemMax - kFixed) / kStageBytes : 8;
-  static constexpr int kTails = kIsLatent ? ((kSmemMax - kFixed - 2 * kStageBytes) >= 2 * kTailBytes ? 2 : 1) : 0;
-  static constexpr int kUsed = kFixed + kStages * kStageBytes + kTails * kTailBytes;
+  static constexpr int kStageCost = kStageBytes + kNoteBytes + 16 * kLoadChunks;  // with its barriers
+  static constexpr int kFit = (kSmemMax - kFixed) / kStageCost;
+  static constexpr int kStages = kIsLatent ? 2 : kFit < 8 ? kFit : 8;
+  static constexpr int kTails = kIsLatent ? ((kSmemMax - kFixed - 2 * kStageCost) >= 2 * kTailBytes ? 2 : 1) : 0;
+  static constexpr int kUsed = kFixed + kStages * kStageCost + kTails * kTailBytes;
   static_assert(kStages >= 2 && kUsed <= kSmemMax, "shared memory");
   static constexpr int kSmem = kUsed > smem_for_columns(kColumns) ? kUsed : smem_for_columns(kColumns);
   static_assert(NH * kValueDim * 4 <= kStages * kStageBytes, "joining buffer");
+  // The chunk whose buffer is free again only after a tile's softmax, and
+  // with it the tile's scales and positions.
+  static constexpr int kNoteChunk = kIsLatent ? 0 : 1;
   // Offsets from the dynamic shared memory's start.
   static constexpr int kOffTail = kStages * kStageBytes;
   static constexpr int kOffQ = kOffTail + kTails * kTailBytes;
@@ -97,18 +109,21 @@ struct Config {
 };
 
 // The small shared state behind the tiles.
-template <int NH, int CHUNKS, int STAGES>
+template <typename C, int NH>
 struct __align__(16) Shared {
-  int32_t best[3][NH];     // running column maxima of a tile, as ordered integers
-  float reference[8][32];  // each softmax warp's copy of its columns' references
-  float factor[NH];        // score factor of a column, then 1 / (32 l)
-  int32_t seen_to[NH], seen_from[NH];  // positions that a column sees: below, from
-  uint64_t full[CHUNKS][STAGES], empty[CHUNKS][STAGES];
+  int32_t best[3][NH];  // column maxima of a tile, as ordered integers
+  float reference[NH];  // the columns' references R, at the end their output factors
+  float factor[NH];     // the columns' score factors
+  int32_t seen_to[C::kSeveral ? NH : 1], seen_from[C::kSeveral ? NH : 1];  // positions that a column sees: below, from
+  float k_scale[C::kStages][kTile];
+  float v_scale[C::kIsLatent ? 1 : C::kStages][C::kIsLatent ? 1 : kTile];
+  int32_t position[C::kSeveral ? C::kStages : 1][C::kSeveral ? kTile : 1];
+  uint32_t valid[C::kStages][4];  // a bit for each key
+  uint64_t full[C::kLoadChunks][C::kStages], empty[C::kLoadChunks][C::kStages];
   uint64_t scores[2], weights, done, queries, drained;
   uint32_t tmem;
   int32_t abort;
 };
-
 __device__ __forceinline__ int32_t ordered(float x) {
   const int32_t b = __float_as_int(x);
   return b >= 0 ? b : b ^ 0x7fffffff;
@@ -164,8 +179,7 @@ __device__ __forceinline__ void split4_f16(const float (&x)[4], uint32_t (&part)
 }
 
 template <typename E>
-__device__ __forceinline__ void load4(const E* p, float (&x)[4]) {
-  const uint2 raw = *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ void unpack4(const uint2 raw, float (&x)[4]) {
   if constexpr (std::is_same<E, __nv_bfloat16>::value) {
     x[0] = __uint_as_float(raw.x << 16);
     x[1] = __uint_as_float(raw.x & 0xffff0000u);
@@ -181,6 +195,26 @@ __device__ __forceinline__ void load4(const E* p, float (&x)[4]) {
   }
 }
 
+// Sums each of a thread's N columns over the warp: lane c gets column c mod N.
+// Each step adds up half of the columns with the lane across and gives the
+// other half away.
+template <int N>
+__device__ __forceinline__ float sum_columns(float (&x)[N], int lane) {
+#pragma unroll
+  for (int half = N / 2; half > 0; half >>= 1) {
+    const bool upper = (lane & half) != 0;
+#pragma unroll
+    for (int c = 0; c < half; ++c) {
+      const float keep = upper ? x[c + half] : x[c], give = upper ? x[c] : x[c + half];
+      x[c] = keep + __shfl_xor_sync(kAllLanes, give, half);
+    }
+  }
+  float y = x[0];
+#pragma unroll
+  for (int d = N; d < 32; d <<= 1) y += __shfl_xor_sync(kAllLanes, y, d);
+  return y;
+}
+
 // A column of the CTA: which query (of the span) and head it is.
 struct Column {
   int32_t query, head;
@@ -193,11 +227,11 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
   using C = Config<SHAPE, NH, T>;
   using E = typename std::conditional<T == 2, __nv_bfloat16, __half>::type;
   extern __shared__ __align__(1024) uint8_t smem[];
-  using S = Shared<NH, C::kLoadChunks, C::kStages>;
-  static_assert(sizeof(S) <= C::kMisc, "shared state");
+  using S = Shared<C, NH>;
+  static_assert(C::kOffMisc + sizeof(S) <= C::kSmem, "shared state");
   S& sh = *reinterpret_cast<S*>(smem + C::kOffMisc);
   const uint32_t base = smem_addr(smem);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(kAllLanes, tid >> 5, 0);
   constexpr int kMmaWarp = C::kThreads / 32 - 1;
   constexpr int kLoadWarp = C::kSoftmax / 32;
 
@@ -205,7 +239,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
   if (tid == 0) {
     for (int c = 0; c < C::kLoadChunks; ++c) {
       for (int b = 0; b < C::kStages; ++b) {
-        mbar_init(smem_addr(&sh.full[c][b]), 128);
+        mbar_init(smem_addr(&sh.full[c][b]), C::kLoaders * (c == C::kNoteChunk ? 64 : 32));
         mbar_init(smem_addr(&sh.empty[c][b]), 1);
       }
     }
@@ -219,12 +253,15 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
-  if (tid < NH) sh.best[0][tid] = ordered(-INFINITY);
+  if (tid < NH) {
+    sh.best[0][tid] = ordered(-INFINITY);
+    sh.reference[tid] = 0.f;
+  }
   if (warp == kMmaWarp) tmem_alloc(smem_addr(&sh.tmem), C::kColumns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = __shfl_sync(kAllLanes, sh.tmem, 0);
   volatile int* abort = &sh.abort;
   pdl_wait();
   pdl_launch_dependents();
@@ -264,51 +301,69 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
       // ================================================== queries, softmax
       const int wg = warp >> 2;
       const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane quadrant, << 16
-      // -- split the queries: a warp takes a column at a time
-      for (int c = warp; c < NH; c += kLoadWarp) {
-        const Column col = column(c);
-        constexpr int kPieces = (C::kKeyDim / 4 + 31) / 32;
-        float x[kPieces][4];
-        uint32_t most = 0;
-        const E* q = static_cast<const E*>(a.q) + static_cast<int64_t>(span.row + col.query) * a.q_row +
-                     static_cast<int64_t>(col.head) * a.q_head;
+      // -- split the queries: a warp takes four columns at a time, so that
+      // their loads overlap
+      constexpr int kPieces = (C::kKeyDim / 4 + 31) / 32;
+      constexpr int kBatch = 4;
+      for (int c0 = warp * kBatch; c0 < NH; c0 += kLoadWarp * kBatch) {
+        uint2 raw[kBatch][kPieces];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int d = (i * 32 + lane) * 4;
-          x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-          if (col.used && d < C::kKeyDim) load4(q + d, x[i]);
+        for (int n = 0; n < kBatch; ++n) {
+          const Column col = column(c0 + n);
+          const E* q = static_cast<const E*>(a.q) + static_cast<int64_t>(span.row + col.query) * a.q_row +
+                       static_cast<int64_t>(col.head) * a.q_head;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(x[i][k]) & 0x7fffffffu);
-        }
-        most = __reduce_max_sync(kAllLanes, most);
-        // The largest magnitude comes to [128, 256): its exponent field is taken off.
-        const int e = max(static_cast<int>(most >> 23), 40);
-        const bool odd = most >= 0x7f800000u;  // an infinity or NaN: the row becomes NaN
-        const float up = odd ? 1.f : __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
-        if (lane == 0) {
-          sh.factor[c] = odd ? NAN : a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
-          const int32_t position = span.position + col.query;
-          sh.seen_to[c] = col.used ? position + 1 : 0x7fffffff;
-          sh.seen_from[c] = col.used && a.window != 0 && position + 1 > static_cast<int64_t>(a.window)
-                                ? position + 1 - static_cast<int32_t>(a.window) : 0;
+          for (int i = 0; i < kPieces; ++i) {
+            const int d = (i * 32 + lane) * 4;
+            raw[n][i] = make_uint2(0u, 0u);
+            if (col.used && d < C::kKeyDim) raw[n][i] = *reinterpret_cast<const uint2*>(q + d);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int d = (i * 32 + lane) * 4;
-          if (d < C::kKeyDim) {
-            float y[4];
+        for (int n = 0; n < kBatch; ++n) {
+          const int c = c0 + n;
+          uint32_t most = 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = odd ? 0.f : x[i][k] * up;
-            uint32_t part[T];
-            split4<T, false>(y, part);
-            const int chunk = d / 128, in = d & 127;
-            const bool narrow = C::kWide == 64 || (C::kIsLatent && chunk == 4);
+          for (int i = 0; i < kPieces; ++i) {
+            float x[4];
+            unpack4<E>(raw[n][i], x);
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-              const int row = t * NH + c;
-              const uint32_t at = narrow ? row * 64 + ((((in >> 4) ^ (row >> 1)) & 3) << 4) + (in & 15)
-                                         : row * 128 + ((((in >> 4) ^ row) & 7) << 4) + (in & 15);
-              st_shared(base + C::kOffQ + chunk * (T * NH * 128) + at, part[t]);
+            for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(x[k]) & 0x7fffffffu);
+          }
+          most = __reduce_max_sync(kAllLanes, most);
+          // The largest magnitude comes to [128, 256): its exponent field is taken off.
+          const int e = max(static_cast<int>(most >> 23), 40);
+          const bool odd = most >= 0x7f800000u;  // an infinity or NaN: the row becomes NaN
+          const float up = odd ? 0.f : __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
+          if (lane == 0) {
+            sh.factor[c] = odd ? NAN : a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
+            if constexpr (C::kSeveral) {
+              const Column col = column(c);
+              const int32_t position = span.position + col.query;
+              sh.seen_to[c] = col.used ? position + 1 : 0x7fffffff;
+              sh.seen_from[c] = col.used && a.window != 0 && position + 1 > static_cast<int64_t>(a.window)
+                                    ? position + 1 - static_cast<int32_t>(a.window) : 0;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            const int d = (i * 32 + lane) * 4;
+            if (d < C::kKeyDim) {
+              float y[4];
+              unpack4<E>(raw[n][i], y);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) y[k] = odd ? 0.f : y[k] * up;
+              uint32_t part[T];
+              split4<T, false>(y, part);
+              const int chunk = d / 128, in = d & 127;
+              const bool narrow = C::kWide == 64 || (C::kIsLatent && chunk == 4);
+#pragma unroll
+              for (int t = 0; t < T; ++t) {
+                const int row = t * NH + c;
+                const uint32_t at = narrow ? row * 64 + ((((in >> 4) ^ (row >> 1)) & 3) << 4) + (in & 15)
+                                           : row * 128 + ((((in >> 4) ^ row) & 7) << 4) + (in & 15);
+                st_shared(base + C::kOffQ + chunk * (T * NH * 128) + at, part[t]);
+              }
             }
           }
         }
@@ -324,35 +379,18 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
 #pragma unroll
       for (int c = 0; c < CW; ++c) l[c] = 0.f;
       float reference = -INFINITY, highest = -INFINITY;  // of column first_col + lane
-      const int32_t mine = tile_begin * kTile + (tid & 127);
       const int32_t all_to = span.position + 1;  // positions below are seen by every query, from
       const int32_t all_from =
           a.window == 0 ? 0
                         : static_cast<int32_t>(max(int64_t{0}, static_cast<int64_t>(span.position) + span.count - a.window));
-      int32_t fetched = fetch_key(a, keys, mine);
-      Key key = locate_key(a, keys, mine, fetched);
-      const int64_t kv_heads = a.cache.kv_heads;
-      float ks = 0.f, vs = 0.f;
-      if (key.valid) {
-        ks = __ldg(a.cache.k_scale + key.block * kv_heads + kv);
-        vs = C::kIsLatent ? ks : __ldg(a.cache.v_scale + key.block * kv_heads + kv);
-      }
-      fetched = fetch_key(a, keys, mine + kTile);
-      if (lane < CW) sh.reference[warp][lane] = 0.f;
-      __syncwarp();
       for (int32_t i = 0; i < steps; ++i) {
-        // The next tile's key and scales, a tile ahead.
-        const int32_t next_j = mine + (i + 1) * kTile;
-        const Key next = i + 1 < steps ? locate_key(a, keys, next_j, fetched) : Key{0u, 0u, 0, false};
-        float next_ks = 0.f, next_vs = 0.f;
-        if (next.valid) {
-          next_ks = __ldg(a.cache.k_scale + next.block * kv_heads + kv);
-          next_vs = C::kIsLatent ? next_ks : __ldg(a.cache.v_scale + next.block * kv_heads + kv);
-        }
-        fetched = i + 2 < steps ? fetch_key(a, keys, next_j + kTile) : -1;
-
         warp_wait(&sh.scores[i & 1], (i >> 1) & 1, abort);
         tc_fence_after();
+        const uint32_t b = i % C::kStages;
+        warp_wait(&sh.full[C::kNoteChunk][b], (i / C::kStages) & 1, abort);
+        const bool valid = (sh.valid[b][warp & 3] >> lane) & 1;
+        const float ks = sh.k_scale[b][tid & 127];
+        const float vs = C::kIsLatent ? ks : sh.v_scale[C::kIsLatent ? 0 : b][C::kIsLatent ? 0 : tid & 127];
         const uint32_t s_at = tmem + lanes + C::kValues * NH + (i & 1) * (T * NH) + first_col;
         float t[CW];
 #pragma unroll
@@ -379,18 +417,21 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float s = (s0[c + k] + s1[c + k] * 0.0625f) * (ks * fs[k]);
-              t[h + c + k] = key.valid ? s : -INFINITY;
+              t[h + c + k] = valid ? s : -INFINITY;
             }
           }
         }
-        if (several && !(key.position < all_to &&
-                         (key.position >= all_from || static_cast<uint32_t>(key.position) < a.sinks))) {
-          const bool sink = static_cast<uint32_t>(key.position) < a.sinks;
+        if constexpr (C::kSeveral) {
+          if (several) {
+            const int32_t at = sh.position[b][tid & 127];
+            const bool sink = static_cast<uint32_t>(at) < a.sinks;
+            if (!(at < all_to && (at >= all_from || sink))) {
 #pragma unroll
-          for (int c = 0; c < CW; ++c) {
-            const bool seen = key.position < sh.seen_to[first_col + c] &&
-                              (key.position >= sh.seen_from[first_col + c] || sink);
-            if (!seen) t[c] = -INFINITY;
+              for (int c = 0; c < CW; ++c) {
+                const bool seen = at < sh.seen_to[first_col + c] && (at >= sh.seen_from[first_col + c] || sink);
+                if (!seen) t[c] = -INFINITY;
+              }
+            }
           }
         }
         // Largest u of each column: lane c of a warp has column c's.
@@ -416,8 +457,9 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
           const float by = !move ? 1.f : reference == -INFINITY ? 0.f : exp2_approx(reference - to);
           reference = to;
           highest = fmaxf(highest, to);
-          __syncwarp();
-          if (lane < CW) sh.reference[warp][lane] = to == -INFINITY ? 0.f : to;
+          // The group's warps all write the same numbers: whoever reads them has
+          // written them, and nobody is still at the tile before.
+          if (lane < CW) sh.reference[first_col + lane] = to == -INFINITY ? 0.f : to;
           __syncwarp();
           if (i > 0) {
             warp_wait(&sh.done, (i - 1) & 1, abort);
@@ -452,7 +494,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
         uint32_t part[CW / 4][T];
 #pragma unroll
         for (int c = 0; c < CW; c += 4) {
-          const float4 r = *reinterpret_cast<const float4*>(&sh.reference[warp][c]);
+          const float4 r = *reinterpret_cast<const float4*>(&sh.reference[first_col + c]);
           const float rs[4] = {r.x, r.y, r.z, r.w};
           float w[4];
 #pragma unroll
@@ -483,9 +525,6 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
         fence_proxy_async();
         tc_fence_before();
         mbar_arrive(smem_addr(&sh.weights));
-        key = next;
-        ks = next_ks;
-        vs = next_vs;
       }
       if (steps > 0) warp_wait(&sh.done, (steps - 1) & 1, abort);
       tc_fence_after();
@@ -493,14 +532,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
       // -- sums over the keys: lanes first, then the group's warps. The
       // weights' buffer is free by now and takes the warps' sums.
       float* sums = reinterpret_cast<float*>(smem + C::kOffP) + wg * (4 * CW);
-      float mine_l = 0.f;
-#pragma unroll
-      for (int c = 0; c < CW; ++c) {
-        float x = l[c];
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(kAllLanes, x, d);
-        if ((lane & (CW - 1)) == c) mine_l = x;
-      }
+      float mine_l = sum_columns<CW>(l, lane);
       if (lane < CW) sums[(warp & 3) * CW + lane] = mine_l;
       named_barrier(2 + wg, 128);
       const int own = lane & (CW - 1);
@@ -534,36 +566,53 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
         }
       }
       __syncwarp();
-      if (lane < CW) sh.reference[warp][lane] = part_of * inverse;
+      if (lane < CW) sh.reference[first_col + lane] = part_of * inverse;
       __syncwarp();
 
-      // -- outputs: straight from TMEM, or by way of shared memory to be joined
-      const int rows_of = SHAPE == kDim64 ? 64 : 128;
-      if (steps > 0 && !__any_sync(kAllLanes, *abort != 0)) {
-        float* joined = reinterpret_cast<float*>(smem);
+      // -- outputs by way of the tiles' shared memory: in float32 to be joined
+      // by the cluster, else as they are stored, in rows of a column
+      constexpr int kRowsOf = SHAPE == kDim64 ? 64 : 128;  // of M = 128
+      const bool failed = __any_sync(kAllLanes, *abort != 0);
+      if (steps > 0 && !failed && (warp & 3) * 32 < kRowsOf) {
 #pragma unroll 1
         for (int m = 0; m < C::kValues; ++m) {
           const int d = m * 128 + (warp & 3) * 32 + lane;
-          if ((warp & 3) * 32 < rows_of) {
-#pragma unroll 1
-            for (int h = 0; h < CW; h += 16) {
-              float o[16];
-              tmem_ld16(tmem + lanes + m * NH + first_col + h, o);
-              tmem_wait_ld(o);
 #pragma unroll
-              for (int c = 0; c < 16; ++c) {
-                const float y = o[c] * sh.reference[warp][h + c];
-                if (ranks > 1) {
-                  joined[(first_col + h + c) * C::kValueDim + d] = y;
-                } else {
-                  const Column col = column(first_col + h + c);
-                  if (col.used) {
-                    E* out = static_cast<E*>(a.out) + static_cast<int64_t>(span.row + col.query) * a.out_row +
-                             static_cast<int64_t>(col.head) * a.out_head;
-                    out[d] = static_cast<E>(y);
-                  }
+          for (int h = 0; h < CW; h += 16) {
+            float o[16];
+            tmem_ld16(tmem + lanes + m * NH + first_col + h, o);
+            tmem_wait_ld(o);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const int at = (first_col + h + c) * C::kValueDim + d;
+              const float y = o[c] * sh.reference[first_col + h + c];
+              if (ranks > 1) {
+                reinterpret_cast<float*>(smem)[at] = y;
+              } else {
+                reinterpret_cast<E*>(smem)[at] = static_cast<E>(y);
+              }
+            }
+          }
+        }
+      }
+      if (ranks == 1) {
+        named_barrier(1, C::kSoftmax);
+        if (!failed) {
+          for (int c = warp; c < NH; c += kLoadWarp) {
+            const Column col = column(c);
+            if (!col.used) continue;
+            E* out = static_cast<E*>(a.out) + static_cast<int64_t>(span.row + col.query) * a.out_row +
+                     static_cast<int64_t>(col.head) * a.out_head;
+            const E* from = reinterpret_cast<const E*>(smem) + c * C::kValueDim;
+            if (a.out_wide) {
+#pragma unroll
+              for (int d = 0; d < C::kValueDim; d += 256) {
+                if (d + lane * 8 < C::kValueDim) {
+                  *reinterpret_cast<uint4*>(out + d + lane * 8) = *reinterpret_cast<const uint4*>(from + d + lane * 8);
                 }
               }
+            } else {
+              for (int d = lane; d < C::kValueDim; d += 32) out[d] = from[d];
             }
           }
         }
@@ -571,52 +620,81 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
       tc_fence_before();
     } else if (warp < kMmaWarp) {
       // ================================================== gathering
-      // A warp gathers 32 of a tile's 128 rows; lane r knows row r's place,
-      // eight lanes copy a 128-byte row (four a 64-byte one).
-      const int w = warp - kLoadWarp;
-      const int32_t mine = tile_begin * kTile + w * 32 + lane;
-      int32_t fetched = steps > 0 ? fetch_key(a, keys, mine) : -1;
-      bool bad = false;
+      // A warp gathers its share of a tile's 128 rows; lane r knows the places
+      // of rows r, r + 32, ..., eight lanes copy a 128-byte row (four a
+      // 64-byte one).
+      constexpr int kShare = kTile / C::kLoaders;   // rows of a warp
+      constexpr int kOwn = kShare / 32;             // rows whose place a lane knows
       constexpr int kLanes = C::kWide / 16;         // lanes to a main row
       constexpr int kRows = 32 / kLanes;            // rows at once
-      constexpr int kTurns = 32 / kRows;
+      constexpr int kTurns = 32 / kRows;            // turns for 32 rows
+      const int w = warp - kLoadWarp;
+      const int32_t mine = tile_begin * kTile + w * kShare + lane;
+      const uint8_t* k_base = a.cache.k + kv * a.cache.k_head;
+      const uint8_t* v_base = a.cache.v + kv * a.cache.v_head;
+      int32_t fetched[kOwn];
+#pragma unroll
+      for (int o = 0; o < kOwn; ++o) fetched[o] = steps > 0 ? fetch_key(a, keys, mine + o * 32) : -1;
+      bool bad = false;
+      uint32_t b = 0, turn = 0;
       for (int32_t i = 0; i < steps; ++i) {
-        const int32_t j = mine + i * kTile;
-        const Key key = locate_key(a, keys, j, fetched);
-        bad |= bad_key(keys, j, fetched, key);
-        fetched = i + 1 < steps ? fetch_key(a, keys, j + kTile) : -1;
-        const uint32_t valid = __ballot_sync(kAllLanes, key.valid);
-        const int64_t k_off = key.block * a.cache.k_block + key.offset * a.cache.k_token;
-        const int64_t v_off = key.block * a.cache.v_block + key.offset * a.cache.v_token;
-        const uint8_t* k_base = a.cache.k + kv * a.cache.k_head;
-        const uint8_t* v_base = a.cache.v + kv * a.cache.v_head;
-        const uint32_t b = i % C::kStages, turn = (i / C::kStages) & 1;
+        Key key[kOwn];
+        uint32_t valid[kOwn];
+        int64_t k_off[kOwn], v_off[kOwn];
+#pragma unroll
+        for (int o = 0; o < kOwn; ++o) {
+          const int32_t j = mine + i * kTile + o * 32;
+          key[o] = locate_key(a, keys, j, fetched[o]);
+          bad |= bad_key(keys, j, fetched[o], key[o]);
+          fetched[o] = i + 1 < steps ? fetch_key(a, keys, j + kTile) : -1;
+          valid[o] = __ballot_sync(kAllLanes, key[o].valid);
+          k_off[o] = key[o].block * a.cache.k_block + key[o].offset * a.cache.k_token;
+          v_off[o] = key[o].block * a.cache.v_block + key[o].offset * a.cache.v_token;
+        }
+        // What the softmax has to know of a key: copied with its tile.
+        auto note = [&]() {
+#pragma unroll
+          for (int o = 0; o < kOwn; ++o) {
+            const int row = w * kShare + o * 32 + lane;
+            const int64_t scale_at = static_cast<int64_t>(key[o].block) * a.cache.kv_heads + kv;
+            cp_async4(smem_addr(&sh.k_scale[b][row]), a.cache.k_scale + scale_at, key[o].valid ? 4 : 0);
+            if constexpr (!C::kIsLatent) {
+              cp_async4(smem_addr(&sh.v_scale[b][row]), a.cache.v_scale + scale_at, key[o].valid ? 4 : 0);
+            }
+            if constexpr (C::kSeveral) sh.position[b][row] = key[o].position;
+            if (lane == 0) sh.valid[b][w * kOwn + o] = valid[o];
+          }
+        };
         const uint32_t stage = base + b * C::kStageBytes;
         if constexpr (C::kIsLatent) {
           const uint8_t* from[kTurns];
 #pragma unroll
           for (int n = 0; n < kTurns; ++n) {
-            from[n] = k_base + __shfl_sync(kAllLanes, k_off, n * kRows + lane / kLanes) + (lane % kLanes) * 16;
+            from[n] = k_base + __shfl_sync(kAllLanes, k_off[0], n * kRows + lane / kLanes) + (lane % kLanes) * 16;
           }
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             warp_wait(&sh.empty[c][b], turn ^ 1, abort);
 #pragma unroll
             for (int n = 0; n < kTurns; ++n) {
-              const int r = n * kRows + lane / kLanes, row = w * 32 + r;
+              const int r = n * kRows + lane / kLanes, row = w * kShare + r;
               const uint32_t dst = stage + c * C::kChunkBytes + row * 128 + (((lane % 8) ^ (row & 7)) << 4);
-              cp_async16(dst, from[n] + c * 128, (valid >> r) & 1 ? 16 : 0);
+              cp_async16(dst, from[n] + c * 128, (valid[0] >> r) & 1 ? 16 : 0);
+            }
+            if (c == C::kNoteChunk) {
+              note();
+              mbar_arrive(smem_addr(&sh.full[c][b]));
             }
             cp_async_arrive(smem_addr(&sh.full[c][b]));
           }
-          const uint32_t tb = i % C::kTails, tt = (i / C::kTails) & 1;
+          const uint32_t tb = C::kTails == 1 ? 0 : b, tt = C::kTails == 1 ? i & 1 : turn;
           warp_wait(&sh.empty[4][tb], tt ^ 1, abort);
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            const int r = n * 8 + lane / 4, row = w * 32 + r;
-            const uint8_t* src = k_base + __shfl_sync(kAllLanes, k_off, r) + 512 + (lane % 4) * 16;
+            const int r = n * 8 + lane / 4, row = w * kShare + r;
+            const uint8_t* src = k_base + __shfl_sync(kAllLanes, k_off[0], r) + 512 + (lane % 4) * 16;
             const uint32_t dst = base + C::kOffTail + tb * C::kTailBytes + row * 64 + (((lane ^ (row >> 1)) & 3) << 4);
-            cp_async16(dst, src, (valid >> r) & 1 ? 16 : 0);
+            cp_async16(dst, src, (valid[0] >> r) & 1 ? 16 : 0);
           }
           cp_async_arrive(smem_addr(&sh.full[4][tb]));
         } else {
@@ -627,15 +705,26 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
             // the keys behind them.
             const uint32_t at = stage + ((SHAPE == kDim64) == (c == 0) ? C::kChunkBytes : 0);
 #pragma unroll
-            for (int n = 0; n < kTurns; ++n) {
-              const int r = n * kRows + lane / kLanes, row = w * 32 + r;
-              const int64_t off = __shfl_sync(kAllLanes, c == 0 ? k_off : v_off, r) + (lane % kLanes) * 16;
-              const uint32_t dst = at + row * C::kWide + (C::kWide == 128 ? ((lane ^ row) & 7) << 4
-                                                                          : ((lane ^ (row >> 1)) & 3) << 4);
-              cp_async16(dst, (c == 0 ? k_base : v_base) + off, (valid >> r) & 1 ? 16 : 0);
+            for (int o = 0; o < kOwn; ++o) {
+#pragma unroll
+              for (int n = 0; n < kTurns; ++n) {
+                const int r = n * kRows + lane / kLanes, row = w * kShare + o * 32 + r;
+                const int64_t off = __shfl_sync(kAllLanes, c == 0 ? k_off[o] : v_off[o], r) + (lane % kLanes) * 16;
+                const uint32_t dst = at + row * C::kWide + (C::kWide == 128 ? ((lane ^ row) & 7) << 4
+                                                                            : ((lane ^ (row >> 1)) & 3) << 4);
+                cp_async16(dst, (c == 0 ? k_base : v_base) + off, (valid[o] >> r) & 1 ? 16 : 0);
+              }
+            }
+            if (c == C::kNoteChunk) {
+              note();
+              mbar_arrive(smem_addr(&sh.full[c][b]));
             }
             cp_async_arrive(smem_addr(&sh.full[c][b]));
           }
+        }
+        if (++b == C::kStages) {
+          b = 0;
+          turn ^= 1;
         }
       }
       cp_async_wait_all();
@@ -643,87 +732,100 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
       if (ranks > 1) cluster_sync();
     } else {
       // ================================================== MMAs
-      if (lane == 0 && steps > 0) {
+      // The whole warp walks the loop, so that addresses stay in uniform
+      // registers; one lane issues.
+      if (steps > 0) {
         constexpr uint32_t kScoreDesc = mma_descriptor(128, T * NH, kE4M3, false, false);
+        constexpr uint32_t kFirstDesc = mma_descriptor(128, NH, kE4M3, true, true);
+        constexpr uint32_t kOtherDesc = mma_descriptor(128, NH, kE5M2, true, true);
         constexpr Swizzle kPSwizzle = NH == 64 ? kSwizzle64 : NH == 32 ? kSwizzle32 : kSwizzleNone;
         constexpr Swizzle kMain = C::kWide == 128 ? kSwizzle128 : kSwizzle64;
-        const uint32_t q_at = base + C::kOffQ, p_at = base + C::kOffP;
-        bool ok = mbar_wait(smem_addr(&sh.queries), 0, abort);
-        int32_t issued = 0;
-        for (int32_t i = 0; ok && i <= steps; ++i) {
+        // Descriptors of the first chunks; further ones are offsets in units of 16 bytes.
+        const uint64_t k_desc = smem_descriptor(base + (SHAPE == kDim64 ? C::kChunkBytes : 0), 16, 8 * C::kWide, kMain);
+        const uint64_t q_desc = smem_descriptor(base + C::kOffQ, 16, 8 * C::kWide, kMain);
+        const uint64_t v_desc = smem_descriptor(base + (SHAPE == kDim128 ? C::kChunkBytes : 0),
+                                                SHAPE == kDim64 ? C::kChunkBytes : 1024, 8 * C::kWide, kMain);
+        const uint64_t p_desc = smem_descriptor(base + C::kOffP, 8 * NH, 8 * NH, kPSwizzle);
+        const bool leader = elect_one();
+        warp_wait(&sh.queries, 0, abort);
+        uint32_t sb = 0, st = 0, ob = 0, ot = 0;  // stage and its turn, of scores and of outputs
+        for (int32_t i = 0; i <= steps; ++i) {
           if (i < steps) {  // scores of tile i
-            const uint32_t b = i % C::kStages, turn = (i / C::kStages) & 1;
             const uint32_t d = tmem + C::kValues * NH + (i & 1) * (T * NH);
-#pragma unroll 1
-            for (int c = 0; ok && c < C::kMainKeys; ++c) {
-              ok = mbar_wait(smem_addr(&sh.full[c][b]), turn, abort);
-              if (!ok) break;
-              fence_proxy_async();
-              const uint32_t k_at = base + b * C::kStageBytes + c * C::kChunkBytes + (SHAPE == kDim64 ? C::kChunkBytes : 0);
-              const uint32_t qc = q_at + c * (T * NH * C::kWide);
 #pragma unroll
-              for (int k = 0; k < C::kWide / 32; ++k) {
-                mma_f8(d, smem_descriptor(k_at + k * 32, 16, 8 * C::kWide, kMain),
-                       smem_descriptor(qc + k * 32, 16, 8 * C::kWide, kMain), kScoreDesc, c + k > 0);
+            for (int c = 0; c < C::kMainKeys; ++c) {
+              warp_wait(&sh.full[c][sb], st, abort);
+              fence_proxy_async();
+              if (leader) {
+                const uint64_t kd = k_desc + ((sb * C::kStageBytes + c * C::kChunkBytes) >> 4);
+                const uint64_t qd = q_desc + ((c * (T * NH * C::kWide)) >> 4);
+#pragma unroll
+                for (int k = 0; k < C::kWide / 32; ++k) mma_f8(d, kd + 2 * k, qd + 2 * k, kScoreDesc, c + k > 0);
               }
+              __syncwarp();
             }
-            if (!ok) break;
             if constexpr (C::kIsLatent) {
-              const uint32_t tb = i % C::kTails;
-              ok = mbar_wait(smem_addr(&sh.full[4][tb]), (i / C::kTails) & 1, abort);
-              if (!ok) break;
+              const uint32_t tb = C::kTails == 1 ? 0 : sb, tt = C::kTails == 1 ? i & 1 : st;
+              warp_wait(&sh.full[4][tb], tt, abort);
               fence_proxy_async();
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                mma_f8(d, smem_descriptor(base + C::kOffTail + tb * C::kTailBytes + k * 32, 16, 512, kSwizzle64),
-                       smem_descriptor(q_at + 4 * (T * NH * 128) + k * 32, 16, 512, kSwizzle64), kScoreDesc, true);
+              if (leader) {
+                const uint64_t kd = smem_descriptor(base + C::kOffTail + tb * C::kTailBytes, 16, 512, kSwizzle64);
+                const uint64_t qd = smem_descriptor(base + C::kOffQ + 4 * (T * NH * 128), 16, 512, kSwizzle64);
+                mma_f8(d, kd, qd, kScoreDesc, true);
+                mma_f8(d, kd + 2, qd + 2, kScoreDesc, true);
+                mma_commit(smem_addr(&sh.empty[4][tb]));
               }
-              mma_commit(smem_addr(&sh.empty[4][tb]));
-            } else {
-              mma_commit(smem_addr(&sh.empty[0][b]));
+            } else if (leader) {
+              mma_commit(smem_addr(&sh.empty[0][sb]));
             }
-            mma_commit(smem_addr(&sh.scores[i & 1]));
+            if (leader) mma_commit(smem_addr(&sh.scores[i & 1]));
+            __syncwarp();
+            if (++sb == C::kStages) {
+              sb = 0;
+              st ^= 1;
+            }
           }
           if (i > 0) {  // outputs of tile i - 1
-            const int32_t o = i - 1;
-            const uint32_t b = o % C::kStages, turn = (o / C::kStages) & 1;
-            ok = mbar_wait(smem_addr(&sh.weights), o & 1, abort);
-            if (!ok) break;
+            warp_wait(&sh.weights, (i - 1) & 1, abort);
             tc_fence_after();
             if constexpr (!C::kIsLatent) {
-              ok = mbar_wait(smem_addr(&sh.full[1][b]), turn, abort);
-              if (!ok) break;
+              warp_wait(&sh.full[1][ob], ot, abort);
               fence_proxy_async();
             }
-#pragma unroll 1
-            for (int c = 0; c < C::kValues; ++c) {
-              const uint32_t v_at = base + b * C::kStageBytes + (SHAPE == kDim128 ? C::kChunkBytes : c * C::kChunkBytes);
+            if (leader) {
 #pragma unroll
-              for (int p = 0; p < T; ++p) {
+              for (int c = 0; c < C::kValues; ++c) {
+                const uint64_t vd = v_desc + ((ob * C::kStageBytes + c * C::kChunkBytes) >> 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  mma_f8(tmem + c * NH,
-                         smem_descriptor(v_at + k * 32 * C::kWide, SHAPE == kDim64 ? C::kChunkBytes : 1024, 8 * C::kWide, kMain),
-                         smem_descriptor(p_at + p * (NH * kTile) + k * 32 * NH, 8 * NH, 8 * NH, kPSwizzle),
-                         p == 0 ? mma_descriptor(128, NH, kE4M3, true, true) : mma_descriptor(128, NH, kE5M2, true, true),
-                         o + p + k > 0);
+                for (int p = 0; p < T; ++p) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    mma_f8(tmem + c * NH, vd + 2 * C::kWide * k, p_desc + ((p * (NH * kTile) + k * 32 * NH) >> 4),
+                           p == 0 ? kFirstDesc : kOtherDesc, p + k > 0 || i > 1);
+                  }
                 }
+                mma_commit(smem_addr(&sh.empty[C::kIsLatent ? c : 1][ob]));
               }
-              mma_commit(smem_addr(&sh.empty[C::kIsLatent ? c : 1][b]));
+              mma_commit(smem_addr(&sh.done));
             }
-            mma_commit(smem_addr(&sh.done));
-            issued = i;
+            __syncwarp();
+            if (++ob == C::kStages) {
+              ob = 0;
+              ot ^= 1;
+            }
           }
         }
-        if (issued < steps) {  // gave up: let what was issued finish before the memory goes
-          mma_commit(smem_addr(&sh.drained));
-          const long long begin = clock64();
-          while (!mbar_try(smem_addr(&sh.drained), 0) && clock64() - begin < 1000000000LL) {
+        if (__any_sync(kAllLanes, *abort != 0)) {  // gave up: let what was issued finish before the memory goes
+          if (leader) {
+            mma_commit(smem_addr(&sh.drained));
+            const long long begin = clock64();
+            while (!mbar_try(smem_addr(&sh.drained), 0) && clock64() - begin < 1000000000LL) {
+            }
+            flag_status(a.status, SILKERN_STATUS_WAIT_TIMEOUT);
           }
-          flag_status(a.status, SILKERN_STATUS_WAIT_TIMEOUT);
+          __syncwarp();
         }
       }
-      __syncwarp();
       if (ranks > 1) cluster_sync();
     }
 
@@ -777,7 +879,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
 template <CacheShape SHAPE, int NH, int T>
 int launch_config(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l) {
   using C = Config<SHAPE, NH, T>;
-  const int rc = allow_shared_memory(reinterpret_cast<const void*>(attend_kernel<SHAPE, NH, T>), C::kSmem);
+  const int rc = allow_launch(reinterpret_cast<const void*>(attend_kernel<SHAPE, NH, T>), C::kSmem);
   if (rc != SILKERN_OK) return rc;
   return launch_pdl(attend_kernel<SHAPE, NH, T>, l.grid, C::kThreads, C::kSmem, l.cluster, l.stream, a, plan);
 }

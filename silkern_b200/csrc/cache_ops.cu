@@ -267,6 +267,7 @@ int check_queries(const silkern_cache_v1* c, const void* q, int64_t q_row, int64
   a->out = out;
   a->out_row = out_row;
   a->out_head = out_head;
+  a->out_wide = out_row % 8 == 0 && out_head % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   a->lse = lse;
   a->scale_log2 = softmax_scale * 1.4426950408889634f;
   a->rows = static_cast<int32_t>(rows);

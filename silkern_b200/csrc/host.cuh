@@ -48,9 +48,10 @@ int launch_pdl(void (*fn)(P...), unsigned grid, unsigned threads, size_t smem, u
   return launch_pdl_grid(fn, dim3(grid, 1, 1), threads, smem, cluster, stream, args...);
 }
 
-// Let `kernel` use `bytes` of dynamic shared memory on the current device. The
-// driver is asked once for each kernel and device.
-inline int allow_shared_memory(const void* kernel, int bytes) {
+// Let `kernel` use `bytes` of dynamic shared memory, all of an SM's shared
+// memory, and clusters of up to 16 CTAs, on the current device. The driver is
+// asked once for each kernel and device.
+inline int allow_launch(const void* kernel, int bytes) {
   static std::mutex mutex;
   static std::vector<std::pair<const void*, int>> granted;
   int device = 0;
@@ -61,6 +62,10 @@ inline int allow_shared_memory(const void* kernel, int bytes) {
       if (g.first == kernel && g.second == device) return SILKERN_OK;
     }
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err == cudaSuccess) {
+      err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    }
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (err == cudaSuccess) granted.emplace_back(kernel, device);
   }
   if (err == cudaSuccess) return SILKERN_OK;

@@ -55,6 +55,7 @@ struct AttendArgs {
   int64_t q_row, q_head;
   void* out;  // (rows, heads, value_dim)
   int64_t out_row, out_head;
+  bool out_wide;  // rows of out start on 16-byte boundaries
   float* lse;  // (rows, heads), contiguous
   int32_t* status;
   float scale_log2;  // softmax_scale * log2(e)
