@@ -35,6 +35,7 @@ int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t strea
   const int32_t per = a.slots != nullptr || group >= columns ? 1 : columns / group;
   AttendPlan plan;
   plan.per = make_fastdiv(static_cast<uint32_t>(per));
+  plan.group = make_fastdiv(static_cast<uint32_t>(group));
   plan.blocks = (group + columns - 1) / columns;
   const int64_t items = a.slots != nullptr ? a.rows : a.rows / per + static_cast<int64_t>(a.sequences);
   int64_t busy = a.slots != nullptr ? a.rows : (a.rows + per - 1) / per;
@@ -48,14 +49,28 @@ int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t strea
     if (seen < keys) keys = seen;
   }
   const int64_t tiles = (keys + 127) / 128;
-  // Few work items: a cluster of up to 16 CTAs takes the tiles of each, as
-  // long as the CTAs still find an SM each and a tile each.
-  const int64_t ctas = busy * a.cache.kv_heads * plan.blocks;
-  const int64_t room = static_cast<int64_t>(multiprocessors()) * (!latent && columns == 16 ? 2 : 1);
+  const int64_t units = items * a.cache.kv_heads * plan.blocks;
+  if (units > 0x3fffffff) return SILKERN_E_SHAPE;
+  const int64_t live = busy * a.cache.kv_heads * plan.blocks;
+  const int64_t sms = multiprocessors(), pipes = !latent && columns == 16 ? 2 : 1;
+  // Few work items: as many CTAs as still find an SM and a tile for each of
+  // their pipelines, up to a cluster of 8, share each item's keys. (16 to a
+  // cluster find room seven times only, 8 fifteen times.)
   unsigned cluster = 1;
-  while (cluster < 16 && ctas * cluster * 2 <= room && tiles >= cluster * 2) cluster *= 2;
-  const int64_t grid = items * a.cache.kv_heads * plan.blocks * cluster;
-  if (grid > 0x7fffffff) return SILKERN_E_SHAPE;
+  while (cluster < 8 && live * cluster * 2 <= sms && tiles >= cluster * 2 * pipes) cluster *= 2;
+  plan.units = static_cast<uint32_t>(units);
+  int64_t grid;
+  if (cluster > 1 || (pipes > 1 && units <= sms && tiles >= pipes)) {
+    plan.whole = 0;
+    grid = units * cluster;
+  } else {
+    // Whole rounds of an item to each pipeline. What is left over after them
+    // goes to the pipelines of a CTA together, if it does not fill more than
+    // half a round.
+    grid = (units + pipes - 1) / pipes < sms ? (units + pipes - 1) / pipes : sms;
+    const int64_t round = grid * pipes, left = units % round;
+    plan.whole = static_cast<uint32_t>(pipes > 1 && left <= grid ? units - left : units);
+  }
   AttendLaunch l{columns, half, static_cast<unsigned>(grid), cluster, stream};
   return key_dim == 64 ? launch_dim64(a, plan, l) : key_dim == 128 ? launch_dim128(a, plan, l) : launch_latent(a, plan, l);
 }

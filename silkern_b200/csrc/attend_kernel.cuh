@@ -27,10 +27,16 @@
 // only when a tile's largest u leaves [R - 4, R + 3.5]: e4m3 ends at 448 =
 // 2^8.8. l, S and O are float32.
 //
-// Warps: 4 or 8 for the softmax (one key each thread), 4 that gather keys and
-// values with cp.async, one that issues the MMAs. Few work items are split
-// over the keys by a thread-block cluster, whose CTAs join their sums and
-// outputs through distributed shared memory: no workspace, one launch.
+// A CTA is one or two pipelines, each a softmax of one key a thread and 16
+// columns a warpgroup, warps that gather keys and values with cp.async, warps
+// that split the queries, and one that issues the MMAs. Every kernel that
+// allocates TMEM has an SM to itself, so a CTA stays on its SM and its
+// pipelines walk through the work items; each role runs ahead as far as the
+// buffers let it, and one item's start and end hide behind its neighbours'.
+// Work items that are few, or left over after whole rounds, are split over
+// their keys: by the pipelines of a CTA and of a thread-block cluster, which
+// join their sums and outputs through (distributed) shared memory. No
+// workspace, one launch.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -50,80 +56,89 @@ namespace silkern {
 enum CacheShape { kDim64, kDim128, kLatent };
 
 constexpr int kTile = 128;
-// A CTA's share of the 228 KB of an SM is at least its share of the 512 TMEM
-// columns, 456 bytes a column with the 1 KB that the SM adds to each CTA. So
-// CTAs of these kernels that fit an SM's shared memory also fit its TMEM, and
-// none waits for TMEM that a member of another waiting cluster holds.
-constexpr int smem_for_columns(int columns) { return columns * 456 - 1024; }
+// All of an SM's shared memory that a CTA can have.
+constexpr int kSharedMemory = 227 * 1024;
 
 template <CacheShape SHAPE, int NH, int T>
 struct Config {
   static constexpr bool kIsLatent = SHAPE == kLatent;
   static constexpr int kKeyDim = SHAPE == kDim64 ? 64 : SHAPE == kDim128 ? 128 : 576;
   static constexpr int kValueDim = SHAPE == kDim64 ? 64 : SHAPE == kDim128 ? 128 : 512;
-  static constexpr int kWide = SHAPE == kDim64 ? 64 : 128;      // row bytes of the main chunks
-  static constexpr int kMainKeys = kIsLatent ? 4 : 1;           // K chunks of kWide bytes
-  static constexpr int kValues = kIsLatent ? 4 : 1;             // V chunks: M = 128 tiles of O^T
-  static constexpr int kLoadChunks = kIsLatent ? 5 : 2;  // barriers: four wide chunks and the tail; else keys, values
+  static constexpr int kWide = SHAPE == kDim64 ? 64 : 128;       // row bytes of the main chunks
+  static constexpr int kMainKeys = kIsLatent ? 4 : 1;            // K chunks of kWide bytes
+  static constexpr int kValues = kIsLatent ? 4 : 1;              // V chunks: M = 128 tiles of O^T
+  static constexpr int kLoadChunks = kIsLatent ? 5 : 2;          // four wide ones and the tail; else keys, values
   static constexpr int kChunkBytes = kWide * kTile;
   static constexpr int kStageBytes = (kIsLatent ? 4 : 2) * kChunkBytes;
   static constexpr int kTailBytes = kIsLatent ? 64 * kTile : 0;  // a latent key's last 64 bytes
-  static constexpr int kGroups = NH >= 32 ? 2 : 1;               // softmax warpgroups, by columns
-  static constexpr int kCols = NH / kGroups;                     // columns of a softmax thread
+  // Pipelines: a narrow column block's softmax is a chain of short steps, and
+  // two of them keep the memory busy.
+  static constexpr int kPipes = !kIsLatent && NH == 16 ? 2 : 1;
+  static constexpr int kGroups = NH / 16;                        // softmax warpgroups, 16 columns each
   static constexpr int kSoftmax = kGroups * 128;
-  // Two CTAs to an SM where a column block is narrow: each hides the other's
-  // start, end and softmax. With 4 + 2 + 1 warps (registers are given out for
-  // eight) both have 128 registers a thread. Otherwise one CTA, with all of
-  // shared memory.
-  static constexpr int kPerSm = !kIsLatent && NH == 16 ? 2 : 1;
-  static constexpr int kLoaders = kPerSm == 2 ? 2 : 4;           // gathering warps
-  static constexpr int kThreads = kSoftmax + kLoaders * 32 + 32;
+  static constexpr int kLoaders = kPipes == 2 ? 2 : 4;           // gathering warps
+  static constexpr int kSplitters = kPipes == 2 ? 1 : 3;         // query warps
+  static constexpr int kPipeWarps = kGroups * 4 + kLoaders + kSplitters + 1;
+  static_assert(kPipeWarps % 4 == 0, "a softmax warp's TMEM lanes go by its number in the CTA");
+  static constexpr int kThreads = kPipes * kPipeWarps * 32;
   static constexpr int kQBytes = T * NH * kKeyDim;
   static constexpr int kPBytes = T * NH * kTile;
   // Columns of several queries see different keys. 64 columns of a latent
   // cache are one query's, so that its shared memory need not hold positions.
   static constexpr bool kSeveral = !(kIsLatent && NH == 64);
   static constexpr int kNoteBytes = kTile * ((kIsLatent ? 4 : 8) + (kSeveral ? 4 : 0)) + 16;  // a tile's scales, positions
-  static constexpr int kMisc = 20 * NH + (kSeveral ? 8 * NH : 0) + 256;
-  static constexpr int kColumnsUsed = kValues * NH + 2 * T * NH;
-  static constexpr int kColumns = kColumnsUsed <= 128 ? 128 : kColumnsUsed <= 256 ? 256 : 512;
+  static constexpr int kMisc = NH * (12 + 4 + 8 + (kSeveral ? 16 : 0)) + 320;
+  // TMEM columns of a pipeline: outputs, and scores twice.
+  static constexpr int kPipeColumns = kValues * NH + 2 * T * NH;
+  static constexpr int kColumnsUsed = kPipes * kPipeColumns;
   static_assert(kColumnsUsed <= 512, "TMEM");
-  static constexpr int kSmemMax = smem_for_columns(512 / kPerSm);
+  static constexpr int kColumns = kColumnsUsed <= 128 ? 128 : kColumnsUsed <= 256 ? 256 : 512;
+  static constexpr int kPipeBytes = kSharedMemory / kPipes / 1024 * 1024;
   static constexpr int kFixed = kQBytes + kPBytes + kMisc;
   static constexpr int kStageCost = kStageBytes + kNoteBytes + 16 * kLoadChunks;  // with its barriers
-  static constexpr int kFit = (kSmemMax - kFixed) / kStageCost;
+  static constexpr int kFit = (kPipeBytes - kFixed) / kStageCost;
   static constexpr int kStages = kIsLatent ? 2 : kFit < 8 ? kFit : 8;
-  static constexpr int kTails = kIsLatent ? ((kSmemMax - kFixed - 2 * kStageCost) >= 2 * kTailBytes ? 2 : 1) : 0;
-  static constexpr int kUsed = kFixed + kStages * kStageCost + kTails * kTailBytes;
-  static_assert(kStages >= 2 && kUsed <= kSmemMax, "shared memory");
-  static constexpr int kSmem = kUsed > smem_for_columns(kColumns) ? kUsed : smem_for_columns(kColumns);
+  static constexpr int kTails = kIsLatent ? ((kPipeBytes - kFixed - 2 * kStageCost) >= 2 * kTailBytes ? 2 : 1) : 0;
+  static_assert(kStages >= 2 && kFixed + kStages * kStageCost + kTails * kTailBytes <= kPipeBytes, "shared memory");
   static_assert(NH * kValueDim * 4 <= kStages * kStageBytes, "joining buffer");
   // The chunk whose buffer is free again only after a tile's softmax, and
   // with it the tile's scales and positions.
   static constexpr int kNoteChunk = kIsLatent ? 0 : 1;
-  // Offsets from the dynamic shared memory's start.
+  // Offsets from the start of a pipeline's shared memory.
   static constexpr int kOffTail = kStages * kStageBytes;
   static constexpr int kOffQ = kOffTail + kTails * kTailBytes;
   static constexpr int kOffP = kOffQ + kQBytes;
   static constexpr int kOffMisc = kOffP + kPBytes;
 };
 
-// The small shared state behind the tiles.
+// A work item as its query warps hand it to the softmax and the MMAs.
+struct Handed {
+  int32_t row, count, position;  // its queries
+  int32_t kv, block;
+  int32_t steps;                 // tiles; -1: no more items
+  int32_t split;                 // whether its keys are split over ranks
+};
+
+// The small shared state of a pipeline, behind its tiles.
 template <typename C, int NH>
 struct __align__(16) Shared {
   int32_t best[3][NH];  // column maxima of a tile, as ordered integers
-  float reference[NH];  // the columns' references R, at the end their output factors
-  float factor[NH];     // the columns' score factors
-  int32_t seen_to[C::kSeveral ? NH : 1], seen_from[C::kSeveral ? NH : 1];  // positions that a column sees: below, from
+  float reference[NH];  // the columns' references R
+  float factor[2][NH];  // the columns' score factors, of this item and the next
+  int32_t seen_to[2][C::kSeveral ? NH : 1], seen_from[2][C::kSeveral ? NH : 1];  // positions a column sees: below, from
   float k_scale[C::kStages][kTile];
   float v_scale[C::kIsLatent ? 1 : C::kStages][C::kIsLatent ? 1 : kTile];
   int32_t position[C::kSeveral ? C::kStages : 1][C::kSeveral ? kTile : 1];
   uint32_t valid[C::kStages][4];  // a bit for each key
+  Handed handed[2];
   uint64_t full[C::kLoadChunks][C::kStages], empty[C::kLoadChunks][C::kStages];
-  uint64_t scores[2], weights, done, queries, drained;
+  uint64_t scores[2], weights, done;
+  uint64_t queries[2], queries_read, finished[2];
+  uint64_t drained;
   uint32_t tmem;
   int32_t abort;
 };
+
 __device__ __forceinline__ int32_t ordered(float x) {
   const int32_t b = __float_as_int(x);
   return b >= 0 ? b : b ^ 0x7fffffff;
@@ -131,9 +146,9 @@ __device__ __forceinline__ int32_t ordered(float x) {
 __device__ __forceinline__ float unordered(int32_t b) { return __int_as_float(b >= 0 ? b : b ^ 0x7fffffff); }
 
 // A whole warp waits. A wait that ran out leaves *abort set, and every later
-// wait returns at once: the loops then run to their end on whatever is there,
-// so that each barrier gets the arrivals it counts, and the results are not
-// stored.
+// wait returns at once: an item's loops then run to their end on whatever is
+// there, so that each barrier gets the arrivals it counts, the results are not
+// stored, and no further item begins.
 __device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   mbar_wait(smem_addr(bar), parity, abort);
   __syncwarp();
@@ -195,6 +210,30 @@ __device__ __forceinline__ void unpack4(const uint2 raw, float (&x)[4]) {
   }
 }
 
+// The bf16 parts of a query by way of fp16 pairs: a scaled bf16 number's 8 bits
+// and what the first part leaves of them are exact there.
+__device__ __forceinline__ void split_query4(const float (&x)[4], uint32_t (&part)[2]) {
+  const uint32_t a = pack_f16x2(x[0], x[1]), b = pack_f16x2(x[2], x[3]);
+  const uint16_t a1 = f16x2_to_e4m3x2(a), b1 = f16x2_to_e4m3x2(b);
+  part[0] = a1 | (static_cast<uint32_t>(b1) << 16);
+  const uint16_t a2 = f16x2_to_e4m3x2(mul16_f16x2(sub_f16x2(a, e4m3x2_to_f16x2(a1))));
+  const uint16_t b2 = f16x2_to_e4m3x2(mul16_f16x2(sub_f16x2(b, e4m3x2_to_f16x2(b1))));
+  part[1] = a2 | (static_cast<uint32_t>(b2) << 16);
+}
+
+// The largest magnitude of four numbers, as the bits of a float's magnitude
+// (which order like unsigned integers, NaN last).
+template <typename E>
+__device__ __forceinline__ uint32_t magnitude4(const uint2 raw) {
+  const uint32_t a = raw.x & 0x7fff7fffu, b = raw.y & 0x7fff7fffu;
+  const uint32_t m = __vmaxu2(a, b);
+  const uint32_t most = max(m & 0xffffu, m >> 16);  // the type's own bits order the same way
+  if constexpr (std::is_same<E, __nv_bfloat16>::value) return most << 16;
+  if (most >= 0x7c00u) return 0x7f800000u;
+  const __half h = *reinterpret_cast<const __half*>(&most);
+  return __float_as_uint(__half2float(h));
+}
+
 // Sums each of a thread's N columns over the warp: lane c gets column c mod N.
 // Each step adds up half of the columns with the lane across and gives the
 // other half away.
@@ -215,25 +254,72 @@ __device__ __forceinline__ float sum_columns(float (&x)[N], int lane) {
   return y;
 }
 
-// A column of the CTA: which query (of the span) and head it is.
+// One work item's share of a rank.
+struct Work {
+  QuerySpan span;
+  KeyList keys;
+  int32_t kv, block;
+  int32_t tiles, begin, steps;  // of the item; this rank's first and number
+};
+
+__device__ __forceinline__ Work find_work(const AttendArgs& a, const AttendPlan& plan, uint32_t unit, uint32_t rank,
+                                          uint32_t ranks) {
+  Work w;
+  w.block = unit % plan.blocks;
+  unit /= plan.blocks;
+  w.kv = unit % a.cache.kv_heads;
+  const int32_t item = unit / a.cache.kv_heads;
+  w.span = QuerySpan{item, 1, 0, 0};
+  w.keys = KeyList{};
+  if (a.slots != nullptr) {
+    w.keys = selected_keys(a, item);
+  } else {
+    w.span = find_span(a, item, plan.per);
+    if (w.span.count > 0) w.keys = window_keys(a, w.span);
+  }
+  w.tiles = (w.keys.n + kTile - 1) / kTile;
+  w.begin = static_cast<int32_t>(static_cast<int64_t>(w.tiles) * rank / ranks);
+  w.steps = static_cast<int32_t>(static_cast<int64_t>(w.tiles) * (rank + 1) / ranks) - w.begin;
+  return w;
+}
+
+// A column of an item: which of its queries, and which head.
 struct Column {
   int32_t query, head;
   bool used;
 };
 
+template <int NH>
+__device__ __forceinline__ Column find_column(const AttendArgs& a, const AttendPlan& plan, int32_t count, int32_t kv,
+                                              int32_t block, int32_t c) {
+  Column r;
+  r.query = plan.per.divisor == 1 ? 0 : static_cast<int32_t>(fastdiv(c, plan.group));
+  const int32_t g = c - r.query * a.heads_per_kv + block * NH;
+  r.head = kv * a.heads_per_kv + g;
+  r.used = r.query < count && g < a.heads_per_kv && (plan.per.divisor == 1 || block == 0);
+  return r;
+}
+
 template <CacheShape SHAPE, int NH, int T>
-__global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, NH, T>::kPerSm)
+__global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ AttendPlan plan) {
   using C = Config<SHAPE, NH, T>;
   using E = typename std::conditional<T == 2, __nv_bfloat16, __half>::type;
-  extern __shared__ __align__(1024) uint8_t smem[];
   using S = Shared<C, NH>;
-  static_assert(C::kOffMisc + sizeof(S) <= C::kSmem, "shared state");
-  S& sh = *reinterpret_cast<S*>(smem + C::kOffMisc);
+  static_assert(C::kOffMisc + sizeof(S) <= C::kPipeBytes, "shared state");
+  extern __shared__ __align__(1024) uint8_t all_smem[];
+  const int lane = threadIdx.x & 31;
+  const int pipe = C::kPipes == 1 ? 0 : __shfl_sync(kAllLanes, threadIdx.x / (C::kPipeWarps * 32), 0);
+  const int tid = threadIdx.x - pipe * (C::kPipeWarps * 32);
+  const int warp = __shfl_sync(kAllLanes, tid >> 5, 0);  // within the pipeline
+  uint8_t* const smem = all_smem + pipe * C::kPipeBytes;
   const uint32_t base = smem_addr(smem);
-  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(kAllLanes, tid >> 5, 0);
-  constexpr int kMmaWarp = C::kThreads / 32 - 1;
+  S& sh = *reinterpret_cast<S*>(smem + C::kOffMisc);
   constexpr int kLoadWarp = C::kSoftmax / 32;
+  constexpr int kSplitWarp = kLoadWarp + C::kLoaders;
+  constexpr int kMmaWarp = C::kPipeWarps - 1;
+  // Named barriers: one for each softmax group, one for them all.
+  constexpr int kFirstGroup = 1 + C::kPipes;
 
   // ---- set up, before the previous grid's results are needed
   if (tid == 0) {
@@ -243,13 +329,18 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
         mbar_init(smem_addr(&sh.empty[c][b]), 1);
       }
     }
-    mbar_init(smem_addr(&sh.scores[0]), 1);
-    mbar_init(smem_addr(&sh.scores[1]), 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_addr(&sh.scores[b]), 1);
+      mbar_init(smem_addr(&sh.queries[b]), C::kSplitters * 32);
+      mbar_init(smem_addr(&sh.finished[b]), C::kSoftmax);
+    }
     mbar_init(smem_addr(&sh.weights), C::kSoftmax);
     mbar_init(smem_addr(&sh.done), 1);
-    mbar_init(smem_addr(&sh.queries), C::kSoftmax);
+    mbar_init(smem_addr(&sh.queries_read), 1);
     mbar_init(smem_addr(&sh.drained), 1);
     sh.abort = 0;
+    sh.handed[0].split = 0;
+    sh.handed[1].split = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
@@ -257,178 +348,91 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
     sh.best[0][tid] = ordered(-INFINITY);
     sh.reference[tid] = 0.f;
   }
-  if (warp == kMmaWarp) tmem_alloc(smem_addr(&sh.tmem), C::kColumns);
+  S& first = *reinterpret_cast<S*>(all_smem + C::kOffMisc);
+  if (pipe == 0 && warp == kMmaWarp) tmem_alloc(smem_addr(&first.tmem), C::kColumns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = __shfl_sync(kAllLanes, sh.tmem, 0);
+  const uint32_t tmem_all = __shfl_sync(kAllLanes, first.tmem, 0);
+  const uint32_t tmem = tmem_all + pipe * C::kPipeColumns;
   volatile int* abort = &sh.abort;
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- which work this CTA has
-  const uint32_t ranks = cluster_size(), rank = cluster_ctarank();
-  uint32_t unit = blockIdx.x / ranks;
-  const int32_t block = unit % plan.blocks;
-  unit /= plan.blocks;
-  const int32_t kv = unit % a.cache.kv_heads;
-  const int32_t item = unit / a.cache.kv_heads;
-  QuerySpan span{item, 1, 0, 0};
-  KeyList keys{};
-  if (a.slots != nullptr) {
-    keys = selected_keys(a, item);
-  } else {
-    span = find_span(a, item, plan.per);
-    if (span.count > 0) keys = window_keys(a, span);
-  }
-  const int32_t tiles = (keys.n + kTile - 1) / kTile;
-  const int32_t tile_begin = static_cast<int32_t>(static_cast<int64_t>(tiles) * rank / ranks);
-  const int32_t tile_end = static_cast<int32_t>(static_cast<int64_t>(tiles) * (rank + 1) / ranks);
-  const int32_t steps = tile_end - tile_begin;
-  const bool several = span.count > 1;  // columns see different keys
-  const int32_t group = a.heads_per_kv;
-  auto column = [&](int32_t c) {
-    Column r;
-    r.query = plan.per.divisor == 1 ? 0 : c / group;
-    const int32_t g = c - r.query * group + block * NH;
-    r.head = kv * group + g;
-    r.used = r.query < span.count && g < group && (plan.per.divisor == 1 || block == 0);
-    return r;
-  };
+  // ---- this pipeline's items: whole ones, then perhaps a rank's share of one
+  const uint32_t ctas = cluster_size();
+  const uint32_t rank = cluster_ctarank() * C::kPipes + pipe, ranks = ctas * C::kPipes;
+  const uint32_t whole_step = gridDim.x * C::kPipes;
+  const uint32_t split_unit = plan.whole + blockIdx.x / ctas;
+  const bool has_split = split_unit < plan.units;
+  // Softmax state that outlives the loop for a split item.
+  float l[16];
+  float reference = -INFINITY;
 
-  if (tiles > 0) {
-    if (warp < kLoadWarp) {
-      // ================================================== queries, softmax
-      const int wg = warp >> 2;
-      const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane quadrant, << 16
-      // -- split the queries: a warp takes four columns at a time, so that
-      // their loads overlap
-      constexpr int kPieces = (C::kKeyDim / 4 + 31) / 32;
-      constexpr int kBatch = 4;
-      for (int c0 = warp * kBatch; c0 < NH; c0 += kLoadWarp * kBatch) {
-        uint2 raw[kBatch][kPieces];
-#pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-          const Column col = column(c0 + n);
-          const E* q = static_cast<const E*>(a.q) + static_cast<int64_t>(span.row + col.query) * a.q_row +
-                       static_cast<int64_t>(col.head) * a.q_head;
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            const int d = (i * 32 + lane) * 4;
-            raw[n][i] = make_uint2(0u, 0u);
-            if (col.used && d < C::kKeyDim) raw[n][i] = *reinterpret_cast<const uint2*>(q + d);
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-          const int c = c0 + n;
-          uint32_t most = 0;
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            float x[4];
-            unpack4<E>(raw[n][i], x);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(x[k]) & 0x7fffffffu);
-          }
-          most = __reduce_max_sync(kAllLanes, most);
-          // The largest magnitude comes to [128, 256): its exponent field is taken off.
-          const int e = max(static_cast<int>(most >> 23), 40);
-          const bool odd = most >= 0x7f800000u;  // an infinity or NaN: the row becomes NaN
-          const float up = odd ? 0.f : __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
-          if (lane == 0) {
-            sh.factor[c] = odd ? NAN : a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
-            if constexpr (C::kSeveral) {
-              const Column col = column(c);
-              const int32_t position = span.position + col.query;
-              sh.seen_to[c] = col.used ? position + 1 : 0x7fffffff;
-              sh.seen_from[c] = col.used && a.window != 0 && position + 1 > static_cast<int64_t>(a.window)
-                                    ? position + 1 - static_cast<int32_t>(a.window) : 0;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            const int d = (i * 32 + lane) * 4;
-            if (d < C::kKeyDim) {
-              float y[4];
-              unpack4<E>(raw[n][i], y);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) y[k] = odd ? 0.f : y[k] * up;
-              uint32_t part[T];
-              split4<T, false>(y, part);
-              const int chunk = d / 128, in = d & 127;
-              const bool narrow = C::kWide == 64 || (C::kIsLatent && chunk == 4);
-#pragma unroll
-              for (int t = 0; t < T; ++t) {
-                const int row = t * NH + c;
-                const uint32_t at = narrow ? row * 64 + ((((in >> 4) ^ (row >> 1)) & 3) << 4) + (in & 15)
-                                           : row * 128 + ((((in >> 4) ^ row) & 7) << 4) + (in & 15);
-                st_shared(base + C::kOffQ + chunk * (T * NH * 128) + at, part[t]);
-              }
-            }
-          }
-        }
-      }
-      fence_proxy_async();
-      mbar_arrive(smem_addr(&sh.queries));
-      named_barrier(1, C::kSoftmax);
-
-      // -- tiles
-      constexpr int CW = C::kCols;
-      const int first_col = wg * CW;
-      float l[CW];
-#pragma unroll
-      for (int c = 0; c < CW; ++c) l[c] = 0.f;
-      float reference = -INFINITY, highest = -INFINITY;  // of column first_col + lane
-      const int32_t all_to = span.position + 1;  // positions below are seen by every query, from
+  if (warp < kLoadWarp) {
+    // ==================================================== softmax
+    const int wg = warp >> 2, thread = tid & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lane quadrant, << 16
+    const int first_col = wg * 16;
+    const int own = lane & 15;  // the column whose reference a lane keeps
+    const int group_barrier = kFirstGroup + pipe * C::kGroups + wg;
+    uint32_t n = 0, n3 = 0, b = 0, turn = 0;  // tiles so far; modulo 3; stage and its turn
+    for (uint32_t seq = 0;; ++seq) {
+      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort);
+      // Everybody stops or nobody: the groups' barriers count on it.
+      if (named_barrier_or(1 + pipe, C::kSoftmax, *abort != 0)) break;
+      const Handed h = sh.handed[seq & 1];
+      if (h.steps < 0) break;
+      const bool several = h.count > 1;  // columns see different keys
+      const int32_t all_to = h.position + 1;  // positions below are seen by every query, from
       const int32_t all_from =
-          a.window == 0 ? 0
-                        : static_cast<int32_t>(max(int64_t{0}, static_cast<int64_t>(span.position) + span.count - a.window));
-      for (int32_t i = 0; i < steps; ++i) {
-        warp_wait(&sh.scores[i & 1], (i >> 1) & 1, abort);
+          a.window == 0 ? 0 : static_cast<int32_t>(max(int64_t{0}, static_cast<int64_t>(h.position) + h.count - a.window));
+#pragma unroll
+      for (int c = 0; c < 16; ++c) l[c] = 0.f;
+      reference = -INFINITY;
+      float highest = -INFINITY;
+      for (int32_t i = 0; i < h.steps; ++i) {
+        warp_wait(&sh.scores[n & 1], (n >> 1) & 1, abort);
         tc_fence_after();
-        const uint32_t b = i % C::kStages;
-        warp_wait(&sh.full[C::kNoteChunk][b], (i / C::kStages) & 1, abort);
+        const uint32_t s_at = tmem + lanes + C::kValues * NH + (n & 1) * (T * NH) + first_col;
+        float t[16], s1[16];
+        tmem_ld16(s_at, t);
+        tmem_ld16(s_at + NH, s1);
+        warp_wait(&sh.full[C::kNoteChunk][b], turn, abort);
         const bool valid = (sh.valid[b][warp & 3] >> lane) & 1;
-        const float ks = sh.k_scale[b][tid & 127];
-        const float vs = C::kIsLatent ? ks : sh.v_scale[C::kIsLatent ? 0 : b][C::kIsLatent ? 0 : tid & 127];
-        const uint32_t s_at = tmem + lanes + C::kValues * NH + (i & 1) * (T * NH) + first_col;
-        float t[CW];
+        const float ks = sh.k_scale[b][thread];
+        const float vs = C::kIsLatent ? ks : sh.v_scale[C::kIsLatent ? 0 : b][C::kIsLatent ? 0 : thread];
+        if constexpr (T == 3) {
+          float s2[16];
+          tmem_ld16(s_at + 2 * NH, s2);
+          tmem_wait_ld(t);
+          tmem_wait_ld(s1);
+          tmem_wait_ld(s2);
 #pragma unroll
-        for (int h = 0; h < CW; h += 16) {
-          float s0[16], s1[16];
-          tmem_ld16(s_at + h, s0);
-          tmem_ld16(s_at + NH + h, s1);
-          if constexpr (T == 3) {
-            float s2[16];
-            tmem_ld16(s_at + 2 * NH + h, s2);
-            tmem_wait_ld(s0);
-            tmem_wait_ld(s1);
-            tmem_wait_ld(s2);
+          for (int c = 0; c < 16; ++c) s1[c] += s2[c] * 0.0625f;
+        } else {
+          tmem_wait_ld(t);
+          tmem_wait_ld(s1);
+        }
 #pragma unroll
-            for (int c = 0; c < 16; ++c) s1[c] += s2[c] * 0.0625f;
-          } else {
-            tmem_wait_ld(s0);
-            tmem_wait_ld(s1);
-          }
+        for (int c = 0; c < 16; c += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&sh.factor[seq & 1][first_col + c]);
+          const float fs[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-          for (int c = 0; c < 16; c += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(&sh.factor[first_col + h + c]);
-            const float fs[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float s = (s0[c + k] + s1[c + k] * 0.0625f) * (ks * fs[k]);
-              t[h + c + k] = valid ? s : -INFINITY;
-            }
+          for (int k = 0; k < 4; ++k) {
+            const float s = (t[c + k] + s1[c + k] * 0.0625f) * (ks * fs[k]);
+            t[c + k] = valid ? s : -INFINITY;
           }
         }
         if constexpr (C::kSeveral) {
           if (several) {
-            const int32_t at = sh.position[b][tid & 127];
+            const int32_t at = sh.position[b][thread];
             const bool sink = static_cast<uint32_t>(at) < a.sinks;
             if (!(at < all_to && (at >= all_from || sink))) {
 #pragma unroll
-              for (int c = 0; c < CW; ++c) {
-                const bool seen = at < sh.seen_to[first_col + c] && (at >= sh.seen_from[first_col + c] || sink);
+              for (int c = 0; c < 16; ++c) {
+                const bool seen = at < sh.seen_to[seq & 1][first_col + c] &&
+                                  (at >= sh.seen_from[seq & 1][first_col + c] || sink);
                 if (!seen) t[c] = -INFINITY;
               }
             }
@@ -439,19 +443,20 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
         const float shift = __log2f(scale > 0.f ? scale : 0x1p-100f);
         float top = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < CW; ++c) {
+        for (int c = 0; c < 16; ++c) {
           const float m = warp_max(t[c] + shift);
-          if ((lane & (CW - 1)) == c) top = m;
+          if (own == c) top = m;
         }
-        int32_t* best = sh.best[i % 3];
-        if (lane < CW) {
+        int32_t* best = sh.best[n3];
+        n3 = n3 == 2 ? 0 : n3 + 1;
+        if (lane < 16) {
           atomicMax(&best[first_col + lane], ordered(top));
-          if ((warp & 3) == 0) sh.best[(i + 1) % 3][first_col + lane] = ordered(-INFINITY);
+          if ((warp & 3) == 0) sh.best[n3][first_col + lane] = ordered(-INFINITY);
         }
-        named_barrier(2 + wg, 128);
-        top = unordered(best[first_col + (lane & (CW - 1))]);
+        named_barrier(group_barrier, 128);
+        top = unordered(best[first_col + own]);
         const bool move = top > reference + 3.5f || (top < reference - 4.f && top > highest - 60.f);
-        bool waited = false;
+        bool waited = i == 0;  // an item's end waits for its last outputs
         if (__any_sync(kAllLanes, move)) {
           const float to = move ? fmaxf(top, highest - 60.f) : reference;
           const float by = !move ? 1.f : reference == -INFINITY ? 0.f : exp2_approx(reference - to);
@@ -459,41 +464,36 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
           highest = fmaxf(highest, to);
           // The group's warps all write the same numbers: whoever reads them has
           // written them, and nobody is still at the tile before.
-          if (lane < CW) sh.reference[first_col + lane] = to == -INFINITY ? 0.f : to;
+          if (lane < 16) sh.reference[first_col + lane] = to == -INFINITY ? 0.f : to;
           __syncwarp();
-          if (i > 0) {
-            warp_wait(&sh.done, (i - 1) & 1, abort);
-            waited = true;
-            tc_fence_after();
+          if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
+          waited = true;
+          tc_fence_after();
+          float f[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            f[c] = __shfl_sync(kAllLanes, by, c);
+            l[c] *= f[c];
           }
-#pragma unroll
-          for (int h = 0; h < CW; h += 16) {
-            float f[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              f[c] = __shfl_sync(kAllLanes, by, h + c);
-              l[h + c] *= f[c];
-            }
-            if (i > 0) {
+          if (i > 0) {
 #pragma unroll 1
-              for (int m = 0; m < C::kValues; ++m) {
-                const uint32_t at = tmem + lanes + m * NH + first_col + h;
-                float o[16];
-                tmem_ld16(at, o);
-                tmem_wait_ld(o);
+            for (int m = 0; m < C::kValues; ++m) {
+              const uint32_t at = tmem + lanes + m * NH + first_col;
+              float o[16];
+              tmem_ld16(at, o);
+              tmem_wait_ld(o);
 #pragma unroll
-                for (int c = 0; c < 16; ++c) o[c] *= f[c];
-                tmem_st16(at, o);
-              }
-              tmem_wait_st();
+              for (int c = 0; c < 16; ++c) o[c] *= f[c];
+              tmem_st16(at, o);
             }
+            tmem_wait_st();
           }
         }
         // Weights. The sum takes them in float32, the tensor core in T parts.
         const float to_value = scale * 32.f;
-        uint32_t part[CW / 4][T];
+        uint32_t part[4][T];
 #pragma unroll
-        for (int c = 0; c < CW; c += 4) {
+        for (int c = 0; c < 16; c += 4) {
           const float4 r = *reinterpret_cast<const float4*>(&sh.reference[first_col + c]);
           const float rs[4] = {r.x, r.y, r.z, r.w};
           float w[4];
@@ -509,144 +509,137 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
             split4<T, true>(w, part[c / 4]);
           }
         }
-        if (i > 0 && !waited) warp_wait(&sh.done, (i - 1) & 1, abort);
-        const int row = tid & 127;
+        if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
+        const uint32_t at = NH == 64 ? thread * 64 + ((wg ^ ((thread >> 1) & 3)) << 4)
+                            : NH == 32 ? thread * 32 + ((wg ^ ((thread >> 2) & 1)) << 4) : thread * 16;
 #pragma unroll
         for (int p = 0; p < T; ++p) {
-#pragma unroll
-          for (int h = 0; h < CW; h += 16) {
-            const int piece = (first_col + h) / 16;
-            const uint32_t at = NH == 64 ? row * 64 + ((piece ^ ((row >> 1) & 3)) << 4)
-                                : NH == 32 ? row * 32 + ((piece ^ ((row >> 2) & 1)) << 4) : row * 16;
-            st_shared_v4(base + C::kOffP + p * (NH * kTile) + at, part[h / 4][p], part[h / 4 + 1][p],
-                         part[h / 4 + 2][p], part[h / 4 + 3][p]);
-          }
+          st_shared_v4(base + C::kOffP + p * (NH * kTile) + at, part[0][p], part[1][p], part[2][p], part[3][p]);
         }
         fence_proxy_async();
         tc_fence_before();
         mbar_arrive(smem_addr(&sh.weights));
+        ++n;
+        if (++b == C::kStages) {
+          b = 0;
+          turn ^= 1;
+        }
       }
-      if (steps > 0) warp_wait(&sh.done, (steps - 1) & 1, abort);
+      if (h.steps > 0) warp_wait(&sh.done, (n - 1) & 1, abort);
       tc_fence_after();
-
-      // -- sums over the keys: lanes first, then the group's warps. The
-      // weights' buffer is free by now and takes the warps' sums.
-      float* sums = reinterpret_cast<float*>(smem + C::kOffP) + wg * (4 * CW);
-      float mine_l = sum_columns<CW>(l, lane);
-      if (lane < CW) sums[(warp & 3) * CW + lane] = mine_l;
-      named_barrier(2 + wg, 128);
-      const int own = lane & (CW - 1);
-      mine_l = (sums[own] + sums[CW + own]) + (sums[2 * CW + own] + sums[3 * CW + own]);
-
-      float whole_l = mine_l, whole_r = reference, part_of = 1.f;
-      if (ranks > 1) {
-        // Every CTA's references and sums go round the cluster.
-        float* joint = reinterpret_cast<float*>(smem + C::kOffP) + 8 * NH;  // references, then sums
-        if ((warp & 3) == 0 && lane < CW) {
-          joint[first_col + lane] = reference;
-          joint[NH + first_col + lane] = mine_l;
-        }
-        cluster_sync();
-        const uint32_t at = smem_addr(joint + first_col + own);
-        whole_r = -INFINITY;
-        for (uint32_t r = 0; r < ranks; ++r) whole_r = fmaxf(whole_r, ld_cluster(at, r));
-        whole_l = 0.f;
-        for (uint32_t r = 0; r < ranks; ++r) {
-          const float rr = ld_cluster(at, r);
-          whole_l += rr == -INFINITY ? 0.f : ld_cluster(at + NH * 4, r) * exp2_approx(rr - whole_r);
-        }
-        part_of = reference == -INFINITY ? 0.f : exp2_approx(reference - whole_r);
-      }
-      const float inverse = whole_l == 0.f ? 0.f : 1.f / (32.f * whole_l);
-      if (rank == 0 && (warp & 3) == 0 && lane < CW && *abort == 0) {
-        const Column col = column(first_col + lane);
-        if (col.used) {
-          a.lse[static_cast<int64_t>(span.row + col.query) * a.heads + col.head] =
-              whole_l == 0.f ? -INFINITY : (whole_r + log2f(whole_l)) * 0.69314718055994531f;
-        }
-      }
-      __syncwarp();
-      if (lane < CW) sh.reference[first_col + lane] = part_of * inverse;
-      __syncwarp();
-
-      // -- outputs by way of the tiles' shared memory: in float32 to be joined
-      // by the cluster, else as they are stored, in rows of a column
-      constexpr int kRowsOf = SHAPE == kDim64 ? 64 : 128;  // of M = 128
+      // Sums over the keys: lanes first, then the group's warps. The weights'
+      // buffer is free by now and takes the warps' sums, then the outputs.
+      float* sums = reinterpret_cast<float*>(smem + C::kOffP + wg * 4096);
+      const float part_l = sum_columns(l, lane);
+      if (lane < 16) sums[(warp & 3) * 16 + lane] = part_l;
+      named_barrier(group_barrier, 128);
+      l[0] = (sums[own] + sums[16 + own]) + (sums[32 + own] + sums[48 + own]);  // column own's
+      if (h.split) break;
+      const float inverse = l[0] == 0.f ? 0.f : 1.f / (32.f * l[0]);
       const bool failed = __any_sync(kAllLanes, *abort != 0);
-      if (steps > 0 && !failed && (warp & 3) * 32 < kRowsOf) {
+      if ((warp & 3) == 0 && lane < 16 && !failed) {
+        const Column col = find_column<NH>(a, plan, h.count, h.kv, h.block, first_col + lane);
+        if (col.used) {
+          a.lse[static_cast<int64_t>(h.row + col.query) * a.heads + col.head] =
+              l[0] == 0.f ? -INFINITY : (reference + log2f(l[0])) * 0.69314718055994531f;
+        }
+      }
+      named_barrier(group_barrier, 128);  // the sums are read
+      // Outputs: a tile of 128 (D 64: 64) by 16 columns at a time through shared
+      // memory, then in rows of a column.
+      constexpr int kRowsOf = SHAPE == kDim64 ? 64 : 128;  // of M = 128
+      constexpr int kPieces = kRowsOf / 8;                 // of 16 bytes in a row
+      constexpr int kTurns = kPieces * 16 / 128;
+      E* staged = reinterpret_cast<E*>(smem + C::kOffP + wg * 4096);
+      E* out[kTurns];
+#pragma unroll
+      for (int k = 0; k < kTurns; ++k) {
+        const int p = thread + k * 128;
+        const Column col = find_column<NH>(a, plan, h.count, h.kv, h.block, first_col + p / kPieces);
+        out[k] = !col.used || failed ? nullptr
+                                     : static_cast<E*>(a.out) + static_cast<int64_t>(h.row + col.query) * a.out_row +
+                                           static_cast<int64_t>(col.head) * a.out_head + p % kPieces * 8;
+      }
 #pragma unroll 1
-        for (int m = 0; m < C::kValues; ++m) {
-          const int d = m * 128 + (warp & 3) * 32 + lane;
+      for (int m = 0; m < C::kValues; ++m) {
+        float o[16];
+        if ((warp & 3) * 32 < kRowsOf) {
+          tmem_ld16(tmem + lanes + m * NH + first_col, o);
+          tmem_wait_ld(o);
 #pragma unroll
-          for (int h = 0; h < CW; h += 16) {
-            float o[16];
-            tmem_ld16(tmem + lanes + m * NH + first_col + h, o);
-            tmem_wait_ld(o);
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const int at = (first_col + h + c) * C::kValueDim + d;
-              const float y = o[c] * sh.reference[first_col + h + c];
-              if (ranks > 1) {
-                reinterpret_cast<float*>(smem)[at] = y;
-              } else {
-                reinterpret_cast<E*>(smem)[at] = static_cast<E>(y);
-              }
-            }
+          for (int c = 0; c < 16; ++c) {
+            staged[c * 128 + thread] = static_cast<E>(o[c] * __shfl_sync(kAllLanes, inverse, c));
           }
         }
-      }
-      if (ranks == 1) {
-        named_barrier(1, C::kSoftmax);
-        if (!failed) {
-          for (int c = warp; c < NH; c += kLoadWarp) {
-            const Column col = column(c);
-            if (!col.used) continue;
-            E* out = static_cast<E*>(a.out) + static_cast<int64_t>(span.row + col.query) * a.out_row +
-                     static_cast<int64_t>(col.head) * a.out_head;
-            const E* from = reinterpret_cast<const E*>(smem) + c * C::kValueDim;
+        named_barrier(group_barrier, 128);
+#pragma unroll
+        for (int k = 0; k < kTurns; ++k) {
+          const int p = thread + k * 128;
+          const uint4 x = *reinterpret_cast<const uint4*>(staged + p / kPieces * 128 + p % kPieces * 8);
+          if (out[k] != nullptr) {
             if (a.out_wide) {
-#pragma unroll
-              for (int d = 0; d < C::kValueDim; d += 256) {
-                if (d + lane * 8 < C::kValueDim) {
-                  *reinterpret_cast<uint4*>(out + d + lane * 8) = *reinterpret_cast<const uint4*>(from + d + lane * 8);
-                }
-              }
+              *reinterpret_cast<uint4*>(out[k] + m * 128) = x;
             } else {
-              for (int d = lane; d < C::kValueDim; d += 32) out[d] = from[d];
+              const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint16_t half = static_cast<uint16_t>(words[e / 2] >> (16 * (e & 1)));
+                reinterpret_cast<uint16_t*>(out[k] + m * 128)[e] = half;
+              }
             }
           }
         }
+        if (m + 1 < C::kValues) named_barrier(group_barrier, 128);
       }
+      // The next item's weights may overwrite any group's part of the buffer,
+      // its outputs these.
+      named_barrier(1 + pipe, C::kSoftmax);
       tc_fence_before();
-    } else if (warp < kMmaWarp) {
-      // ================================================== gathering
-      // A warp gathers its share of a tile's 128 rows; lane r knows the places
-      // of rows r, r + 32, ..., eight lanes copy a 128-byte row (four a
-      // 64-byte one).
-      constexpr int kShare = kTile / C::kLoaders;   // rows of a warp
-      constexpr int kOwn = kShare / 32;             // rows whose place a lane knows
-      constexpr int kLanes = C::kWide / 16;         // lanes to a main row
-      constexpr int kRows = 32 / kLanes;            // rows at once
-      constexpr int kTurns = 32 / kRows;            // turns for 32 rows
-      const int w = warp - kLoadWarp;
-      const int32_t mine = tile_begin * kTile + w * kShare + lane;
-      const uint8_t* k_base = a.cache.k + kv * a.cache.k_head;
-      const uint8_t* v_base = a.cache.v + kv * a.cache.v_head;
+      mbar_arrive(smem_addr(&sh.finished[seq & 1]));
+    }
+    tc_fence_before();
+  } else if (warp < kSplitWarp) {
+    // ==================================================== gathering
+    // A warp gathers its share of a tile's 128 rows; lane r knows the places
+    // of rows r, r + 32, ..., eight lanes copy a 128-byte row (four a 64-byte
+    // one).
+    constexpr int kShare = kTile / C::kLoaders;   // rows of a warp
+    constexpr int kOwn = kShare / 32;             // rows whose place a lane knows
+    constexpr int kLanes = C::kWide / 16;         // lanes to a main row
+    constexpr int kRows = 32 / kLanes;            // rows at once
+    constexpr int kTurns = 32 / kRows;            // turns for 32 rows
+    const int w = warp - kLoadWarp;
+    bool bad = false;
+    uint32_t b = 0, turn = 0, tail_turn = 0;
+    uint32_t unit = blockIdx.x * C::kPipes + pipe;
+    bool shared = false;  // at the split item
+    while (true) {
+      Work work;
+      if (unit < plan.whole) {
+        work = find_work(a, plan, unit, 0, 1);
+        unit += whole_step;
+      } else if (has_split && !shared) {
+        work = find_work(a, plan, split_unit, rank, ranks);
+        shared = true;
+      } else {
+        break;
+      }
+      const uint8_t* k_base = a.cache.k + work.kv * a.cache.k_head;
+      const uint8_t* v_base = a.cache.v + work.kv * a.cache.v_head;
+      const int32_t mine = work.begin * kTile + w * kShare + lane;
       int32_t fetched[kOwn];
 #pragma unroll
-      for (int o = 0; o < kOwn; ++o) fetched[o] = steps > 0 ? fetch_key(a, keys, mine + o * 32) : -1;
-      bool bad = false;
-      uint32_t b = 0, turn = 0;
-      for (int32_t i = 0; i < steps; ++i) {
+      for (int o = 0; o < kOwn; ++o) fetched[o] = work.steps > 0 ? fetch_key(a, work.keys, mine + o * 32) : -1;
+      for (int32_t i = 0; i < work.steps; ++i) {
         Key key[kOwn];
         uint32_t valid[kOwn];
         int64_t k_off[kOwn], v_off[kOwn];
 #pragma unroll
         for (int o = 0; o < kOwn; ++o) {
           const int32_t j = mine + i * kTile + o * 32;
-          key[o] = locate_key(a, keys, j, fetched[o]);
-          bad |= bad_key(keys, j, fetched[o], key[o]);
-          fetched[o] = i + 1 < steps ? fetch_key(a, keys, j + kTile) : -1;
+          key[o] = locate_key(a, work.keys, j, fetched[o]);
+          bad |= bad_key(work.keys, j, fetched[o], key[o]);
+          fetched[o] = i + 1 < work.steps ? fetch_key(a, work.keys, j + kTile) : -1;
           valid[o] = __ballot_sync(kAllLanes, key[o].valid);
           k_off[o] = key[o].block * a.cache.k_block + key[o].offset * a.cache.k_token;
           v_off[o] = key[o].block * a.cache.v_block + key[o].offset * a.cache.v_token;
@@ -656,7 +649,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
 #pragma unroll
           for (int o = 0; o < kOwn; ++o) {
             const int row = w * kShare + o * 32 + lane;
-            const int64_t scale_at = static_cast<int64_t>(key[o].block) * a.cache.kv_heads + kv;
+            const int64_t scale_at = static_cast<int64_t>(key[o].block) * a.cache.kv_heads + work.kv;
             cp_async4(smem_addr(&sh.k_scale[b][row]), a.cache.k_scale + scale_at, key[o].valid ? 4 : 0);
             if constexpr (!C::kIsLatent) {
               cp_async4(smem_addr(&sh.v_scale[b][row]), a.cache.v_scale + scale_at, key[o].valid ? 4 : 0);
@@ -687,7 +680,8 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
             }
             cp_async_arrive(smem_addr(&sh.full[c][b]));
           }
-          const uint32_t tb = C::kTails == 1 ? 0 : b, tt = C::kTails == 1 ? i & 1 : turn;
+          const uint32_t tb = C::kTails == 1 ? 0 : b, tt = C::kTails == 1 ? tail_turn : turn;
+          tail_turn ^= 1;
           warp_wait(&sh.empty[4][tb], tt ^ 1, abort);
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
@@ -727,161 +721,336 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, Config<SHAPE, 
           turn ^= 1;
         }
       }
-      cp_async_wait_all();
-      if (__any_sync(kAllLanes, bad) && lane == 0) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
-      if (ranks > 1) cluster_sync();
-    } else {
-      // ================================================== MMAs
-      // The whole warp walks the loop, so that addresses stay in uniform
-      // registers; one lane issues.
-      if (steps > 0) {
-        constexpr uint32_t kScoreDesc = mma_descriptor(128, T * NH, kE4M3, false, false);
-        constexpr uint32_t kFirstDesc = mma_descriptor(128, NH, kE4M3, true, true);
-        constexpr uint32_t kOtherDesc = mma_descriptor(128, NH, kE5M2, true, true);
-        constexpr Swizzle kPSwizzle = NH == 64 ? kSwizzle64 : NH == 32 ? kSwizzle32 : kSwizzleNone;
-        constexpr Swizzle kMain = C::kWide == 128 ? kSwizzle128 : kSwizzle64;
-        // Descriptors of the first chunks; further ones are offsets in units of 16 bytes.
-        const uint64_t k_desc = smem_descriptor(base + (SHAPE == kDim64 ? C::kChunkBytes : 0), 16, 8 * C::kWide, kMain);
-        const uint64_t q_desc = smem_descriptor(base + C::kOffQ, 16, 8 * C::kWide, kMain);
-        const uint64_t v_desc = smem_descriptor(base + (SHAPE == kDim128 ? C::kChunkBytes : 0),
-                                                SHAPE == kDim64 ? C::kChunkBytes : 1024, 8 * C::kWide, kMain);
-        const uint64_t p_desc = smem_descriptor(base + C::kOffP, 8 * NH, 8 * NH, kPSwizzle);
-        const bool leader = elect_one();
-        warp_wait(&sh.queries, 0, abort);
-        uint32_t sb = 0, st = 0, ob = 0, ot = 0;  // stage and its turn, of scores and of outputs
-        for (int32_t i = 0; i <= steps; ++i) {
-          if (i < steps) {  // scores of tile i
-            const uint32_t d = tmem + C::kValues * NH + (i & 1) * (T * NH);
+    }
+    cp_async_wait_all();
+    if (__any_sync(kAllLanes, bad) && lane == 0) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
+  } else if (warp < kMmaWarp) {
+    // ==================================================== queries
+    // Find the next item, bring its queries, split them as soon as the last
+    // scores of the item before are done, and hand it on. Items without keys
+    // end here: out 0, lse -inf.
+    const int w = warp - kSplitWarp;
+    uint32_t unit = blockIdx.x * C::kPipes + pipe, seq = 0;
+    bool shared = false;
+    while (true) {
+      Work work;
+      bool end = false;
+      const bool split = unit >= plan.whole;
+      if (!split) {
+        work = find_work(a, plan, unit, 0, 1);
+        unit += whole_step;
+      } else if (has_split && !shared) {
+        work = find_work(a, plan, split_unit, rank, ranks);
+        shared = true;
+      } else {
+        end = true;
+      }
+      constexpr int kPieces = (C::kKeyDim / 4 + 31) / 32;
+      constexpr int kBatch = 2;
+      uint2 raw[kBatch][kPieces];
+      auto bring = [&](int c0) {
 #pragma unroll
-            for (int c = 0; c < C::kMainKeys; ++c) {
-              warp_wait(&sh.full[c][sb], st, abort);
-              fence_proxy_async();
-              if (leader) {
-                const uint64_t kd = k_desc + ((sb * C::kStageBytes + c * C::kChunkBytes) >> 4);
-                const uint64_t qd = q_desc + ((c * (T * NH * C::kWide)) >> 4);
+        for (int n = 0; n < kBatch; ++n) {
+          const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, c0 + n);
+          const E* q = static_cast<const E*>(a.q) + static_cast<int64_t>(work.span.row + col.query) * a.q_row +
+                       static_cast<int64_t>(col.head) * a.q_head;
 #pragma unroll
-                for (int k = 0; k < C::kWide / 32; ++k) mma_f8(d, kd + 2 * k, qd + 2 * k, kScoreDesc, c + k > 0);
-              }
-              __syncwarp();
-            }
-            if constexpr (C::kIsLatent) {
-              const uint32_t tb = C::kTails == 1 ? 0 : sb, tt = C::kTails == 1 ? i & 1 : st;
-              warp_wait(&sh.full[4][tb], tt, abort);
-              fence_proxy_async();
-              if (leader) {
-                const uint64_t kd = smem_descriptor(base + C::kOffTail + tb * C::kTailBytes, 16, 512, kSwizzle64);
-                const uint64_t qd = smem_descriptor(base + C::kOffQ + 4 * (T * NH * 128), 16, 512, kSwizzle64);
-                mma_f8(d, kd, qd, kScoreDesc, true);
-                mma_f8(d, kd + 2, qd + 2, kScoreDesc, true);
-                mma_commit(smem_addr(&sh.empty[4][tb]));
-              }
-            } else if (leader) {
-              mma_commit(smem_addr(&sh.empty[0][sb]));
-            }
-            if (leader) mma_commit(smem_addr(&sh.scores[i & 1]));
-            __syncwarp();
-            if (++sb == C::kStages) {
-              sb = 0;
-              st ^= 1;
+          for (int i = 0; i < kPieces; ++i) {
+            const int d = (i * 32 + lane) * 4;
+            raw[n][i] = make_uint2(0u, 0u);
+            if (col.used && c0 + n < NH && d < C::kKeyDim) raw[n][i] = *reinterpret_cast<const uint2*>(q + d);
+          }
+        }
+      };
+      if (!end) {
+        if (work.tiles == 0) {
+          if (!split || rank == 0) {
+            for (int c = w; c < NH; c += C::kSplitters) {
+              const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, c);
+              if (!col.used) continue;
+              const int64_t row = work.span.row + col.query;
+              E* out = static_cast<E*>(a.out) + row * a.out_row + static_cast<int64_t>(col.head) * a.out_head;
+              for (int d = lane; d < C::kValueDim; d += 32) out[d] = static_cast<E>(0.f);
+              if (lane == 0) a.lse[row * a.heads + col.head] = -INFINITY;
             }
           }
-          if (i > 0) {  // outputs of tile i - 1
-            warp_wait(&sh.weights, (i - 1) & 1, abort);
-            tc_fence_after();
-            if constexpr (!C::kIsLatent) {
-              warp_wait(&sh.full[1][ob], ot, abort);
-              fence_proxy_async();
+          continue;
+        }
+        bring(w * kBatch);
+      }
+      if (seq > 0) warp_wait(&sh.queries_read, (seq - 1) & 1, abort);
+      if (seq > 1) warp_wait(&sh.finished[seq & 1], ((seq >> 1) - 1) & 1, abort);
+      if (__any_sync(kAllLanes, *abort != 0)) break;  // what was handed on stays
+      if (end) {
+        if (w == 0 && lane == 0) sh.handed[seq & 1].steps = -1;
+        __syncwarp();
+        mbar_arrive(smem_addr(&sh.queries[seq & 1]));
+        break;
+      }
+      if (w == 0 && lane == 0) {
+        sh.handed[seq & 1] = Handed{work.span.row, work.span.count, work.span.position, work.kv, work.block, work.steps,
+                                    split ? 1 : 0};
+      }
+      for (int c0 = w * kBatch; c0 < NH; c0 += C::kSplitters * kBatch) {
+        uint2 now[kBatch][kPieces];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) now[n][i] = raw[n][i];
+        }
+        if (c0 + C::kSplitters * kBatch < NH) bring(c0 + C::kSplitters * kBatch);  // the next columns' loads
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+          const int c = c0 + n;
+          uint32_t most = 0;
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) most = max(most, magnitude4<E>(now[n][i]));
+          most = __reduce_max_sync(kAllLanes, most);
+          // The largest magnitude comes to [128, 256): its exponent field is taken off.
+          const int e = max(static_cast<int>(most >> 23), 40);
+          const bool odd = most >= 0x7f800000u;  // an infinity or NaN: the row becomes NaN
+          const float up = __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
+          if (lane == 0) {
+            sh.factor[seq & 1][c] = odd ? NAN : a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
+            if constexpr (C::kSeveral) {
+              const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, c);
+              const int32_t position = work.span.position + col.query;
+              sh.seen_to[seq & 1][c] = col.used ? position + 1 : 0x7fffffff;
+              sh.seen_from[seq & 1][c] = col.used && a.window != 0 && position + 1 > static_cast<int64_t>(a.window)
+                                             ? position + 1 - static_cast<int32_t>(a.window) : 0;
             }
-            if (leader) {
+          }
 #pragma unroll
-              for (int c = 0; c < C::kValues; ++c) {
-                const uint64_t vd = v_desc + ((ob * C::kStageBytes + c * C::kChunkBytes) >> 4);
+          for (int i = 0; i < kPieces; ++i) {
+            const int d = (i * 32 + lane) * 4;
+            if (d < C::kKeyDim) {
+              float y[4];
+              unpack4<E>(now[n][i], y);
 #pragma unroll
-                for (int p = 0; p < T; ++p) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    mma_f8(tmem + c * NH, vd + 2 * C::kWide * k, p_desc + ((p * (NH * kTile) + k * 32 * NH) >> 4),
-                           p == 0 ? kFirstDesc : kOtherDesc, p + k > 0 || i > 1);
-                  }
-                }
-                mma_commit(smem_addr(&sh.empty[C::kIsLatent ? c : 1][ob]));
+              for (int k = 0; k < 4; ++k) y[k] = odd ? 0.f : y[k] * up;
+              uint32_t part[T];
+              if constexpr (T == 2) {
+                split_query4(y, part);
+              } else {
+                split4<T, false>(y, part);
               }
-              mma_commit(smem_addr(&sh.done));
-            }
-            __syncwarp();
-            if (++ob == C::kStages) {
-              ob = 0;
-              ot ^= 1;
+              const int chunk = d / 128, in = d & 127;
+              const bool narrow = C::kWide == 64 || (C::kIsLatent && chunk == 4);
+#pragma unroll
+              for (int t = 0; t < T; ++t) {
+                const int row = t * NH + c;
+                const uint32_t at = narrow ? row * 64 + ((((in >> 4) ^ (row >> 1)) & 3) << 4) + (in & 15)
+                                           : row * 128 + ((((in >> 4) ^ row) & 7) << 4) + (in & 15);
+                st_shared(base + C::kOffQ + chunk * (T * NH * 128) + at, part[t]);
+              }
             }
           }
         }
-        if (__any_sync(kAllLanes, *abort != 0)) {  // gave up: let what was issued finish before the memory goes
-          if (leader) {
-            mma_commit(smem_addr(&sh.drained));
-            const long long begin = clock64();
-            while (!mbar_try(smem_addr(&sh.drained), 0) && clock64() - begin < 1000000000LL) {
+      }
+      fence_proxy_async();
+      mbar_arrive(smem_addr(&sh.queries[seq & 1]));
+      ++seq;
+      if (split) break;
+    }
+  } else {
+    // ==================================================== MMAs
+    // The whole warp walks the loops, so that addresses stay in uniform
+    // registers; one lane issues.
+    constexpr uint32_t kScoreDesc = mma_descriptor(128, T * NH, kE4M3, false, false);
+    constexpr uint32_t kFirstDesc = mma_descriptor(128, NH, kE4M3, true, true);
+    constexpr uint32_t kOtherDesc = mma_descriptor(128, NH, kE5M2, true, true);
+    constexpr Swizzle kPSwizzle = NH == 64 ? kSwizzle64 : NH == 32 ? kSwizzle32 : kSwizzleNone;
+    constexpr Swizzle kMain = C::kWide == 128 ? kSwizzle128 : kSwizzle64;
+    // Descriptors of the first chunks; further ones are offsets in units of 16 bytes.
+    const uint64_t k_desc = smem_descriptor(base + (SHAPE == kDim64 ? C::kChunkBytes : 0), 16, 8 * C::kWide, kMain);
+    const uint64_t q_desc = smem_descriptor(base + C::kOffQ, 16, 8 * C::kWide, kMain);
+    const uint64_t v_desc = smem_descriptor(base + (SHAPE == kDim128 ? C::kChunkBytes : 0),
+                                            SHAPE == kDim64 ? C::kChunkBytes : 1024, 8 * C::kWide, kMain);
+    const uint64_t p_desc = smem_descriptor(base + C::kOffP, 8 * NH, 8 * NH, kPSwizzle);
+    const bool leader = elect_one();
+    uint32_t sb = 0, st = 0, ob = 0, ot = 0, tail_turn = 0;  // stage and its turn, of scores and of outputs
+    uint32_t n = 0;                                          // tiles before this item
+    bool more = true;
+    for (uint32_t seq = 0; more; ++seq) {
+      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort);
+      if (__any_sync(kAllLanes, *abort != 0)) break;
+      const int32_t steps = __shfl_sync(kAllLanes, sh.handed[seq & 1].steps, 0);
+      more = steps >= 0 && __shfl_sync(kAllLanes, sh.handed[seq & 1].split, 0) == 0;
+      for (int32_t i = 0; steps > 0 && i <= steps; ++i) {
+        if (i < steps) {  // scores of tile i
+          const uint32_t d = tmem + C::kValues * NH + ((n + i) & 1) * (T * NH);
+#pragma unroll
+          for (int c = 0; c < C::kMainKeys; ++c) {
+            warp_wait(&sh.full[c][sb], st, abort);
+            fence_proxy_async();
+            if (leader) {
+              const uint64_t kd = k_desc + ((sb * C::kStageBytes + c * C::kChunkBytes) >> 4);
+              const uint64_t qd = q_desc + ((c * (T * NH * C::kWide)) >> 4);
+#pragma unroll
+              for (int k = 0; k < C::kWide / 32; ++k) mma_f8(d, kd + 2 * k, qd + 2 * k, kScoreDesc, c + k > 0);
             }
-            flag_status(a.status, SILKERN_STATUS_WAIT_TIMEOUT);
+            __syncwarp();
+          }
+          if constexpr (C::kIsLatent) {
+            const uint32_t tb = C::kTails == 1 ? 0 : sb, tt = C::kTails == 1 ? tail_turn : st;
+            tail_turn ^= 1;
+            warp_wait(&sh.full[4][tb], tt, abort);
+            fence_proxy_async();
+            if (leader) {
+              const uint64_t kd = smem_descriptor(base + C::kOffTail + tb * C::kTailBytes, 16, 512, kSwizzle64);
+              const uint64_t qd = smem_descriptor(base + C::kOffQ + 4 * (T * NH * 128), 16, 512, kSwizzle64);
+              mma_f8(d, kd, qd, kScoreDesc, true);
+              mma_f8(d, kd + 2, qd + 2, kScoreDesc, true);
+              mma_commit(smem_addr(&sh.empty[4][tb]));
+            }
+          } else if (leader) {
+            mma_commit(smem_addr(&sh.empty[0][sb]));
+          }
+          if (leader) {
+            mma_commit(smem_addr(&sh.scores[(n + i) & 1]));
+            if (i + 1 == steps) mma_commit(smem_addr(&sh.queries_read));
           }
           __syncwarp();
+          if (++sb == C::kStages) {
+            sb = 0;
+            st ^= 1;
+          }
+        }
+        if (i > 0) {  // outputs of tile i - 1
+          warp_wait(&sh.weights, (n + i - 1) & 1, abort);
+          tc_fence_after();
+          if constexpr (!C::kIsLatent) {
+            warp_wait(&sh.full[1][ob], ot, abort);
+            fence_proxy_async();
+          }
+          if (leader) {
+#pragma unroll
+            for (int c = 0; c < C::kValues; ++c) {
+              const uint64_t vd = v_desc + ((ob * C::kStageBytes + c * C::kChunkBytes) >> 4);
+#pragma unroll
+              for (int p = 0; p < T; ++p) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  mma_f8(tmem + c * NH, vd + 2 * C::kWide * k, p_desc + ((p * (NH * kTile) + k * 32 * NH) >> 4),
+                         p == 0 ? kFirstDesc : kOtherDesc, p + k > 0 || i > 1);
+                }
+              }
+              mma_commit(smem_addr(&sh.empty[C::kIsLatent ? c : 1][ob]));
+            }
+            mma_commit(smem_addr(&sh.done));
+          }
+          __syncwarp();
+          if (++ob == C::kStages) {
+            ob = 0;
+            ot ^= 1;
+          }
         }
       }
-      if (ranks > 1) cluster_sync();
+      if (steps > 0) n += steps;
     }
-
-    if (ranks > 1) {
-      // ==================================================== joining
-      cluster_sync();
-      const float* joint = reinterpret_cast<const float*>(smem + C::kOffP) + 8 * NH;
-      for (int32_t e = (static_cast<int32_t>(rank) * C::kThreads + tid) * 4; e < NH * C::kValueDim;
-           e += static_cast<int32_t>(ranks) * C::kThreads * 4) {
-        const int32_t c = e / C::kValueDim, d = e - c * C::kValueDim;
-        const Column col = column(c);
-        if (!col.used) continue;
-        float4 y{0.f, 0.f, 0.f, 0.f};
-        for (uint32_t r = 0; r < ranks; ++r) {
-          if (ld_cluster(smem_addr(joint + c), r) == -INFINITY) continue;  // rank r saw nothing
-          const float4 x = ld_cluster4(base + e * 4, r);
-          y.x += x.x;
-          y.y += x.y;
-          y.z += x.z;
-          y.w += x.w;
+    if (__any_sync(kAllLanes, *abort != 0)) {  // gave up: let what was issued finish before the memory goes
+      if (leader) {
+        mma_commit(smem_addr(&sh.drained));
+        const long long begin = clock64();
+        while (!mbar_try(smem_addr(&sh.drained), 0) && clock64() - begin < 1000000000LL) {
         }
-        E* out = static_cast<E*>(a.out) + static_cast<int64_t>(span.row + col.query) * a.out_row +
-                 static_cast<int64_t>(col.head) * a.out_head + d;
-        if (*abort == 0) {
-          out[0] = static_cast<E>(y.x);
-          out[1] = static_cast<E>(y.y);
-          out[2] = static_cast<E>(y.z);
-          out[3] = static_cast<E>(y.w);
-        }
+        flag_status(a.status, SILKERN_STATUS_WAIT_TIMEOUT);
       }
-      cluster_sync();  // nobody's shared memory goes before it was read
-    }
-  } else if (rank == 0) {
-    // Nothing to see: out 0, lse -inf.
-    for (int c = warp; c < NH; c += C::kThreads / 32) {
-      const Column col = column(c);
-      if (!col.used) continue;
-      const int64_t row = span.row + col.query;
-      E* out = static_cast<E*>(a.out) + row * a.out_row + static_cast<int64_t>(col.head) * a.out_head;
-      for (int d = lane; d < C::kValueDim; d += 32) out[d] = static_cast<E>(0.f);
-      if (lane == 0) a.lse[row * a.heads + col.head] = -INFINITY;
+      __syncwarp();
     }
   }
+
   __syncthreads();
-  if (warp == kMmaWarp) {
+  // ---- a split item: its ranks, which all see the same tiles, join
+  const Work last = has_split ? find_work(a, plan, split_unit, rank, ranks) : Work{};
+  if (has_split && last.tiles > 0) {
+    float* joint = reinterpret_cast<float*>(smem + C::kOffP) + 8 * NH;  // references, then sums
+    float* joined = reinterpret_cast<float*>(smem);                     // outputs
+    const int first_col = (warp >> 2) * 16, own = lane & 15;
+    if (warp < kLoadWarp && (warp & 3) == 0 && lane < 16) {
+      joint[first_col + lane] = reference;
+      joint[NH + first_col + lane] = l[0];
+    }
+    cluster_sync();
+    // Rank r is pipeline r mod kPipes of CTA r / kPipes.
+    const uint32_t origin = smem_addr(all_smem);
+    auto place = [&](const float* p, uint32_t r) {
+      return origin + (r % C::kPipes) * C::kPipeBytes + (smem_addr(p) - base);
+    };
+    if (warp < kLoadWarp) {
+      const float* at = joint + first_col + own;
+      float whole_r = -INFINITY, whole_l = 0.f;
+      for (uint32_t r = 0; r < ranks; ++r) whole_r = fmaxf(whole_r, ld_cluster(place(at, r), r / C::kPipes));
+      for (uint32_t r = 0; r < ranks; ++r) {
+        const float rr = ld_cluster(place(at, r), r / C::kPipes);
+        whole_l += rr == -INFINITY ? 0.f : ld_cluster(place(at + NH, r), r / C::kPipes) * exp2_approx(rr - whole_r);
+      }
+      const float inverse = whole_l == 0.f ? 0.f : 1.f / (32.f * whole_l);
+      const float by = reference == -INFINITY ? 0.f : exp2_approx(reference - whole_r) * inverse;
+      if (rank == 0 && (warp & 3) == 0 && lane < 16 && *abort == 0) {
+        const Column col = find_column<NH>(a, plan, last.span.count, last.kv, last.block, first_col + lane);
+        if (col.used) {
+          a.lse[static_cast<int64_t>(last.span.row + col.query) * a.heads + col.head] =
+              whole_l == 0.f ? -INFINITY : (whole_r + log2f(whole_l)) * 0.69314718055994531f;
+        }
+      }
+      __syncwarp();
+      tc_fence_after();
+      if (last.steps > 0 && (SHAPE != kDim64 || (warp & 3) < 2)) {
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+#pragma unroll 1
+        for (int m = 0; m < C::kValues; ++m) {
+          float o[16];
+          tmem_ld16(tmem + lanes + m * NH + first_col, o);
+          tmem_wait_ld(o);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            joined[(first_col + c) * C::kValueDim + m * 128 + (tid & 127)] = o[c] * __shfl_sync(kAllLanes, by, c);
+          }
+        }
+      }
+    }
+    cluster_sync();
+    constexpr int kRankThreads = C::kPipeWarps * 32;
+    for (int32_t e = (static_cast<int32_t>(rank) * kRankThreads + tid) * 4; e < NH * C::kValueDim;
+         e += static_cast<int32_t>(ranks) * kRankThreads * 4) {
+      const int32_t c = e / C::kValueDim, d = e - c * C::kValueDim;
+      const Column col = find_column<NH>(a, plan, last.span.count, last.kv, last.block, c);
+      if (!col.used) continue;
+      float4 y{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t r = 0; r < ranks; ++r) {
+        if (ld_cluster(place(joint + c, r), r / C::kPipes) == -INFINITY) continue;  // rank r saw nothing
+        const float4 x = ld_cluster4(place(joined + e, r), r / C::kPipes);
+        y.x += x.x;
+        y.y += x.y;
+        y.z += x.z;
+        y.w += x.w;
+      }
+      E* out = static_cast<E*>(a.out) + static_cast<int64_t>(last.span.row + col.query) * a.out_row +
+               static_cast<int64_t>(col.head) * a.out_head + d;
+      if (*abort == 0) {
+        out[0] = static_cast<E>(y.x);
+        out[1] = static_cast<E>(y.y);
+        out[2] = static_cast<E>(y.z);
+        out[3] = static_cast<E>(y.w);
+      }
+    }
+    cluster_sync();  // nobody's shared memory goes before it was read
+    tc_fence_before();
+    __syncthreads();
+  }
+  if (pipe == 0 && warp == kMmaWarp) {
     tc_fence_after();
-    tmem_free(tmem, C::kColumns);
+    tmem_free(tmem_all, C::kColumns);
   }
 }
 
 template <CacheShape SHAPE, int NH, int T>
 int launch_config(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l) {
   using C = Config<SHAPE, NH, T>;
-  const int rc = allow_launch(reinterpret_cast<const void*>(attend_kernel<SHAPE, NH, T>), C::kSmem);
+  const int rc = allow_launch(reinterpret_cast<const void*>(attend_kernel<SHAPE, NH, T>), kSharedMemory);
   if (rc != SILKERN_OK) return rc;
-  return launch_pdl(attend_kernel<SHAPE, NH, T>, l.grid, C::kThreads, C::kSmem, l.cluster, l.stream, a, plan);
+  return launch_pdl(attend_kernel<SHAPE, NH, T>, l.grid, C::kThreads, kSharedMemory, l.cluster, l.stream, a, plan);
 }
 
 template <CacheShape SHAPE>

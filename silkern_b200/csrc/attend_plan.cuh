@@ -7,8 +7,12 @@
 namespace silkern {
 
 struct AttendPlan {
-  FastDiv per;     // queries of one sequence that share a CTA
+  FastDiv per;     // queries of one sequence that share a work item
+  FastDiv group;   // by heads to a cache head
   int32_t blocks;  // column blocks of one (item, cache head)
+  // Work items: [0, whole) go to a pipeline each, [whole, units) are split
+  // over the pipelines of a cluster each.
+  uint32_t whole, units;
 };
 
 struct AttendLaunch {

@@ -44,6 +44,17 @@ __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// The same, and whether any of the threads says yes.
+__device__ __forceinline__ bool named_barrier_or(int id, int threads, bool yes) {
+  uint32_t any;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n"
+      " selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(yes)), "r"(id), "r"(threads)
+      : "memory");
+  return any != 0;
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -224,6 +235,11 @@ __device__ __forceinline__ uint32_t e5m2x2_to_f16x2(uint16_t v) {
 __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul16_f16x2(uint32_t a) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x4c004c00u));
   return r;
 }
 
