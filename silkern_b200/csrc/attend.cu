@@ -1,5 +1,7 @@
 // Launch of the cache's attention: how many columns a CTA takes and how many
 // CTAs share a work item's keys.
+#include <numeric>
+
 #include "attend_plan.cuh"
 #include "host.cuh"
 #include "paged.cuh"
@@ -19,9 +21,29 @@ int multiprocessors() {
   return n;
 }
 
+// One tensor's rows of a token and head: the pitch that divides its strides,
+// and the strides in units of it. False where a row's number passes 31 bits.
+struct Rows {
+  int64_t pitch;
+  uint32_t block, token, head;
+};
+bool find_rows(const PagedCache& c, int64_t block, int64_t token, int64_t head, Rows* r) {
+  int64_t pitch = 0;
+  if (c.num_blocks > 1) pitch = std::gcd(pitch, block);
+  if (c.block.divisor > 1) pitch = std::gcd(pitch, token);
+  if (c.kv_heads > 1) pitch = std::gcd(pitch, head);
+  if (pitch == 0) pitch = 16;
+  const int64_t last = (c.num_blocks - int64_t{1}) * (block / pitch) + (c.block.divisor - int64_t{1}) * (token / pitch) +
+                       (c.kv_heads - int64_t{1}) * (head / pitch);
+  if (last >= 0x7ffffffe) return false;
+  *r = Rows{pitch, static_cast<uint32_t>(block / pitch), static_cast<uint32_t>(token / pitch),
+            static_cast<uint32_t>(head / pitch)};
+  return true;
+}
+
 }  // namespace
 
-int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
+int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
   const bool latent = key_dim == 576, half = type == SILKERN_F16;
   const int32_t group = a.heads_per_kv;
   // Queries that may share a CTA's keys: one for a selected row; for
@@ -37,7 +59,7 @@ int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t strea
   plan.per = make_fastdiv(static_cast<uint32_t>(per));
   plan.group = make_fastdiv(static_cast<uint32_t>(group));
   plan.blocks = (group + columns - 1) / columns;
-  const int64_t items = a.slots != nullptr ? a.rows : a.rows / per + static_cast<int64_t>(a.sequences);
+  const int64_t items = a.slots != nullptr ? a.rows : (a.rows + static_cast<int64_t>(per - 1) * a.sequences) / per;
   int64_t busy = a.slots != nullptr ? a.rows : (a.rows + per - 1) / per;
   if (a.slots == nullptr && busy < a.sequences) busy = a.sequences < a.rows ? a.sequences : a.rows;
   const int64_t most = a.slots != nullptr ? a.width : static_cast<int64_t>(a.table_width) * a.cache.block.divisor;
@@ -71,6 +93,20 @@ int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t strea
     const int64_t round = grid * pipes, left = units % round;
     plan.whole = static_cast<uint32_t>(pipes > 1 && left <= grid ? units - left : units);
   }
+  Rows k, v;
+  PagedCache& c = a.cache;
+  if (!find_rows(c, c.k_block, c.k_token, c.k_head, &k) ||
+      !find_rows(c, c.v_block, c.v_token, c.v_head, &v)) {
+    return SILKERN_E_CACHE;
+  }
+  c.k_block_rows = k.block;
+  c.k_token_rows = k.token;
+  c.k_head_rows = k.head;
+  c.k_pitch = k.pitch;
+  c.v_block_rows = v.block;
+  c.v_token_rows = v.token;
+  c.v_head_rows = v.head;
+  c.v_pitch = v.pitch;
   AttendLaunch l{columns, half, static_cast<unsigned>(grid), cluster, stream};
   return key_dim == 64 ? launch_dim64(a, plan, l) : key_dim == 128 ? launch_dim128(a, plan, l) : launch_latent(a, plan, l);
 }

@@ -28,8 +28,9 @@
 // 2^8.8. l, S and O are float32.
 //
 // A CTA is one or two pipelines, each a softmax of one key a thread and 16
-// columns a warpgroup, warps that gather keys and values with cp.async, warps
-// that split the queries, and one that issues the MMAs. Every kernel that
+// columns a warpgroup, warps that gather keys and values with cp.async (the TMA
+// unit's four-row gathers took 61 cycles for 512 bytes of an SM here, these
+// copies about 12), warps that split the queries, and one that issues the MMAs. Every kernel that
 // allocates TMEM has an SM to itself, so a CTA stays on its SM and its
 // pipelines walk through the work items; each role runs ahead as far as the
 // buffers let it, and one item's start and end hide behind its neighbours'.
@@ -560,6 +561,9 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
                                      : static_cast<E*>(a.out) + static_cast<int64_t>(h.row + col.query) * a.out_row +
                                            static_cast<int64_t>(col.head) * a.out_head + p % kPieces * 8;
       }
+      float inv[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) inv[c] = __shfl_sync(kAllLanes, inverse, c);
 #pragma unroll 1
       for (int m = 0; m < C::kValues; ++m) {
         float o[16];
@@ -568,7 +572,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           tmem_wait_ld(o);
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
-            staged[c * 128 + thread] = static_cast<E>(o[c] * __shfl_sync(kAllLanes, inverse, c));
+            staged[c * 128 + thread] = static_cast<E>(o[c] * inv[c]);
           }
         }
         named_barrier(group_barrier, 128);
@@ -601,14 +605,21 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
   } else if (warp < kSplitWarp) {
     // ==================================================== gathering
     // A warp gathers its share of a tile's 128 rows; lane r knows the places
-    // of rows r, r + 32, ..., eight lanes copy a 128-byte row (four a 64-byte
-    // one).
-    constexpr int kShare = kTile / C::kLoaders;   // rows of a warp
-    constexpr int kOwn = kShare / 32;             // rows whose place a lane knows
-    constexpr int kLanes = C::kWide / 16;         // lanes to a main row
-    constexpr int kRows = 32 / kLanes;            // rows at once
-    constexpr int kTurns = 32 / kRows;            // turns for 32 rows
+    // of rows r, r + 32, ... (-1: masked, filled with zeros), eight lanes copy
+    // a 128-byte row, four a 64-byte one. All places come round before the
+    // first copy, so that the copies follow one another without a wait.
+    constexpr int kShare = kTile / C::kLoaders;  // rows of a warp
+    constexpr int kOwn = kShare / 32;            // rows whose place a lane knows
+    constexpr int kLanes = C::kWide / 16;        // lanes to a main row
+    constexpr int kRows = 32 / kLanes;           // rows at once
+    constexpr int kTurns = kShare / kRows;       // turns for a warp's rows
     const int w = warp - kLoadWarp;
+    const int sub = lane / kLanes;
+    // Swizzled place of a lane's 16 bytes, in even and odd turns.
+    const uint32_t in_even = C::kWide == 128 ? ((lane ^ sub) & 7) << 4 : ((lane ^ (sub >> 1)) & 3) << 4;
+    const uint32_t in_odd = C::kWide == 128 ? ((lane ^ (sub + 4)) & 7) << 4 : in_even;
+    const bool alike = a.cache.k_block_rows == a.cache.v_block_rows && a.cache.k_token_rows == a.cache.v_token_rows &&
+                       a.cache.k_head_rows == a.cache.v_head_rows;
     bool bad = false;
     uint32_t b = 0, turn = 0, tail_turn = 0;
     uint32_t unit = blockIdx.x * C::kPipes + pipe;
@@ -624,97 +635,93 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       } else {
         break;
       }
-      const uint8_t* k_base = a.cache.k + work.kv * a.cache.k_head;
-      const uint8_t* v_base = a.cache.v + work.kv * a.cache.v_head;
+      const uint32_t k_first = work.kv * a.cache.k_head_rows, v_first = work.kv * a.cache.v_head_rows;
       const int32_t mine = work.begin * kTile + w * kShare + lane;
       int32_t fetched[kOwn];
 #pragma unroll
       for (int o = 0; o < kOwn; ++o) fetched[o] = work.steps > 0 ? fetch_key(a, work.keys, mine + o * 32) : -1;
       for (int32_t i = 0; i < work.steps; ++i) {
-        Key key[kOwn];
-        uint32_t valid[kOwn];
-        int64_t k_off[kOwn], v_off[kOwn];
+        int32_t k_row[kOwn], v_row[kOwn], position[kOwn];
+        uint32_t page[kOwn];
 #pragma unroll
         for (int o = 0; o < kOwn; ++o) {
           const int32_t j = mine + i * kTile + o * 32;
-          key[o] = locate_key(a, work.keys, j, fetched[o]);
-          bad |= bad_key(work.keys, j, fetched[o], key[o]);
+          const Key key = locate_key(a, work.keys, j, fetched[o]);
+          bad |= bad_key(work.keys, j, fetched[o], key);
           fetched[o] = i + 1 < work.steps ? fetch_key(a, work.keys, j + kTile) : -1;
-          valid[o] = __ballot_sync(kAllLanes, key[o].valid);
-          k_off[o] = key[o].block * a.cache.k_block + key[o].offset * a.cache.k_token;
-          v_off[o] = key[o].block * a.cache.v_block + key[o].offset * a.cache.v_token;
+          page[o] = key.block;
+          position[o] = key.position;
+          k_row[o] = key.valid ? static_cast<int32_t>(k_first + key.block * a.cache.k_block_rows + key.offset * a.cache.k_token_rows) : -1;
+          v_row[o] = key.valid ? static_cast<int32_t>(v_first + key.block * a.cache.v_block_rows + key.offset * a.cache.v_token_rows) : -1;
         }
+        int32_t row[kTurns];
+#pragma unroll
+        for (int n = 0; n < kTurns; ++n) {
+          row[n] = __shfl_sync(kAllLanes, k_row[n * kRows / 32], (n * kRows) % 32 + sub);
+        }
+        // Copies `kWide` bytes of every row, from column x on, to a chunk.
+        auto copy = [&](uint32_t to, const uint8_t* from, int64_t pitch) {
+          to += (w * kShare + sub) * C::kWide;
+          from += (lane % kLanes) * 16;
+#pragma unroll
+          for (int n = 0; n < kTurns; ++n) {
+            cp_async16(to + n * kRows * C::kWide + (n & 1 ? in_odd : in_even), from + max(row[n], 0) * pitch,
+                       row[n] < 0 ? 0 : 16);
+          }
+        };
         // What the softmax has to know of a key: copied with its tile.
         auto note = [&]() {
 #pragma unroll
           for (int o = 0; o < kOwn; ++o) {
-            const int row = w * kShare + o * 32 + lane;
-            const int64_t scale_at = static_cast<int64_t>(key[o].block) * a.cache.kv_heads + work.kv;
-            cp_async4(smem_addr(&sh.k_scale[b][row]), a.cache.k_scale + scale_at, key[o].valid ? 4 : 0);
-            if constexpr (!C::kIsLatent) {
-              cp_async4(smem_addr(&sh.v_scale[b][row]), a.cache.v_scale + scale_at, key[o].valid ? 4 : 0);
-            }
-            if constexpr (C::kSeveral) sh.position[b][row] = key[o].position;
-            if (lane == 0) sh.valid[b][w * kOwn + o] = valid[o];
+            const int at = w * kShare + o * 32 + lane;
+            const int64_t scale_at = static_cast<int64_t>(page[o]) * a.cache.kv_heads + work.kv;
+            const uint32_t size = k_row[o] < 0 ? 0 : 4;
+            cp_async4(smem_addr(&sh.k_scale[b][at]), a.cache.k_scale + scale_at, size);
+            if constexpr (!C::kIsLatent) cp_async4(smem_addr(&sh.v_scale[b][at]), a.cache.v_scale + scale_at, size);
+            if constexpr (C::kSeveral) sh.position[b][at] = position[o];
+            const uint32_t valid = __ballot_sync(kAllLanes, k_row[o] >= 0);
+            if (lane == 0) sh.valid[b][w * kOwn + o] = valid;
           }
+          mbar_arrive(smem_addr(&sh.full[C::kNoteChunk][b]));
         };
         const uint32_t stage = base + b * C::kStageBytes;
         if constexpr (C::kIsLatent) {
-          const uint8_t* from[kTurns];
 #pragma unroll
-          for (int n = 0; n < kTurns; ++n) {
-            from[n] = k_base + __shfl_sync(kAllLanes, k_off[0], n * kRows + lane / kLanes) + (lane % kLanes) * 16;
-          }
-#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             warp_wait(&sh.empty[c][b], turn ^ 1, abort);
-#pragma unroll
-            for (int n = 0; n < kTurns; ++n) {
-              const int r = n * kRows + lane / kLanes, row = w * kShare + r;
-              const uint32_t dst = stage + c * C::kChunkBytes + row * 128 + (((lane % 8) ^ (row & 7)) << 4);
-              cp_async16(dst, from[n] + c * 128, (valid[0] >> r) & 1 ? 16 : 0);
-            }
-            if (c == C::kNoteChunk) {
-              note();
-              mbar_arrive(smem_addr(&sh.full[c][b]));
-            }
+            copy(stage + c * C::kChunkBytes, a.cache.k + c * 128, a.cache.k_pitch);
+            if (c == C::kNoteChunk) note();
             cp_async_arrive(smem_addr(&sh.full[c][b]));
           }
           const uint32_t tb = C::kTails == 1 ? 0 : b, tt = C::kTails == 1 ? tail_turn : turn;
           tail_turn ^= 1;
           warp_wait(&sh.empty[4][tb], tt ^ 1, abort);
+          const uint32_t to = base + C::kOffTail + tb * C::kTailBytes + (w * kShare + lane / 4) * 64 +
+                              (((lane ^ (lane >> 3)) & 3) << 4);
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int r = n * 8 + lane / 4, row = w * kShare + r;
-            const uint8_t* src = k_base + __shfl_sync(kAllLanes, k_off[0], r) + 512 + (lane % 4) * 16;
-            const uint32_t dst = base + C::kOffTail + tb * C::kTailBytes + row * 64 + (((lane ^ (row >> 1)) & 3) << 4);
-            cp_async16(dst, src, (valid[0] >> r) & 1 ? 16 : 0);
+          for (int n = 0; n < kShare / 8; ++n) {
+            const int32_t r = __shfl_sync(kAllLanes, k_row[n * 8 / 32], (n * 8) % 32 + lane / 4);
+            cp_async16(to + n * 512, a.cache.k + 512 + (lane % 4) * 16 + max(r, 0) * a.cache.k_pitch, r < 0 ? 0 : 16);
           }
           cp_async_arrive(smem_addr(&sh.full[4][tb]));
         } else {
+          // 64-byte rows: values first, so that their second half of M reads
+          // the keys behind them.
+          const uint32_t keys_at = stage + (SHAPE == kDim64 ? C::kChunkBytes : 0);
+          const uint32_t values_at = stage + (SHAPE == kDim64 ? 0 : C::kChunkBytes);
+          warp_wait(&sh.empty[0][b], turn ^ 1, abort);
+          copy(keys_at, a.cache.k, a.cache.k_pitch);
+          cp_async_arrive(smem_addr(&sh.full[0][b]));
+          if (!alike) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            warp_wait(&sh.empty[c][b], turn ^ 1, abort);
-            // 64-byte rows: values first, so that their second half of M reads
-            // the keys behind them.
-            const uint32_t at = stage + ((SHAPE == kDim64) == (c == 0) ? C::kChunkBytes : 0);
-#pragma unroll
-            for (int o = 0; o < kOwn; ++o) {
-#pragma unroll
-              for (int n = 0; n < kTurns; ++n) {
-                const int r = n * kRows + lane / kLanes, row = w * kShare + o * 32 + r;
-                const int64_t off = __shfl_sync(kAllLanes, c == 0 ? k_off[o] : v_off[o], r) + (lane % kLanes) * 16;
-                const uint32_t dst = at + row * C::kWide + (C::kWide == 128 ? ((lane ^ row) & 7) << 4
-                                                                            : ((lane ^ (row >> 1)) & 3) << 4);
-                cp_async16(dst, (c == 0 ? k_base : v_base) + off, (valid[o] >> r) & 1 ? 16 : 0);
-              }
+            for (int n = 0; n < kTurns; ++n) {
+              row[n] = __shfl_sync(kAllLanes, v_row[n * kRows / 32], (n * kRows) % 32 + sub);
             }
-            if (c == C::kNoteChunk) {
-              note();
-              mbar_arrive(smem_addr(&sh.full[c][b]));
-            }
-            cp_async_arrive(smem_addr(&sh.full[c][b]));
           }
+          warp_wait(&sh.empty[1][b], turn ^ 1, abort);
+          copy(values_at, a.cache.v, a.cache.v_pitch);
+          note();
+          cp_async_arrive(smem_addr(&sh.full[1][b]));
         }
         if (++b == C::kStages) {
           b = 0;
@@ -777,6 +784,13 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           continue;
         }
         bring(w * kBatch);
+        for (int e = (w * 32 + lane) * 64; e < NH * C::kKeyDim; e += C::kSplitters * 32 * 64) {
+          const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, e / C::kKeyDim);
+          if (col.used) {
+            prefetch_l2_line(static_cast<const E*>(a.q) + static_cast<int64_t>(work.span.row + col.query) * a.q_row +
+                             static_cast<int64_t>(col.head) * a.q_head + e % C::kKeyDim);
+          }
+        }
       }
       if (seq > 0) warp_wait(&sh.queries_read, (seq - 1) & 1, abort);
       if (seq > 1) warp_wait(&sh.finished[seq & 1], ((seq >> 1) - 1) & 1, abort);
@@ -882,7 +896,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < C::kMainKeys; ++c) {
             warp_wait(&sh.full[c][sb], st, abort);
-            fence_proxy_async();
+            fence_proxy_async();  // the copies wrote through the generic proxy
             if (leader) {
               const uint64_t kd = k_desc + ((sb * C::kStageBytes + c * C::kChunkBytes) >> 4);
               const uint64_t qd = q_desc + ((c * (T * NH * C::kWide)) >> 4);

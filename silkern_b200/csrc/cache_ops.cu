@@ -13,7 +13,7 @@
 
 namespace silkern {
 
-int launch_attend(const AttendArgs& a, int key_dim, int type, cudaStream_t stream);
+int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream);
 
 namespace {
 
@@ -363,7 +363,7 @@ extern "C" int silkern_attend_window_v1(const silkern_cache_v1* cache, const voi
   if (!cu_tokens || !lengths || !req_ids || !block_table) return SILKERN_E_NULL;
   rc = check_queries(cache, q, q_row, q_head, type, rows, heads, out, out_row, out_head, lse, softmax_scale, &a);
   if (rc != SILKERN_OK) return rc;
-  if (sequences < 1 || rows + sequences > 0x7fffffff || table_rows < 1 || table_width < 1 ||
+  if (sequences < 1 || rows + 64 * sequences > 0x7fffffff || table_rows < 1 || table_width < 1 ||
       table_width > 0x7fffffff) {
     return SILKERN_E_SHAPE;
   }

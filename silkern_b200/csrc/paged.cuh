@@ -24,6 +24,9 @@ struct PagedCache {
   const float* v_scale;
   int64_t k_block, k_token, k_head;  // strides in bytes, multiples of 16
   int64_t v_block, v_token, v_head;
+  // The same in rows of a common pitch, which divides the strides (attention only).
+  uint32_t k_block_rows, k_token_rows, k_head_rows, v_block_rows, v_token_rows, v_head_rows;
+  int64_t k_pitch, v_pitch;
   uint32_t num_blocks;
   uint32_t kv_heads;
   FastDiv block;  // by block_size
@@ -94,10 +97,14 @@ struct QuerySpan {
 };
 
 // The span of up to `per` queries that work item `item` stands for. Sequence
-// b owns the items [cu[b] / per + b, cu[b + 1] / per + b + 1), which is at
-// least one for each `per` of its tokens, so rows / per + sequences items
-// cover any cu_tokens that ascends to at most `rows`. The warp's lanes search
-// together, 32 boundaries a step.
+// b owns the items from (cu[b] + (per - 1) b) / per on, which leaves each
+// sequence at least one for each `per` of its tokens, so that
+// (rows + (per - 1) sequences) / per items cover any cu_tokens that ascends to
+// at most `rows`, and one for each sequence where each has one token. The
+// warp's lanes search together, 32 boundaries a step.
+__device__ __forceinline__ int32_t first_item(const FastDiv& per, int32_t cu, int32_t b) {
+  return static_cast<int32_t>(fastdiv(static_cast<uint32_t>(cu) + (per.divisor - 1) * static_cast<uint32_t>(b), per));
+}
 __device__ __forceinline__ QuerySpan find_span(const AttendArgs& a, int32_t item, const FastDiv& per) {
   const int32_t lane = threadIdx.x & 31;
   int32_t low = 0, high = a.sequences;  // the last b in [low, high) with first_item(b) <= item
@@ -107,7 +114,7 @@ __device__ __forceinline__ QuerySpan find_span(const AttendArgs& a, int32_t item
     bool before = false;
     if (b < high) {
       const int32_t cu = min(max(__ldg(a.cu_tokens + b), 0), a.rows);
-      before = static_cast<int32_t>(fastdiv(cu, per)) + b <= item;
+      before = first_item(per, cu, b) <= item;
     }
     const uint32_t hits = __ballot_sync(kAllLanes, before);
     const int32_t last = hits == 0 ? 0 : 31 - __clz(hits);
@@ -117,7 +124,7 @@ __device__ __forceinline__ QuerySpan find_span(const AttendArgs& a, int32_t item
   QuerySpan s{0, 0, low, 0};
   const int32_t begin = min(max(__ldg(a.cu_tokens + low), 0), a.rows);
   const int32_t end = min(max(__ldg(a.cu_tokens + low + 1), begin), a.rows);
-  const int32_t chunk = item - (static_cast<int32_t>(fastdiv(begin, per)) + low);
+  const int32_t chunk = item - first_item(per, begin, low);
   const int64_t row = begin + static_cast<int64_t>(chunk) * per.divisor;
   if (chunk < 0 || row >= end) return s;
   s.row = static_cast<int32_t>(row);
@@ -179,32 +186,32 @@ __device__ __forceinline__ KeyList window_keys(const AttendArgs& a, const QueryS
 }
 
 // fetch: the one dependent load of key j (a slot or a table entry), issued
-// ahead; locate: what that value says.
+// ahead, for lists that are not empty; locate: what that value says. The load
+// is unconditional, at a place inside the list, so that nothing waits for it
+// before locate.
 __device__ __forceinline__ uint32_t local_token(const KeyList& l, uint32_t j) {
   return j < l.sinks_end ? j : j + l.skip;
 }
 __device__ __forceinline__ int32_t fetch_key(const AttendArgs& a, const KeyList& l, int32_t j) {
-  if (j >= l.n) return -1;
-  if (!l.table) return __ldg(l.source + j);
-  const uint32_t page = fastdiv(local_token(l, j), a.cache.block);
-  return page < l.table_width ? __ldg(l.source + page) : -1;
+  uint32_t at = min(j, l.n - 1);
+  if (l.table) at = min(fastdiv(local_token(l, at), a.cache.block), l.table_width - 1);
+  return __ldg(l.source + at);
 }
 __device__ __forceinline__ Key locate_key(const AttendArgs& a, const KeyList& l, int32_t j, int32_t fetched) {
   Key k{0u, 0u, 0, false};
-  if (j >= l.n) return k;
   if (!l.table) {
-    k.valid = fetched >= 0 && static_cast<uint32_t>(fetched) < a.total_slots;
+    k.valid = j < l.n && static_cast<uint32_t>(fetched) < a.total_slots;  // negative ones are above
     if (k.valid) {
       k.block = fastdiv(fetched, a.cache.block);
       k.offset = fetched - k.block * a.cache.block.divisor;
     }
     return k;
   }
-  k.valid = static_cast<uint32_t>(fetched) < a.cache.num_blocks;
+  const uint32_t local = local_token(l, j), page = fastdiv(local, a.cache.block);
+  k.valid = j < l.n && page < l.table_width && static_cast<uint32_t>(fetched) < a.cache.num_blocks;
   if (k.valid) {
-    const uint32_t local = local_token(l, j);
     k.block = fetched;
-    k.offset = local - fastdiv(local, a.cache.block) * a.cache.block.divisor;
+    k.offset = local - page * a.cache.block.divisor;
     k.position = static_cast<int32_t>(a.own.position(local));
   }
   return k;
