@@ -24,8 +24,9 @@
 // tile's largest u, P'_j = 2^(u_j - R + 5) goes to the tensor core and
 // 2^(log2 p_j - R) to the sum, so out = O / (32 l) and lse = (R + log2 l) ln 2
 // hold for any scales in [2^-100, 2^100]. R moves, and O and l are rescaled,
-// only when a tile's largest u leaves [R - 4, R + 3.5]: e4m3 ends at 448 =
-// 2^8.8. l, S and O are float32.
+// only when a tile's largest u leaves [R - 4, R + 3.5] (e4m3 ends at 448 =
+// 2^8.8): at once when it passes the upper end, within four tiles below the
+// lower. l, S and O are float32.
 //
 // A CTA is one or two pipelines, each a softmax of one key a thread and 16
 // columns a warpgroup, warps that gather keys and values with cp.async (the TMA
@@ -77,8 +78,8 @@ struct Config {
   static constexpr int kPipes = !kIsLatent && NH == 16 ? 2 : 1;
   static constexpr int kGroups = NH / 16;                        // softmax warpgroups, 16 columns each
   static constexpr int kSoftmax = kGroups * 128;
-  static constexpr int kLoaders = kPipes == 2 ? 2 : 4;           // gathering warps
-  static constexpr int kSplitters = kPipes == 2 ? 1 : 3;         // query warps
+  static constexpr int kLoaders = kPipes == 2 || NH == 64 ? 2 : 4;  // gathering warps
+  static constexpr int kSplitters = kPipes == 2 ? 1 : NH == 64 ? 5 : 3;  // query warps
   static constexpr int kPipeWarps = kGroups * 4 + kLoaders + kSplitters + 1;
   static_assert(kPipeWarps % 4 == 0, "a softmax warp's TMEM lanes go by its number in the CTA");
   static constexpr int kThreads = kPipes * kPipeWarps * 32;
@@ -124,7 +125,7 @@ struct Handed {
 template <typename C, int NH>
 struct __align__(16) Shared {
   int32_t best[3][NH];  // column maxima of a tile, as ordered integers
-  float reference[NH];  // the columns' references R
+  float reference[NH];  // 5 - R of the columns' references R
   float factor[2][NH];  // the columns' score factors, of this item and the next
   int32_t seen_to[2][C::kSeveral ? NH : 1], seen_from[2][C::kSeveral ? NH : 1];  // positions a column sees: below, from
   float k_scale[C::kStages][kTile];
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
   }
   if (tid < NH) {
     sh.best[0][tid] = ordered(-INFINITY);
-    sh.reference[tid] = 0.f;
+    sh.reference[tid] = 5.f;
   }
   S& first = *reinterpret_cast<S*>(all_smem + C::kOffMisc);
   if (pipe == 0 && warp == kMmaWarp) tmem_alloc(smem_addr(&first.tmem), C::kColumns);
@@ -415,14 +416,16 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           tmem_wait_ld(t);
           tmem_wait_ld(s1);
         }
+        // u = log2(p) + log2(vscale): where the key is masked, -inf.
+        const float scale = vs > 0.f ? fminf(fmaxf(vs, 0x1p-100f), 0x1p+100f) : vs == 0.f ? 0x1p-100f : vs;  // NaN stays
+        const float shift = valid ? __log2f(scale) : -INFINITY;
 #pragma unroll
         for (int c = 0; c < 16; c += 4) {
           const float4 f = *reinterpret_cast<const float4*>(&sh.factor[seq & 1][first_col + c]);
           const float fs[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float s = (t[c + k] + s1[c + k] * 0.0625f) * (ks * fs[k]);
-            t[c + k] = valid ? s : -INFINITY;
+            t[c + k] = fmaf(fmaf(s1[c + k], 0.0625f, t[c + k]), ks * fs[k], shift);
           }
         }
         if constexpr (C::kSeveral) {
@@ -439,75 +442,101 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
             }
           }
         }
-        // Largest u of each column: lane c of a warp has column c's.
-        const float scale = vs > 0.f ? fminf(fmaxf(vs, 0x1p-100f), 0x1p+100f) : vs;  // 0 and NaN stay
-        const float shift = __log2f(scale > 0.f ? scale : 0x1p-100f);
-        float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float m = warp_max(t[c] + shift);
-          if (own == c) top = m;
-        }
-        int32_t* best = sh.best[n3];
-        n3 = n3 == 2 ? 0 : n3 + 1;
-        if (lane < 16) {
-          atomicMax(&best[first_col + lane], ordered(top));
-          if ((warp & 3) == 0) sh.best[n3][first_col + lane] = ordered(-INFINITY);
-        }
-        named_barrier(group_barrier, 128);
-        top = unordered(best[first_col + own]);
-        const bool move = top > reference + 3.5f || (top < reference - 4.f && top > highest - 60.f);
+        // Weights x = 2^(u - R + 5). Every fourth tile, and any whose largest x
+        // passes 2^8.5, first finds its columns' largest u and moves the
+        // references that it left. (Each tile doing so cost 360 of 2100 cycles.)
         bool waited = i == 0;  // an item's end waits for its last outputs
-        if (__any_sync(kAllLanes, move)) {
-          const float to = move ? fmaxf(top, highest - 60.f) : reference;
-          const float by = !move ? 1.f : reference == -INFINITY ? 0.f : exp2_approx(reference - to);
-          reference = to;
-          highest = fmaxf(highest, to);
-          // The group's warps all write the same numbers: whoever reads them has
-          // written them, and nobody is still at the tile before.
-          if (lane < 16) sh.reference[first_col + lane] = to == -INFINITY ? 0.f : to;
-          __syncwarp();
-          if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
-          waited = true;
-          tc_fence_after();
-          float f[16];
+        bool look = (i & 3) == 0;
+        float w[16];
+        while (true) {
+          if (look) {
+            float top = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            f[c] = __shfl_sync(kAllLanes, by, c);
-            l[c] *= f[c];
-          }
-          if (i > 0) {
-#pragma unroll 1
-            for (int m = 0; m < C::kValues; ++m) {
-              const uint32_t at = tmem + lanes + m * NH + first_col;
-              float o[16];
-              tmem_ld16(at, o);
-              tmem_wait_ld(o);
-#pragma unroll
-              for (int c = 0; c < 16; ++c) o[c] *= f[c];
-              tmem_st16(at, o);
+            for (int c = 0; c < 16; ++c) {
+              const float m = warp_max(t[c]);  // lane c of a warp has column c's
+              if (own == c) top = m;
             }
-            tmem_wait_st();
+            int32_t* best = sh.best[n3];
+            n3 = n3 == 2 ? 0 : n3 + 1;
+            if (lane < 16) {
+              atomicMax(&best[first_col + lane], ordered(top));
+              if ((warp & 3) == 0) sh.best[n3][first_col + lane] = ordered(-INFINITY);
+            }
+            named_barrier(group_barrier, 128);
+            top = unordered(best[first_col + own]);
+            const bool move = top > reference + 3.5f || (top < reference - 4.f && top > highest - 60.f);
+            if (__any_sync(kAllLanes, move)) {
+              const float to = move ? fmaxf(top, highest - 60.f) : reference;
+              const float by = !move ? 1.f : reference == -INFINITY ? 0.f : exp2_approx(reference - to);
+              reference = to;
+              highest = fmaxf(highest, to);
+              // The group's warps all write the same numbers: whoever reads them has
+              // written them, and nobody is still at the tile before.
+              if (lane < 16) sh.reference[first_col + lane] = to == -INFINITY ? 0.f : 5.f - to;
+              __syncwarp();
+              if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
+              waited = true;
+              tc_fence_after();
+              float f[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                f[c] = __shfl_sync(kAllLanes, by, c);
+                l[c] *= f[c];
+              }
+              if (i > 0) {
+#pragma unroll 1
+                for (int m = 0; m < C::kValues; ++m) {
+                  const uint32_t at = tmem + lanes + m * NH + first_col;
+                  float o[16];
+                  tmem_ld16(at, o);
+                  tmem_wait_ld(o);
+#pragma unroll
+                  for (int c = 0; c < 16; ++c) o[c] *= f[c];
+                  tmem_st16(at, o);
+                }
+                tmem_wait_st();
+              }
+            }
           }
+          float largest = 0.f;
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) {
+            const float4 r = *reinterpret_cast<const float4*>(&sh.reference[first_col + c]);
+            const float rs[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              w[c + k] = exp2_approx(t[c + k] + rs[k]);
+              largest = fmaxf(largest, w[c + k]);
+            }
+          }
+          if (look) break;
+          look = named_barrier_or(group_barrier, 128, largest > 362.f);
+          if (!look) break;
         }
-        // Weights. The sum takes them in float32, the tensor core in T parts.
-        const float to_value = scale * 32.f;
+        // The sum takes the weights in float32, without the value's scale; the
+        // tensor core in T parts.
+        const float to_sum = scale == scale ? __fdividef(0.03125f, scale) : 1.f;  // a NaN comes with the weights that see it
+        const bool dead = vs == 0.f;  // values that count as 0, whatever their codes
         uint32_t part[4][T];
 #pragma unroll
         for (int c = 0; c < 16; c += 4) {
-          const float4 r = *reinterpret_cast<const float4*>(&sh.reference[first_col + c]);
-          const float rs[4] = {r.x, r.y, r.z, r.w};
-          float w[4];
+          float x[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float p = exp2_approx(t[c + k] - rs[k]);
-            l[c + k] += p;
-            w[k] = p * to_value;
+            l[c + k] = fmaf(w[c + k], to_sum, l[c + k]);
+            x[k] = w[c + k];
           }
           if constexpr (T == 2) {
-            split4_f16(w, part[c / 4]);
+            split4_f16(x, part[c / 4]);
           } else {
-            split4<T, true>(w, part[c / 4]);
+            split4<T, true>(x, part[c / 4]);
+          }
+        }
+        if (dead) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int p = 0; p < T; ++p) part[c][p] = 0;
           }
         }
         if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
@@ -823,7 +852,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           // The largest magnitude comes to [128, 256): its exponent field is taken off.
           const int e = max(static_cast<int>(most >> 23), 40);
           const bool odd = most >= 0x7f800000u;  // an infinity or NaN: the row becomes NaN
-          const float up = __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
+          const float up = odd ? 0.f : __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
           if (lane == 0) {
             sh.factor[seq & 1][c] = odd ? NAN : a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
             if constexpr (C::kSeveral) {
@@ -834,29 +863,27 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
                                              ? position + 1 - static_cast<int32_t>(a.window) : 0;
             }
           }
+          // A lane's four columns of piece i are bytes 4 lane on of chunk i; a
+          // part's rows lie NH rows behind the part before.
+          const uint32_t wide_at = base + C::kOffQ + c * 128 + ((((lane >> 2) ^ c) & 7) << 4) + (lane & 3) * 4;
+          const uint32_t narrow_at = base + C::kOffQ + c * 64 + ((((lane >> 2) ^ (c >> 1)) & 3) << 4) + (lane & 3) * 4;
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
-            const int d = (i * 32 + lane) * 4;
-            if (d < C::kKeyDim) {
-              float y[4];
-              unpack4<E>(now[n][i], y);
+            const bool narrow = C::kWide == 64 || (C::kIsLatent && i == 4);
+            if (narrow && lane >= 16) continue;
+            float y[4];
+            unpack4<E>(now[n][i], y);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) y[k] = odd ? 0.f : y[k] * up;
-              uint32_t part[T];
-              if constexpr (T == 2) {
-                split_query4(y, part);
-              } else {
-                split4<T, false>(y, part);
-              }
-              const int chunk = d / 128, in = d & 127;
-              const bool narrow = C::kWide == 64 || (C::kIsLatent && chunk == 4);
+            for (int k = 0; k < 4; ++k) y[k] *= up;
+            uint32_t part[T];
+            if constexpr (T == 2) {
+              split_query4(y, part);
+            } else {
+              split4<T, false>(y, part);
+            }
 #pragma unroll
-              for (int t = 0; t < T; ++t) {
-                const int row = t * NH + c;
-                const uint32_t at = narrow ? row * 64 + ((((in >> 4) ^ (row >> 1)) & 3) << 4) + (in & 15)
-                                           : row * 128 + ((((in >> 4) ^ row) & 7) << 4) + (in & 15);
-                st_shared(base + C::kOffQ + chunk * (T * NH * 128) + at, part[t]);
-              }
+            for (int t = 0; t < T; ++t) {
+              st_shared((narrow ? narrow_at + t * (NH * 64) : wide_at + t * (NH * 128)) + i * (T * NH * 128), part[t]);
             }
           }
         }

@@ -193,7 +193,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // The largest of a warp's values, NaN left aside.
 __device__ __forceinline__ float warp_max(float x) {
   float y;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
 // Pairs: the first argument goes into the low half.

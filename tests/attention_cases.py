@@ -43,14 +43,14 @@ def score_error(q, k_cache, k_scale, softmax_scale):
 def assert_attention(out, lse, want, q, k_cache, k_scale, softmax_scale):
     """out within half a step of the output's type, plus what the weights' errors make.
 
-    A weight enters the product as x = 2^(u - R + 5), with the tile's largest x
-    in [2, 2^8.5], in parts of 8 bits. A first e4m3 part leaves at most
+    A weight enters the product as x = 2^(u - R + 5), with the largest x of its
+    tile, or of one of the four before, in [2, 2^8.5], in parts of 8 bits. A first e4m3 part leaves at most
     max(2^-4 2^e, 2^-10) for x in [2^e, 2^(e + 1)); an e5m2 part leaves of a
     remainder r at most half a step of r's binade, which is 2^-3 of the
     binade's start, or 2^-17 below 2^-14. So two parts (bf16) leave at most
     max(2^-8 x, 2^-14), with 2^-11 x more from their way through fp16, and
     three (fp16) max(2^-12 x, 2^-17): relative errors of 2^-8 + 2^-11 and 2^-12
-    in each weight, and 2^-15 and 2^-18 of the largest weight of its tile. The
+    in each weight, and 2^-15 and 2^-18 of the largest weight of that tile. The
     score's own error counts twice, in the weight and in the sum."""
     ref_out, ref_lse, spread, near = want
     u = HALF_STEP[out.dtype]
