@@ -73,9 +73,9 @@ def attend_row(q, slot, k_cache, v_cache, k_scale, v_scale, softmax_scale):
     ``spread`` (heads, value_dim) is the weighted mean of the values'
     magnitudes: an error of relative size u in each weight moves ``out`` by at
     most ``u * spread``. ``near`` is the same with each weight replaced by the
-    largest among its neighbours, up to 639 places away: an error of u times
-    the largest weight of some run of 128 that begins at most 512 places before
-    a weight's own moves ``out`` by at most ``u * near``."""
+    largest among its neighbours, up to 127 places away: an error of u times
+    the largest weight of a weight's run of 128 moves ``out`` by at most
+    ``u * near``."""
     heads, kv_heads = q.shape[0], k_cache.shape[2]
     value_dim = 512 if v_cache is None else v_cache.shape[3]
     if slot.numel() == 0:
@@ -91,7 +91,7 @@ def attend_row(q, slot, k_cache, v_cache, k_scale, v_scale, softmax_scale):
     weight = torch.exp(score - lse[..., None])
     out = torch.einsum("hgn,nhd->hgd", weight, v)
     spread = torch.einsum("hgn,nhd->hgd", weight, v.abs())
-    around = torch.nn.functional.max_pool1d(weight, 1279, stride=1, padding=639)
+    around = torch.nn.functional.max_pool1d(weight, 255, stride=1, padding=127)
     near = torch.einsum("hgn,nhd->hgd", around, v.abs())
     return out.reshape(heads, value_dim), lse.reshape(heads), spread.reshape(heads, value_dim), near.reshape(heads, value_dim)
 

@@ -24,9 +24,8 @@
 // tile's largest u, P'_j = 2^(u_j - R + 5) goes to the tensor core and
 // 2^(log2 p_j - R) to the sum, so out = O / (32 l) and lse = (R + log2 l) ln 2
 // hold for any scales in [2^-100, 2^100]. R moves, and O and l are rescaled,
-// only when a tile's largest u leaves [R - 4, R + 3.5] (e4m3 ends at 448 =
-// 2^8.8): at once when it passes the upper end, within four tiles below the
-// lower. l, S and O are float32.
+// only when a tile's largest u leaves [R - 4, R + 3.5]: e4m3 ends at 448 =
+// 2^8.8. l, S and O are float32.
 //
 // A CTA is one or two pipelines, each a softmax of one key a thread and 16
 // columns a warpgroup, warps that gather keys and values with cp.async (the TMA
@@ -133,6 +132,8 @@ struct __align__(16) Shared {
   int32_t position[C::kSeveral ? C::kStages : 1][C::kSeveral ? kTile : 1];
   uint32_t valid[C::kStages][4];  // a bit for each key
   Handed handed[2];
+  Handed last;          // the split item, as soon as it is known
+  int32_t last_known;
   uint64_t full[C::kLoadChunks][C::kStages], empty[C::kLoadChunks][C::kStages];
   uint64_t scores[2], weights, done;
   uint64_t queries[2], queries_read, finished[2];
@@ -341,8 +342,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     mbar_init(smem_addr(&sh.queries_read), 1);
     mbar_init(smem_addr(&sh.drained), 1);
     sh.abort = 0;
-    sh.handed[0].split = 0;
-    sh.handed[1].split = 0;
+    sh.last_known = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
@@ -442,89 +442,69 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
             }
           }
         }
-        // Weights x = 2^(u - R + 5). Every fourth tile, and any whose largest x
-        // passes 2^8.5, first finds its columns' largest u and moves the
-        // references that it left. (Each tile doing so cost 360 of 2100 cycles.)
-        bool waited = i == 0;  // an item's end waits for its last outputs
-        bool look = (i & 3) == 0;
-        float w[16];
-        while (true) {
-          if (look) {
-            float top = -INFINITY;
+        // Largest u of each column: lane c of a warp has column c's.
+        float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float m = warp_max(t[c]);  // lane c of a warp has column c's
-              if (own == c) top = m;
-            }
-            int32_t* best = sh.best[n3];
-            n3 = n3 == 2 ? 0 : n3 + 1;
-            if (lane < 16) {
-              atomicMax(&best[first_col + lane], ordered(top));
-              if ((warp & 3) == 0) sh.best[n3][first_col + lane] = ordered(-INFINITY);
-            }
-            named_barrier(group_barrier, 128);
-            top = unordered(best[first_col + own]);
-            const bool move = top > reference + 3.5f || (top < reference - 4.f && top > highest - 60.f);
-            if (__any_sync(kAllLanes, move)) {
-              const float to = move ? fmaxf(top, highest - 60.f) : reference;
-              const float by = !move ? 1.f : reference == -INFINITY ? 0.f : exp2_approx(reference - to);
-              reference = to;
-              highest = fmaxf(highest, to);
-              // The group's warps all write the same numbers: whoever reads them has
-              // written them, and nobody is still at the tile before.
-              if (lane < 16) sh.reference[first_col + lane] = to == -INFINITY ? 0.f : 5.f - to;
-              __syncwarp();
-              if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
-              waited = true;
-              tc_fence_after();
-              float f[16];
-#pragma unroll
-              for (int c = 0; c < 16; ++c) {
-                f[c] = __shfl_sync(kAllLanes, by, c);
-                l[c] *= f[c];
-              }
-              if (i > 0) {
-#pragma unroll 1
-                for (int m = 0; m < C::kValues; ++m) {
-                  const uint32_t at = tmem + lanes + m * NH + first_col;
-                  float o[16];
-                  tmem_ld16(at, o);
-                  tmem_wait_ld(o);
-#pragma unroll
-                  for (int c = 0; c < 16; ++c) o[c] *= f[c];
-                  tmem_st16(at, o);
-                }
-                tmem_wait_st();
-              }
-            }
-          }
-          float largest = 0.f;
-#pragma unroll
-          for (int c = 0; c < 16; c += 4) {
-            const float4 r = *reinterpret_cast<const float4*>(&sh.reference[first_col + c]);
-            const float rs[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              w[c + k] = exp2_approx(t[c + k] + rs[k]);
-              largest = fmaxf(largest, w[c + k]);
-            }
-          }
-          if (look) break;
-          look = named_barrier_or(group_barrier, 128, largest > 362.f);
-          if (!look) break;
+        for (int c = 0; c < 16; ++c) {
+          const float m = warp_max(t[c]);
+          if (own == c) top = m;
         }
-        // The sum takes the weights in float32, without the value's scale; the
-        // tensor core in T parts.
+        int32_t* best = sh.best[n3];
+        n3 = n3 == 2 ? 0 : n3 + 1;
+        if (lane < 16) {
+          atomicMax(&best[first_col + lane], ordered(top));
+          if ((warp & 3) == 0) sh.best[n3][first_col + lane] = ordered(-INFINITY);
+        }
+        named_barrier(group_barrier, 128);
+        top = unordered(best[first_col + own]);
+        const bool move = top > reference + 3.5f || (top < reference - 4.f && top > highest - 60.f);
+        bool waited = i == 0;  // an item's end waits for its last outputs
+        if (__any_sync(kAllLanes, move)) {
+          const float to = move ? fmaxf(top, highest - 60.f) : reference;
+          const float by = !move ? 1.f : reference == -INFINITY ? 0.f : exp2_approx(reference - to);
+          reference = to;
+          highest = fmaxf(highest, to);
+          // The group's warps all write the same numbers: whoever reads them has
+          // written them, and nobody is still at the tile before.
+          if (lane < 16) sh.reference[first_col + lane] = to == -INFINITY ? 0.f : 5.f - to;
+          __syncwarp();
+          if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
+          waited = true;
+          tc_fence_after();
+          float f[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            f[c] = __shfl_sync(kAllLanes, by, c);
+            l[c] *= f[c];
+          }
+          if (i > 0) {
+#pragma unroll 1
+            for (int m = 0; m < C::kValues; ++m) {
+              const uint32_t at = tmem + lanes + m * NH + first_col;
+              float o[16];
+              tmem_ld16(at, o);
+              tmem_wait_ld(o);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) o[c] *= f[c];
+              tmem_st16(at, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        // Weights x = 2^(u - R + 5). The sum takes them in float32, without the
+        // value's scale; the tensor core in T parts.
         const float to_sum = scale == scale ? __fdividef(0.03125f, scale) : 1.f;  // a NaN comes with the weights that see it
         const bool dead = vs == 0.f;  // values that count as 0, whatever their codes
         uint32_t part[4][T];
 #pragma unroll
         for (int c = 0; c < 16; c += 4) {
+          const float4 r = *reinterpret_cast<const float4*>(&sh.reference[first_col + c]);
+          const float rs[4] = {r.x, r.y, r.z, r.w};
           float x[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            l[c + k] = fmaf(w[c + k], to_sum, l[c + k]);
-            x[k] = w[c + k];
+            x[k] = exp2_approx(t[c + k] + rs[k]);
+            l[c + k] = fmaf(x[k], to_sum, l[c + k]);
           }
           if constexpr (T == 2) {
             split4_f16(x, part[c / 4]);
@@ -666,7 +646,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       }
       const uint32_t k_first = work.kv * a.cache.k_head_rows, v_first = work.kv * a.cache.v_head_rows;
       const int32_t mine = work.begin * kTile + w * kShare + lane;
-      int32_t fetched[kOwn];
+      int32_t fetched[kOwn];  // slots or table entries, a tile ahead
 #pragma unroll
       for (int o = 0; o < kOwn; ++o) fetched[o] = work.steps > 0 ? fetch_key(a, work.keys, mine + o * 32) : -1;
       for (int32_t i = 0; i < work.steps; ++i) {
@@ -677,7 +657,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           const int32_t j = mine + i * kTile + o * 32;
           const Key key = locate_key(a, work.keys, j, fetched[o]);
           bad |= bad_key(work.keys, j, fetched[o], key);
-          fetched[o] = i + 1 < work.steps ? fetch_key(a, work.keys, j + kTile) : -1;
+          fetched[o] = fetch_key(a, work.keys, j + kTile);
           page[o] = key.block;
           position[o] = key.position;
           k_row[o] = key.valid ? static_cast<int32_t>(k_first + key.block * a.cache.k_block_rows + key.offset * a.cache.k_token_rows) : -1;
@@ -778,23 +758,28 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       } else if (has_split && !shared) {
         work = find_work(a, plan, split_unit, rank, ranks);
         shared = true;
+        if (w == 0 && lane == 0) {
+          sh.last = Handed{work.span.row, work.span.count, work.span.position, work.kv, work.block, work.steps,
+                           work.tiles > 0 ? 1 : 0};
+          sh.last_known = 1;
+        }
       } else {
         end = true;
       }
       constexpr int kPieces = (C::kKeyDim / 4 + 31) / 32;
-      constexpr int kBatch = 2;
+      constexpr int kBatch = 4;  // columns whose loads overlap
       uint2 raw[kBatch][kPieces];
       auto bring = [&](int c0) {
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
           const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, c0 + n);
-          const E* q = static_cast<const E*>(a.q) + static_cast<int64_t>(work.span.row + col.query) * a.q_row +
-                       static_cast<int64_t>(col.head) * a.q_head;
+          const int64_t at = col.used ? static_cast<int64_t>(work.span.row + col.query) * a.q_row +
+                                            static_cast<int64_t>(col.head) * a.q_head : 0;
+          const E* q = static_cast<const E*>(a.q) + at + lane * 4;
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
-            const int d = (i * 32 + lane) * 4;
             raw[n][i] = make_uint2(0u, 0u);
-            if (col.used && c0 + n < NH && d < C::kKeyDim) raw[n][i] = *reinterpret_cast<const uint2*>(q + d);
+            if (col.used && (i * 32 + lane) * 4 < C::kKeyDim) raw[n][i] = ld_global_v2(q + i * 128);
           }
         }
       };
@@ -812,14 +797,17 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           }
           continue;
         }
-        bring(w * kBatch);
-        for (int e = (w * 32 + lane) * 64; e < NH * C::kKeyDim; e += C::kSplitters * 32 * 64) {
-          const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, e / C::kKeyDim);
-          if (col.used) {
-            prefetch_l2_line(static_cast<const E*>(a.q) + static_cast<int64_t>(work.span.row + col.query) * a.q_row +
-                             static_cast<int64_t>(col.head) * a.q_head + e % C::kKeyDim);
-          }
+        // Towards L2, while the item before still needs the buffer (unused
+        // columns: the first row, so that the lanes stay together).
+        for (int e = w * 32; e < NH * C::kKeyDim / 64; e += C::kSplitters * 32) {
+          const int first = min(e + lane, NH * C::kKeyDim / 64 - 1) * 64;
+          const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, first / C::kKeyDim);
+          const int64_t at = col.used ? static_cast<int64_t>(work.span.row + col.query) * a.q_row +
+                                            static_cast<int64_t>(col.head) * a.q_head + first % C::kKeyDim : 0;
+          prefetch_l2_line(static_cast<const E*>(a.q) + at);
         }
+        __syncwarp();
+        bring(w * kBatch);
       }
       if (seq > 0) warp_wait(&sh.queries_read, (seq - 1) & 1, abort);
       if (seq > 1) warp_wait(&sh.finished[seq & 1], ((seq >> 1) - 1) & 1, abort);
@@ -835,13 +823,16 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
                                     split ? 1 : 0};
       }
       for (int c0 = w * kBatch; c0 < NH; c0 += C::kSplitters * kBatch) {
+        // The next batch comes during this one, where registers allow it.
+        constexpr bool kEarly = !C::kIsLatent;
+        if (!kEarly && c0 != w * kBatch) bring(c0);
         uint2 now[kBatch][kPieces];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) now[n][i] = raw[n][i];
         }
-        if (c0 + C::kSplitters * kBatch < NH) bring(c0 + C::kSplitters * kBatch);  // the next columns' loads
+        if (kEarly && c0 + C::kSplitters * kBatch < NH) bring(c0 + C::kSplitters * kBatch);
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
           const int c = c0 + n;
@@ -863,6 +854,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
                                              ? position + 1 - static_cast<int32_t>(a.window) : 0;
             }
           }
+          __syncwarp();
           // A lane's four columns of piece i are bytes 4 lane on of chunk i; a
           // part's rows lie NH rows behind the part before.
           const uint32_t wide_at = base + C::kOffQ + c * 128 + ((((lane >> 2) ^ c) & 7) << 4) + (lane & 3) * 4;
@@ -870,7 +862,6 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
             const bool narrow = C::kWide == 64 || (C::kIsLatent && i == 4);
-            if (narrow && lane >= 16) continue;
             float y[4];
             unpack4<E>(now[n][i], y);
 #pragma unroll
@@ -881,9 +872,11 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
             } else {
               split4<T, false>(y, part);
             }
+            if (!narrow || lane < 16) {
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-              st_shared((narrow ? narrow_at + t * (NH * 64) : wide_at + t * (NH * 128)) + i * (T * NH * 128), part[t]);
+              for (int t = 0; t < T; ++t) {
+                st_shared((narrow ? narrow_at + t * (NH * 64) : wide_at + t * (NH * 128)) + i * (T * NH * 128), part[t]);
+              }
             }
           }
         }
@@ -917,75 +910,80 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       if (__any_sync(kAllLanes, *abort != 0)) break;
       const int32_t steps = __shfl_sync(kAllLanes, sh.handed[seq & 1].steps, 0);
       more = steps >= 0 && __shfl_sync(kAllLanes, sh.handed[seq & 1].split, 0) == 0;
-      for (int32_t i = 0; steps > 0 && i <= steps; ++i) {
-        if (i < steps) {  // scores of tile i
-          const uint32_t d = tmem + C::kValues * NH + ((n + i) & 1) * (T * NH);
+      auto scores = [&](int32_t i) {
+        const uint32_t d = tmem + C::kValues * NH + ((n + i) & 1) * (T * NH);
 #pragma unroll
-          for (int c = 0; c < C::kMainKeys; ++c) {
-            warp_wait(&sh.full[c][sb], st, abort);
-            fence_proxy_async();  // the copies wrote through the generic proxy
-            if (leader) {
-              const uint64_t kd = k_desc + ((sb * C::kStageBytes + c * C::kChunkBytes) >> 4);
-              const uint64_t qd = q_desc + ((c * (T * NH * C::kWide)) >> 4);
-#pragma unroll
-              for (int k = 0; k < C::kWide / 32; ++k) mma_f8(d, kd + 2 * k, qd + 2 * k, kScoreDesc, c + k > 0);
-            }
-            __syncwarp();
-          }
-          if constexpr (C::kIsLatent) {
-            const uint32_t tb = C::kTails == 1 ? 0 : sb, tt = C::kTails == 1 ? tail_turn : st;
-            tail_turn ^= 1;
-            warp_wait(&sh.full[4][tb], tt, abort);
-            fence_proxy_async();
-            if (leader) {
-              const uint64_t kd = smem_descriptor(base + C::kOffTail + tb * C::kTailBytes, 16, 512, kSwizzle64);
-              const uint64_t qd = smem_descriptor(base + C::kOffQ + 4 * (T * NH * 128), 16, 512, kSwizzle64);
-              mma_f8(d, kd, qd, kScoreDesc, true);
-              mma_f8(d, kd + 2, qd + 2, kScoreDesc, true);
-              mma_commit(smem_addr(&sh.empty[4][tb]));
-            }
-          } else if (leader) {
-            mma_commit(smem_addr(&sh.empty[0][sb]));
-          }
+        for (int c = 0; c < C::kMainKeys; ++c) {
+          warp_wait(&sh.full[c][sb], st, abort);
+          fence_proxy_async();  // the copies wrote through the generic proxy
           if (leader) {
-            mma_commit(smem_addr(&sh.scores[(n + i) & 1]));
-            if (i + 1 == steps) mma_commit(smem_addr(&sh.queries_read));
+            const uint64_t kd = k_desc + ((sb * C::kStageBytes + c * C::kChunkBytes) >> 4);
+            const uint64_t qd = q_desc + ((c * (T * NH * C::kWide)) >> 4);
+#pragma unroll
+            for (int k = 0; k < C::kWide / 32; ++k) mma_f8(d, kd + 2 * k, qd + 2 * k, kScoreDesc, c + k > 0);
           }
           __syncwarp();
-          if (++sb == C::kStages) {
-            sb = 0;
-            st ^= 1;
-          }
         }
-        if (i > 0) {  // outputs of tile i - 1
-          warp_wait(&sh.weights, (n + i - 1) & 1, abort);
-          tc_fence_after();
-          if constexpr (!C::kIsLatent) {
-            warp_wait(&sh.full[1][ob], ot, abort);
-            fence_proxy_async();
-          }
+        if constexpr (C::kIsLatent) {
+          const uint32_t tb = C::kTails == 1 ? 0 : sb, tt = C::kTails == 1 ? tail_turn : st;
+          tail_turn ^= 1;
+          warp_wait(&sh.full[4][tb], tt, abort);
+          fence_proxy_async();
           if (leader) {
+            const uint64_t kd = smem_descriptor(base + C::kOffTail + tb * C::kTailBytes, 16, 512, kSwizzle64);
+            const uint64_t qd = smem_descriptor(base + C::kOffQ + 4 * (T * NH * 128), 16, 512, kSwizzle64);
+            mma_f8(d, kd, qd, kScoreDesc, true);
+            mma_f8(d, kd + 2, qd + 2, kScoreDesc, true);
+            mma_commit(smem_addr(&sh.empty[4][tb]));
+          }
+        } else if (leader) {
+          mma_commit(smem_addr(&sh.empty[0][sb]));
+        }
+        if (leader) {
+          mma_commit(smem_addr(&sh.scores[(n + i) & 1]));
+          if (i + 1 == steps) mma_commit(smem_addr(&sh.queries_read));
+        }
+        __syncwarp();
+        if (++sb == C::kStages) {
+          sb = 0;
+          st ^= 1;
+        }
+      };
+      auto outputs = [&](int32_t i) {
+        warp_wait(&sh.weights, (n + i) & 1, abort);
+        tc_fence_after();
+        if constexpr (!C::kIsLatent) {
+          warp_wait(&sh.full[1][ob], ot, abort);
+          fence_proxy_async();
+        }
+        if (leader) {
 #pragma unroll
-            for (int c = 0; c < C::kValues; ++c) {
-              const uint64_t vd = v_desc + ((ob * C::kStageBytes + c * C::kChunkBytes) >> 4);
+          for (int c = 0; c < C::kValues; ++c) {
+            const uint64_t vd = v_desc + ((ob * C::kStageBytes + c * C::kChunkBytes) >> 4);
 #pragma unroll
-              for (int p = 0; p < T; ++p) {
+            for (int p = 0; p < T; ++p) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  mma_f8(tmem + c * NH, vd + 2 * C::kWide * k, p_desc + ((p * (NH * kTile) + k * 32 * NH) >> 4),
-                         p == 0 ? kFirstDesc : kOtherDesc, p + k > 0 || i > 1);
-                }
+              for (int k = 0; k < 4; ++k) {
+                mma_f8(tmem + c * NH, vd + 2 * C::kWide * k, p_desc + ((p * (NH * kTile) + k * 32 * NH) >> 4),
+                       p == 0 ? kFirstDesc : kOtherDesc, p + k > 0 || i > 0);
               }
-              mma_commit(smem_addr(&sh.empty[C::kIsLatent ? c : 1][ob]));
             }
-            mma_commit(smem_addr(&sh.done));
+            mma_commit(smem_addr(&sh.empty[C::kIsLatent ? c : 1][ob]));
           }
-          __syncwarp();
-          if (++ob == C::kStages) {
-            ob = 0;
-            ot ^= 1;
-          }
+          mma_commit(smem_addr(&sh.done));
         }
+        __syncwarp();
+        if (++ob == C::kStages) {
+          ob = 0;
+          ot ^= 1;
+        }
+      };
+      // Scores run a tile ahead of the outputs, so that a softmax overlaps the
+      // next tile's scores.
+#pragma unroll 1
+      for (int32_t i = 0; i <= steps && steps > 0; ++i) {
+        if (i < steps) scores(i);
+        if (i > 0) outputs(i - 1);
       }
       if (steps > 0) n += steps;
     }
@@ -1003,8 +1001,17 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
 
   __syncthreads();
   // ---- a split item: its ranks, which all see the same tiles, join
-  const Work last = has_split ? find_work(a, plan, split_unit, rank, ranks) : Work{};
-  if (has_split && last.tiles > 0) {
+  Handed last{};
+  if (has_split) {
+    if (sh.last_known != 0) {
+      last = sh.last;
+    } else {  // the query warps gave up before it
+      const Work work = find_work(a, plan, split_unit, rank, ranks);
+      last = Handed{work.span.row, work.span.count, work.span.position, work.kv, work.block, work.steps, work.tiles > 0 ? 1 : 0};
+    }
+  }
+  if (last.split) {
+    constexpr int kMostRanks = 16;
     float* joint = reinterpret_cast<float*>(smem + C::kOffP) + 8 * NH;  // references, then sums
     float* joined = reinterpret_cast<float*>(smem);                     // outputs
     const int first_col = (warp >> 2) * 16, own = lane & 15;
@@ -1020,33 +1027,47 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     };
     if (warp < kLoadWarp) {
       const float* at = joint + first_col + own;
+      float rr[kMostRanks], ll[kMostRanks];
+#pragma unroll
+      for (uint32_t r = 0; r < kMostRanks; ++r) {
+        rr[r] = -INFINITY;
+        ll[r] = 0.f;
+        if (r < ranks) {
+          rr[r] = ld_cluster(place(at, r), r / C::kPipes);
+          ll[r] = ld_cluster(place(at + NH, r), r / C::kPipes);
+        }
+      }
       float whole_r = -INFINITY, whole_l = 0.f;
-      for (uint32_t r = 0; r < ranks; ++r) whole_r = fmaxf(whole_r, ld_cluster(place(at, r), r / C::kPipes));
-      for (uint32_t r = 0; r < ranks; ++r) {
-        const float rr = ld_cluster(place(at, r), r / C::kPipes);
-        whole_l += rr == -INFINITY ? 0.f : ld_cluster(place(at + NH, r), r / C::kPipes) * exp2_approx(rr - whole_r);
+#pragma unroll
+      for (uint32_t r = 0; r < kMostRanks; ++r) whole_r = fmaxf(whole_r, rr[r]);
+#pragma unroll
+      for (uint32_t r = 0; r < kMostRanks; ++r) {
+        if (rr[r] != -INFINITY) whole_l += ll[r] * exp2_approx(rr[r] - whole_r);
       }
       const float inverse = whole_l == 0.f ? 0.f : 1.f / (32.f * whole_l);
       const float by = reference == -INFINITY ? 0.f : exp2_approx(reference - whole_r) * inverse;
       if (rank == 0 && (warp & 3) == 0 && lane < 16 && *abort == 0) {
-        const Column col = find_column<NH>(a, plan, last.span.count, last.kv, last.block, first_col + lane);
+        const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, first_col + lane);
         if (col.used) {
-          a.lse[static_cast<int64_t>(last.span.row + col.query) * a.heads + col.head] =
+          a.lse[static_cast<int64_t>(last.row + col.query) * a.heads + col.head] =
               whole_l == 0.f ? -INFINITY : (whole_r + log2f(whole_l)) * 0.69314718055994531f;
         }
       }
       __syncwarp();
       tc_fence_after();
-      if (last.steps > 0 && (SHAPE != kDim64 || (warp & 3) < 2)) {
+      if (SHAPE != kDim64 || (warp & 3) < 2) {
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
 #pragma unroll 1
         for (int m = 0; m < C::kValues; ++m) {
           float o[16];
-          tmem_ld16(tmem + lanes + m * NH + first_col, o);
-          tmem_wait_ld(o);
+          if (last.steps > 0) {
+            tmem_ld16(tmem + lanes + m * NH + first_col, o);
+            tmem_wait_ld(o);
+          }
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
-            joined[(first_col + c) * C::kValueDim + m * 128 + (tid & 127)] = o[c] * __shfl_sync(kAllLanes, by, c);
+            const float f = __shfl_sync(kAllLanes, by, c);
+            joined[(first_col + c) * C::kValueDim + m * 128 + (tid & 127)] = last.steps > 0 ? o[c] * f : 0.f;
           }
         }
       }
@@ -1056,18 +1077,25 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     for (int32_t e = (static_cast<int32_t>(rank) * kRankThreads + tid) * 4; e < NH * C::kValueDim;
          e += static_cast<int32_t>(ranks) * kRankThreads * 4) {
       const int32_t c = e / C::kValueDim, d = e - c * C::kValueDim;
-      const Column col = find_column<NH>(a, plan, last.span.count, last.kv, last.block, c);
+      const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, c);
       if (!col.used) continue;
       float4 y{0.f, 0.f, 0.f, 0.f};
-      for (uint32_t r = 0; r < ranks; ++r) {
-        if (ld_cluster(place(joint + c, r), r / C::kPipes) == -INFINITY) continue;  // rank r saw nothing
-        const float4 x = ld_cluster4(place(joined + e, r), r / C::kPipes);
-        y.x += x.x;
-        y.y += x.y;
-        y.z += x.z;
-        y.w += x.w;
+      for (uint32_t r0 = 0; r0 < ranks; r0 += 4) {
+        float4 x[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+          x[k] = float4{0.f, 0.f, 0.f, 0.f};
+          if (r0 + k < ranks) x[k] = ld_cluster4(place(joined + e, r0 + k), (r0 + k) / C::kPipes);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+          y.x += x[k].x;
+          y.y += x[k].y;
+          y.z += x[k].z;
+          y.w += x[k].w;
+        }
       }
-      E* out = static_cast<E*>(a.out) + static_cast<int64_t>(last.span.row + col.query) * a.out_row +
+      E* out = static_cast<E*>(a.out) + static_cast<int64_t>(last.row + col.query) * a.out_row +
                static_cast<int64_t>(col.head) * a.out_head + d;
       if (*abort == 0) {
         out[0] = static_cast<E>(y.x);

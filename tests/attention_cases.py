@@ -43,8 +43,8 @@ def score_error(q, k_cache, k_scale, softmax_scale):
 def assert_attention(out, lse, want, q, k_cache, k_scale, softmax_scale):
     """out within half a step of the output's type, plus what the weights' errors make.
 
-    A weight enters the product as x = 2^(u - R + 5), with the largest x of its
-    tile, or of one of the four before, in [2, 2^8.5], in parts of 8 bits. A first e4m3 part leaves at most
+    A weight enters the product as x = 2^(u - R + 5), with the tile's largest x
+    in [2, 2^8.5], in parts of 8 bits. A first e4m3 part leaves at most
     max(2^-4 2^e, 2^-10) for x in [2^e, 2^(e + 1)); an e5m2 part leaves of a
     remainder r at most half a step of r's binade, which is 2^-3 of the
     binade's start, or 2^-17 below 2^-14. So two parts (bf16) leave at most
