@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         end = true;
       }
       constexpr int kPieces = (C::kKeyDim / 4 + 31) / 32;
-      constexpr int kBatch = 4;  // columns whose loads overlap
+      constexpr int kBatch = 2;  // columns whose loads overlap
       uint2 raw[kBatch][kPieces];
       auto bring = [&](int c0) {
 #pragma unroll
@@ -823,16 +823,13 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
                                     split ? 1 : 0};
       }
       for (int c0 = w * kBatch; c0 < NH; c0 += C::kSplitters * kBatch) {
-        // The next batch comes during this one, where registers allow it.
-        constexpr bool kEarly = !C::kIsLatent;
-        if (!kEarly && c0 != w * kBatch) bring(c0);
         uint2 now[kBatch][kPieces];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) now[n][i] = raw[n][i];
         }
-        if (kEarly && c0 + C::kSplitters * kBatch < NH) bring(c0 + C::kSplitters * kBatch);
+        if (c0 + C::kSplitters * kBatch < NH) bring(c0 + C::kSplitters * kBatch);  // the next ones come during these
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
           const int c = c0 + n;
@@ -1012,8 +1009,9 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
   }
   if (last.split) {
     constexpr int kMostRanks = 16;
+    const uint32_t share = NH / ranks;  // both are powers of two, ranks at most 16
     float* joint = reinterpret_cast<float*>(smem + C::kOffP) + 8 * NH;  // references, then sums
-    float* joined = reinterpret_cast<float*>(smem);                     // outputs
+    float* joined = reinterpret_cast<float*>(smem);                     // outputs: (rank, column of this rank, value)
     const int first_col = (warp >> 2) * 16, own = lane & 15;
     if (warp < kLoadWarp && (warp & 3) == 0 && lane < 16) {
       joint[first_col + lane] = reference;
@@ -1055,11 +1053,15 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       }
       __syncwarp();
       tc_fence_after();
+      // Rank r joins the columns [r, r + 1) * share, and gets every rank's part
+      // of them: stores need no answer, loads would wait for one.
       if (SHAPE != kDim64 || (warp & 3) < 2) {
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
 #pragma unroll 1
         for (int m = 0; m < C::kValues; ++m) {
           float o[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) o[c] = 0.f;
           if (last.steps > 0) {
             tmem_ld16(tmem + lanes + m * NH + first_col, o);
             tmem_wait_ld(o);
@@ -1067,44 +1069,34 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             const float f = __shfl_sync(kAllLanes, by, c);
-            joined[(first_col + c) * C::kValueDim + m * 128 + (tid & 127)] = last.steps > 0 ? o[c] * f : 0.f;
+            const uint32_t to = (first_col + c) / share, col = (first_col + c) % share;
+            st_cluster(place(joined + (rank * share + col) * C::kValueDim + m * 128 + (tid & 127), to), to / C::kPipes,
+                       last.steps > 0 ? o[c] * f : 0.f);
           }
         }
       }
     }
-    cluster_sync();
+    cluster_sync();  // the last time that a CTA touches another's memory is before
     constexpr int kRankThreads = C::kPipeWarps * 32;
-    for (int32_t e = (static_cast<int32_t>(rank) * kRankThreads + tid) * 4; e < NH * C::kValueDim;
-         e += static_cast<int32_t>(ranks) * kRankThreads * 4) {
+    for (int32_t e = tid * 4; e < static_cast<int32_t>(share) * C::kValueDim; e += kRankThreads * 4) {
       const int32_t c = e / C::kValueDim, d = e - c * C::kValueDim;
-      const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, c);
-      if (!col.used) continue;
+      const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, rank * share + c);
+      if (!col.used || *abort != 0) continue;
       float4 y{0.f, 0.f, 0.f, 0.f};
-      for (uint32_t r0 = 0; r0 < ranks; r0 += 4) {
-        float4 x[4];
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-          x[k] = float4{0.f, 0.f, 0.f, 0.f};
-          if (r0 + k < ranks) x[k] = ld_cluster4(place(joined + e, r0 + k), (r0 + k) / C::kPipes);
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-          y.x += x[k].x;
-          y.y += x[k].y;
-          y.z += x[k].z;
-          y.w += x[k].w;
-        }
+      for (uint32_t r = 0; r < ranks; ++r) {
+        const float4 x = *reinterpret_cast<const float4*>(joined + r * share * C::kValueDim + e);
+        y.x += x.x;
+        y.y += x.y;
+        y.z += x.z;
+        y.w += x.w;
       }
       E* out = static_cast<E*>(a.out) + static_cast<int64_t>(last.row + col.query) * a.out_row +
                static_cast<int64_t>(col.head) * a.out_head + d;
-      if (*abort == 0) {
-        out[0] = static_cast<E>(y.x);
-        out[1] = static_cast<E>(y.y);
-        out[2] = static_cast<E>(y.z);
-        out[3] = static_cast<E>(y.w);
-      }
+      out[0] = static_cast<E>(y.x);
+      out[1] = static_cast<E>(y.y);
+      out[2] = static_cast<E>(y.z);
+      out[3] = static_cast<E>(y.w);
     }
-    cluster_sync();  // nobody's shared memory goes before it was read
     tc_fence_before();
     __syncthreads();
   }

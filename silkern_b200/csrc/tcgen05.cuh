@@ -70,15 +70,10 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
   return v;
 }
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v) {
   uint32_t remote;
-  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(remote)
-               : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
 // ------------------------------------------------------------- copies
