@@ -37,7 +37,7 @@ import math
 from silkern_b200 import _native
 from silkern_b200.contract import _validate_dcp_config
 from silkern_b200.errors import LocalizationError
-from silkern_b200.kernels import _check_status, _device_scope, _is_int
+from silkern_b200.kernels import _check_status, _is_int
 
 #: Dimensions of a latent cache: keys, and the leading part that is the value.
 LATENT_KEY_DIM = 576
@@ -61,36 +61,56 @@ def _type_code(torch, dtype):
     return code
 
 
-def _on_device(torch, tensors, what: str):
-    """The device that every given tensor is on."""
-    device = None
+def _on_device(torch, tensors, what: str) -> int:
+    """The index of the device that every given tensor is on."""
+    device = -1
+    tensor = torch.Tensor
     for t in tensors:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor):
+        if not isinstance(t, tensor):
             raise LocalizationError(f"all {what} buffers must be torch tensors")
-        if not t.is_cuda:
-            raise LocalizationError(f"all {what} buffers must be CUDA tensors")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise LocalizationError(f"all {what} buffers must be on the same device")
+        index = t.get_device()
+        if index != device:
+            if not t.is_cuda:
+                raise LocalizationError(f"all {what} buffers must be CUDA tensors")
+            if device >= 0:
+                raise LocalizationError(f"all {what} buffers must be on the same device")
+            device = index
     return device
 
 
+def _launch(torch, device: int, what: str, entry, *args) -> None:
+    """Call ``entry(*args, stream)`` on the current stream of ``device``."""
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch.cuda.current_device():
+        code = entry(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            code = entry(*args, stream)
+    if code:
+        _native.check(code, what)
+
+
 def _check_ints(torch, tensors, names: str) -> None:
+    int32 = torch.int32
     for t in tensors:
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not int32 or not t.is_contiguous()):
             raise LocalizationError(f"{names} must be contiguous int32 tensors")
+
+
+def _status_pointer(torch, status, device: int):
+    return None if status is None else _check_status(torch, status, torch.device("cuda", device))
 
 
 def _cache(torch, k_cache, v_cache, k_scale, v_scale) -> _native.Cache:
     """The checked ``silkern_cache_v1`` of a cache's tensors."""
     if (v_cache is None) != (v_scale is None):
         raise LocalizationError("v_cache and v_scale are both given or both None")
-    if k_cache.ndim != 4 or (v_cache is not None and v_cache.ndim != 4):
+    shape = k_cache.shape
+    if len(shape) != 4:
         raise LocalizationError("caches must be (num_blocks, block_size, kv_heads, dim)")
-    blocks, block_size, kv_heads, dim = k_cache.shape
+    blocks, block_size, kv_heads, dim = shape
     if blocks < 1 or block_size < 1 or kv_heads < 1:
         raise LocalizationError("cache dimensions must be positive")
     if block_size > 65536 or blocks * block_size > _INT32_MAX:
@@ -99,38 +119,27 @@ def _cache(torch, k_cache, v_cache, k_scale, v_scale) -> _native.Cache:
         if kv_heads != 1 or dim != LATENT_KEY_DIM:
             raise LocalizationError(
                 f"a cache without values is latent: one head and dim {LATENT_KEY_DIM}")
-    elif dim not in (64, 128) or v_cache.shape != k_cache.shape:
+    elif dim not in (64, 128) or v_cache.shape != shape:
         raise LocalizationError("k_cache and v_cache must have the same shape, dim 64 or 128")
-    strides = []
+    scales = (blocks, kv_heads)
+    numbers = []
     for cache, scale in ((k_cache, k_scale), (v_cache, v_scale)):
         if cache is None:
-            strides += (0, 0, 0)
+            numbers.append((None, None, 0, 0, 0))
             continue
-        if cache.dtype != torch.float8_e4m3fn:
+        if cache.dtype is not torch.float8_e4m3fn:
             raise LocalizationError("caches must use float8_e4m3fn")
-        if scale.dtype != torch.float32 or scale.shape != (blocks, kv_heads) or not scale.is_contiguous():
+        if scale.dtype is not torch.float32 or scale.shape != scales or not scale.is_contiguous():
             raise LocalizationError("scales must be contiguous float32 (num_blocks, kv_heads)")
         sb, st, sh, sd = cache.stride()
-        if sd != 1 or sb % 16 or st % 16 or sh % 16 or cache.data_ptr() % 16:
+        pointer = cache.data_ptr()
+        if sd != 1 or (sb | st | sh | pointer) & 15:
             raise LocalizationError(
                 "caches need unit column stride, other strides that are multiples of 16 and 16-byte alignment")
-        strides += (sb, st, sh)
-    return _native.Cache(
-        k_cache.data_ptr(), None if v_cache is None else v_cache.data_ptr(), k_scale.data_ptr(),
-        None if v_scale is None else v_scale.data_ptr(), blocks, block_size, kv_heads, dim,
-        LATENT_VALUE_DIM if v_cache is None else dim, *strides)
-
-
-def _check_separate(outputs, others) -> None:
-    """No output shares storage with another output or with an input."""
-    taken = {t.untyped_storage().data_ptr() for t in others if t is not None}
-    for t in outputs:
-        if t is None:
-            continue
-        storage = t.untyped_storage().data_ptr()
-        if storage in taken:
-            raise LocalizationError("outputs must not share storage with inputs or with each other")
-        taken.add(storage)
+        numbers.append((pointer, scale.data_ptr(), sb, st, sh))
+    (k, ks, kb, kt, kh), (v, vs, vb, vt, vh) = numbers
+    return _native.Cache(k, v, ks, vs, blocks, block_size, kv_heads, dim,
+                         LATENT_VALUE_DIM if v_cache is None else dim, kb, kt, kh, vb, vt, vh)
 
 
 def _check_table(block_table) -> None:
@@ -139,32 +148,38 @@ def _check_table(block_table) -> None:
 
 
 def _check_owner(block_size, dcp_size, dcp_rank, dcp_interleave) -> None:
-    _validate_dcp_config(dcp_size, dcp_rank, dcp_interleave)
+    if not (type(dcp_size) is type(dcp_rank) is type(dcp_interleave) is int
+            and 0 <= dcp_rank < dcp_size and dcp_interleave > 0):
+        _validate_dcp_config(dcp_size, dcp_rank, dcp_interleave)
     if block_size % dcp_interleave:
         raise LocalizationError("the cache's block_size must be divisible by dcp_interleave")
     if dcp_size * dcp_interleave > _INT32_MAX:
         raise LocalizationError("dcp_size * dcp_interleave must be below 2**31")
 
 
-def _check_queries(torch, q, k_cache, out, lse, softmax_scale) -> tuple[int, int]:
-    """Checks of an attention call's queries and results: (rows, type code)."""
-    code = _type_code(torch, q.dtype)
-    if q.ndim != 3 or q.shape[2] != k_cache.shape[3]:
+def _check_queries(torch, q, cache, out, lse, softmax_scale):
+    """Checks of an attention call's queries and results: (rows, heads, q's row
+    and head stride, out's, type code)."""
+    dtype = q.dtype
+    code = _type_code(torch, dtype)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != cache.key_dim:
         raise LocalizationError("q must be (rows, heads, key_dim) with the cache's key_dim")
-    rows, heads, dim = q.shape
-    if rows < 1 or heads < 1 or heads > 65535 or heads % k_cache.shape[2]:
+    rows, heads, _ = shape
+    if rows < 1 or heads < 1 or heads > 65535 or heads % cache.kv_heads:
         raise LocalizationError("q needs at least one row, and heads in a positive multiple of the cache's heads")
-    value_dim = LATENT_VALUE_DIM if dim == LATENT_KEY_DIM else dim
-    if out.dtype != q.dtype or out.shape != (rows, heads, value_dim) or out.stride(2) != 1:
-        raise LocalizationError(f"out must be (rows, heads, {value_dim}) of q's type with unit column stride")
-    if lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous():
+    out_row, out_head, out_column = out.stride() if out.ndim == 3 else (0, 0, 0)
+    if out.dtype is not dtype or out.shape != (rows, heads, cache.value_dim) or out_column != 1:
+        raise LocalizationError(f"out must be (rows, heads, {cache.value_dim}) of q's type with unit column stride")
+    if lse.dtype is not torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous():
         raise LocalizationError("lse must be contiguous float32 (rows, heads)")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    q_row, q_head, q_column = q.stride()
+    if q_column != 1 or (q_row | q_head) & 7 or q.data_ptr() & 15:
         raise LocalizationError(
             "q needs unit column stride, other strides that are multiples of 8 and 16-byte alignment")
     if not math.isfinite(softmax_scale):
         raise LocalizationError("softmax_scale must be finite")
-    return rows, code
+    return rows, heads, q_row, q_head, out_row, out_head, code
 
 
 def append_quantized(
@@ -220,34 +235,28 @@ def append_quantized(
     if (values is None) != (v_cache is None):
         raise LocalizationError("values are given exactly when the cache has values")
     tokens = keys.shape[0] if keys.ndim == 3 else 0
+    wanted = (tokens, cache.kv_heads, cache.key_dim)
+    places = []
     for new in (keys, values):
-        if new is not None and (new.dtype != keys.dtype or tuple(new.shape) != (tokens, cache.kv_heads, cache.key_dim)
-                                or tokens < 1 or new.stride(2) != 1):
+        if new is None:
+            places += (None, 0, 0)
+            continue
+        row, head, column = new.stride() if new.ndim == 3 else (0, 0, 0)
+        if new.dtype is not keys.dtype or new.shape != wanted or tokens < 1 or column != 1:
             raise LocalizationError(
                 "keys and values must be (tokens, kv_heads, dim) of one type with unit column stride")
+        places += (new.data_ptr(), row, head)
     sequences = starts.shape[0] if starts.ndim == 1 else 0
     if sequences < 1 or cu_tokens.shape != (sequences + 1,) or req_ids.shape != (sequences,):
         raise LocalizationError("starts and req_ids need one element per sequence, cu_tokens one more")
     _check_table(block_table)
     _check_owner(cache.block_size, dcp_size, dcp_rank, dcp_interleave)
-    _check_separate((k_scale, v_scale), (keys, values, cu_tokens, starts, req_ids, block_table, k_cache, v_cache))
-    inputs = {t.untyped_storage().data_ptr() for t in (keys, values, cu_tokens, starts, req_ids, block_table)
-              if t is not None}
-    if any(t is not None and t.untyped_storage().data_ptr() in inputs for t in (k_cache, v_cache)):
-        raise LocalizationError("caches must not share storage with inputs")
-    status_ptr = _check_status(torch, status, device)
-
-    lib = _native.load()
-    with _device_scope(torch, device):
-        rc = lib.silkern_append_quantized_v1(
-            ctypes.addressof(cache), keys.data_ptr(), keys.stride(0), keys.stride(1),
-            None if values is None else values.data_ptr(),
-            0 if values is None else values.stride(0), 0 if values is None else values.stride(1),
-            code, tokens, cu_tokens.data_ptr(), starts.data_ptr(), req_ids.data_ptr(), sequences,
-            block_table.data_ptr(), block_table.shape[0], block_table.shape[1],
-            int(dcp_size), int(dcp_rank), int(dcp_interleave), status_ptr,
-            torch.cuda.current_stream(device).cuda_stream)
-    _native.check(rc, "append_quantized")
+    status_ptr = _status_pointer(torch, status, device)
+    table_rows, table_width = block_table.shape
+    _launch(torch, device, "append_quantized", _native.load().silkern_append_quantized_v1,
+            ctypes.addressof(cache), *places, code, tokens, cu_tokens.data_ptr(), starts.data_ptr(),
+            req_ids.data_ptr(), sequences, block_table.data_ptr(), table_rows, table_width, int(dcp_size),
+            int(dcp_rank), int(dcp_interleave), status_ptr)
 
 
 def attend_selected(
@@ -285,24 +294,20 @@ def attend_selected(
     device = _on_device(torch, (q, slots, k_cache, v_cache, k_scale, v_scale, out, lse, counts), "attention")
     _check_ints(torch, (counts,), "counts")
     cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
-    rows, code = _check_queries(torch, q, k_cache, out, lse, softmax_scale)
-    if slots.dtype != torch.int32 or slots.ndim != 2 or slots.shape[0] != rows or slots.shape[1] < 1:
+    rows, heads, q_row, q_head, out_row, out_head, code = _check_queries(torch, q, cache, out, lse, softmax_scale)
+    if slots.dtype is not torch.int32 or slots.ndim != 2 or slots.shape[0] != rows or slots.shape[1] < 1:
         raise LocalizationError("slots must be int32 with one non-empty row for each row of q")
-    if slots.stride(1) != 1:
+    slots_row, slots_column = slots.stride()
+    width = slots.shape[1]
+    if slots_column != 1 and width > 1:
         raise LocalizationError("slots must have unit column stride")
     if counts is not None and counts.shape != (rows,):
         raise LocalizationError("counts must contain one element per row")
-    _check_separate((out, lse), (q, slots, counts, k_cache, v_cache, k_scale, v_scale))
-    status_ptr = _check_status(torch, status, device)
-
-    lib = _native.load()
-    with _device_scope(torch, device):
-        rc = lib.silkern_attend_selected_v1(
-            ctypes.addressof(cache), q.data_ptr(), q.stride(0), q.stride(1), code, rows, q.shape[1],
-            slots.data_ptr(), slots.stride(0), slots.shape[1], None if counts is None else counts.data_ptr(),
-            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), softmax_scale, status_ptr,
-            torch.cuda.current_stream(device).cuda_stream)
-    _native.check(rc, "attend_selected")
+    status_ptr = _status_pointer(torch, status, device)
+    _launch(torch, device, "attend_selected", _native.load().silkern_attend_selected_v1,
+            ctypes.addressof(cache), q.data_ptr(), q_row, q_head, code, rows, heads, slots.data_ptr(), slots_row,
+            width, None if counts is None else counts.data_ptr(), out.data_ptr(), out_row, out_head,
+            lse.data_ptr(), softmax_scale, status_ptr)
 
 
 def attend_window(
@@ -352,7 +357,7 @@ def attend_window(
         "attention")
     _check_ints(torch, (cu_tokens, lengths, req_ids, block_table), "cu_tokens, lengths, req_ids and block_table")
     cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
-    rows, code = _check_queries(torch, q, k_cache, out, lse, softmax_scale)
+    rows, heads, q_row, q_head, out_row, out_head, code = _check_queries(torch, q, cache, out, lse, softmax_scale)
     sequences = lengths.shape[0] if lengths.ndim == 1 else 0
     if sequences < 1 or cu_tokens.shape != (sequences + 1,) or req_ids.shape != (sequences,):
         raise LocalizationError("lengths and req_ids need one element per sequence, cu_tokens one more")
@@ -360,18 +365,13 @@ def attend_window(
     _check_owner(cache.block_size, dcp_size, dcp_rank, dcp_interleave)
     if not _is_int(window) or not 0 <= window <= _INT32_MAX or not _is_int(sinks) or not 0 <= sinks <= _INT32_MAX:
         raise LocalizationError("window and sinks must be non-negative int32 integers")
-    _check_separate((out, lse), (q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale))
-    status_ptr = _check_status(torch, status, device)
-
-    lib = _native.load()
-    with _device_scope(torch, device):
-        rc = lib.silkern_attend_window_v1(
-            ctypes.addressof(cache), q.data_ptr(), q.stride(0), q.stride(1), code, rows, q.shape[1],
-            cu_tokens.data_ptr(), lengths.data_ptr(), req_ids.data_ptr(), sequences, block_table.data_ptr(),
-            block_table.shape[0], block_table.shape[1], int(window), int(sinks), int(dcp_size), int(dcp_rank),
-            int(dcp_interleave), out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), softmax_scale,
-            status_ptr, torch.cuda.current_stream(device).cuda_stream)
-    _native.check(rc, "attend_window")
+    status_ptr = _status_pointer(torch, status, device)
+    table_rows, table_width = block_table.shape
+    _launch(torch, device, "attend_window", _native.load().silkern_attend_window_v1,
+            ctypes.addressof(cache), q.data_ptr(), q_row, q_head, code, rows, heads, cu_tokens.data_ptr(),
+            lengths.data_ptr(), req_ids.data_ptr(), sequences, block_table.data_ptr(), table_rows, table_width,
+            int(window), int(sinks), int(dcp_size), int(dcp_rank), int(dcp_interleave), out.data_ptr(), out_row,
+            out_head, lse.data_ptr(), softmax_scale, status_ptr)
 
 
 def merge_partials(outs, lses, out, lse=None) -> None:
@@ -388,24 +388,21 @@ def merge_partials(outs, lses, out, lse=None) -> None:
     import torch
 
     device = _on_device(torch, (outs, lses, out, lse), "merge")
-    code = _type_code(torch, outs.dtype)
-    if outs.ndim != 4 or min(outs.shape) < 1:
+    dtype = outs.dtype
+    code = _type_code(torch, dtype)
+    if outs.ndim != 4 or outs.numel() < 1:
         raise LocalizationError("outs must be a non-empty (ranks, rows, heads, dim)")
     ranks, rows, heads, dim = outs.shape
-    if out.dtype != outs.dtype or out.shape != (rows, heads, dim):
+    if out.dtype is not dtype or out.shape != (rows, heads, dim):
         raise LocalizationError("out must be (rows, heads, dim) of the type of outs")
-    if outs.stride(3) != 1 or out.stride(2) != 1:
+    in_rank, in_row, in_head, in_column = outs.stride()
+    out_row, out_head, out_column = out.stride()
+    if dim > 1 and (in_column != 1 or out_column != 1):
         raise LocalizationError("outs and out must have unit column stride")
-    if lses.dtype != torch.float32 or lses.shape != (ranks, rows, heads) or not lses.is_contiguous():
+    if lses.dtype is not torch.float32 or lses.shape != (ranks, rows, heads) or not lses.is_contiguous():
         raise LocalizationError("lses must be contiguous float32 (ranks, rows, heads)")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous()):
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous()):
         raise LocalizationError("lse must be contiguous float32 (rows, heads)")
-    _check_separate((out, lse), (outs, lses))
-
-    lib = _native.load()
-    with _device_scope(torch, device):
-        rc = lib.silkern_merge_partials_v1(
-            outs.data_ptr(), outs.stride(0), outs.stride(1), outs.stride(2), lses.data_ptr(), code, ranks, rows,
-            heads, dim, out.data_ptr(), out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(),
-            torch.cuda.current_stream(device).cuda_stream)
-    _native.check(rc, "merge_partials")
+    _launch(torch, device, "merge_partials", _native.load().silkern_merge_partials_v1,
+            outs.data_ptr(), in_rank, in_row, in_head, lses.data_ptr(), code, ranks, rows, heads, dim,
+            out.data_ptr(), out_row, out_head, None if lse is None else lse.data_ptr())

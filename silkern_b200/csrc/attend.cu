@@ -11,6 +11,8 @@ namespace silkern {
 
 namespace {
 
+constexpr int64_t kMostCluster = 8;
+
 int multiprocessors() {
   int device = 0, n = 0;
   if (cudaGetDevice(&device) != cudaSuccess ||
@@ -53,34 +55,45 @@ int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
   // A latent cache's fp16 queries have three parts: 64 columns of them do not
   // fit the shared memory beside the keys.
   const int widest = latent && half ? 32 : 64;
-  const int columns = want <= 16 ? 16 : want <= 32 || widest == 32 || (latent && group <= 32) ? 32 : 64;
-  const int32_t per = a.slots != nullptr || group >= columns ? 1 : columns / group;
+  int columns = want <= 16 ? 16 : want <= 32 || widest == 32 || (latent && group <= 32) ? 32 : 64;
+  const int64_t sms = multiprocessors();
+  int32_t per;
+  int64_t blocks, items, live, tiles;
+  while (true) {
+    per = a.slots != nullptr || group >= columns ? 1 : columns / group;
+    blocks = (group + columns - 1) / columns;
+    items = a.slots != nullptr ? a.rows : (a.rows + static_cast<int64_t>(per - 1) * a.sequences) / per;
+    int64_t busy = a.slots != nullptr ? a.rows : (a.rows + per - 1) / per;
+    if (a.slots == nullptr && busy < a.sequences) busy = a.sequences < a.rows ? a.sequences : a.rows;
+    live = busy * a.cache.kv_heads * blocks;
+    int64_t keys = a.slots != nullptr ? a.width : static_cast<int64_t>(a.table_width) * a.cache.block.divisor;
+    if (a.slots == nullptr && a.window != 0) {
+      // This rank's share of what a CTA's queries see, and a run of owned tokens more.
+      const int64_t seen = (static_cast<int64_t>(a.window) + a.sinks + per) / a.own.group.divisor * a.own.interleave.divisor +
+                           2 * a.own.interleave.divisor;
+      if (seen < keys) keys = seen;
+    }
+    tiles = (keys + 127) / 128;
+    // While clusters over all keys still leave half of the SMs without work,
+    // half the columns to a CTA: its queries are split, and its outputs
+    // joined, in half the time (one row of 128 heads: 21.3 -> 17.4 us).
+    if (columns == 16 || live * 2 * (tiles < kMostCluster ? tiles : kMostCluster) > sms) break;
+    columns /= 2;
+  }
+  const int64_t units = items * a.cache.kv_heads * blocks, pipes = !latent && columns == 16 ? 2 : 1;
+  if (units > 0x3fffffff) return SILKERN_E_SHAPE;
   AttendPlan plan;
   plan.per = make_fastdiv(static_cast<uint32_t>(per));
   plan.group = make_fastdiv(static_cast<uint32_t>(group));
-  plan.blocks = (group + columns - 1) / columns;
-  const int64_t items = a.slots != nullptr ? a.rows : (a.rows + static_cast<int64_t>(per - 1) * a.sequences) / per;
-  int64_t busy = a.slots != nullptr ? a.rows : (a.rows + per - 1) / per;
-  if (a.slots == nullptr && busy < a.sequences) busy = a.sequences < a.rows ? a.sequences : a.rows;
-  const int64_t most = a.slots != nullptr ? a.width : static_cast<int64_t>(a.table_width) * a.cache.block.divisor;
-  int64_t keys = most;
-  if (a.slots == nullptr && a.window != 0) {
-    // This rank's share of what a CTA's queries see, and a run of owned tokens more.
-    const int64_t seen = (static_cast<int64_t>(a.window) + a.sinks + per) / a.own.group.divisor * a.own.interleave.divisor +
-                         2 * a.own.interleave.divisor;
-    if (seen < keys) keys = seen;
-  }
-  const int64_t tiles = (keys + 127) / 128;
-  const int64_t units = items * a.cache.kv_heads * plan.blocks;
-  if (units > 0x3fffffff) return SILKERN_E_SHAPE;
-  const int64_t live = busy * a.cache.kv_heads * plan.blocks;
-  const int64_t sms = multiprocessors(), pipes = !latent && columns == 16 ? 2 : 1;
-  // Few work items: as many CTAs as still find an SM and a tile for each of
-  // their pipelines, up to a cluster of 8, share each item's keys. (16 to a
-  // cluster find room seven times only, 8 fifteen times.)
-  unsigned cluster = 1;
-  while (cluster < 8 && live * cluster * 2 <= sms && tiles >= cluster * 2 * pipes) cluster *= 2;
+  plan.blocks = static_cast<int32_t>(blocks);
   plan.units = static_cast<uint32_t>(units);
+  // Few work items: as many CTAs as still find an SM and a tile for each of
+  // their pipelines, up to a cluster of 8, share each item's keys. How many
+  // clusters find room at once is the occupancy calculator's answer for these
+  // kernels (148 SMs: 74 of 2, 33 of 4, 15 of 8; 7 of 16).
+  unsigned cluster = 1;
+  const int64_t room[3] = {sms / 2, sms * 33 / 148, sms * 15 / 148};
+  for (int k = 0; k < 3 && live <= room[k] && tiles >= cluster * 2 * pipes; ++k) cluster *= 2;
   int64_t grid;
   if (cluster > 1 || (pipes > 1 && units <= sms && tiles >= pipes)) {
     plan.whole = 0;

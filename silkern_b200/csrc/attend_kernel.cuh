@@ -988,7 +988,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       if (leader) {
         mma_commit(smem_addr(&sh.drained));
         const long long begin = clock64();
-        while (!mbar_try(smem_addr(&sh.drained), 0) && clock64() - begin < 1000000000LL) {
+        while (!mbar_try(smem_addr(&sh.drained), 0) && clock64() - begin < 4000000000LL) {
         }
         flag_status(a.status, SILKERN_STATUS_WAIT_TIMEOUT);
       }

@@ -24,7 +24,7 @@ struct AppendArgs {
   const void* keys;
   const void* values;
   int64_t key_token, key_head, value_token, value_head;  // elements
-  int32_t key_dim, value_dim;
+  bool wide;  // new values lie on 16-byte boundaries, eight by eight
   int32_t tokens, sequences;
   const int32_t* cu_tokens;
   const int32_t* starts;
@@ -37,8 +37,6 @@ struct AppendArgs {
   int32_t* status;
 };
 
-constexpr int kAppendThreads = 128;
-
 // The scale that a largest magnitude asks for: the smallest power of two w
 // with 448 w >= m, from the bits of m (448 = 0.875 * 2^9, so with m = f 2^e,
 // f in [0.5, 1), w = 2^(e - 9), or twice that where f > 0.875).
@@ -48,6 +46,11 @@ __device__ __forceinline__ float scale_for(float m) {
   const float f = frexpf(m, &e);
   const int p = e - 9 + (f > 0.875f ? 1 : 0);
   return ldexpf(1.f, min(max(p, -100), 100));
+}
+
+__device__ __forceinline__ int64_t first_append_item(const AppendArgs& a, int32_t cu, int32_t b) {
+  const int64_t n = cu + (2 * static_cast<int64_t>(a.page_tokens.divisor) - 2) * b;
+  return n <= 0x7fffffff ? fastdiv(static_cast<uint32_t>(n), a.page_tokens) : n / a.page_tokens.divisor;
 }
 
 __device__ __forceinline__ uint8_t to_e4m3(float x) {
@@ -60,11 +63,18 @@ __device__ __forceinline__ float from_e4m3(uint8_t code) {
 }
 
 // One CTA for each (page that a sequence's tokens touch, head, keys or
-// values). Sequence b owns the items from cu[b] / page_tokens + 2 b on: n new
-// tokens touch at most n / page_tokens + 2 pages of a rank.
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
-  __shared__ uint32_t most_shared[kAppendThreads / 32];
+// values). Sequence b owns the items from (cu[b] + (2 p - 2) b) / p on, p the
+// positions from page to page: n new tokens touch at most (n + 2 p - 2) / p
+// pages of a rank. A CTA reads its new values once, 16 bytes a thread at a
+// time, and keeps the first kKept of a thread's for the second pass. What
+// bounds a decode step's call is its launch and the chain of dependent loads
+// (item, request, page, tokens); a prompt's, its few pages: 8192 tokens of a
+// latent cache over two ranks are 64 of them.
+template <typename T, int DIM, int THREADS>
+__global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int kPieces = DIM / 8;  // of 8 values in a token
+  constexpr int kKept = 9;
+  __shared__ uint32_t most_shared[THREADS / 32];
   pdl_wait();
   pdl_launch_dependents();
   const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -78,7 +88,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     bool before = false;
     if (b < high) {
       const int32_t cu = min(max(__ldg(a.cu_tokens + b), 0), a.tokens);
-      before = static_cast<int64_t>(fastdiv(cu, a.page_tokens)) + 2 * static_cast<int64_t>(b) <= item;
+      before = first_append_item(a, cu, b) <= item;
     }
     const uint32_t hits = __ballot_sync(kAllLanes, before);
     const int32_t last = hits == 0 ? 0 : 31 - __clz(hits);
@@ -87,7 +97,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   }
   const int32_t begin = min(max(__ldg(a.cu_tokens + low), 0), a.tokens);
   const int32_t end = min(max(__ldg(a.cu_tokens + low + 1), begin), a.tokens);
-  const int64_t page_index = item - (static_cast<int64_t>(fastdiv(begin, a.page_tokens)) + 2 * static_cast<int64_t>(low));
+  const int64_t page_index = item - first_append_item(a, begin, low);
   if (page_index < 0 || begin == end) return;
   const int32_t start = __ldg(a.starts + low);
   const int32_t req = __ldg(a.req_ids + low);
@@ -114,52 +124,107 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     if (threadIdx.x == 0) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
     return;
   }
-  const int32_t dim = is_value ? a.value_dim : a.key_dim;
   const int64_t src_token = is_value ? a.value_token : a.key_token;
-  const T* src = static_cast<const T*>(is_value ? a.values : a.keys) + head * (is_value ? a.value_head : a.key_head);
+  const T* src = static_cast<const T*>(is_value ? a.values : a.keys) + head * (is_value ? a.value_head : a.key_head) +
+                 begin * src_token;
   const int64_t dst_token = is_value ? a.cache.v_token : a.cache.k_token;
   uint8_t* dst = const_cast<uint8_t*>(is_value ? a.cache.v : a.cache.k) +
                  block * (is_value ? a.cache.v_block : a.cache.k_block) +
                  head * (is_value ? a.cache.v_head : a.cache.k_head);
   float* scale = const_cast<float*>(is_value ? a.cache.v_scale : a.cache.k_scale) +
                  static_cast<int64_t>(block) * a.cache.kv_heads + head;
-  const int32_t count = static_cast<int32_t>(hi - lo), total = count * dim;
+  const int32_t skip = static_cast<int32_t>(lo - page_first), count = static_cast<int32_t>(hi - lo);
+  const int32_t total = count * kPieces;
+  const float held_scale = *scale;
+  auto read = [&](int32_t i) {
+    const int32_t t = i / kPieces, d = (i - t * kPieces) * 8;
+    const T* p = src + static_cast<int64_t>(a.own.position(lo + t) - static_cast<uint32_t>(start)) * src_token + d;
+    uint4 x;
+    if (a.wide) {
+      x = __ldg(reinterpret_cast<const uint4*>(p));
+    } else {
+      T* e = reinterpret_cast<T*>(&x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = p[k];
+    }
+    return x;
+  };
   // The largest magnitude by its bits: NaN > infinity > finite.
+  uint4 kept[kKept];
   uint32_t most = 0;
-  for (int32_t i = threadIdx.x; i < total; i += kAppendThreads) {
-    const int32_t t = i / dim, d = i - t * dim;
-    const int64_t row = begin + static_cast<int64_t>(a.own.position(lo + t)) - start;
-    most = max(most, __float_as_uint(static_cast<float>(src[row * src_token + d])) & 0x7fffffffu);
+  auto see = [&](const uint4& x) {
+    const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) most = max(most, __float_as_uint(static_cast<float>(e[k])) & 0x7fffffffu);
+  };
+#pragma unroll
+  for (int n = 0; n < kKept; ++n) {
+    const int32_t i = threadIdx.x + n * THREADS;
+    if (i < total) kept[n] = read(i);
   }
+#pragma unroll
+  for (int n = 0; n < kKept; ++n) {
+    if (static_cast<int32_t>(threadIdx.x) + n * THREADS < total) see(kept[n]);
+  }
+  for (int32_t i = threadIdx.x + kKept * THREADS; i < total; i += THREADS) see(read(i));
   most = __reduce_max_sync(kAllLanes, most);
   if (lane == 0) most_shared[warp] = most;
-  __syncthreads();
+  __syncthreads();  // every thread has read the old scale as well
 #pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, most_shared[w]);
-  const bool fresh = lo == page_first;
-  const float old = fresh ? 0.f : *scale;
+  for (int w = 0; w < THREADS / 32; ++w) most = max(most, most_shared[w]);
+  const bool fresh = skip == 0;
+  const float old = fresh ? 0.f : held_scale;
   const float want = most >= 0x7f800000u ? NAN : scale_for(__uint_as_float(most));
   const float use = want != want || old != old ? NAN : fmaxf(old, want);
-  __syncthreads();  // every thread has read the old scale
   if (threadIdx.x == 0) *scale = use;
   const bool live = use > 0.f;  // false for 0 and NaN
-  for (int32_t i = threadIdx.x; i < total; i += kAppendThreads) {
-    const int32_t t = i / dim, d = i - t * dim;
-    const int64_t row = begin + static_cast<int64_t>(a.own.position(lo + t)) - start;
-    const float x = static_cast<float>(src[row * src_token + d]);
-    dst[static_cast<int64_t>(lo - page_first + t) * dst_token + d] = live ? to_e4m3(__fdiv_rn(x, use)) : 0;
+  // A power of two divides as its reciprocal multiplies, exactly; a scale that
+  // somebody else set may be another number.
+  const bool power = (__float_as_uint(use) & 0x007fffffu) == 0;
+  const float inverse = __fdiv_rn(1.f, use);
+  auto write = [&](int32_t i, const uint4& x) {
+    const int32_t t = i / kPieces, d = (i - t * kPieces) * 8;
+    const T* e = reinterpret_cast<const T*>(&x);
+    uint2 codes = make_uint2(0u, 0u);
+    uint8_t* c = reinterpret_cast<uint8_t*>(&codes);
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float v = static_cast<float>(e[k]);
+        c[k] = to_e4m3(power ? v * inverse : __fdiv_rn(v, use));
+      }
+    }
+    *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(skip + t) * dst_token + d) = codes;
+  };
+#pragma unroll
+  for (int n = 0; n < kKept; ++n) {
+    const int32_t i = threadIdx.x + n * THREADS;
+    if (i < total) write(i, kept[n]);
   }
-  if (!fresh && live && use > old) {
-    const uint32_t skip = lo - static_cast<uint32_t>(page_first);
+  for (int32_t i = threadIdx.x + kKept * THREADS; i < total; i += THREADS) write(i, read(i));
+  if (!fresh && live && use > old) {  // what the page held, in the new scale
     const float ratio = __fdiv_rn(old, use);
-    for (int32_t i = threadIdx.x; i < (static_cast<int32_t>(block_size) - count) * dim; i += kAppendThreads) {
-      int32_t t = i / dim;
-      const int32_t d = i - t * dim;
-      if (static_cast<uint32_t>(t) >= skip) t += count;
-      uint8_t* p = dst + t * dst_token + d;
-      *p = to_e4m3(from_e4m3(*p) * ratio);
+    for (int32_t i = threadIdx.x; i < (static_cast<int32_t>(block_size) - count) * (DIM / 16); i += THREADS) {
+      int32_t t = i / (DIM / 16);
+      const int32_t d = (i - t * (DIM / 16)) * 16;
+      if (t >= skip) t += count;
+      uint4* p = reinterpret_cast<uint4*>(dst + static_cast<int64_t>(t) * dst_token + d);
+      uint4 x = *p;
+      uint8_t* c = reinterpret_cast<uint8_t*>(&x);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) c[k] = to_e4m3(from_e4m3(c[k]) * ratio);
+      *p = x;
     }
   }
+}
+
+template <typename T, int DIM>
+void (*append_for(bool pages))(AppendArgs) {
+  return pages ? append_kernel<T, DIM, 512> : append_kernel<T, DIM, 128>;
+}
+template <typename T>
+void (*append_for(int dim, bool pages))(AppendArgs) {
+  return dim == 64 ? append_for<T, 64>(pages) : dim == 128 ? append_for<T, 128>(pages) : append_for<T, 576>(pages);
 }
 
 // ---------------------------------------------------------------- merge
@@ -176,8 +241,11 @@ struct MergeArgs {
 
 constexpr int kMergeWarps = 8;
 
-// One warp for each (row, head).
-template <typename T>
+// One warp for each (row, head): lane r has rank r's weight, and every lane
+// eight columns at a time of all ranks, four loads on their way at once. A
+// call reads and writes each byte once: it is bound by memory (8 ranks, 128
+// rows of 128 heads of 512: 152 MB).
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ MergeArgs a) {
   pdl_wait();
   pdl_launch_dependents();
@@ -186,26 +254,110 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
   if (pair >= a.pairs) return;
   const int64_t row = pair / a.heads;
   const int64_t head = pair - row * a.heads;
-  float top = -INFINITY;
-  for (int i = 0; i < a.ranks; ++i) top = fmaxf(top, a.lses[i * a.pairs + pair]);
+  const float mine = lane < a.ranks ? a.lses[lane * a.pairs + pair] : -INFINITY;
+  float top = mine;
+  for (int i = 32 + lane; i < a.ranks; i += 32) top = fmaxf(top, a.lses[i * a.pairs + pair]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kAllLanes, top, d));
   const float base = top == -INFINITY ? 0.f : top;
+  const float weight = expf(mine - base);
   float total = 0.f;
-  for (int i = 0; i < a.ranks; ++i) total += expf(a.lses[i * a.pairs + pair] - base);
+  for (int i = 0; i < min(a.ranks, 32); ++i) total += __shfl_sync(kAllLanes, weight, i);
+  for (int i = 32; i < a.ranks; ++i) total += expf(a.lses[i * a.pairs + pair] - base);
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const T* src = static_cast<const T*>(a.outs) + row * a.outs_row + head * a.outs_head;
   T* dst = static_cast<T*>(a.out) + row * a.out_row + head * a.out_head;
-  for (int d = lane; d < a.dim; d += 32) {
-    float x = 0.f;
-    for (int i = 0; i < a.ranks; ++i) {
-      const float l = a.lses[i * a.pairs + pair];
-      if (l != -INFINITY) x += expf(l - base) * inv * static_cast<float>(src[i * a.outs_rank + d]);
+  // The weight of rank i; 0 and `read` false where its lse is -inf.
+  auto weight_of = [&](int i, bool& read) {
+    const float l = i < 32 ? __shfl_sync(kAllLanes, mine, i & 31) : a.lses[i * a.pairs + pair];
+    const float w = i < 32 ? __shfl_sync(kAllLanes, weight, i & 31) : expf(l - base);
+    read = l != -INFINITY;
+    return read ? w * inv : 0.f;
+  };
+  constexpr int kStep = WIDE ? 256 : 32;
+  for (int d0 = 0; d0 < a.dim; d0 += kStep) {
+    if constexpr (WIDE) {
+      const int d = d0 + lane * 8;
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int i0 = 0; i0 < a.ranks; i0 += 4) {
+        uint4 raw[4];
+        float w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          raw[k] = make_uint4(0u, 0u, 0u, 0u);
+          w[k] = 0.f;
+          if (i0 + k < a.ranks) {
+            bool read;
+            w[k] = weight_of(i0 + k, read);
+            if (read && d < a.dim) raw[k] = __ldcs(reinterpret_cast<const uint4*>(src + (i0 + k) * a.outs_rank + d));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const T* v = reinterpret_cast<const T*>(&raw[k]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = fmaf(w[k], static_cast<float>(v[e]), x[e]);
+        }
+      }
+      if (d < a.dim) {
+        uint4 packed;
+        T* v = reinterpret_cast<T*>(&packed);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = static_cast<T>(x[e]);
+        *reinterpret_cast<uint4*>(dst + d) = packed;
+      }
+    } else {
+      const int d = d0 + lane;
+      float x = 0.f;
+      for (int i = 0; i < a.ranks; ++i) {
+        bool read;
+        const float w = weight_of(i, read);
+        if (read && d < a.dim) x = fmaf(w, static_cast<float>(src[i * a.outs_rank + d]), x);
+      }
+      if (d < a.dim) dst[d] = static_cast<T>(x);
     }
-    dst[d] = static_cast<T>(x);
   }
   if (a.lse != nullptr && lane == 0) a.lse[pair] = top + logf(total);
 }
 
 // ---------------------------------------------------------------- checks
+
+// The bytes that a buffer covers, from its address to its last element.
+struct Range {
+  uintptr_t begin, end;
+};
+Range range_of(const void* base, int64_t bytes) {
+  const uintptr_t b = reinterpret_cast<uintptr_t>(base);
+  return base == nullptr ? Range{0, 0} : Range{b, b + static_cast<uintptr_t>(bytes)};
+}
+int64_t extent(int64_t count, int64_t stride) { return (count - 1) * stride; }
+
+// Whether an output shares memory with another output or an input.
+template <int N, int M>
+bool shares(const Range (&outputs)[N], const Range (&inputs)[M]) {
+  for (int i = 0; i < N; ++i) {
+    if (outputs[i].begin == outputs[i].end) continue;
+    for (int j = 0; j < M; ++j) {
+      if (outputs[i].begin < inputs[j].end && inputs[j].begin < outputs[i].end) return true;
+    }
+    for (int j = 0; j < i; ++j) {
+      if (outputs[i].begin < outputs[j].end && outputs[j].begin < outputs[i].end) return true;
+    }
+  }
+  return false;
+}
+
+Range range_of_keys(const silkern_cache_v1* c) {
+  return range_of(c->k, extent(c->num_blocks, c->k_block) + extent(c->block_size, c->k_token) +
+                            extent(c->kv_heads, c->k_head) + c->key_dim);
+}
+Range range_of_values(const silkern_cache_v1* c) {
+  return range_of(c->v, extent(c->num_blocks, c->v_block) + extent(c->block_size, c->v_token) +
+                            extent(c->kv_heads, c->v_head) + c->value_dim);
+}
+Range range_of_scales(const silkern_cache_v1* c, const float* scale) {
+  return range_of(scale, c->num_blocks * c->kv_heads * 4);
+}
 
 int check_cache(const silkern_cache_v1* c, PagedCache* out) {
   if (c == nullptr || c->k == nullptr || c->k_scale == nullptr) return SILKERN_E_NULL;
@@ -250,6 +402,19 @@ int check_owner(int32_t block_size, int32_t dcp_size, int32_t dcp_rank, int32_t 
   out->interleave = make_fastdiv(static_cast<uint32_t>(interleave));
   out->rank_first = static_cast<uint32_t>(dcp_rank) * static_cast<uint32_t>(interleave);
   return SILKERN_OK;
+}
+
+// The results of an attention call share no memory with each other, with the
+// cache or the queries, nor with `index`, the call's other buffers.
+template <int N>
+bool results_alone(const silkern_cache_v1* c, const AttendArgs& a, const Range (&index)[N]) {
+  const int64_t rows = a.rows, heads = a.heads;
+  const Range results[2] = {range_of(a.out, 2 * (extent(rows, a.out_row) + extent(heads, a.out_head) + c->value_dim)),
+                            range_of(a.lse, 4 * rows * heads)};
+  const Range read[5] = {range_of(a.q, 2 * (extent(rows, a.q_row) + extent(heads, a.q_head) + c->key_dim)),
+                         range_of_keys(c), range_of_values(c), range_of_scales(c, c->k_scale),
+                         range_of_scales(c, c->v_scale)};
+  return !shares(results, read) && !shares(results, index);
 }
 
 int check_queries(const silkern_cache_v1* c, const void* q, int64_t q_row, int64_t q_head, int32_t type,
@@ -303,14 +468,25 @@ extern "C" int silkern_append_quantized_v1(const silkern_cache_v1* cache, const 
   }
   rc = check_owner(cache->block_size, dcp_size, dcp_rank, dcp_interleave, &a.own);
   if (rc != SILKERN_OK) return rc;
+  const Range written[4] = {range_of_scales(cache, cache->k_scale), range_of_scales(cache, cache->v_scale),
+                            range_of_keys(cache), Range{0, 0}};
+  const int64_t dims = cache->kv_heads - int64_t{1};
+  const Range read[6] = {range_of(keys, 2 * (extent(tokens, key_token) + dims * key_head + cache->key_dim)),
+                         range_of(values, 2 * (extent(tokens, value_token) + dims * value_head + cache->value_dim)),
+                         range_of(cu_tokens, 4 * (sequences + 1)), range_of(starts, 4 * sequences),
+                         range_of(req_ids, 4 * sequences), range_of(block_table, 4 * table_rows * table_width)};
+  // Keys and values may lie in one buffer, page by page or row by row.
+  const Range values_too[1] = {range_of_values(cache)};
+  const Range scales[2] = {written[0], written[1]};
+  if (shares(written, read) || shares(values_too, read) || shares(values_too, scales)) return SILKERN_E_ALIAS;
   a.keys = keys;
   a.values = values;
   a.key_token = key_token;
   a.key_head = key_head;
   a.value_token = value_token;
   a.value_head = value_head;
-  a.key_dim = cache->key_dim;
-  a.value_dim = cache->value_dim;
+  a.wide = (key_token | key_head | value_token | value_head) % 8 == 0 &&
+           (reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) % 16 == 0;
   a.tokens = static_cast<int32_t>(tokens);
   a.sequences = static_cast<int32_t>(sequences);
   a.cu_tokens = cu_tokens;
@@ -322,11 +498,16 @@ extern "C" int silkern_append_quantized_v1(const silkern_cache_v1* cache, const 
   const int64_t page_tokens = static_cast<int64_t>(cache->block_size) * dcp_size;
   a.page_tokens = make_fastdiv(static_cast<uint32_t>(page_tokens > 0x7fffffff ? 0x7fffffff : page_tokens));
   a.status = status;
-  const int64_t items = tokens / a.page_tokens.divisor + 2 * sequences;
+  const int64_t step = a.page_tokens.divisor;
+  const int64_t items = (tokens + (2 * step - 2) * sequences) / step;
   if (items > 0x7fffffff) return SILKERN_E_SHAPE;
-  void (*fn)(AppendArgs) = type == SILKERN_BF16 ? append_kernel<__nv_bfloat16> : append_kernel<__half>;
+  // A few tokens to a sequence: small CTAs. (Half a page of the widest cache
+  // fills the large ones.)
+  const bool pages = tokens > 8 * sequences;
+  void (*fn)(AppendArgs) = type == SILKERN_BF16 ? append_for<__nv_bfloat16>(cache->key_dim, pages)
+                                                : append_for<__half>(cache->key_dim, pages);
   return launch_pdl_grid(fn, dim3(static_cast<unsigned>(items), static_cast<unsigned>(cache->kv_heads), latent ? 1 : 2),
-                         kAppendThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
+                         pages ? 512 : 128, 0, 1, static_cast<cudaStream_t>(stream), a);
 }
 
 extern "C" int silkern_attend_selected_v1(const silkern_cache_v1* cache, const void* q, int64_t q_row, int64_t q_head,
@@ -347,6 +528,8 @@ extern "C" int silkern_attend_selected_v1(const silkern_cache_v1* cache, const v
   a.counts = counts;
   a.total_slots = static_cast<uint32_t>(cache->num_blocks * cache->block_size);
   a.status = status;
+  const Range index[2] = {range_of(slots, 4 * (extent(rows, slots_row) + width)), range_of(counts, 4 * rows)};
+  if (!results_alone(cache, a, index)) return SILKERN_E_ALIAS;
   return launch_attend(a, cache->key_dim, type, static_cast<cudaStream_t>(stream));
 }
 
@@ -380,6 +563,9 @@ extern "C" int silkern_attend_window_v1(const silkern_cache_v1* cache, const voi
   a.window = static_cast<uint32_t>(window);
   a.sinks = static_cast<uint32_t>(sinks);
   a.status = status;
+  const Range index[4] = {range_of(cu_tokens, 4 * (sequences + 1)), range_of(lengths, 4 * sequences),
+                          range_of(req_ids, 4 * sequences), range_of(block_table, 4 * table_rows * table_width)};
+  if (!results_alone(cache, a, index)) return SILKERN_E_ALIAS;
   return launch_attend(a, cache->key_dim, type, static_cast<cudaStream_t>(stream));
 }
 
@@ -395,7 +581,17 @@ extern "C" int silkern_merge_partials_v1(const void* outs, int64_t outs_rank, in
   }
   MergeArgs a{outs, lses, out, lse, outs_rank, outs_row, outs_head, out_row, out_head, rows * heads,
               static_cast<int32_t>(ranks), static_cast<int32_t>(heads), static_cast<int32_t>(dim)};
-  void (*fn)(MergeArgs) = type == SILKERN_BF16 ? merge_kernel<__nv_bfloat16> : merge_kernel<__half>;
+  const Range written[2] = {range_of(out, 2 * (extent(rows, out_row) + extent(heads, out_head) + dim)),
+                            range_of(lse, 4 * rows * heads)};
+  const Range read[2] = {
+      range_of(outs, 2 * (extent(ranks, outs_rank) + extent(rows, outs_row) + extent(heads, outs_head) + dim)),
+      range_of(lses, 4 * ranks * rows * heads)};
+  if (shares(written, read)) return SILKERN_E_ALIAS;
+  // 16 bytes at a time where every row of columns allows it.
+  const bool wide = (dim | outs_rank | outs_row | outs_head | out_row | out_head) % 8 == 0 &&
+                    (reinterpret_cast<uintptr_t>(outs) | reinterpret_cast<uintptr_t>(out)) % 16 == 0;
+  void (*fn)(MergeArgs) = type == SILKERN_BF16 ? (wide ? merge_kernel<__nv_bfloat16, true> : merge_kernel<__nv_bfloat16, false>)
+                                               : (wide ? merge_kernel<__half, true> : merge_kernel<__half, false>);
   const int64_t ctas = (a.pairs + kMergeWarps - 1) / kMergeWarps;
   if (ctas > 0x7fffffff) return SILKERN_E_SHAPE;
   return launch_pdl(fn, static_cast<unsigned>(ctas), kMergeWarps * 32, 0, 1, static_cast<cudaStream_t>(stream), a);
