@@ -71,7 +71,7 @@ def _on_device(torch, tensors, what: str) -> int:
         if not isinstance(t, tensor):
             raise LocalizationError(f"all {what} buffers must be torch tensors")
         index = t.get_device()
-        if index != device:
+        if index != device or index < 0:
             if not t.is_cuda:
                 raise LocalizationError(f"all {what} buffers must be CUDA tensors")
             if device >= 0:

@@ -1040,7 +1040,8 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       for (uint32_t r = 0; r < kMostRanks; ++r) whole_r = fmaxf(whole_r, rr[r]);
 #pragma unroll
       for (uint32_t r = 0; r < kMostRanks; ++r) {
-        if (rr[r] != -INFINITY) whole_l += ll[r] * exp2_approx(rr[r] - whole_r);
+        // (A rank without a reference saw nothing, or only what is not a number.)
+        whole_l += rr[r] == -INFINITY ? ll[r] : ll[r] * exp2_approx(rr[r] - whole_r);
       }
       const float inverse = whole_l == 0.f ? 0.f : 1.f / (32.f * whole_l);
       const float by = reference == -INFINITY ? 0.f : exp2_approx(reference - whole_r) * inverse;

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__
     const int32_t b = low + lane * step;
     bool before = false;
     if (b < high) {
-      const int32_t cu = min(max(__ldg(a.cu_tokens + b), 0), a.tokens);
+      const int32_t cu = min(max(load_int(a.cu_tokens + b), 0), a.tokens);
       before = first_append_item(a, cu, b) <= item;
     }
     const uint32_t hits = __ballot_sync(kAllLanes, before);
@@ -95,12 +95,12 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__
     low += last * step;
     high = min(high, low + step);
   }
-  const int32_t begin = min(max(__ldg(a.cu_tokens + low), 0), a.tokens);
-  const int32_t end = min(max(__ldg(a.cu_tokens + low + 1), begin), a.tokens);
+  const int32_t begin = min(max(load_int(a.cu_tokens + low), 0), a.tokens);
+  const int32_t end = min(max(load_int(a.cu_tokens + low + 1), begin), a.tokens);
   const int64_t page_index = item - first_append_item(a, begin, low);
   if (page_index < 0 || begin == end) return;
-  const int32_t start = __ldg(a.starts + low);
-  const int32_t req = __ldg(a.req_ids + low);
+  const int32_t start = load_int(a.starts + low);
+  const int32_t req = load_int(a.req_ids + low);
   const int64_t stop = static_cast<int64_t>(start) + (end - begin);
   if (start < 0 || stop > 0x7fffffff) {
     if (page_index == 0 && threadIdx.x == 0) flag_status(a.status, SILKERN_STATUS_BAD_LENGTH);
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__
   if (page_first >= last) return;
   const uint32_t lo = page_first > first ? static_cast<uint32_t>(page_first) : first;
   const uint32_t hi = page_first + block_size < last ? static_cast<uint32_t>(page_first) + block_size : last;
-  const int32_t block = page < a.table_width ? __ldg(a.table + static_cast<int64_t>(req) * a.table_width + page) : -1;
+  const int32_t block = page < a.table_width ? load_int(a.table + static_cast<int64_t>(req) * a.table_width + page) : -1;
   if (static_cast<uint32_t>(block) >= a.cache.num_blocks) {
     if (threadIdx.x == 0) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
     return;
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__
     const T* p = src + static_cast<int64_t>(a.own.position(lo + t) - static_cast<uint32_t>(start)) * src_token + d;
     uint4 x;
     if (a.wide) {
-      x = __ldg(reinterpret_cast<const uint4*>(p));
+      x = *reinterpret_cast<const uint4*>(p);
     } else {
       T* e = reinterpret_cast<T*>(&x);
 #pragma unroll
@@ -521,7 +521,7 @@ extern "C" int silkern_attend_selected_v1(const silkern_cache_v1* cache, const v
   if (slots == nullptr) return SILKERN_E_NULL;
   rc = check_queries(cache, q, q_row, q_head, type, rows, heads, out, out_row, out_head, lse, softmax_scale, &a);
   if (rc != SILKERN_OK) return rc;
-  if (width < 1 || width > 0x7fffffff - 1024) return SILKERN_E_SHAPE;
+  if (width < 1 || width > 0x7fffffff - 4096) return SILKERN_E_SHAPE;
   a.slots = slots;
   a.slots_row = slots_row;
   a.width = static_cast<int32_t>(width);

@@ -17,6 +17,14 @@ namespace silkern {
 
 constexpr uint32_t kAllLanes = 0xffffffffu;
 
+// A load that stays behind griddepcontrol.wait, and takes the coherent path:
+// the grid before may have written what it reads.
+__device__ __forceinline__ int32_t load_int(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 struct PagedCache {
   const uint8_t* k;
   const uint8_t* v;  // the keys again for a latent cache
@@ -113,7 +121,7 @@ __device__ __forceinline__ QuerySpan find_span(const AttendArgs& a, int32_t item
     const int32_t b = low + lane * step;
     bool before = false;
     if (b < high) {
-      const int32_t cu = min(max(__ldg(a.cu_tokens + b), 0), a.rows);
+      const int32_t cu = min(max(load_int(a.cu_tokens + b), 0), a.rows);
       before = first_item(per, cu, b) <= item;
     }
     const uint32_t hits = __ballot_sync(kAllLanes, before);
@@ -122,18 +130,21 @@ __device__ __forceinline__ QuerySpan find_span(const AttendArgs& a, int32_t item
     high = min(high, low + step);
   }
   QuerySpan s{0, 0, low, 0};
-  const int32_t begin = min(max(__ldg(a.cu_tokens + low), 0), a.rows);
-  const int32_t end = min(max(__ldg(a.cu_tokens + low + 1), begin), a.rows);
+  const int32_t begin = min(max(load_int(a.cu_tokens + low), 0), a.rows);
+  const int32_t end = min(max(load_int(a.cu_tokens + low + 1), begin), a.rows);
   const int32_t chunk = item - first_item(per, begin, low);
   const int64_t row = begin + static_cast<int64_t>(chunk) * per.divisor;
   if (chunk < 0 || row >= end) return s;
   s.row = static_cast<int32_t>(row);
   s.count = min(static_cast<int32_t>(per.divisor), end - s.row);
-  const int64_t position = static_cast<int64_t>(__ldg(a.lengths + low)) - (end - s.row);
+  const int64_t position = static_cast<int64_t>(load_int(a.lengths + low)) - (end - s.row);
   s.position = static_cast<int32_t>(max(position, int64_t{-0x7fffffff}));
-  if (__ldg(a.lengths + low) < end - begin && lane == 0) flag_status(a.status, 2);
+  if (load_int(a.lengths + low) < end - begin && lane == 0) flag_status(a.status, 2);
   return s;
 }
+
+// Key numbers are 32-bit integers, and so are those a few tiles past the last.
+constexpr uint32_t kMostKeys = 0x7fffffffu - 4096u;
 
 // The keys that one work item reads, in order: j in [0, n).
 struct KeyList {
@@ -154,7 +165,7 @@ struct Key {
 __device__ __forceinline__ KeyList selected_keys(const AttendArgs& a, int32_t row) {
   KeyList l{a.slots + row * a.slots_row, a.width, 0, 0, 0, 0};
   if (a.counts != nullptr) {
-    const int32_t c = __ldg(a.counts + row);
+    const int32_t c = load_int(a.counts + row);
     l.n = min(max(c, 0), a.width);
     if (c != l.n && (threadIdx.x & 31) == 0) flag_status(a.status, 2);
   }
@@ -165,7 +176,7 @@ __device__ __forceinline__ KeyList selected_keys(const AttendArgs& a, int32_t ro
 // windows, clipped to this rank's tokens.
 __device__ __forceinline__ KeyList window_keys(const AttendArgs& a, const QuerySpan& s) {
   KeyList l{nullptr, 0, 1, 0, 0, a.table_width};
-  const int32_t req = __ldg(a.req_ids + s.seq);
+  const int32_t req = load_int(a.req_ids + s.seq);
   if (req < 0 || req >= a.table_rows) {
     if ((threadIdx.x & 31) == 0) flag_status(a.status, 1);
     return l;
@@ -181,7 +192,9 @@ __device__ __forceinline__ KeyList window_keys(const AttendArgs& a, const QueryS
   const uint32_t head_end = a.window == 0 ? 0u : a.own.owned_before(min(a.sinks, begin));
   l.sinks_end = head_end;
   l.skip = tail_begin - head_end;
-  l.n = static_cast<int32_t>(head_end + (tail_end - tail_begin));
+  const uint32_t n = head_end + (tail_end - tail_begin);
+  l.n = static_cast<int32_t>(min(n, kMostKeys));
+  if (n > kMostKeys && (threadIdx.x & 31) == 0) flag_status(a.status, 2);
   return l;
 }
 
@@ -195,7 +208,7 @@ __device__ __forceinline__ uint32_t local_token(const KeyList& l, uint32_t j) {
 __device__ __forceinline__ int32_t fetch_key(const AttendArgs& a, const KeyList& l, int32_t j) {
   uint32_t at = min(j, l.n - 1);
   if (l.table) at = min(fastdiv(local_token(l, at), a.cache.block), l.table_width - 1);
-  return __ldg(l.source + at);
+  return load_int(l.source + at);
 }
 __device__ __forceinline__ Key locate_key(const AttendArgs& a, const KeyList& l, int32_t j, int32_t fetched) {
   Key k{0u, 0u, 0, false};

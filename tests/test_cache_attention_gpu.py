@@ -563,3 +563,200 @@ def test_a_decode_step_over_ranks_is_attention_over_the_whole_selection(latent) 
     loose = 2.0**-10 * 2.0**-5 * (1 + float(q.double().abs().sum(-1).max()) * scale * 4)
     assert float(((out.double() - want).abs() - 3 * 2.0**-8 * spread).max()) <= loose
     assert float((lse.double() - want_lse).abs().max()) <= loose
+
+
+# --------------------------------------------------------------------------------------- refusals, far places
+
+def good_calls():
+    """name -> (launcher, positional buffers by name, keywords) of calls that are right."""
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    k, v, ks, vs = make_cache(4, 16, 2, 64, seed=50)
+    q, out, lse = randn(3, 4, 64, dtype=torch.bfloat16, seed=51), *results(3, 4, 64, torch.bfloat16)
+    cache = dict(k_cache=k, v_cache=v, k_scale=ks, v_scale=vs)
+    table = ints(0, 1, 2, 3).view(2, 2)
+    sequence = dict(cu_tokens=ints(0, 2, 3), lengths=ints(5, 9), req_ids=ints(0, 1), block_table=table)
+    new = randn(3, 2, 64, dtype=torch.bfloat16, seed=52)
+    return {
+        "selected": (silkern.attend_selected, dict(q=q, slots=table.repeat(2, 1)[:3], **cache, out=out, lse=lse),
+                     dict(softmax_scale=0.1)),
+        "window": (silkern.attend_window, dict(q=q, **sequence, **cache, out=out, lse=lse), dict(softmax_scale=0.1)),
+        "append": (silkern.append_quantized, dict(keys=new, values=new.clone(), **cache, cu_tokens=ints(0, 2, 3),
+                                                  starts=ints(0, 4), req_ids=ints(0, 1), block_table=table), {}),
+        "merge": (silkern.merge_partials, dict(outs=randn(2, 3, 4, 64, dtype=torch.bfloat16, seed=53),
+                                               lses=torch.zeros((2, 3, 4), device="cuda"), out=out, lse=lse), {}),
+    }
+
+
+REFUSED = [
+    ("selected window", "q", lambda t: t.float(), "bfloat16 or float16"),
+    ("selected window", "q", lambda t: t[:, :3], "multiple of the cache's heads"),
+    ("selected window", "q", lambda t: t[..., :32], "key_dim"),
+    ("selected window", "q", lambda t: t[:0], "at least one row"),
+    ("selected window", "q", lambda t: torch.cat([t, t], -1).view(3, 4, 64, 2)[..., 0], "unit column stride"),
+    ("selected window", "q", lambda t: torch.cat([t, t], -1)[..., 1:65], "16-byte alignment"),
+    ("selected window", "out", lambda t: t.half(), "of q's type"),
+    ("selected window", "out", lambda t: t[:2], "out must be"),
+    ("selected window", "lse", lambda t: t.double(), "float32"),
+    ("selected window", "lse", lambda t: t.t().contiguous().t(), "contiguous"),
+    ("selected window append", "k_cache", lambda t: t.view(torch.uint8), "float8_e4m3fn"),
+    ("selected window append", "k_cache", lambda t: t[0], "num_blocks, block_size"),
+    ("selected window append", "v_cache", lambda t: t[:2], "the same shape"),
+    ("selected window append", "v_cache", lambda t: None, "both given or both None"),
+    ("selected window append", "k_scale", lambda t: t.half(), "scales must be"),
+    ("selected window append", "v_scale", lambda t: t.t().contiguous().t(), "scales must be"),
+    ("selected", "slots", lambda t: t.long(), "slots must be int32"),
+    ("selected", "slots", lambda t: t[:2], "slots must be int32"),
+    ("selected", "slots", lambda t: t.t().contiguous().t(), "unit column stride"),
+    ("window append", "cu_tokens", lambda t: t[:2], "cu_tokens one more"),
+    ("window append", "req_ids", lambda t: t.long(), "contiguous int32"),
+    ("window append", "block_table", lambda t: t[0], "2D"),
+    ("window", "lengths", lambda t: t[:1], "one element per sequence"),
+    ("append", "keys", lambda t: t[:, :1], "must be (tokens"),
+    ("append", "values", lambda t: t.half(), "of one type"),
+    ("append", "values", lambda t: None, "exactly when"),
+    ("merge", "outs", lambda t: t[0], "ranks, rows, heads, dim"),
+    ("merge", "lses", lambda t: t.half(), "lses must be"),
+    ("merge", "out", lambda t: t.half(), "type of outs"),
+    ("merge", "lse", lambda t: t[:2], "lse must be"),
+    ("selected window append merge", "any", lambda t: t.cpu(), "CUDA tensors"),
+]
+
+
+@pytest.mark.parametrize("names,buffer,change,message", REFUSED, ids=[f"{r[1]}-{r[3][:12]}" for r in REFUSED])
+def test_launchers_refuse(names, buffer, change, message) -> None:
+    for name in names.split():
+        call, buffers, kw = good_calls()[name]
+        call(*buffers.values(), **kw)
+        for which in list(buffers) if buffer == "any" else [buffer]:
+            wrong = dict(buffers)
+            wrong[which] = change(wrong[which])
+            with pytest.raises(silkern.LocalizationError) as caught:
+                call(*wrong.values(), **kw)
+            assert message in str(caught.value), (name, which, str(caught.value))
+
+
+@pytest.mark.parametrize("names,kw,message", [
+    ("selected window", dict(softmax_scale=math.inf), "finite"), ("window", dict(window=-1), "window and sinks"),
+    ("window", dict(sinks=2.0), "window and sinks"), ("window append", dict(dcp_size=0), "dcp"),
+    ("window append", dict(dcp_rank=True), "integers"), ("window append", dict(dcp_interleave=3), "divisible"),
+    ("selected window append", dict(status=torch.zeros(1)), "status"), ("selected", dict(counts=torch.zeros(2, dtype=torch.int32)), ""),
+])
+def test_launchers_refuse_numbers(names, kw, message) -> None:
+    for name in names.split():
+        call, buffers, more = good_calls()[name]
+        with pytest.raises(silkern.LocalizationError) as caught:
+            call(*buffers.values(), **{**more, **kw})
+        assert message in str(caught.value)
+
+
+def test_results_must_not_lie_in_inputs() -> None:
+    call, b, kw = good_calls()["selected"]
+    for which, other in (("out", b["q"]), ("lse", b["k_scale"].flatten().repeat(2)[:12].view(3, 4))):
+        with pytest.raises(silkern.LocalizationError, match="overlaps"):
+            wrong = {**b, which: other}
+            if which == "lse":
+                wrong["k_scale"] = other.view(-1)[:8].view(4, 2)
+            call(*wrong.values(), **kw)
+
+
+@pytest.mark.parametrize("shape", ["d128", "latent"])
+def test_places_past_32_bits(shape) -> None:
+    """Slots whose bytes lie more than 4 GB into the cache, and append to them."""
+    dim, value_dim, latent = SHAPES[shape]
+    heads = 1 if latent else 2
+    blocks = 70_000 if latent else 300_000  # 5.2 and 2 x 4.9 GB
+    block_size = 128 if latent else 64
+    small = make_cache(6, block_size, heads, dim, latent=latent, seed=60)
+    cache = [None if t is None else torch.zeros((blocks, *t.shape[1:]), dtype=t.dtype, device="cuda") for t in small]
+    places = torch.tensor([0, blocks // 3, blocks // 2, blocks - 3, blocks - 2, blocks - 1]).cuda()
+    for t, s in zip(cache, small):
+        if t is not None:
+            t.view(torch.uint8)[places] = s.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else s.view(torch.uint8)
+    assert cache[0].numel() > 2**32
+    g = torch.Generator().manual_seed(61)
+    local = torch.randint(0, 6 * block_size, (3, 500), generator=g).cuda()
+    slots = (places[local // block_size] * block_size + local % block_size).to(torch.int32)
+    q = randn(3, 8, dim, dtype=torch.bfloat16, seed=62)
+    out, lse = selected(q, slots, cache, value_dim, softmax_scale=dim**-0.5)
+    near, near_lse = selected(q, local.to(torch.int32), small, value_dim, softmax_scale=dim**-0.5)
+    assert torch.equal(out, near) and torch.equal(lse, near_lse)
+    x = torch.randn((200, heads, dim), generator=g).to(torch.bfloat16).cuda()
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    args = (x, None if latent else x), (ints(0, 200), ints(0), ints(0))
+    silkern.append_quantized(*args[0], *cache, *args[1], places[2:].to(torch.int32)[None])
+    silkern.append_quantized(*args[0], *small, *args[1], ints(2, 3, 4, 5)[None])
+    torch.cuda.synchronize()
+    same_cache([None if t is None else t[places] for t in cache], small)
+
+
+def test_grids_that_follow_one_another_see_what_was_written() -> None:
+    """Append, localize, attend and merge back to back, on fresh values each
+    time: each kernel starts before the one ahead ends, and reads its results."""
+    g = torch.Generator().manual_seed(70)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = [t.clone() for t in make_cache(64, 16, 1, 128, seed=71)]
+    table = torch.randperm(64, generator=g).to(torch.int32).view(2, 32).cuda()
+    req, cu, starts = ints([0, 1]), ints([0, 400, 800]), ints([0, 0])
+    q = randn(2, 16, 128, dtype=torch.bfloat16, seed=72)
+    got = []
+    for step in range(12):
+        x = torch.randn((800, 1, 128), generator=g).to(torch.bfloat16).cuda()
+        tokens = torch.stack([torch.randperm(400, generator=g)[:300] for _ in range(2)]).to(torch.int32).cuda()
+        slots, counts = torch.empty_like(tokens), torch.empty(2, dtype=torch.int32, device="cuda")
+        out, lse = results(2, 16, 128, torch.bfloat16)
+        whole, whole_lse = results(2, 16, 128, torch.bfloat16)
+        torch.cuda.synchronize()
+        silkern.append_quantized(x, x, *cache, cu, starts, req, table)
+        silkern.localize_rowwise(req, table, tokens, slots, counts, block_size=16, dcp_size=1, dcp_rank=0)
+        silkern.attend_selected(q, slots, *cache, out, lse, softmax_scale=0.09)
+        silkern.merge_partials(out[None], lse[None], whole, whole_lse)
+        torch.cuda.synchronize()
+        want = oracle.attend_selected(q, slots, *cache, softmax_scale=0.09)
+        assert_attention(out, lse, want, q, cache[0], cache[2], 0.09)
+        assert torch.equal(whole, out)
+        got.append(out)
+    assert not torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("rows,heads", [(16, 16), (19, 16), (37, 16), (75, 16), (150, 16), (310, 16), (444, 64), (520, 64)])
+@pytest.mark.parametrize("shape", ["d64", "latent"])
+def test_batches_around_the_splitting_rules(shape, rows, heads) -> None:
+    """Batches on both sides of where clusters, a CTA's pipelines and leftover
+    items split the keys, with rows of every length among them."""
+    dim, value_dim, latent = SHAPES[shape]
+    cache = make_cache(40, 64, 1, dim, latent=latent, seed=80)
+    g = torch.Generator().manual_seed(rows)
+    slots = torch.randint(0, 2560, (rows, 600), generator=g, dtype=torch.int32)
+    counts = torch.randint(0, 601, (rows,), generator=g, dtype=torch.int32)
+    counts[-5:] = torch.tensor([0, 600, 1, 128, 129])
+    slots, counts = slots.cuda(), counts.cuda()
+    q = randn(rows, heads, dim, dtype=torch.bfloat16, seed=81)
+    out, lse = selected(q, slots, cache, value_dim, softmax_scale=dim**-0.5, counts=counts)
+    want = oracle.attend_selected(q, slots, *cache, softmax_scale=dim**-0.5, counts=counts)
+    assert_attention(out, lse, want, q, cache[0], cache[2], dim**-0.5)
+
+
+def test_odd_queries() -> None:
+    """Zero, tiny, huge and unlike heads of one CTA; a NaN or infinity in one
+    head's query makes that head NaN and no other."""
+    cache = make_cache(4, 64, 1, 128, seed=90)
+    slots = torch.arange(200, dtype=torch.int32).view(1, 200).cuda()
+    for dtype in TYPES:
+        q = randn(1, 12, 128, dtype=dtype, seed=91)
+        q[0, 1] = 0
+        q[0, 2] *= 2.0**-20 if dtype == torch.float16 else 2.0**-60
+        q[0, 3] *= 300.0
+        q[0, 4, 5:] = 0
+        q[0, 5] = 0
+        q[0, 5, 7] = 2.0**-14
+        out, lse = selected(q, slots, cache, 128, softmax_scale=0.09)
+        want = oracle.attend_selected(q, slots, *cache, softmax_scale=0.09)
+        for h in range(12):  # a bound of its own for each head
+            assert_attention(out[:, h : h + 1], lse[:, h : h + 1].contiguous(), tuple(t[:, h : h + 1] for t in want),
+                             q[:, h : h + 1], cache[0], cache[2], 0.09)
+        q[0, 6, 9], q[0, 7, 3] = math.nan, math.inf
+        after, after_lse = selected(q, slots, cache, 128, softmax_scale=0.09)
+        odd = torch.zeros(12, dtype=torch.bool, device="cuda")
+        odd[6:8] = True
+        assert bool(after[0, odd].isnan().all()) and bool(after_lse[0, odd].isnan().all())
+        assert torch.equal(after[0, ~odd], out[0, ~odd]) and torch.equal(after_lse[0, ~odd], lse[0, ~odd])
