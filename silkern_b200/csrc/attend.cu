@@ -80,7 +80,7 @@ int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
     if (columns == 16 || live * 2 * (tiles < kMostCluster ? tiles : kMostCluster) > sms) break;
     columns /= 2;
   }
-  const int64_t units = items * a.cache.kv_heads * blocks, pipes = !latent && columns == 16 ? 2 : 1;
+  const int64_t units = items * a.cache.kv_heads * blocks, pipes = !latent && columns <= 32 ? 2 : 1;
   if (units > 0x3fffffff) return SILKERN_E_SHAPE;
   AttendPlan plan;
   plan.per = make_fastdiv(static_cast<uint32_t>(per));

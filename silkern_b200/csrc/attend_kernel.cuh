@@ -74,7 +74,7 @@ struct Config {
   static constexpr int kTailBytes = kIsLatent ? 64 * kTile : 0;  // a latent key's last 64 bytes
   // Pipelines: a narrow column block's softmax is a chain of short steps, and
   // two of them keep the memory busy.
-  static constexpr int kPipes = !kIsLatent && NH == 16 ? 2 : 1;
+  static constexpr int kPipes = !kIsLatent && NH <= 32 ? 2 : 1;
   static constexpr int kGroups = NH / 16;                        // softmax warpgroups, 16 columns each
   static constexpr int kSoftmax = kGroups * 128;
   static constexpr int kLoaders = kPipes == 2 || NH == 64 ? 2 : 4;  // gathering warps
