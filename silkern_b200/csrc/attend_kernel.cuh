@@ -88,7 +88,7 @@ struct Config {
   // cache are one query's, so that its shared memory need not hold positions.
   static constexpr bool kSeveral = !(kIsLatent && NH == 64);
   static constexpr int kNoteBytes = kTile * ((kIsLatent ? 4 : 8) + (kSeveral ? 4 : 0)) + 16;  // a tile's scales, positions
-  static constexpr int kMisc = NH * (12 + 4 + 8 + (kSeveral ? 16 : 0)) + 320;
+  static constexpr int kMisc = NH * (12 + 4 + 8) + 320;
   // TMEM columns of a pipeline: outputs, and scores twice.
   static constexpr int kPipeColumns = kValues * NH + 2 * T * NH;
   static constexpr int kColumnsUsed = kPipes * kPipeColumns;
@@ -126,7 +126,6 @@ struct __align__(16) Shared {
   int32_t best[3][NH];  // column maxima of a tile, as ordered integers
   float reference[NH];  // 5 - R of the columns' references R
   float factor[2][NH];  // the columns' score factors, of this item and the next
-  int32_t seen_to[2][C::kSeveral ? NH : 1], seen_from[2][C::kSeveral ? NH : 1];  // positions a column sees: below, from
   float k_scale[C::kStages][kTile];
   float v_scale[C::kIsLatent ? 1 : C::kStages][C::kIsLatent ? 1 : kTile];
   int32_t position[C::kSeveral ? C::kStages : 1][C::kSeveral ? kTile : 1];
@@ -168,16 +167,14 @@ __device__ __forceinline__ void split4(const float (&x)[4], uint32_t (&part)[T])
     const bool wide = WEIGHT && t > 0;
     const uint16_t lo = wide ? f32_to_e5m2x2(r[0], r[1]) : f32_to_e4m3x2(r[0], r[1]);
     const uint16_t hi = wide ? f32_to_e5m2x2(r[2], r[3]) : f32_to_e4m3x2(r[2], r[3]);
-    part[t] = lo | (static_cast<uint32_t>(hi) << 16);
+    part[t] = join16(lo, hi);
     if (t + 1 < T) {
       const uint32_t a = wide ? e5m2x2_to_f16x2(lo) : e4m3x2_to_f16x2(lo);
       const uint32_t b = wide ? e5m2x2_to_f16x2(hi) : e4m3x2_to_f16x2(hi);
       const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
       const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
-      r[0] -= fa.x;
-      r[1] -= fa.y;
-      r[2] -= fb.x;
-      r[3] -= fb.y;
+      fma_pair(fa.x, fa.y, -1.f, -1.f, r[0], r[1], r[0], r[1]);
+      fma_pair(fb.x, fb.y, -1.f, -1.f, r[2], r[3], r[2], r[3]);
       if (!WEIGHT) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[i] *= 16.f;
@@ -190,10 +187,10 @@ __device__ __forceinline__ void split4(const float (&x)[4], uint32_t (&part)[T])
 __device__ __forceinline__ void split4_f16(const float (&x)[4], uint32_t (&part)[2]) {
   const uint32_t a = pack_f16x2(x[0], x[1]), b = pack_f16x2(x[2], x[3]);
   const uint16_t a1 = f16x2_to_e4m3x2(a), b1 = f16x2_to_e4m3x2(b);
-  part[0] = a1 | (static_cast<uint32_t>(b1) << 16);
+  part[0] = join16(a1, b1);
   const uint16_t a2 = f16x2_to_e5m2x2(sub_f16x2(a, e4m3x2_to_f16x2(a1)));
   const uint16_t b2 = f16x2_to_e5m2x2(sub_f16x2(b, e4m3x2_to_f16x2(b1)));
-  part[1] = a2 | (static_cast<uint32_t>(b2) << 16);
+  part[1] = join16(a2, b2);
 }
 
 template <typename E>
@@ -218,10 +215,10 @@ __device__ __forceinline__ void unpack4(const uint2 raw, float (&x)[4]) {
 __device__ __forceinline__ void split_query4(const float (&x)[4], uint32_t (&part)[2]) {
   const uint32_t a = pack_f16x2(x[0], x[1]), b = pack_f16x2(x[2], x[3]);
   const uint16_t a1 = f16x2_to_e4m3x2(a), b1 = f16x2_to_e4m3x2(b);
-  part[0] = a1 | (static_cast<uint32_t>(b1) << 16);
+  part[0] = join16(a1, b1);
   const uint16_t a2 = f16x2_to_e4m3x2(mul16_f16x2(sub_f16x2(a, e4m3x2_to_f16x2(a1))));
   const uint16_t b2 = f16x2_to_e4m3x2(mul16_f16x2(sub_f16x2(b, e4m3x2_to_f16x2(b1))));
-  part[1] = a2 | (static_cast<uint32_t>(b2) << 16);
+  part[1] = join16(a2, b2);
 }
 
 // The largest magnitude of four numbers, as the bits of a float's magnitude
@@ -411,7 +408,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           tmem_wait_ld(s1);
           tmem_wait_ld(s2);
 #pragma unroll
-          for (int c = 0; c < 16; ++c) s1[c] += s2[c] * 0.0625f;
+          for (int c = 0; c < 16; c += 2) fma_pair(s2[c], s2[c + 1], 0.0625f, 0.0625f, s1[c], s1[c + 1], s1[c], s1[c + 1]);
         } else {
           tmem_wait_ld(t);
           tmem_wait_ld(s1);
@@ -422,22 +419,30 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 16; c += 4) {
           const float4 f = *reinterpret_cast<const float4*>(&sh.factor[seq & 1][first_col + c]);
-          const float fs[4] = {f.x, f.y, f.z, f.w};
+          float fs[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            t[c + k] = fmaf(fmaf(s1[c + k], 0.0625f, t[c + k]), ks * fs[k], shift);
+          for (int k = 0; k < 4; k += 2) {
+            mul_pair(fs[k], fs[k + 1], ks, ks, fs[k], fs[k + 1]);
+            fma_pair(s1[c + k], s1[c + k + 1], 0.0625f, 0.0625f, t[c + k], t[c + k + 1], t[c + k], t[c + k + 1]);
+            fma_pair(t[c + k], t[c + k + 1], fs[k], fs[k + 1], shift, shift, t[c + k], t[c + k + 1]);
           }
         }
         if constexpr (C::kSeveral) {
           if (several) {
+            // The key is seen by the queries from its own position on, in a window
+            // by the next window - 1 as well, or as a sink by all after it: a run
+            // of the columns.
             const int32_t at = sh.position[b][thread];
-            const bool sink = static_cast<uint32_t>(at) < a.sinks;
+            const bool sink = a.window == 0 || static_cast<uint32_t>(at) < a.sinks;
             if (!(at < all_to && (at >= all_from || sink))) {
+              const int64_t ahead = static_cast<int64_t>(at) - h.position;  // the first query that sees it
+              const int32_t from = static_cast<int32_t>(min(max(ahead, int64_t{0}), int64_t{NH})) * a.heads_per_kv;
+              const int32_t to = sink ? NH : static_cast<int32_t>(min(max(ahead + a.window, int64_t{0}), int64_t{NH})) * a.heads_per_kv;
+              const uint32_t seen = (0xffffu << min(max(from - first_col, 0), 16)) &
+                                    ~(0xffffu << min(max(to - first_col, 0), 16));
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
-                const bool seen = at < sh.seen_to[seq & 1][first_col + c] &&
-                                  (at >= sh.seen_from[seq & 1][first_col + c] || sink);
-                if (!seen) t[c] = -INFINITY;
+                if (!((seen >> c) & 1)) t[c] = -INFINITY;
               }
             }
           }
@@ -502,9 +507,11 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           const float rs[4] = {r.x, r.y, r.z, r.w};
           float x[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[k] = exp2_approx(t[c + k] + rs[k]);
-            l[c + k] = fmaf(x[k], to_sum, l[c + k]);
+          for (int k = 0; k < 4; k += 2) {
+            add_pair(t[c + k], t[c + k + 1], rs[k], rs[k + 1], x[k], x[k + 1]);
+            x[k] = exp2_approx(x[k]);
+            x[k + 1] = exp2_approx(x[k + 1]);
+            fma_pair(x[k], x[k + 1], to_sum, to_sum, l[c + k], l[c + k + 1], l[c + k], l[c + k + 1]);
           }
           if constexpr (T == 2) {
             split4_f16(x, part[c / 4]);
@@ -843,13 +850,6 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           const float up = odd ? 0.f : __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
           if (lane == 0) {
             sh.factor[seq & 1][c] = odd ? NAN : a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
-            if constexpr (C::kSeveral) {
-              const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, c);
-              const int32_t position = work.span.position + col.query;
-              sh.seen_to[seq & 1][c] = col.used ? position + 1 : 0x7fffffff;
-              sh.seen_from[seq & 1][c] = col.used && a.window != 0 && position + 1 > static_cast<int64_t>(a.window)
-                                             ? position + 1 - static_cast<int32_t>(a.window) : 0;
-            }
           }
           __syncwarp();
           // A lane's four columns of piece i are bytes 4 lane on of chunk i; a

@@ -185,6 +185,30 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 
 // ------------------------------------------------------------- numbers
 
+// Two at a time: z = a b + c, z = a b, z = a + b.
+__device__ __forceinline__ void fma_pair(float a0, float a1, float b0, float b1, float c0, float c1, float& z0, float& z1) {
+  asm("{\n .reg .b64 a, b, c, z;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 z, a, b, c;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(z0), "=f"(z1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul_pair(float a0, float a1, float b0, float b1, float& z0, float& z1) {
+  asm("{\n .reg .b64 a, b, z;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 z, a, b;\n"
+      " mov.b64 {%0, %1}, z;\n}"
+      : "=f"(z0), "=f"(z1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add_pair(float a0, float a1, float b0, float b1, float& z0, float& z1) {
+  asm("{\n .reg .b64 a, b, z;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 z, a, b;\n"
+      " mov.b64 {%0, %1}, z;\n}"
+      : "=f"(z0), "=f"(z1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ uint32_t join16(uint16_t lo, uint16_t hi) {
+  uint32_t r;
+  asm("mov.b32 %0, {%1, %2};" : "=r"(r) : "h"(lo), "h"(hi));
+  return r;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
