@@ -25,8 +25,13 @@ contract says (silkern/contract.py:8-36).
 
 Every buffer is the caller's; nothing is allocated and nothing synchronises, so
 calls can be captured in a CUDA graph. They run on the current stream of the
-buffers' device. Each raises :class:`LocalizationError` before launch on an
-unsupported binding or geometry.
+buffers' device. While ``torch.compile`` traces the caller, each routes through
+its op of the same name (:mod:`silkern_b200.ops`). Each raises
+:class:`LocalizationError` before launch on an unsupported binding or geometry.
+
+Attention expects what :func:`append_quantized` writes: finite codes (no NaN
+code, 0x7f or 0xff, at a token that any query of the call sees) and scales that
+are 0, NaN or in [2**-100, 2**100].
 """
 
 from __future__ import annotations
@@ -34,10 +39,10 @@ from __future__ import annotations
 import ctypes
 import math
 
-from silkern_b200 import _native
+from silkern_b200 import _native, ops
 from silkern_b200.contract import _validate_dcp_config
 from silkern_b200.errors import LocalizationError
-from silkern_b200.kernels import _check_status, _is_int
+from silkern_b200.kernels import _check_status, _compiling, _is_int, _traced_op
 
 #: Dimensions of a latent cache: keys, and the leading part that is the value.
 LATENT_KEY_DIM = 576
@@ -82,6 +87,8 @@ def _on_device(torch, tensors, what: str) -> int:
 
 def _launch(torch, device: int, what: str, entry, *args) -> None:
     """Call ``entry(*args, stream)`` on the current stream of ``device``."""
+    if not ops.registered():
+        ops.register()
     stream = torch._C._cuda_getCurrentRawStream(device)
     if device == torch.cuda.current_device():
         code = entry(*args, stream)
@@ -226,6 +233,10 @@ def append_quantized(
     """
     import torch
 
+    if _compiling(torch):
+        return _traced_op(torch, "append_quantized")(
+            keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table, dcp_size,
+            dcp_rank, dcp_interleave, status)
     device = _on_device(
         torch, (keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table),
         "append")
@@ -291,6 +302,9 @@ def attend_selected(
     """
     import torch
 
+    if _compiling(torch):
+        return _traced_op(torch, "attend_selected")(
+            q, slots, k_cache, v_cache, k_scale, v_scale, out, lse, softmax_scale, counts, status)
     device = _on_device(torch, (q, slots, k_cache, v_cache, k_scale, v_scale, out, lse, counts), "attention")
     _check_ints(torch, (counts,), "counts")
     cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
@@ -352,6 +366,10 @@ def attend_window(
     """
     import torch
 
+    if _compiling(torch):
+        return _traced_op(torch, "attend_window")(
+            q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale, out, lse,
+            softmax_scale, window, sinks, dcp_size, dcp_rank, dcp_interleave, status)
     device = _on_device(
         torch, (q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale, out, lse),
         "attention")
@@ -387,6 +405,8 @@ def merge_partials(outs, lses, out, lse=None) -> None:
     """
     import torch
 
+    if _compiling(torch):
+        return _traced_op(torch, "merge_partials")(outs, lses, out, lse)
     device = _on_device(torch, (outs, lses, out, lse), "merge")
     dtype = outs.dtype
     code = _type_code(torch, dtype)

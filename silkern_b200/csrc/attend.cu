@@ -93,7 +93,9 @@ int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
   // kernels (148 SMs: 74 of 2, 33 of 4, 15 of 8; 7 of 16).
   unsigned cluster = 1;
   const int64_t room[3] = {sms / 2, sms * 33 / 148, sms * 15 / 148};
-  for (int k = 0; k < 3 && live <= room[k] && tiles >= cluster * 2 * pipes; ++k) cluster *= 2;
+  for (int k = 0; k < 3 && live <= room[k] && tiles >= cluster * 2 * pipes && units * cluster * 2 <= 0x7fffffff; ++k) {
+    cluster *= 2;
+  }
   int64_t grid;
   if (cluster > 1 || (pipes > 1 && units <= sms && tiles >= pipes)) {
     plan.whole = 0;

@@ -425,7 +425,8 @@ int check_queries(const silkern_cache_v1* c, const void* q, int64_t q_row, int64
   if (rows < 1 || rows > 0x7fffffff) return SILKERN_E_SHAPE;
   if (heads < 1 || heads > 65535 || heads % c->kv_heads != 0) return SILKERN_E_HEADS;
   if (q_row % 8 != 0 || q_head % 8 != 0 || reinterpret_cast<uintptr_t>(q) % 16 != 0) return SILKERN_E_CACHE;
-  if (!std::isfinite(softmax_scale)) return SILKERN_E_ATTEND;
+  a->scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (!std::isfinite(a->scale_log2)) return SILKERN_E_ATTEND;
   a->q = q;
   a->q_row = q_row;
   a->q_head = q_head;
@@ -434,11 +435,9 @@ int check_queries(const silkern_cache_v1* c, const void* q, int64_t q_row, int64
   a->out_head = out_head;
   a->out_wide = out_row % 8 == 0 && out_head % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   a->lse = lse;
-  a->scale_log2 = softmax_scale * 1.4426950408889634f;
   a->rows = static_cast<int32_t>(rows);
   a->heads = heads;
   a->heads_per_kv = heads / c->kv_heads;
-  a->one = make_fastdiv(1);
   return SILKERN_OK;
 }
 

@@ -88,7 +88,6 @@ struct AttendArgs {
   int32_t sequences;
   uint32_t window;  // 0: the whole context
   uint32_t sinks;
-  FastDiv one;  // by 1
   Ownership own;
 };
 

@@ -15,7 +15,7 @@ torch = pytest.importorskip("torch")
 
 import silkern_b200 as silkern  # noqa: E402
 from oracle import attention as oracle  # noqa: E402
-from silkern_b200 import _native  # noqa: E402
+from silkern_b200 import _native, ops  # noqa: E402
 from silkern_b200.build import build  # noqa: E402
 from tests.attention_cases import make_cache  # noqa: E402
 
@@ -207,3 +207,55 @@ def test_oracle_append_scales_are_the_smallest_powers_of_two() -> None:
         s = float(scale[0, 0])
         assert math.frexp(s)[0] == 0.5 and 448 * s >= min(most, 448 * 2.0**100)
         assert s == 2.0**-100 or s / 2 * 448 < most
+
+
+# ---------------------------------------------------------------------- further refusals, ops
+
+def test_a_scale_that_overflows_in_base_two_is_refused(lib) -> None:
+    """3e38 is a float32, 3e38 * log2(e) is not."""
+    assert selected(lib, cache(), scale=3e38) == 12
+    assert window(lib, cache(), scale=-3e38) == 12
+
+
+def test_ops_mark_exactly_the_written_buffers() -> None:
+    ops.register()
+    written = {name: {a.name for a in getattr(torch.ops.silkern_b200, name).default._schema.arguments
+                      if a.alias_info is not None and a.alias_info.is_write}
+               for name in ("append_quantized", "attend_selected", "attend_window", "merge_partials")}
+    assert written == {"append_quantized": {"k_cache", "v_cache", "k_scale", "v_scale", "status"},
+                       "attend_selected": {"out", "lse", "status"}, "attend_window": {"out", "lse", "status"},
+                       "merge_partials": {"out", "lse"}}
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_launchers_trace_as_op_nodes_without_a_graph_break(latent) -> None:
+    """One node for each of the four launchers, and fake implementations that
+    launch nothing; the backend only inspects the graph."""
+    ops.register()
+    graphs = []
+
+    def inspect(gm, example_inputs):
+        graphs.append(gm)
+        return lambda *args: None
+
+    k, v, ks, vs = make_cache(2, 4, 1, 576 if latent else 64, latent=latent, device="cpu")
+    dim, value_dim = (576, 512) if latent else (64, 64)
+    q = torch.zeros((1, 2, dim), dtype=torch.bfloat16)
+    new = torch.zeros((1, 1, dim), dtype=torch.bfloat16)
+    ints = torch.zeros(2, dtype=torch.int32)
+    table = torch.zeros((1, 1), dtype=torch.int32)
+    outs, lses = torch.zeros((2, 1, 2, value_dim), dtype=torch.bfloat16), torch.zeros(2, 1, 2)
+    out = torch.zeros((1, 2, value_dim), dtype=torch.bfloat16)
+
+    def step(q, new, ints, one, table, outs, lses, out):
+        silkern.append_quantized(new, None if latent else new, k, v, ks, vs, ints, one, one, table)
+        silkern.attend_selected(q, table, k, v, ks, vs, outs[0], lses[0], softmax_scale=0.1, counts=one)
+        silkern.attend_window(q, ints, one, one, table, k, v, ks, vs, outs[1], lses[1], softmax_scale=0.1, window=3)
+        silkern.merge_partials(outs, lses, out)
+
+    torch._dynamo.reset()
+    torch.compile(step, backend=inspect, fullgraph=True)(q, new, ints, ints[:1].clone(), table, outs, lses, out)
+    assert len(graphs) == 1
+    targets = [str(node.target) for node in graphs[0].graph.nodes if node.op == "call_function"]
+    for name in ("append_quantized", "attend_selected", "attend_window", "merge_partials"):
+        assert sum(f"silkern_b200.{name}" in t for t in targets) == 1

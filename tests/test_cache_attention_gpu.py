@@ -760,3 +760,56 @@ def test_odd_queries() -> None:
         odd[6:8] = True
         assert bool(after[0, odd].isnan().all()) and bool(after_lse[0, odd].isnan().all())
         assert torch.equal(after[0, ~odd], out[0, ~odd]) and torch.equal(after_lse[0, ~odd], lse[0, ~odd])
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_compiled_step_in_a_graph_is_the_eager_step(latent) -> None:
+    """append, both attentions and merge under torch.compile, captured and
+    replayed: bit for bit what the launchers give when called one by one."""
+    from silkern_b200 import ops
+
+    ops.register()
+    dim, value_dim, heads = (576, 512, 32) if latent else (128, 128, 16)
+    kv_heads = 1 if latent else 4
+    cache = [t if t is None else t.clone() for t in make_cache(12, 16, kv_heads, dim, latent=latent, seed=50)]
+    other = [t if t is None else t.clone() for t in cache]
+    table = torch.randperm(12, generator=torch.Generator().manual_seed(51)).to(torch.int32).view(3, 4).cuda()
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    cu, starts, lengths, req = ints(0, 1, 2, 3), ints(20, 0, 47), ints(21, 1, 48), ints(1, 0, 2)
+    slots = torch.randint(-1, 192, (3, 70), dtype=torch.int32, generator=torch.Generator().manual_seed(52)).cuda()
+    q = randn(3, heads, dim, dtype=torch.bfloat16, seed=53)
+    new = randn(3, kv_heads, dim, dtype=torch.bfloat16, seed=54)
+
+    def step(cache, outs, lses, out, lse):
+        silkern.append_quantized(new, None if latent else new, *cache, cu, starts, req, table)
+        silkern.attend_selected(q, slots, *cache, outs[0], lses[0], softmax_scale=0.05)
+        silkern.attend_window(q, cu, lengths, req, table, *cache, outs[1], lses[1], softmax_scale=0.05, window=30, sinks=2)
+        silkern.merge_partials(outs, lses, out, lse)
+
+    def buffers():
+        return (torch.zeros((2, 3, heads, value_dim), dtype=torch.bfloat16, device="cuda"),
+                torch.zeros((2, 3, heads), device="cuda"), *results(3, heads, value_dim, torch.bfloat16))
+
+    want = buffers()
+    step(cache, *want)
+    torch.cuda.synchronize()
+    got = buffers()
+    torch._dynamo.reset()
+    compiled = torch.compile(step, fullgraph=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            compiled(other, *got)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        compiled(other, *got)
+    for t in got:
+        t.zero_()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    same_cache(other, cache)
