@@ -11,8 +11,6 @@ namespace silkern {
 
 namespace {
 
-constexpr int64_t kMostCluster = 8;
-
 int multiprocessors() {
   int device = 0, n = 0;
   if (cudaGetDevice(&device) != cudaSuccess ||
@@ -77,7 +75,7 @@ int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
     // While clusters over all keys still leave half of the SMs without work,
     // half the columns to a CTA: its queries are split, and its outputs
     // joined, in half the time (one row of 128 heads: 21.4 -> 12.5 us).
-    if (columns == 16 || live * 2 * (tiles < kMostCluster ? tiles : kMostCluster) > sms) break;
+    if (columns == 16 || live * 2 * (tiles < 8 ? tiles : 8) > sms) break;
     columns /= 2;
   }
   const int64_t units = items * a.cache.kv_heads * blocks, pipes = !latent && columns <= 32 ? 2 : 1;
@@ -87,14 +85,21 @@ int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
   plan.group = make_fastdiv(static_cast<uint32_t>(group));
   plan.blocks = static_cast<int32_t>(blocks);
   plan.units = static_cast<uint32_t>(units);
-  // Few work items: as many CTAs as still find an SM and a tile for each of
-  // their pipelines, up to a cluster of 8, share each item's keys. How many
-  // clusters find room at once is the occupancy calculator's answer for these
-  // kernels (148 SMs: 74 of 2, 33 of 4, 15 of 8; 7 of 16).
+  // Few work items: CTAs share each item's keys, as a cluster of up to 16 that
+  // leaves room for a cluster of every item, and of the sizes that give a
+  // pipeline equally many tiles at most the smallest. Clusters come in any
+  // size, since SMs do: of a B200's 148, clusters of 8 reach 120, of 9 or 3
+  // 135, of 6 132.
   unsigned cluster = 1;
-  const int64_t room[3] = {sms / 2, sms * 33 / 148, sms * 15 / 148};
-  for (int k = 0; k < 3 && live <= room[k] && tiles >= cluster * 2 * pipes && units * cluster * 2 <= 0x7fffffff; ++k) {
-    cluster *= 2;
+  if (live * 2 <= sms) {
+    int64_t least = (tiles + pipes - 1) / pipes;  // tiles of a pipeline
+    for (unsigned size = 2; size <= kMostCluster; ++size) {
+      const int64_t ranks = size * pipes, most = (tiles + ranks - 1) / ranks;
+      if (most < least && tiles >= ranks && units * size <= 0x7fffffff && live <= resident_clusters(size)) {
+        cluster = size;
+        least = most;
+      }
+    }
   }
   int64_t grid;
   if (cluster > 1 || (pipes > 1 && units <= sms && tiles >= pipes)) {

@@ -101,7 +101,8 @@ struct Config {
   static constexpr int kStages = kIsLatent ? 2 : kFit < 8 ? kFit : 8;
   static constexpr int kTails = kIsLatent ? ((kPipeBytes - kFixed - 2 * kStageCost) >= 2 * kTailBytes ? 2 : 1) : 0;
   static_assert(kStages >= 2 && kFixed + kStages * kStageCost + kTails * kTailBytes <= kPipeBytes, "shared memory");
-  static_assert(NH * kValueDim * 4 <= kStages * kStageBytes, "joining buffer");
+  // Ranks that may share an item, and the columns that their shares round up to.
+  static constexpr int kMostRanks = kMostCluster * kPipes;
   // The chunk whose buffer is free again only after a tile's softmax, and
   // with it the tile's scales and positions.
   static constexpr int kNoteChunk = kIsLatent ? 0 : 1;
@@ -110,6 +111,7 @@ struct Config {
   static constexpr int kOffQ = kOffTail + kTails * kTailBytes;
   static constexpr int kOffP = kOffQ + kQBytes;
   static constexpr int kOffMisc = kOffP + kPBytes;
+  static_assert((NH + kMostRanks - 1) * kValueDim * 4 <= kOffP, "joining buffer");
 };
 
 // A work item as its query warps hand it to the softmax and the MMAs.
@@ -1008,8 +1010,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     }
   }
   if (last.split) {
-    constexpr int kMostRanks = 16;
-    const uint32_t share = NH / ranks;  // both are powers of two, ranks at most 16
+    const uint32_t share = (NH + ranks - 1) / ranks;                    // columns of a rank at most
     float* joint = reinterpret_cast<float*>(smem + C::kOffP) + 8 * NH;  // references, then sums
     float* joined = reinterpret_cast<float*>(smem);                     // outputs: (rank, column of this rank, value)
     const int first_col = (warp >> 2) * 16, own = lane & 15;
@@ -1021,28 +1022,33 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     // Rank r is pipeline r mod kPipes of CTA r / kPipes.
     const uint32_t origin = smem_addr(all_smem);
     auto place = [&](const float* p, uint32_t r) {
-      return origin + (r % C::kPipes) * C::kPipeBytes + (smem_addr(p) - base);
+      return map_cluster(origin + (r % C::kPipes) * C::kPipeBytes + (smem_addr(p) - base), r / C::kPipes);
     };
     if (warp < kLoadWarp) {
+      // A column's ranks, the even ones in one lane and the odd ones in another.
       const float* at = joint + first_col + own;
-      float rr[kMostRanks], ll[kMostRanks];
+      constexpr int kHalf = C::kMostRanks / 2;
+      float rr[kHalf], ll[kHalf];
 #pragma unroll
-      for (uint32_t r = 0; r < kMostRanks; ++r) {
-        rr[r] = -INFINITY;
-        ll[r] = 0.f;
+      for (uint32_t k = 0; k < kHalf; ++k) {
+        const uint32_t r = 2 * k + (lane >> 4);
+        rr[k] = -INFINITY;
+        ll[k] = 0.f;
         if (r < ranks) {
-          rr[r] = ld_cluster(place(at, r), r / C::kPipes);
-          ll[r] = ld_cluster(place(at + NH, r), r / C::kPipes);
+          rr[k] = ld_cluster(place(at, r));
+          ll[k] = ld_cluster(place(at + NH, r));
         }
       }
       float whole_r = -INFINITY, whole_l = 0.f;
 #pragma unroll
-      for (uint32_t r = 0; r < kMostRanks; ++r) whole_r = fmaxf(whole_r, rr[r]);
+      for (uint32_t k = 0; k < kHalf; ++k) whole_r = fmaxf(whole_r, rr[k]);
+      whole_r = fmaxf(whole_r, __shfl_xor_sync(kAllLanes, whole_r, 16));
 #pragma unroll
-      for (uint32_t r = 0; r < kMostRanks; ++r) {
+      for (uint32_t k = 0; k < kHalf; ++k) {
         // (A rank without a reference saw nothing, or only what is not a number.)
-        whole_l += rr[r] == -INFINITY ? ll[r] : ll[r] * exp2_approx(rr[r] - whole_r);
+        whole_l += rr[k] == -INFINITY ? ll[k] : ll[k] * exp2_approx(rr[k] - whole_r);
       }
+      whole_l += __shfl_xor_sync(kAllLanes, whole_l, 16);
       const float inverse = whole_l == 0.f ? 0.f : 1.f / (32.f * whole_l);
       const float by = reference == -INFINITY ? 0.f : exp2_approx(reference - whole_r) * inverse;
       if (rank == 0 && (warp & 3) == 0 && lane < 16 && *abort == 0) {
@@ -1054,8 +1060,12 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       }
       __syncwarp();
       tc_fence_after();
-      // Rank r joins the columns [r, r + 1) * share, and gets every rank's part
-      // of them: stores need no answer, loads would wait for one.
+      // Rank r joins the columns from NH r / ranks to NH (r + 1) / ranks, and
+      // gets every rank's part of them: stores need no answer, loads would wait
+      // for one.
+      const uint32_t joiner = ((first_col + own + 1) * ranks - 1) / NH;
+      const uint32_t joined_at =
+          place(joined + (rank * share + first_col + own - NH * joiner / ranks) * C::kValueDim, joiner);
       if (SHAPE != kDim64 || (warp & 3) < 2) {
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
 #pragma unroll 1
@@ -1070,18 +1080,18 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             const float f = __shfl_sync(kAllLanes, by, c);
-            const uint32_t to = (first_col + c) / share, col = (first_col + c) % share;
-            st_cluster(place(joined + (rank * share + col) * C::kValueDim + m * 128 + (tid & 127), to), to / C::kPipes,
-                       last.steps > 0 ? o[c] * f : 0.f);
+            const uint32_t to = __shfl_sync(kAllLanes, joined_at, c);
+            st_cluster(to + (m * 128 + (tid & 127)) * 4, last.steps > 0 ? o[c] * f : 0.f);
           }
         }
       }
     }
     cluster_sync();  // the last time that a CTA touches another's memory is before
     constexpr int kRankThreads = C::kPipeWarps * 32;
-    for (int32_t e = tid * 4; e < static_cast<int32_t>(share) * C::kValueDim; e += kRankThreads * 4) {
+    const int32_t mine = NH * rank / ranks, joins = NH * (rank + 1) / ranks - mine;
+    for (int32_t e = tid * 4; e < joins * C::kValueDim; e += kRankThreads * 4) {
       const int32_t c = e / C::kValueDim, d = e - c * C::kValueDim;
-      const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, rank * share + c);
+      const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, mine + c);
       if (!col.used || *abort != 0) continue;
       float4 y{0.f, 0.f, 0.f, 0.f};
       for (uint32_t r = 0; r < ranks; ++r) {

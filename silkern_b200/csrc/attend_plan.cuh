@@ -6,6 +6,9 @@
 
 namespace silkern {
 
+// CTAs of a thread-block cluster at most.
+constexpr int kMostCluster = 16;
+
 struct AttendPlan {
   FastDiv per;     // queries of one sequence that share a work item
   FastDiv group;   // by heads to a cache head
@@ -21,6 +24,10 @@ struct AttendLaunch {
   unsigned grid, cluster;
   cudaStream_t stream;
 };
+
+// How many clusters of `size` CTAs of these kernels (which all take a whole SM)
+// the current device holds at once. Asked once for each device; 0 on failure.
+int resident_clusters(int size);
 
 int launch_dim64(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);
 int launch_dim128(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);

@@ -813,3 +813,19 @@ def test_compiled_step_in_a_graph_is_the_eager_step(latent) -> None:
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     same_cache(other, cache)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("heads", [5, 30, 64])
+@pytest.mark.parametrize("rows", [1, 2, 8, 11, 15, 21, 26, 33, 44])
+def test_items_shared_by_clusters_of_any_size(shape, dtype, heads, rows) -> None:
+    """As many rows as clusters of 16, 10, 9, 6, 5, 4 and 3 have room for, or a
+    row more or less: ranks that are no power of two, more ranks than columns."""
+    dim, value_dim, latent = SHAPES[shape]
+    cache = make_cache(90, 64, 1, dim, latent=latent, seed=rows)
+    slots = torch.randint(-1, 90 * 64, (rows, 4229), dtype=torch.int32, generator=torch.Generator().manual_seed(rows)).cuda()
+    q = randn(rows, heads, dim, dtype=dtype, seed=heads)
+    out, lse = selected(q, slots, cache, value_dim, softmax_scale=dim**-0.5)
+    want = oracle.attend_selected(q, slots, *cache, softmax_scale=dim**-0.5)
+    assert_attention(out, lse, want, q, cache[0], cache[2], dim**-0.5)
