@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         end = true;
       }
       constexpr int kPieces = (C::kKeyDim / 4 + 31) / 32;
-      constexpr int kBatch = 2;  // columns whose loads overlap
+      constexpr int kBatch = 2;  // columns side by side: a column's own steps follow one another
       uint2 raw[kBatch][kPieces];
       auto bring = [&](int c0) {
 #pragma unroll
@@ -839,43 +839,48 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           for (int i = 0; i < kPieces; ++i) now[n][i] = raw[n][i];
         }
         if (c0 + C::kSplitters * kBatch < NH) bring(c0 + C::kSplitters * kBatch);  // the next ones come during these
+        uint32_t most[kBatch];
+        float up[kBatch];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
-          const int c = c0 + n;
-          uint32_t most = 0;
+          most[n] = 0;
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) most = max(most, magnitude4<E>(now[n][i]));
-          most = __reduce_max_sync(kAllLanes, most);
+          for (int i = 0; i < kPieces; ++i) most[n] = max(most[n], magnitude4<E>(now[n][i]));
+        }
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) most[n] = __reduce_max_sync(kAllLanes, most[n]);
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
           // The largest magnitude comes to [128, 256): its exponent field is taken off.
-          const int e = max(static_cast<int>(most >> 23), 40);
-          const bool odd = most >= 0x7f800000u;  // an infinity or NaN: the row becomes NaN
-          const float up = odd ? 0.f : __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
-          if (lane == 0) {
-            sh.factor[seq & 1][c] = odd ? NAN : a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
-          }
-          __syncwarp();
-          // A lane's four columns of piece i are bytes 4 lane on of chunk i; a
-          // part's rows lie NH rows behind the part before.
-          const uint32_t wide_at = base + C::kOffQ + c * 128 + ((((lane >> 2) ^ c) & 7) << 4) + (lane & 3) * 4;
-          const uint32_t narrow_at = base + C::kOffQ + c * 64 + ((((lane >> 2) ^ (c >> 1)) & 3) << 4) + (lane & 3) * 4;
+          const int e = max(static_cast<int>(most[n] >> 23), 40);
+          const bool odd = most[n] >= 0x7f800000u;  // an infinity or NaN: the row becomes NaN
+          up[n] = odd ? 0.f : __uint_as_float(static_cast<uint32_t>(134 + 127 - e) << 23);
+          if (lane == n) sh.factor[seq & 1][c0 + n] = odd ? NAN : a.scale_log2 * __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
+        }
+        __syncwarp();
+        // A lane's four columns of piece i are bytes 4 lane on of chunk i; a
+        // part's rows lie NH rows behind the part before.
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            const bool narrow = C::kWide == 64 || (C::kIsLatent && i == 4);
+        for (int i = 0; i < kPieces; ++i) {
+          const bool narrow = C::kWide == 64 || (C::kIsLatent && i == 4);
+#pragma unroll
+          for (int n = 0; n < kBatch; ++n) {
+            const int c = c0 + n;
             float y[4];
             unpack4<E>(now[n][i], y);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] *= up;
+            mul_pair(y[0], y[1], up[n], up[n], y[0], y[1]);
+            mul_pair(y[2], y[3], up[n], up[n], y[2], y[3]);
             uint32_t part[T];
             if constexpr (T == 2) {
               split_query4(y, part);
             } else {
               split4<T, false>(y, part);
             }
+            const uint32_t at = base + C::kOffQ + (lane & 3) * 4 + i * (T * NH * 128) +
+                                (narrow ? c * 64 + ((((lane >> 2) ^ (c >> 1)) & 3) << 4) : c * 128 + ((((lane >> 2) ^ c) & 7) << 4));
             if (!narrow || lane < 16) {
 #pragma unroll
-              for (int t = 0; t < T; ++t) {
-                st_shared((narrow ? narrow_at + t * (NH * 64) : wide_at + t * (NH * 128)) + i * (T * NH * 128), part[t]);
-              }
+              for (int t = 0; t < T; ++t) st_shared(at + t * (NH * (narrow ? 64 : 128)), part[t]);
             }
           }
         }
