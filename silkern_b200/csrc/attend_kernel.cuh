@@ -30,14 +30,21 @@
 // A CTA is one or two pipelines, each a softmax of one key a thread and 16
 // columns a warpgroup, warps that gather keys and values with cp.async (the TMA
 // unit's four-row gathers took 61 cycles for 512 bytes of an SM here, these
-// copies about 12), warps that split the queries, and one that issues the MMAs. Every kernel that
-// allocates TMEM has an SM to itself, so a CTA stays on its SM and its
-// pipelines walk through the work items; each role runs ahead as far as the
+// copies about 12), warps that split the queries, and one that issues the MMAs.
+// The kernel takes all of an SM's shared memory, so a CTA stays on its SM and
+// its pipelines walk through the work items; each role runs ahead as far as the
 // buffers let it, and one item's start and end hide behind its neighbours'.
 // Work items that are few, or left over after whole rounds, are split over
 // their keys: by the pipelines of a CTA and of a thread-block cluster, which
 // join their sums and outputs through (distributed) shared memory. No
 // workspace, one launch.
+//
+// Measured: a decode step of 128 sequences, 8 heads of 128, window 4096 (1.02
+// GB): 197-209 us, 5.2 TB/s, bound by memory. 256 rows of 512 latent keys, 128
+// heads: 85 us, 428 TFLOP/s, bound by an item's start and end (four tiles
+// between them). 4001 queries of a prompt, window 1024, heads of 64, fp16: 256
+// us, bound by the softmax's instructions. One row over 131072 tokens: 80 us,
+// 3.3 TB/s on the 80 SMs that clusters for 8 heads reach.
 #pragma once
 
 #include <cuda_bf16.h>
