@@ -20,12 +20,23 @@
 // N (their scores are added in float32, each with its own scale); P's parts
 // are added up in the accumulator.
 //
-// Weights: with u_j = log2(p_j) + log2(vscale_j) and R a reference near the
-// tile's largest u, P'_j = 2^(u_j - R + 5) goes to the tensor core and
-// 2^(log2 p_j - R) to the sum, so out = O / (32 l) and lse = (R + log2 l) ln 2
-// hold for any scales in [2^-100, 2^100]. R moves, and O and l are rescaled,
-// only when a tile's largest u leaves [R - 4, R + 3.5]: e4m3 ends at 448 =
-// 2^8.8. l, S and O are float32.
+// Weights: with s_j = log2(p_j), u_j = s_j + log2(vscale_j) and R a reference
+// near the tile's largest u, P'_j = 2^(u_j - R + 5) goes to the tensor core, and
+// 2^(s_j - Q) to the sum l: out = O 2^(R - Q) / (32 l), lse = (Q + log2 l) ln 2.
+// R moves, and O is rescaled, only when a tile's largest u leaves [R - 4, R +
+// 3.5]: e4m3 ends at 448 = 2^8.8. l, S and O are float32.
+//
+// The sum's own reference Q: as long as an item's value scales lie within
+// 2^kUsual of 1, Q is R, and 2^(s_j - Q) is P'_j 2^-5 / vscale_j. R is at most
+// the largest u so far, and at least 60 below it and 3.5 below the tile's, so
+// that l is at most 2^31 keys of 2^(3.5 + kUsual + 60), in float32 with room;
+// and P' of a key 40 below the largest s is above 2^(5 - 40 - 2 kUsual), which
+// is not flushed. From the first tile with another scale on (0, whose values
+// count nothing, goes into u as 2^-100) each warp keeps a Q of its own, the
+// largest s of its keys, and takes a second exponential for the sum; at the
+// item's end O and l come to one reference again. That holds for any scales in
+// [2^-100, 2^100], in any order, and costs the usual ones 0 to 4 % (a flag of
+// the tile, looked at behind the barrier that the maxima need anyway).
 //
 // A CTA is one or two pipelines, each a softmax of one key a thread and 16
 // columns a warpgroup, warps that gather keys and values with cp.async (the TMA
@@ -64,6 +75,9 @@ namespace silkern {
 enum CacheShape { kDim64, kDim128, kLatent };
 
 constexpr int kTile = 128;
+// Value scales from 2^-kUsual to 2^kUsual share the sum's reference with the
+// outputs': every page of values with a largest magnitude from 2^-15 to 2^32.
+constexpr float kUsual = 24.f;
 // All of an SM's shared memory that a CTA can have.
 constexpr int kSharedMemory = 227 * 1024;
 
@@ -133,8 +147,8 @@ struct Handed {
 template <typename C, int NH>
 struct __align__(16) Shared {
   int32_t best[3][NH];  // column maxima of a tile, as ordered integers
-  float reference[NH];  // 5 - R of the columns' references R
-  float factor[2][NH];  // the columns' score factors, of this item and the next
+  alignas(16) float reference[NH];  // 5 - R of the columns' references R; read four at a time, like the factors
+  alignas(16) float factor[2][NH];  // the columns' score factors, of this item and the next
   float k_scale[C::kStages][kTile];
   float v_scale[C::kIsLatent ? 1 : C::kStages][C::kIsLatent ? 1 : kTile];
   int32_t position[C::kSeveral ? C::kStages : 1][C::kSeveral ? kTile : 1];
@@ -142,6 +156,7 @@ struct __align__(16) Shared {
   Handed handed[2];
   Handed last;          // the split item, as soon as it is known
   int32_t last_known;
+  uint32_t unusual[C::kGroups];  // the last item with an unusual scale, counted from 1
   uint64_t full[C::kLoadChunks][C::kStages], empty[C::kLoadChunks][C::kStages];
   uint64_t scores[2], weights, done;
   uint64_t queries[2], queries_read, finished[2];
@@ -263,6 +278,14 @@ __device__ __forceinline__ float sum_columns(float (&x)[N], int lane) {
   return y;
 }
 
+// 2^x in two factors, since R may lie further below Q than float32 goes: the
+// first is 1 down to x = -60.
+__device__ __forceinline__ float2 exp2_factors(float x) {
+  const bool far = x < -60.f;
+  const float y = exp2_approx(far ? 0.5f * x : x);
+  return make_float2(far ? y : 1.f, y);
+}
+
 // One work item's share of a rank.
 struct Work {
   QuerySpan span;
@@ -356,6 +379,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     sh.best[0][tid] = ordered(-INFINITY);
     sh.reference[tid] = 5.f;
   }
+  if (tid < C::kGroups) sh.unusual[tid] = 0;
   S& first = *reinterpret_cast<S*>(all_smem + C::kOffMisc);
   if (pipe == 0 && warp == kMmaWarp) tmem_alloc(smem_addr(&first.tmem), C::kColumns);
   tc_fence_before();
@@ -375,7 +399,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
   const bool has_split = split_unit < plan.units;
   // Softmax state that outlives the loop for a split item.
   float l[16];
-  float reference = -INFINITY;
+  float reference = -INFINITY;  // R of column `own`
 
   if (warp < kLoadWarp) {
     // ==================================================== softmax
@@ -399,17 +423,23 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       for (int c = 0; c < 16; ++c) l[c] = 0.f;
       reference = -INFINITY;
       float highest = -INFINITY;
-      for (int32_t i = 0; i < h.steps; ++i) {
+      float t[16];              // a tile's scores, then u
+      bool valid;               // this thread's key of it: whether it counts,
+      float vs, scale, shift;   // its values' scale, the one used, its logarithm
+      float top;                // column own's largest u
+      float own_reference;      // Q of column own, where it is the warp's own
+      // A tile up to its columns' maxima.
+      auto begin_tile = [&]() {
         warp_wait(&sh.scores[n & 1], (n >> 1) & 1, abort);
         tc_fence_after();
         const uint32_t s_at = tmem + lanes + C::kValues * NH + (n & 1) * (T * NH) + first_col;
-        float t[16], s1[16];
+        float s1[16];
         tmem_ld16(s_at, t);
         tmem_ld16(s_at + NH, s1);
         warp_wait(&sh.full[C::kNoteChunk][b], turn, abort);
-        const bool valid = (sh.valid[b][warp & 3] >> lane) & 1;
+        valid = (sh.valid[b][warp & 3] >> lane) & 1;
         const float ks = sh.k_scale[b][thread];
-        const float vs = C::kIsLatent ? ks : sh.v_scale[C::kIsLatent ? 0 : b][C::kIsLatent ? 0 : thread];
+        vs = C::kIsLatent ? ks : sh.v_scale[C::kIsLatent ? 0 : b][C::kIsLatent ? 0 : thread];
         if constexpr (T == 3) {
           float s2[16];
           tmem_ld16(s_at + 2 * NH, s2);
@@ -423,8 +453,8 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           tmem_wait_ld(s1);
         }
         // u = log2(p) + log2(vscale): where the key is masked, -inf.
-        const float scale = vs > 0.f ? fminf(fmaxf(vs, 0x1p-100f), 0x1p+100f) : vs == 0.f ? 0x1p-100f : vs;  // NaN stays
-        const float shift = valid ? __log2f(scale) : -INFINITY;
+        scale = vs > 0.f ? fminf(fmaxf(vs, 0x1p-100f), 0x1p+100f) : vs == 0.f ? 0x1p-100f : vs;  // NaN stays
+        shift = valid ? __log2f(scale) : -INFINITY;
 #pragma unroll
         for (int c = 0; c < 16; c += 4) {
           const float4 f = *reinterpret_cast<const float4*>(&sh.factor[seq & 1][first_col + c]);
@@ -457,7 +487,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           }
         }
         // Largest u of each column: lane c of a warp has column c's.
-        float top = -INFINITY;
+        top = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
           const float m = warp_max(t[c]);
@@ -469,8 +499,15 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           atomicMax(&best[first_col + lane], ordered(top));
           if ((warp & 3) == 0) sh.best[n3][first_col + lane] = ordered(-INFINITY);
         }
+        if (valid && !(fabsf(shift) <= kUsual)) sh.unusual[wg] = seq + 1;
         named_barrier(group_barrier, 128);
         top = unordered(best[first_col + own]);
+      };
+      // The rest, with the sum's reference R, or (APART) one of the warp's own.
+      // False, and nothing done, where it has to be the latter.
+      auto end_tile = [&](int32_t i, auto apart_tag) {
+        constexpr bool APART = decltype(apart_tag)::value;
+        if (!APART && __any_sync(kAllLanes, sh.unusual[wg] == seq + 1)) return false;
         const bool move = top > reference + 3.5f || (top < reference - 4.f && top > highest - 60.f);
         bool waited = i == 0;  // an item's end waits for its last outputs
         if (__any_sync(kAllLanes, move)) {
@@ -489,7 +526,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             f[c] = __shfl_sync(kAllLanes, by, c);
-            l[c] *= f[c];
+            if (!APART) l[c] *= f[c];
           }
           if (i > 0) {
 #pragma unroll 1
@@ -505,9 +542,23 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
             tmem_wait_st();
           }
         }
+        if constexpr (APART) {
+          const float back = valid && shift == shift ? shift : 0.f;  // u is -inf or NaN by itself
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float s = t[c] - back, most = warp_max(s);
+            float q = __shfl_sync(kAllLanes, own_reference, c);
+            if (most > q) {
+              l[c] *= q == -INFINITY ? 1.f : exp2_approx(q - most);
+              q = most;
+              if (own == c) own_reference = q;
+            }
+            l[c] += exp2_approx(q == -INFINITY ? s : s - q);
+          }
+        }
         // Weights x = 2^(u - R + 5). The sum takes them in float32, without the
         // value's scale; the tensor core in T parts.
-        const float to_sum = scale == scale ? __fdividef(0.03125f, scale) : 1.f;  // a NaN comes with the weights that see it
+        const float to_sum = __fdividef(0.03125f, scale);
         const bool dead = vs == 0.f;  // values that count as 0, whatever their codes
         uint32_t part[4][T];
 #pragma unroll
@@ -520,7 +571,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
             add_pair(t[c + k], t[c + k + 1], rs[k], rs[k + 1], x[k], x[k + 1]);
             x[k] = exp2_approx(x[k]);
             x[k + 1] = exp2_approx(x[k + 1]);
-            fma_pair(x[k], x[k + 1], to_sum, to_sum, l[c + k], l[c + k + 1], l[c + k], l[c + k + 1]);
+            if (!APART) fma_pair(x[k], x[k + 1], to_sum, to_sum, l[c + k], l[c + k + 1], l[c + k], l[c + k + 1]);
           }
           if constexpr (T == 2) {
             split4_f16(x, part[c / 4]);
@@ -550,6 +601,51 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           b = 0;
           turn ^= 1;
         }
+        return true;
+      };
+      int32_t i = 0;
+      bool apart = false;
+      for (; i < h.steps; ++i) {
+        begin_tile();
+        if (!end_tile(i, std::false_type{})) {
+          apart = true;
+          break;
+        }
+      }
+      if (apart) {  // from here on all of the group's warps are
+        own_reference = reference;
+        while (true) {
+          end_tile(i, std::true_type{});
+          if (++i == h.steps) break;
+          begin_tile();
+        }
+        // One reference for the item's end: 2^32 above the largest Q of the
+        // warps, so that O fits as well, whatever the scales and the keys.
+        warp_wait(&sh.done, (n - 1) & 1, abort);
+        tc_fence_after();
+        float* qs = reinterpret_cast<float*>(smem + C::kOffP + wg * 4096) + 64;
+        if (lane < 16) qs[(warp & 3) * 16 + lane] = own_reference;
+        named_barrier(group_barrier, 128);
+        float to = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) to = fmaxf(to, qs[w * 16 + own] + 32.f);
+        // (Without a reference, a sum is 0 or not a number, and so are the outputs.)
+        const float by = own_reference == -INFINITY ? 1.f : exp2_approx(own_reference - to);
+        const float2 down = reference == -INFINITY ? make_float2(1.f, 1.f) : exp2_factors(reference - to);
+        reference = to;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) l[c] *= __shfl_sync(kAllLanes, by, c);
+#pragma unroll 1
+        for (int m = 0; m < C::kValues; ++m) {
+          const uint32_t at = tmem + lanes + m * NH + first_col;
+          float o[16];
+          tmem_ld16(at, o);
+          tmem_wait_ld(o);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) o[c] = o[c] * __shfl_sync(kAllLanes, down.x, c) * __shfl_sync(kAllLanes, down.y, c);
+          tmem_st16(at, o);
+        }
+        tmem_wait_st();
       }
       if (h.steps > 0) warp_wait(&sh.done, (n - 1) & 1, abort);
       tc_fence_after();
@@ -1062,7 +1158,9 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       }
       whole_l += __shfl_xor_sync(kAllLanes, whole_l, 16);
       const float inverse = whole_l == 0.f ? 0.f : 1.f / (32.f * whole_l);
-      const float by = reference == -INFINITY ? 0.f : exp2_approx(reference - whole_r) * inverse;
+      const float2 down = reference == -INFINITY ? make_float2(1.f, 0.f) : exp2_factors(reference - whole_r);
+      const float by = down.y * inverse;
+      const bool far = __any_sync(kAllLanes, down.x != 1.f);
       if (rank == 0 && (warp & 3) == 0 && lane < 16 && *abort == 0) {
         const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, first_col + lane);
         if (col.used) {
@@ -1088,6 +1186,10 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           if (last.steps > 0) {
             tmem_ld16(tmem + lanes + m * NH + first_col, o);
             tmem_wait_ld(o);
+            if (far) {
+#pragma unroll
+              for (int c = 0; c < 16; ++c) o[c] *= __shfl_sync(kAllLanes, down.x, c);
+            }
           }
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
