@@ -27,6 +27,7 @@ SOURCES = [
     os.path.join(CSRC, "attend_dim64.cu"),
     os.path.join(CSRC, "attend_dim128.cu"),
     os.path.join(CSRC, "attend_latent.cu"),
+    os.path.join(CSRC, "status.cu"),
 ]
 DEPENDS = SOURCES + [
     os.path.join(CSRC, "fastdiv.cuh"),

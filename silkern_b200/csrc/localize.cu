@@ -1275,28 +1275,6 @@ extern "C" int silkern_count_segment_mismatches_v1(const int32_t* a, const int32
   return SILKERN_OK;
 }
 
-extern "C" const char* silkern_status_string_v1(int code) {
-  switch (code) {
-    case SILKERN_OK: return "ok";
-    case SILKERN_E_NULL: return "a required buffer pointer is NULL";
-    case SILKERN_E_SHAPE: return "batch, width or block-table dimensions are out of range";
-    case SILKERN_E_DCP: return "invalid dcp configuration";
-    case SILKERN_E_BLOCK_SIZE: return "block_size must be a positive integer divisible by dcp_interleave";
-    case SILKERN_E_TILE: return "unsupported tile_size";
-    case SILKERN_E_ALIAS: return "an output buffer overlaps an input or another output";
-    case SILKERN_E_GEOMETRY: return "explicit launch geometry rejected";
-    case SILKERN_E_SCRATCH:
-      return "batch x tiles exceeds the allocation-free entry point's static workspace";
-    case SILKERN_E_CACHE: return "unsupported cache geometry, stride or alignment";
-    case SILKERN_E_HEADS: return "heads must be a positive multiple of the cache's heads";
-    case SILKERN_E_TYPE: return "element type must be bfloat16 or float16";
-    case SILKERN_E_ATTEND: return "window, sinks or softmax scale out of range";
-    default: break;
-  }
-  if (code < 0) return cudaGetErrorString(static_cast<cudaError_t>(-code));
-  return "unknown status";
-}
-
 extern "C" int silkern_abi_version_v1(void) { return SILKERN_ABI_VERSION; }
 
 extern "C" int64_t silkern_fastdiv_selftest_v1(uint32_t divisor, uint32_t n_begin, uint32_t n_count) {

@@ -89,6 +89,14 @@ def test_traffic_is_used_only_for_the_kernel_source_it_was_captured_from(tmp_pat
     assert bench._traffic(3)["bytes"] is None
 
 
+@pytest.mark.parametrize("config", sorted(bench.WORKLOADS))
+def test_the_committed_traffic_is_of_the_converter_as_it_is(config) -> None:
+    """A change beside the converter's kernel leaves its source, and so the
+    capture's digest, alone."""
+    traffic = bench._traffic(config)
+    assert traffic["bytes"], traffic["source"]
+
+
 def test_reference_arm_line_on_cpu() -> None:
     proc = subprocess.run(
         [sys.executable, os.path.join(REPO, "bench.py"), "--impl", "reference", "--steps", "2",
