@@ -574,8 +574,9 @@ extern "C" int silkern_merge_partials_v1(const void* outs, int64_t outs_rank, in
                                          void* stream) {
   if (outs == nullptr || lses == nullptr || out == nullptr) return SILKERN_E_NULL;
   if (type != SILKERN_BF16 && type != SILKERN_F16) return SILKERN_E_TYPE;
+  // (The kernel's column numbers step past dim by up to 255.)
   if (ranks < 1 || ranks > 0x7fffffff || rows < 1 || heads < 1 || heads > 0x7fffffff || dim < 1 ||
-      dim > 0x7fffffff || rows > (int64_t{1} << 31) * kMergeWarps / heads - kMergeWarps) {
+      dim > 0x7fffffff - 255 || rows > (int64_t{1} << 31) * kMergeWarps / heads - kMergeWarps) {
     return SILKERN_E_SHAPE;
   }
   MergeArgs a{outs, lses, out, lse, outs_rank, outs_row, outs_head, out_row, out_head, rows * heads,

@@ -259,3 +259,11 @@ def test_launchers_trace_as_op_nodes_without_a_graph_break(latent) -> None:
     targets = [str(node.target) for node in graphs[0].graph.nodes if node.op == "call_function"]
     for name in ("append_quantized", "attend_selected", "attend_window", "merge_partials"):
         assert sum(f"silkern_b200.{name}" in t for t in targets) == 1
+
+
+def test_merge_refuses_columns_past_its_numbers(lib) -> None:
+    """Columns are counted in 32 bits, up to 256 at a step: from 2**31 - 255 on
+    the count would turn negative and never end."""
+    for dim in (2**31 - 255, 2**31 - 1, 2**31):
+        assert merge(lib, dim=dim) == 2
+    assert merge(lib, dim=2**31 - 256, out=Q + 64) == 6  # a size that can be counted, found to overlap
