@@ -66,22 +66,30 @@ def _type_code(torch, dtype):
     return code
 
 
-def _on_device(torch, tensors, what: str) -> int:
-    """The index of the device that every given tensor is on."""
+def _on_device(torch, required, optional, what: str) -> int:
+    """The index of the device that the buffers are on: every required one, and
+    the optional ones that are not None."""
     device = -1
+    host = mixed = False
     tensor = torch.Tensor
-    for t in tensors:
-        if t is None:
-            continue
-        if not isinstance(t, tensor):
-            raise LocalizationError(f"all {what} buffers must be torch tensors")
-        index = t.get_device()
-        if index != device or index < 0:
-            if not t.is_cuda:
-                raise LocalizationError(f"all {what} buffers must be CUDA tensors")
-            if device >= 0:
-                raise LocalizationError(f"all {what} buffers must be on the same device")
-            device = index
+    for tensors, may_lack in ((required, False), (optional, True)):
+        for t in tensors:
+            if t is None and may_lack:
+                continue
+            if not isinstance(t, tensor):
+                raise LocalizationError(f"all {what} buffers must be torch tensors")
+            index = t.get_device()
+            if index != device or index < 0:
+                if not t.is_cuda:
+                    host = True
+                elif device >= 0:
+                    mixed = True
+                else:
+                    device = index
+    if host:
+        raise LocalizationError(f"all {what} buffers must be CUDA tensors")
+    if mixed:
+        raise LocalizationError(f"all {what} buffers must be on the same device")
     return device
 
 
@@ -237,9 +245,8 @@ def append_quantized(
         return _traced_op(torch, "append_quantized")(
             keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table, dcp_size,
             dcp_rank, dcp_interleave, status)
-    device = _on_device(
-        torch, (keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table),
-        "append")
+    device = _on_device(torch, (keys, k_cache, k_scale, cu_tokens, starts, req_ids, block_table),
+                        (values, v_cache, v_scale), "append")
     code = _type_code(torch, keys.dtype)
     _check_ints(torch, (cu_tokens, starts, req_ids, block_table), "cu_tokens, starts, req_ids and block_table")
     cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
@@ -305,7 +312,7 @@ def attend_selected(
     if _compiling(torch):
         return _traced_op(torch, "attend_selected")(
             q, slots, k_cache, v_cache, k_scale, v_scale, out, lse, softmax_scale, counts, status)
-    device = _on_device(torch, (q, slots, k_cache, v_cache, k_scale, v_scale, out, lse, counts), "attention")
+    device = _on_device(torch, (q, slots, k_cache, k_scale, out, lse), (v_cache, v_scale, counts), "attention")
     _check_ints(torch, (counts,), "counts")
     cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
     rows, heads, q_row, q_head, out_row, out_head, code = _check_queries(torch, q, cache, out, lse, softmax_scale)
@@ -370,9 +377,8 @@ def attend_window(
         return _traced_op(torch, "attend_window")(
             q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale, out, lse,
             softmax_scale, window, sinks, dcp_size, dcp_rank, dcp_interleave, status)
-    device = _on_device(
-        torch, (q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale, out, lse),
-        "attention")
+    device = _on_device(torch, (q, cu_tokens, lengths, req_ids, block_table, k_cache, k_scale, out, lse),
+                        (v_cache, v_scale), "attention")
     _check_ints(torch, (cu_tokens, lengths, req_ids, block_table), "cu_tokens, lengths, req_ids and block_table")
     cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
     rows, heads, q_row, q_head, out_row, out_head, code = _check_queries(torch, q, cache, out, lse, softmax_scale)
@@ -407,7 +413,7 @@ def merge_partials(outs, lses, out, lse=None) -> None:
 
     if _compiling(torch):
         return _traced_op(torch, "merge_partials")(outs, lses, out, lse)
-    device = _on_device(torch, (outs, lses, out, lse), "merge")
+    device = _on_device(torch, (outs, lses, out), (lse,), "merge")
     dtype = outs.dtype
     code = _type_code(torch, dtype)
     if outs.ndim != 4 or outs.numel() < 1:

@@ -267,3 +267,36 @@ def test_merge_refuses_columns_past_its_numbers(lib) -> None:
     for dim in (2**31 - 255, 2**31 - 1, 2**31):
         assert merge(lib, dim=dim) == 2
     assert merge(lib, dim=2**31 - 256, out=Q + 64) == 6  # a size that can be counted, found to overlap
+
+
+# ---------------------------------------------------------------------- bindings that are not what a call needs
+
+def host_calls():
+    """name -> (launcher, buffers by name, keywords): right but for lying on the host, which is looked at
+    after what these tests ask for."""
+    k, v, ks, vs = make_cache(2, 4, 1, 64, device="cpu")
+    cache = dict(k_cache=k, v_cache=v, k_scale=ks, v_scale=vs)
+    q, out, lse = torch.zeros((1, 1, 64), dtype=torch.bfloat16), torch.zeros((1, 1, 64), dtype=torch.bfloat16), torch.zeros(1, 1)
+    cu, one, table = torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32)
+    return {
+        "selected": (silkern.attend_selected, dict(q=q, slots=table, **cache, out=out, lse=lse), dict(softmax_scale=1.0)),
+        "window": (silkern.attend_window, dict(q=q, cu_tokens=cu, lengths=one, req_ids=one, block_table=table, **cache,
+                                               out=out, lse=lse), dict(softmax_scale=1.0)),
+        "append": (silkern.append_quantized, dict(keys=q, values=q.clone(), **cache, cu_tokens=cu, starts=one, req_ids=one,
+                                                  block_table=table), {}),
+        "merge": (silkern.merge_partials, dict(outs=q[None], lses=lse[None], out=out, lse=lse.clone()), {}),
+    }
+
+
+OPTIONAL = {"v_cache", "v_scale", "values"}
+
+
+@pytest.mark.parametrize("name", ["selected", "window", "append", "merge"])
+def test_a_missing_buffer_is_refused(name) -> None:
+    call, buffers, kw = host_calls()[name]
+    for which in buffers:
+        if which in OPTIONAL or (name, which) == ("merge", "lse"):
+            continue
+        for wrong in (None, 3, [1.0]):
+            with pytest.raises(silkern.LocalizationError, match="must be torch tensors"):
+                call(**{**buffers, which: wrong}, **kw)
