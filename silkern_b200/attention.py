@@ -28,6 +28,8 @@ calls can be captured in a CUDA graph. They run on the current stream of the
 buffers' device. While ``torch.compile`` traces the caller, each routes through
 its op of the same name (:mod:`silkern_b200.ops`). Each raises
 :class:`LocalizationError` before launch on an unsupported binding or geometry.
+They are for serving and have no backward pass: while gradients are recorded, a
+buffer that requires grad is refused.
 
 Attention expects what :func:`append_quantized` writes: finite codes (no NaN
 code, 0x7f or 0xff, at a token that any query of the call sees) and scales that
@@ -64,6 +66,16 @@ def _type_code(torch, dtype):
     if code is None:
         raise LocalizationError("queries, new tokens and outputs must be bfloat16 or float16")
     return code
+
+
+def _refuse_gradients(torch, *tensors) -> None:
+    """The operators have no backward pass; autograd would lose them silently."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if getattr(t, "requires_grad", False):
+                raise LocalizationError(
+                    "no gradient flows through the cache's operators: call them under torch.no_grad() or "
+                    "torch.inference_mode(), or detach their buffers")
 
 
 def _on_device(torch, required, optional, what: str) -> int:
@@ -241,6 +253,7 @@ def append_quantized(
     """
     import torch
 
+    _refuse_gradients(torch, keys, values, k_cache, v_cache, k_scale, v_scale)
     if _compiling(torch):
         return _traced_op(torch, "append_quantized")(
             keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table, dcp_size,
@@ -309,6 +322,7 @@ def attend_selected(
     """
     import torch
 
+    _refuse_gradients(torch, q, k_cache, v_cache, k_scale, v_scale, out, lse)
     if _compiling(torch):
         return _traced_op(torch, "attend_selected")(
             q, slots, k_cache, v_cache, k_scale, v_scale, out, lse, softmax_scale, counts, status)
@@ -373,6 +387,7 @@ def attend_window(
     """
     import torch
 
+    _refuse_gradients(torch, q, k_cache, v_cache, k_scale, v_scale, out, lse)
     if _compiling(torch):
         return _traced_op(torch, "attend_window")(
             q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale, out, lse,
@@ -411,6 +426,7 @@ def merge_partials(outs, lses, out, lse=None) -> None:
     """
     import torch
 
+    _refuse_gradients(torch, outs, lses, out, lse)
     if _compiling(torch):
         return _traced_op(torch, "merge_partials")(outs, lses, out, lse)
     device = _on_device(torch, (outs, lses, out), (lse,), "merge")

@@ -300,3 +300,28 @@ def test_a_missing_buffer_is_refused(name) -> None:
         for wrong in (None, 3, [1.0]):
             with pytest.raises(silkern.LocalizationError, match="must be torch tensors"):
                 call(**{**buffers, which: wrong}, **kw)
+
+
+GRADIENTS = [("selected", "q"), ("selected", "out"), ("selected", "lse"), ("selected", "k_scale"), ("window", "q"),
+             ("window", "v_scale"), ("append", "keys"), ("append", "values"), ("append", "k_scale"), ("merge", "outs"),
+             ("merge", "lses"), ("merge", "out")]
+
+
+@pytest.mark.parametrize("name,which", GRADIENTS)
+def test_a_call_that_autograd_records_is_refused(name, which) -> None:
+    """There is no backward pass: a result without a graph would drop the gradients."""
+    call, buffers, kw = host_calls()[name]
+    buffers[which] = buffers[which].clone().requires_grad_()
+    with pytest.raises(silkern.LocalizationError, match="no gradient"):
+        call(**buffers, **kw)
+    with torch.no_grad(), pytest.raises(silkern.LocalizationError, match="must be CUDA tensors"):
+        call(**buffers, **kw)
+
+
+def test_a_traced_call_that_autograd_records_is_refused() -> None:
+    ops.register()
+    call, buffers, kw = host_calls()["merge"]
+    buffers["outs"] = buffers["outs"].clone().requires_grad_()
+    torch._dynamo.reset()
+    with pytest.raises(Exception, match="no gradient"):
+        torch.compile(lambda b: call(**b), backend="eager", fullgraph=True)(buffers)
