@@ -184,6 +184,15 @@ def _check_owner(block_size, dcp_size, dcp_rank, dcp_interleave) -> None:
         raise LocalizationError("dcp_size * dcp_interleave must be below 2**31")
 
 
+def _check_scale(softmax_scale) -> None:
+    try:
+        finite = math.isfinite(softmax_scale)
+    except (TypeError, ValueError, RuntimeError) as error:  # RuntimeError: a tensor of several elements
+        raise LocalizationError("softmax_scale must be a finite number") from error
+    if not finite:
+        raise LocalizationError("softmax_scale must be finite")
+
+
 def _check_queries(torch, q, cache, out, lse, softmax_scale):
     """Checks of an attention call's queries and results: (rows, heads, q's row
     and head stride, out's, type code)."""
@@ -204,8 +213,7 @@ def _check_queries(torch, q, cache, out, lse, softmax_scale):
     if q_column != 1 or (q_row | q_head) & 7 or q.data_ptr() & 15:
         raise LocalizationError(
             "q needs unit column stride, other strides that are multiples of 8 and 16-byte alignment")
-    if not math.isfinite(softmax_scale):
-        raise LocalizationError("softmax_scale must be finite")
+    _check_scale(softmax_scale)
     return rows, heads, q_row, q_head, out_row, out_head, code
 
 

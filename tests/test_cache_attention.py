@@ -325,3 +325,13 @@ def test_a_traced_call_that_autograd_records_is_refused() -> None:
     torch._dynamo.reset()
     with pytest.raises(Exception, match="no gradient"):
         torch.compile(lambda b: call(**b), backend="eager", fullgraph=True)(buffers)
+
+
+@pytest.mark.parametrize("scale", ["0.1", None, 0.1j, [0.1], torch.ones(2), math.inf, -math.inf, math.nan])
+def test_a_softmax_scale_that_is_no_finite_number_is_refused(scale) -> None:
+    from silkern_b200 import attention
+
+    with pytest.raises(silkern.LocalizationError, match="finite"):
+        attention._check_scale(scale)
+    for good in (0.1, 2, torch.tensor(0.5)):
+        attention._check_scale(good)
