@@ -310,6 +310,10 @@ int silkern_topk_localize_explicit_v2(const float* logits, int64_t logits_stride
  * visible tokens are finite (neither 0x7f nor 0xff). num_blocks * block_size
  * is below 2^31 and block_size at most 65536. Addresses of k and v are multiples
  * of 16.
+ *
+ * SILKERN_E_ALIAS: what a call writes shares memory with what it reads. Buffers
+ * with equal largest strides may lie between one another's rows; others are
+ * compared as whole ranges of memory.
  */
 typedef struct silkern_cache_v1 {
   void* k;

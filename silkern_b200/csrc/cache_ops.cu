@@ -322,41 +322,73 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
 
 // ---------------------------------------------------------------- checks
 
-// The bytes that a buffer covers, from its address to its last element.
-struct Range {
-  uintptr_t begin, end;
-};
-Range range_of(const void* base, int64_t bytes) {
-  const uintptr_t b = reinterpret_cast<uintptr_t>(base);
-  return base == nullptr ? Range{0, 0} : Range{b, b + static_cast<uintptr_t>(bytes)};
-}
-int64_t extent(int64_t count, int64_t stride) { return (count - 1) * stride; }
+// The bytes of a strided buffer: `bytes` from every place begin + i stride[0] +
+// j stride[1] + ..., i below count[0] and so on, largest strides first.
+struct Place {
+  uintptr_t begin = 0;
+  int64_t bytes = 0;
+  int dims = 0;
+  int64_t count[3], stride[3];
 
+  Place(const void* base, int64_t inner) : begin(reinterpret_cast<uintptr_t>(base)), bytes(base == nullptr ? 0 : inner) {}
+  Place&& along(int64_t n, int64_t step) && {
+    if (n > 1) {
+      int at = dims++;
+      for (; at > 0 && stride[at - 1] < step; --at) {
+        count[at] = count[at - 1];
+        stride[at] = stride[at - 1];
+      }
+      count[at] = n;
+      stride[at] = step;
+    }
+    return static_cast<Place&&>(*this);
+  }
+  // From the first byte to behind the last, of the dimensions from `from` on.
+  int64_t extent(int from) const {
+    int64_t n = bytes;
+    for (int i = from; i < dims; ++i) n += (count[i] - 1) * stride[i];
+    return n;
+  }
+};
+
+// Whether a's dimensions from `i` on at 0 and b's from `j` on at `shift` share
+// no byte. Buffers that take turns in memory, as column slices of one tensor
+// or pages of one allocation do, have their largest stride in common: what lies
+// between two of its steps is then compared alone. Else by their extents.
+bool apart(const Place& a, int i, const Place& b, int j, int64_t shift) {
+  if (shift >= a.extent(i) || shift + b.extent(j) <= 0) return true;
+  if (i == a.dims || j == b.dims || a.stride[i] != b.stride[j] || a.stride[i] < 1) return false;
+  const int64_t step = a.stride[i];
+  if (a.extent(i + 1) > step || b.extent(j + 1) > step) return false;
+  const int64_t ahead = (shift % step + step) % step;
+  return apart(a, i + 1, b, j + 1, ahead) && apart(a, i + 1, b, j + 1, ahead - step);
+}
+bool shares(const Place& a, const Place& b) {
+  return a.bytes != 0 && b.bytes != 0 &&
+         !apart(a, 0, b, 0, static_cast<int64_t>(b.begin) - static_cast<int64_t>(a.begin));
+}
 // Whether an output shares memory with another output or an input.
 template <int N, int M>
-bool shares(const Range (&outputs)[N], const Range (&inputs)[M]) {
+bool shares(const Place (&outputs)[N], const Place (&inputs)[M]) {
   for (int i = 0; i < N; ++i) {
-    if (outputs[i].begin == outputs[i].end) continue;
     for (int j = 0; j < M; ++j) {
-      if (outputs[i].begin < inputs[j].end && inputs[j].begin < outputs[i].end) return true;
+      if (shares(outputs[i], inputs[j])) return true;
     }
     for (int j = 0; j < i; ++j) {
-      if (outputs[i].begin < outputs[j].end && outputs[j].begin < outputs[i].end) return true;
+      if (shares(outputs[i], outputs[j])) return true;
     }
   }
   return false;
 }
 
-Range range_of_keys(const silkern_cache_v1* c) {
-  return range_of(c->k, extent(c->num_blocks, c->k_block) + extent(c->block_size, c->k_token) +
-                            extent(c->kv_heads, c->k_head) + c->key_dim);
+Place place_of_keys(const silkern_cache_v1* c) {
+  return Place(c->k, c->key_dim).along(c->num_blocks, c->k_block).along(c->block_size, c->k_token).along(c->kv_heads, c->k_head);
 }
-Range range_of_values(const silkern_cache_v1* c) {
-  return range_of(c->v, extent(c->num_blocks, c->v_block) + extent(c->block_size, c->v_token) +
-                            extent(c->kv_heads, c->v_head) + c->value_dim);
+Place place_of_values(const silkern_cache_v1* c) {
+  return Place(c->v, c->value_dim).along(c->num_blocks, c->v_block).along(c->block_size, c->v_token).along(c->kv_heads, c->v_head);
 }
-Range range_of_scales(const silkern_cache_v1* c, const float* scale) {
-  return range_of(scale, c->num_blocks * c->kv_heads * 4);
+Place place_of_scales(const silkern_cache_v1* c, const float* scale) {
+  return Place(scale, c->num_blocks * c->kv_heads * 4);
 }
 
 int check_cache(const silkern_cache_v1* c, PagedCache* out) {
@@ -407,13 +439,13 @@ int check_owner(int32_t block_size, int32_t dcp_size, int32_t dcp_rank, int32_t 
 // The results of an attention call share no memory with each other, with the
 // cache or the queries, nor with `index`, the call's other buffers.
 template <int N>
-bool results_alone(const silkern_cache_v1* c, const AttendArgs& a, const Range (&index)[N]) {
+bool results_alone(const silkern_cache_v1* c, const AttendArgs& a, const Place (&index)[N]) {
   const int64_t rows = a.rows, heads = a.heads;
-  const Range results[2] = {range_of(a.out, 2 * (extent(rows, a.out_row) + extent(heads, a.out_head) + c->value_dim)),
-                            range_of(a.lse, 4 * rows * heads)};
-  const Range read[5] = {range_of(a.q, 2 * (extent(rows, a.q_row) + extent(heads, a.q_head) + c->key_dim)),
-                         range_of_keys(c), range_of_values(c), range_of_scales(c, c->k_scale),
-                         range_of_scales(c, c->v_scale)};
+  const Place results[2] = {Place(a.out, 2 * c->value_dim).along(rows, 2 * a.out_row).along(heads, 2 * a.out_head),
+                            Place(a.lse, 4 * rows * heads)};
+  const Place read[5] = {Place(a.q, 2 * c->key_dim).along(rows, 2 * a.q_row).along(heads, 2 * a.q_head),
+                         place_of_keys(c), place_of_values(c), place_of_scales(c, c->k_scale),
+                         place_of_scales(c, c->v_scale)};
   return !shares(results, read) && !shares(results, index);
 }
 
@@ -467,16 +499,15 @@ extern "C" int silkern_append_quantized_v1(const silkern_cache_v1* cache, const 
   }
   rc = check_owner(cache->block_size, dcp_size, dcp_rank, dcp_interleave, &a.own);
   if (rc != SILKERN_OK) return rc;
-  const Range written[4] = {range_of_scales(cache, cache->k_scale), range_of_scales(cache, cache->v_scale),
-                            range_of_keys(cache), Range{0, 0}};
-  const int64_t dims = cache->kv_heads - int64_t{1};
-  const Range read[6] = {range_of(keys, 2 * (extent(tokens, key_token) + dims * key_head + cache->key_dim)),
-                         range_of(values, 2 * (extent(tokens, value_token) + dims * value_head + cache->value_dim)),
-                         range_of(cu_tokens, 4 * (sequences + 1)), range_of(starts, 4 * sequences),
-                         range_of(req_ids, 4 * sequences), range_of(block_table, 4 * table_rows * table_width)};
+  const Place written[3] = {place_of_scales(cache, cache->k_scale), place_of_scales(cache, cache->v_scale),
+                            place_of_keys(cache)};
+  const Place read[6] = {Place(keys, 2 * cache->key_dim).along(tokens, 2 * key_token).along(cache->kv_heads, 2 * key_head),
+                         Place(values, 2 * cache->value_dim).along(tokens, 2 * value_token).along(cache->kv_heads, 2 * value_head),
+                         Place(cu_tokens, 4 * (sequences + 1)), Place(starts, 4 * sequences),
+                         Place(req_ids, 4 * sequences), Place(block_table, 4 * table_rows * table_width)};
   // Keys and values may lie in one buffer, page by page or row by row.
-  const Range values_too[1] = {range_of_values(cache)};
-  const Range scales[2] = {written[0], written[1]};
+  const Place values_too[1] = {place_of_values(cache)};
+  const Place scales[2] = {written[0], written[1]};
   if (shares(written, read) || shares(values_too, read) || shares(values_too, scales)) return SILKERN_E_ALIAS;
   a.keys = keys;
   a.values = values;
@@ -527,7 +558,7 @@ extern "C" int silkern_attend_selected_v1(const silkern_cache_v1* cache, const v
   a.counts = counts;
   a.total_slots = static_cast<uint32_t>(cache->num_blocks * cache->block_size);
   a.status = status;
-  const Range index[2] = {range_of(slots, 4 * (extent(rows, slots_row) + width)), range_of(counts, 4 * rows)};
+  const Place index[2] = {Place(slots, 4 * width).along(rows, 4 * slots_row), Place(counts, 4 * rows)};
   if (!results_alone(cache, a, index)) return SILKERN_E_ALIAS;
   return launch_attend(a, cache->key_dim, type, static_cast<cudaStream_t>(stream));
 }
@@ -562,8 +593,8 @@ extern "C" int silkern_attend_window_v1(const silkern_cache_v1* cache, const voi
   a.window = static_cast<uint32_t>(window);
   a.sinks = static_cast<uint32_t>(sinks);
   a.status = status;
-  const Range index[4] = {range_of(cu_tokens, 4 * (sequences + 1)), range_of(lengths, 4 * sequences),
-                          range_of(req_ids, 4 * sequences), range_of(block_table, 4 * table_rows * table_width)};
+  const Place index[4] = {Place(cu_tokens, 4 * (sequences + 1)), Place(lengths, 4 * sequences),
+                          Place(req_ids, 4 * sequences), Place(block_table, 4 * table_rows * table_width)};
   if (!results_alone(cache, a, index)) return SILKERN_E_ALIAS;
   return launch_attend(a, cache->key_dim, type, static_cast<cudaStream_t>(stream));
 }
@@ -581,11 +612,10 @@ extern "C" int silkern_merge_partials_v1(const void* outs, int64_t outs_rank, in
   }
   MergeArgs a{outs, lses, out, lse, outs_rank, outs_row, outs_head, out_row, out_head, rows * heads,
               static_cast<int32_t>(ranks), static_cast<int32_t>(heads), static_cast<int32_t>(dim)};
-  const Range written[2] = {range_of(out, 2 * (extent(rows, out_row) + extent(heads, out_head) + dim)),
-                            range_of(lse, 4 * rows * heads)};
-  const Range read[2] = {
-      range_of(outs, 2 * (extent(ranks, outs_rank) + extent(rows, outs_row) + extent(heads, outs_head) + dim)),
-      range_of(lses, 4 * ranks * rows * heads)};
+  const Place written[2] = {Place(out, 2 * dim).along(rows, 2 * out_row).along(heads, 2 * out_head),
+                            Place(lse, 4 * rows * heads)};
+  const Place read[2] = {Place(outs, 2 * dim).along(ranks, 2 * outs_rank).along(rows, 2 * outs_row).along(heads, 2 * outs_head),
+                         Place(lses, 4 * ranks * rows * heads)};
   if (shares(written, read)) return SILKERN_E_ALIAS;
   // 16 bytes at a time where every row of columns allows it.
   const bool wide = (dim | outs_rank | outs_row | outs_head | out_row | out_head) % 8 == 0 &&

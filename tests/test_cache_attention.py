@@ -335,3 +335,11 @@ def test_a_softmax_scale_that_is_no_finite_number_is_refused(scale) -> None:
         attention._check_scale(scale)
     for good in (0.1, 2, torch.tensor(0.5)):
         attention._check_scale(good)
+
+
+@pytest.mark.parametrize("offset", [0, 2 * 128, 2 * 255, 2 * 1023, -2 * 16, 2 * 1024 * 3 + 2 * 200])
+def test_results_between_the_rows_of_their_inputs_may_not_reach_into_them(lib, offset) -> None:
+    """Rows of 1024 elements: q has the first 256 of each, out would have 256 that meet them."""
+    assert selected(lib, cache(), rows=4, q_row=1024, out_row=1024, out=Q + offset) == 6
+    assert selected(lib, cache(), rows=4, q_row=1024, out_row=1040, out=Q + 2 * 256) == 6  # steps that differ
+    assert selected(lib, cache(), rows=4, q_row=1024, out_row=1024, out=OUT, lse=OUT + 2 * 256) == 6

@@ -829,3 +829,39 @@ def test_items_shared_by_clusters_of_any_size(shape, dtype, heads, rows) -> None
     out, lse = selected(q, slots, cache, value_dim, softmax_scale=dim**-0.5)
     want = oracle.attend_selected(q, slots, *cache, softmax_scale=dim**-0.5)
     assert_attention(out, lse, want, q, cache[0], cache[2], dim**-0.5)
+
+
+# -------------------------------------------------------------------------------- buffers that lie between one another
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_results_between_the_rows_and_heads_of_the_queries(shape) -> None:
+    """q and out as column slices of one buffer, by rows and by heads: no byte is both."""
+    dim, value_dim, latent = SHAPES[shape]
+    cache = make_cache(9, 32, 1, dim, latent=latent, seed=100)
+    slots = torch.randint(-1, 288, (5, 150), generator=torch.Generator().manual_seed(101), dtype=torch.int32).cuda()
+    whole = randn(5, 4, dim, dtype=torch.bfloat16, seed=102)
+    want = selected(whole, slots, cache, value_dim, softmax_scale=0.07)
+    rows = torch.zeros((5, 4 * dim + 4 * value_dim + 8), dtype=torch.bfloat16, device="cuda")
+    heads = torch.zeros((5, 4, dim + value_dim + 16), dtype=torch.bfloat16, device="cuda")
+    for q, out in ((rows[:, : 4 * dim].unflatten(1, (4, dim)), rows[:, 4 * dim : -8].unflatten(1, (4, value_dim))),
+                   (heads[..., :dim], heads[..., dim : dim + value_dim])):
+        q.copy_(whole)
+        lse = torch.empty((5, 4), device="cuda")
+        silkern.attend_selected(q, slots, *cache, out, lse, softmax_scale=0.07)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and torch.equal(q, whole)
+        with pytest.raises(silkern.LocalizationError, match="overlaps"):
+            silkern.attend_selected(q, slots, *cache, q[..., :value_dim], lse, softmax_scale=0.07)
+
+
+def test_merge_between_its_partial_results() -> None:
+    """One buffer of (rows, ranks + 1, heads, dim) holds the partial outputs and their join."""
+    outs = randn(3, 6, 4, 64, dtype=torch.float16, seed=103)
+    lses = torch.randn((3, 6, 4), generator=torch.Generator().manual_seed(104)).cuda()
+    want, want_lse = results(6, 4, 64, torch.float16)
+    silkern.merge_partials(outs, lses, want, want_lse)
+    held = torch.zeros((6, 4, 4, 64), dtype=torch.float16, device="cuda")
+    held[:, :3] = outs.transpose(0, 1)
+    silkern.merge_partials(held[:, :3].transpose(0, 1), lses, held[:, 3], want_lse)
+    assert torch.equal(held[:, 3], want) and torch.equal(held[:, :3].transpose(0, 1), outs)
+    with pytest.raises(silkern.LocalizationError, match="overlaps"):
+        silkern.merge_partials(held[:, :3].transpose(0, 1), lses, held[:, 2], want_lse)
