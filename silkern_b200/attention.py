@@ -241,7 +241,8 @@ def append_quantized(
 
     ``keys`` is (tokens, kv_heads, key_dim) in bfloat16 or float16, ``values``
     (tokens, kv_heads, value_dim) of the same type, or ``None`` for a latent
-    cache; both have unit column stride. Sequence ``b`` has the tokens
+    cache; both have unit column stride. Key and value cache may take turns in
+    one buffer, page by page or row by row, but share no byte. Sequence ``b`` has the tokens
     ``cu_tokens[b]:cu_tokens[b + 1]`` (int32, one more element than sequences),
     at the positions from ``starts[b]`` on of the request ``req_ids[b]``. The
     positions of this rank go through ``block_table[req_ids[b]]`` into their

@@ -507,8 +507,7 @@ extern "C" int silkern_append_quantized_v1(const silkern_cache_v1* cache, const 
                          Place(req_ids, 4 * sequences), Place(block_table, 4 * table_rows * table_width)};
   // Keys and values may lie in one buffer, page by page or row by row.
   const Place values_too[1] = {place_of_values(cache)};
-  const Place scales[2] = {written[0], written[1]};
-  if (shares(written, read) || shares(values_too, read) || shares(values_too, scales)) return SILKERN_E_ALIAS;
+  if (shares(written, read) || shares(values_too, read) || shares(values_too, written)) return SILKERN_E_ALIAS;
   a.keys = keys;
   a.values = values;
   a.key_token = key_token;

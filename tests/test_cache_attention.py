@@ -343,3 +343,11 @@ def test_results_between_the_rows_of_their_inputs_may_not_reach_into_them(lib, o
     assert selected(lib, cache(), rows=4, q_row=1024, out_row=1024, out=Q + offset) == 6
     assert selected(lib, cache(), rows=4, q_row=1024, out_row=1040, out=Q + 2 * 256) == 6  # steps that differ
     assert selected(lib, cache(), rows=4, q_row=1024, out_row=1024, out=OUT, lse=OUT + 2 * 256) == 6
+
+
+def test_append_refuses_keys_and_values_in_the_same_place(lib) -> None:
+    """Keys and values are written by CTAs of their own: they may take turns in one buffer, not share it."""
+    for v in (K, K + 16 * 256 * 3, K + 128, K - 16 * 256):
+        assert append(lib, cache(v=v)) == 6
+    halves = dict(k_block=2 * 16 * 256, v_block=2 * 16 * 256)  # (num_blocks, 2, block_size, kv_heads, dim)
+    assert append(lib, cache(v=K + 16 * 256 - 16, **halves)) == 6
