@@ -49,7 +49,7 @@ extern "C" {
 #define SILKERN_E_DCP 3          /* invalid dcp_size / dcp_rank / interleave */
 #define SILKERN_E_BLOCK_SIZE 4   /* block_size < 1 or not divisible by interleave */
 #define SILKERN_E_TILE 5         /* unsupported tile_size */
-#define SILKERN_E_ALIAS 6        /* an output overlaps an input or another output */
+#define SILKERN_E_ALIAS 6        /* an output overlaps an input, another output or itself */
 #define SILKERN_E_GEOMETRY 7     /* explicit launch geometry rejected */
 #define SILKERN_E_SCRATCH 8      /* batch x tiles exceeds SILKERN_NOALLOC_MAX_TILES */
 #define SILKERN_E_CACHE 9        /* unsupported cache geometry, stride or alignment */
@@ -311,7 +311,8 @@ int silkern_topk_localize_explicit_v2(const float* logits, int64_t logits_stride
  * is below 2^31 and block_size at most 65536. Addresses of k and v are multiples
  * of 16.
  *
- * SILKERN_E_ALIAS: what a call writes shares memory with what it reads. Buffers
+ * SILKERN_E_ALIAS: what a call writes shares memory with what it reads, or two
+ * of its own elements do (a stride below what the smaller ones span). Buffers
  * with equal largest strides may lie between one another's rows; others are
  * compared as whole ranges of memory.
  */

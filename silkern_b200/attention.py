@@ -28,7 +28,8 @@ calls can be captured in a CUDA graph. They run on the current stream of the
 buffers' device. While ``torch.compile`` traces the caller, each routes through
 its op of the same name (:mod:`silkern_b200.ops`). Each raises
 :class:`LocalizationError` before launch on an unsupported binding or geometry.
-What a call writes shares no memory with what it reads, or the call is refused;
+What a call writes shares no memory with what it reads, nor with itself (as an
+expanded tensor does), or the call is refused;
 buffers that lie between one another's rows, as column slices of one tensor do,
 share none (where their largest strides are equal: others are compared as whole
 ranges of memory). They are for serving and have no backward pass: while gradients are recorded, a

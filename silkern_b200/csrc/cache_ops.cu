@@ -363,14 +363,22 @@ bool apart(const Place& a, int i, const Place& b, int j, int64_t shift) {
   const int64_t ahead = (shift % step + step) % step;
   return apart(a, i + 1, b, j + 1, ahead) && apart(a, i + 1, b, j + 1, ahead - step);
 }
+// Whether every step of a dimension leaves the smaller ones' extent behind.
+bool single(const Place& a) {
+  for (int i = 0; i < a.dims; ++i) {
+    if (a.stride[i] < a.extent(i + 1)) return false;
+  }
+  return true;
+}
 bool shares(const Place& a, const Place& b) {
   return a.bytes != 0 && b.bytes != 0 &&
          !apart(a, 0, b, 0, static_cast<int64_t>(b.begin) - static_cast<int64_t>(a.begin));
 }
-// Whether an output shares memory with another output or an input.
+// Whether an output shares memory with another output, an input or itself.
 template <int N, int M>
 bool shares(const Place (&outputs)[N], const Place (&inputs)[M]) {
   for (int i = 0; i < N; ++i) {
+    if (!single(outputs[i])) return true;
     for (int j = 0; j < M; ++j) {
       if (shares(outputs[i], inputs[j])) return true;
     }

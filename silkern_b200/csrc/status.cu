@@ -13,7 +13,7 @@ extern "C" const char* silkern_status_string_v1(int code) {
     case SILKERN_E_DCP: return "invalid dcp configuration";
     case SILKERN_E_BLOCK_SIZE: return "block_size must be a positive integer divisible by dcp_interleave";
     case SILKERN_E_TILE: return "unsupported tile_size";
-    case SILKERN_E_ALIAS: return "an output buffer overlaps an input or another output";
+    case SILKERN_E_ALIAS: return "an output buffer overlaps an input, another output or itself";
     case SILKERN_E_GEOMETRY: return "explicit launch geometry rejected";
     case SILKERN_E_SCRATCH:
       return "batch x tiles exceeds the allocation-free entry point's static workspace";

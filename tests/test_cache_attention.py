@@ -351,3 +351,15 @@ def test_append_refuses_keys_and_values_in_the_same_place(lib) -> None:
         assert append(lib, cache(v=v)) == 6
     halves = dict(k_block=2 * 16 * 256, v_block=2 * 16 * 256)  # (num_blocks, 2, block_size, kv_heads, dim)
     assert append(lib, cache(v=K + 16 * 256 - 16, **halves)) == 6
+
+
+def test_outputs_that_overlap_themselves_are_refused(lib) -> None:
+    """Expanded outputs, and strides that are less than what they step over."""
+    for row, head in ((0, 128), (256, 0), (128, 128), (256, 64), (248, 128), (8, 8)):
+        assert selected(lib, cache(), out_row=row, out_head=head) == 6
+    for blocks, tokens, heads in ((0, 256, 128), (16 * 256, 0, 128), (16 * 256, 256, 0), (16 * 256, 128, 128), (256, 256, 128)):
+        layout = dict(k_block=blocks, k_token=tokens, k_head=heads)
+        assert append(lib, cache(**layout)) == 6
+        assert append(lib, cache(**{name.replace("k_", "v_"): n for name, n in layout.items()})) == 6
+    assert lib.silkern_merge_partials_v1(Q, 32, 16, 8, IDX, 0, 2, 2, 2, 8, OUT, 0, 8, LSE, None) == 6
+    assert lib.silkern_merge_partials_v1(Q, 32, 16, 8, IDX, 0, 2, 2, 2, 8, OUT, 16, 4, LSE, None) == 6
