@@ -363,3 +363,15 @@ def test_outputs_that_overlap_themselves_are_refused(lib) -> None:
         assert append(lib, cache(**{name.replace("k_", "v_"): n for name, n in layout.items()})) == 6
     assert lib.silkern_merge_partials_v1(Q, 32, 16, 8, IDX, 0, 2, 2, 2, 8, OUT, 0, 8, LSE, None) == 6
     assert lib.silkern_merge_partials_v1(Q, 32, 16, 8, IDX, 0, 2, 2, 2, 8, OUT, 16, 4, LSE, None) == 6
+
+
+def test_strides_past_the_row_numbers_are_refused(lib) -> None:
+    """A row's number, in steps of what divides the strides, has to fit 31 bits: 16-byte steps reach 2**35 bytes."""
+    far = dict(num_blocks=2, k_head=16 * 11, k_token=16 * 22, k_block=2**35)
+    values = {name.replace("k_", "v_"): n for name, n in far.items()}
+    results = dict(out=2**45, lse=2**46)  # behind the caches' bytes
+    for c in (cache(**far), cache(**values)):
+        assert selected(lib, c, **results) == 9
+        assert window(lib, c, **results) == 9
+    latent = cache(latent=True, num_blocks=2, k_token=592, k_block=2**35)
+    assert selected(lib, latent, out_row=1024, out_head=512, **results) == 9

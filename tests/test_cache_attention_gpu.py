@@ -865,3 +865,64 @@ def test_merge_between_its_partial_results() -> None:
     assert torch.equal(held[:, 3], want) and torch.equal(held[:, :3].transpose(0, 1), outs)
     with pytest.raises(silkern.LocalizationError, match="overlaps"):
         silkern.merge_partials(held[:, :3].transpose(0, 1), lses, held[:, 2], want_lse)
+
+
+# ---------------------------------------------------------------------------------------- keys and values laid out apart
+
+LAYOUTS = ["unlike", "heads_first_values", "pages", "rows", "heads", "spread_pages"]
+
+
+def cache_in_layout(layout, blocks, block_size, kv_heads, dim, seed):
+    """The same cache, as two contiguous tensors and in a layout of K and V that is given by name."""
+    plain = make_cache(blocks, block_size, kv_heads, dim, seed=seed)
+    byte = dict(dtype=torch.uint8, device="cuda")
+    if layout == "unlike":  # keys token by token with room between, values head by head
+        k = torch.full((blocks, block_size, kv_heads + 1, dim + 16), 0x7F, **byte)[:, :, 1:, 16:]
+        v = torch.full((blocks, kv_heads, block_size, dim), 0x7F, **byte).permute(0, 2, 1, 3)
+    elif layout == "heads_first_values":  # pages of values among one another
+        k = torch.full((blocks, block_size, kv_heads, dim), 0x7F, **byte)
+        v = torch.full((block_size, kv_heads, blocks, dim), 0x7F, **byte).permute(2, 0, 1, 3)
+    elif layout == "pages":
+        k, v = torch.full((blocks, 2, block_size, kv_heads, dim), 0x7F, **byte).unbind(1)
+    elif layout == "rows":
+        k, v = torch.full((blocks, block_size, 2, kv_heads, dim), 0x7F, **byte).unbind(2)
+    elif layout == "heads":
+        k, v = torch.full((blocks, block_size, kv_heads, 2, dim), 0x7F, **byte).unbind(3)
+    else:  # a page of keys after every third page
+        k = torch.full((3 * blocks, block_size, kv_heads, dim), 0x7F, **byte)[2::3]
+        v = torch.full((blocks, block_size, kv_heads, dim), 0x7F, **byte)
+    for view, codes in ((k, plain[0]), (v, plain[1])):
+        view.copy_(codes.view(torch.uint8))
+    return plain, (k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn), plain[2].clone(), plain[3].clone())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("kv_heads,dim", [(3, 64), (2, 128), (1, 128)])
+def test_keys_and_values_in_layouts_of_their_own(kv_heads, dim, layout, dtype) -> None:
+    """Attention and append see places, not layouts: bit for bit what two
+    contiguous tensors give, which is held against 64 bits."""
+    plain, apart = cache_in_layout(layout, 24, 16, kv_heads, dim, seed=110)
+    g = torch.Generator().manual_seed(111)
+    heads = 4 * kv_heads
+    slots = torch.randint(-1, 24 * 16, (90, 500), generator=g, dtype=torch.int32).cuda()
+    table = torch.randperm(24, generator=g).to(torch.int32).view(2, 12).cuda()
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = randn(90, heads, dim, dtype=dtype, seed=112)
+    place = (ints(0, 50, 90), ints(192, 150), ints(1, 0), table)
+    for rows in (1, 90):
+        got = selected(q[:rows], slots[:rows], apart, dim, softmax_scale=0.1)
+        want = selected(q[:rows], slots[:rows], plain, dim, softmax_scale=0.1)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert_attention(*want, oracle.attend_selected(q[:rows], slots[:rows], *plain, softmax_scale=0.1), q[:rows], plain[0],
+                         plain[2], 0.1)
+    got, want = results(90, heads, dim, dtype), results(90, heads, dim, dtype)
+    silkern.attend_window(q, *place, *apart, *got, softmax_scale=0.1, window=60, sinks=3)
+    silkern.attend_window(q, *place, *plain, *want, softmax_scale=0.1, window=60, sinks=3)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    new = [torch.randn((90, kv_heads, dim), generator=g).to(dtype).cuda() for _ in range(2)]
+    order = (ints(0, 50, 90), ints(100, 3), ints(1, 0), table)
+    same = oracle.append(*new, *plain, *order)
+    silkern.append_quantized(*new, *apart, *order)
+    torch.cuda.synchronize()
+    same_cache(apart, same)
