@@ -340,8 +340,9 @@ typedef struct silkern_cache_v1 {
  * token is left out. */
 #define SILKERN_STATUS_BAD_SLOT 8
 /* Status bit of the attention entry points: a wait inside the kernel ran out
- * of its bound. The outputs of the work items concerned are not valid. It
- * does not occur in a working launch. */
+ * of its bound, and the pipeline of warps concerned gave up. The results of all
+ * of its work items, and those of an item that it shared with others, are NaN.
+ * It does not occur in a working launch. */
 #define SILKERN_STATUS_WAIT_TIMEOUT 16
 
 /*
@@ -427,6 +428,16 @@ int silkern_merge_partials_v1(const void* outs, int64_t outs_rank, int64_t outs_
                               int64_t outs_head, const float* lses, int32_t type, int64_t ranks,
                               int64_t rows, int64_t heads, int64_t dim, void* out, int64_t out_row,
                               int64_t out_head, float* lse, void* stream);
+
+/*
+ * Bound, in cycles of an SM's clock, on each wait of the attention kernels for
+ * another warp. 0 to 2^32; 4e9, about two seconds, to begin with. Holds
+ * for launches, and captures into graphs, from then on in the whole process.
+ * Returns the bound before; with a value out of range, changes nothing. For
+ * debuggers and other slow surroundings, and for tests: with 0 a kernel gives up
+ * at once, and says so as SILKERN_STATUS_WAIT_TIMEOUT does.
+ */
+int64_t silkern_attend_wait_bound_v1(int64_t cycles);
 
 /* Static text for a return code (positive SILKERN_E*, 0, or -cudaError_t). */
 const char* silkern_status_string_v1(int code);

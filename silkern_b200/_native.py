@@ -110,6 +110,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_ptr, _i64, _i64, _i64, _ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr],
     ),
+    "silkern_attend_wait_bound_v1": (_i64, [_i64]),
     "silkern_status_string_v1": (ctypes.c_char_p, [ctypes.c_int]),
     "silkern_abi_version_v1": (ctypes.c_int, []),
     "silkern_fastdiv_selftest_v1": (_i64, [_u32, _u32, _u32]),

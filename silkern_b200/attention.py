@@ -55,7 +55,7 @@ LATENT_KEY_DIM = 576
 LATENT_VALUE_DIM = 512
 #: Status bits (OR-ed into ``status``) besides SILKERN_STATUS_BAD_REQUEST (1)
 #: and STATUS_BAD_LENGTH (2): a slot or page outside the cache, left out; and a
-#: wait inside a kernel that ran out of its bound.
+#: wait inside an attention kernel that ran out of its bound, whose results are NaN.
 STATUS_BAD_SLOT = 8
 STATUS_WAIT_TIMEOUT = 16
 

@@ -1,5 +1,6 @@
 // Launch of the cache's attention: how many columns a CTA takes and how many
 // CTAs share a work item's keys.
+#include <atomic>
 #include <numeric>
 
 #include "attend_plan.cuh"
@@ -10,6 +11,9 @@
 namespace silkern {
 
 namespace {
+
+// About two seconds.
+std::atomic<int64_t> wait_bound{4000000000};
 
 int multiprocessors() {
   int device = 0, n = 0;
@@ -44,6 +48,7 @@ bool find_rows(const PagedCache& c, int64_t block, int64_t token, int64_t head, 
 }  // namespace
 
 int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
+  a.wait_cycles = wait_bound.load(std::memory_order_relaxed);
   const bool latent = key_dim == 576, half = type == SILKERN_F16;
   const int32_t group = a.heads_per_kv;
   // Queries that may share a CTA's keys: one for a selected row; for
@@ -138,3 +143,8 @@ int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
 }
 
 }  // namespace silkern
+
+extern "C" int64_t silkern_attend_wait_bound_v1(int64_t cycles) {
+  if (cycles < 0 || cycles > (int64_t{1} << 32)) return silkern::wait_bound.load(std::memory_order_relaxed);
+  return silkern::wait_bound.exchange(cycles, std::memory_order_relaxed);
+}

@@ -172,11 +172,11 @@ __device__ __forceinline__ int32_t ordered(float x) {
 __device__ __forceinline__ float unordered(int32_t b) { return __int_as_float(b >= 0 ? b : b ^ 0x7fffffff); }
 
 // A whole warp waits. A wait that ran out leaves *abort set, and every later
-// wait returns at once: an item's loops then run to their end on whatever is
-// there, so that each barrier gets the arrivals it counts, the results are not
-// stored, and no further item begins.
-__device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  mbar_wait(smem_addr(bar), parity, abort);
+// wait returns after a try or two (some 4 us): the gathering and the MMAs end, a
+// softmax runs through its item's tiles on whatever is there, so that its
+// groups' barriers get the arrivals they count, and no further item begins.
+__device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int64_t bound) {
+  mbar_wait(smem_addr(bar), parity, abort, bound);
   __syncwarp();
 }
 
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     mbar_init(smem_addr(&sh.done), 1);
     mbar_init(smem_addr(&sh.queries_read), 1);
     mbar_init(smem_addr(&sh.drained), 1);
-    sh.abort = 0;
+    sh.abort = a.wait_cycles == 0 ? 1 : 0;
     sh.last_known = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
@@ -388,6 +388,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
   const uint32_t tmem_all = __shfl_sync(kAllLanes, first.tmem, 0);
   const uint32_t tmem = tmem_all + pipe * C::kPipeColumns;
   volatile int* abort = &sh.abort;
+  const int64_t bound = a.wait_cycles;
   pdl_wait();
   pdl_launch_dependents();
 
@@ -410,7 +411,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     const int group_barrier = kFirstGroup + pipe * C::kGroups + wg;
     uint32_t n = 0, n3 = 0, b = 0, turn = 0;  // tiles so far; modulo 3; stage and its turn
     for (uint32_t seq = 0;; ++seq) {
-      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort);
+      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort, bound);
       // Everybody stops or nobody: the groups' barriers count on it.
       if (named_barrier_or(1 + pipe, C::kSoftmax, *abort != 0)) break;
       const Handed h = sh.handed[seq & 1];
@@ -430,13 +431,13 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       float own_reference;      // Q of column own, where it is the warp's own
       // A tile up to its columns' maxima.
       auto begin_tile = [&]() {
-        warp_wait(&sh.scores[n & 1], (n >> 1) & 1, abort);
+        warp_wait(&sh.scores[n & 1], (n >> 1) & 1, abort, bound);
         tc_fence_after();
         const uint32_t s_at = tmem + lanes + C::kValues * NH + (n & 1) * (T * NH) + first_col;
         float s1[16];
         tmem_ld16(s_at, t);
         tmem_ld16(s_at + NH, s1);
-        warp_wait(&sh.full[C::kNoteChunk][b], turn, abort);
+        warp_wait(&sh.full[C::kNoteChunk][b], turn, abort, bound);
         valid = (sh.valid[b][warp & 3] >> lane) & 1;
         const float ks = sh.k_scale[b][thread];
         vs = C::kIsLatent ? ks : sh.v_scale[C::kIsLatent ? 0 : b][C::kIsLatent ? 0 : thread];
@@ -519,7 +520,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           // written them, and nobody is still at the tile before.
           if (lane < 16) sh.reference[first_col + lane] = to == -INFINITY ? 0.f : 5.f - to;
           __syncwarp();
-          if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
+          if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort, bound);
           waited = true;
           tc_fence_after();
           float f[16];
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
             for (int p = 0; p < T; ++p) part[c][p] = 0;
           }
         }
-        if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort);
+        if (!waited) warp_wait(&sh.done, (n - 1) & 1, abort, bound);
         const uint32_t at = NH == 64 ? thread * 64 + ((wg ^ ((thread >> 1) & 3)) << 4)
                             : NH == 32 ? thread * 32 + ((wg ^ ((thread >> 2) & 1)) << 4) : thread * 16;
 #pragma unroll
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         }
         // One reference for the item's end: 2^32 above the largest Q of the
         // warps, so that O fits as well, whatever the scales and the keys.
-        warp_wait(&sh.done, (n - 1) & 1, abort);
+        warp_wait(&sh.done, (n - 1) & 1, abort, bound);
         tc_fence_after();
         float* qs = reinterpret_cast<float*>(smem + C::kOffP + wg * 4096) + 64;
         if (lane < 16) qs[(warp & 3) * 16 + lane] = own_reference;
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         }
         tmem_wait_st();
       }
-      if (h.steps > 0) warp_wait(&sh.done, (n - 1) & 1, abort);
+      if (h.steps > 0) warp_wait(&sh.done, (n - 1) & 1, abort, bound);
       tc_fence_after();
       // Sums over the keys: lanes first, then the group's warps. The weights'
       // buffer is free by now and takes the warps' sums, then the outputs.
@@ -809,14 +810,14 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         if constexpr (C::kIsLatent) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            warp_wait(&sh.empty[c][b], turn ^ 1, abort);
+            warp_wait(&sh.empty[c][b], turn ^ 1, abort, bound);
             copy(stage + c * C::kChunkBytes, a.cache.k + c * 128, a.cache.k_pitch);
             if (c == C::kNoteChunk) note();
             cp_async_arrive(smem_addr(&sh.full[c][b]));
           }
           const uint32_t tb = C::kTails == 1 ? 0 : b, tt = C::kTails == 1 ? tail_turn : turn;
           tail_turn ^= 1;
-          warp_wait(&sh.empty[4][tb], tt ^ 1, abort);
+          warp_wait(&sh.empty[4][tb], tt ^ 1, abort, bound);
           const uint32_t to = base + C::kOffTail + tb * C::kTailBytes + (w * kShare + lane / 4) * 64 +
                               (((lane ^ (lane >> 3)) & 3) << 4);
 #pragma unroll
@@ -830,7 +831,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           // the keys behind them.
           const uint32_t keys_at = stage + (SHAPE == kDim64 ? C::kChunkBytes : 0);
           const uint32_t values_at = stage + (SHAPE == kDim64 ? 0 : C::kChunkBytes);
-          warp_wait(&sh.empty[0][b], turn ^ 1, abort);
+          warp_wait(&sh.empty[0][b], turn ^ 1, abort, bound);
           copy(keys_at, a.cache.k, a.cache.k_pitch);
           cp_async_arrive(smem_addr(&sh.full[0][b]));
           if (!alike) {
@@ -839,7 +840,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
               row[n] = __shfl_sync(kAllLanes, v_row[n * kRows / 32], (n * kRows) % 32 + sub);
             }
           }
-          warp_wait(&sh.empty[1][b], turn ^ 1, abort);
+          warp_wait(&sh.empty[1][b], turn ^ 1, abort, bound);
           copy(values_at, a.cache.v, a.cache.v_pitch);
           note();
           cp_async_arrive(smem_addr(&sh.full[1][b]));
@@ -848,7 +849,9 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
           b = 0;
           turn ^= 1;
         }
+        if (__any_sync(kAllLanes, *abort != 0)) break;
       }
+      if (__any_sync(kAllLanes, *abort != 0)) break;
     }
     cp_async_wait_all();
     if (__any_sync(kAllLanes, bad) && lane == 0) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
@@ -921,8 +924,8 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         __syncwarp();
         bring(w * kBatch);
       }
-      if (seq > 0) warp_wait(&sh.queries_read, (seq - 1) & 1, abort);
-      if (seq > 1) warp_wait(&sh.finished[seq & 1], ((seq >> 1) - 1) & 1, abort);
+      if (seq > 0) warp_wait(&sh.queries_read, (seq - 1) & 1, abort, bound);
+      if (seq > 1) warp_wait(&sh.finished[seq & 1], ((seq >> 1) - 1) & 1, abort, bound);
       if (__any_sync(kAllLanes, *abort != 0)) break;  // what was handed on stays
       if (end) {
         if (w == 0 && lane == 0) sh.handed[seq & 1].steps = -1;
@@ -1013,7 +1016,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     uint32_t n = 0;                                          // tiles before this item
     bool more = true;
     for (uint32_t seq = 0; more; ++seq) {
-      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort);
+      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort, bound);
       if (__any_sync(kAllLanes, *abort != 0)) break;
       const int32_t steps = __shfl_sync(kAllLanes, sh.handed[seq & 1].steps, 0);
       more = steps >= 0 && __shfl_sync(kAllLanes, sh.handed[seq & 1].split, 0) == 0;
@@ -1021,7 +1024,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         const uint32_t d = tmem + C::kValues * NH + ((n + i) & 1) * (T * NH);
 #pragma unroll
         for (int c = 0; c < C::kMainKeys; ++c) {
-          warp_wait(&sh.full[c][sb], st, abort);
+          warp_wait(&sh.full[c][sb], st, abort, bound);
           fence_proxy_async();  // the copies wrote through the generic proxy
           if (leader) {
             const uint64_t kd = k_desc + ((sb * C::kStageBytes + c * C::kChunkBytes) >> 4);
@@ -1034,7 +1037,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         if constexpr (C::kIsLatent) {
           const uint32_t tb = C::kTails == 1 ? 0 : sb, tt = C::kTails == 1 ? tail_turn : st;
           tail_turn ^= 1;
-          warp_wait(&sh.full[4][tb], tt, abort);
+          warp_wait(&sh.full[4][tb], tt, abort, bound);
           fence_proxy_async();
           if (leader) {
             const uint64_t kd = smem_descriptor(base + C::kOffTail + tb * C::kTailBytes, 16, 512, kSwizzle64);
@@ -1057,10 +1060,10 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         }
       };
       auto outputs = [&](int32_t i) {
-        warp_wait(&sh.weights, (n + i) & 1, abort);
+        warp_wait(&sh.weights, (n + i) & 1, abort, bound);
         tc_fence_after();
         if constexpr (!C::kIsLatent) {
-          warp_wait(&sh.full[1][ob], ot, abort);
+          warp_wait(&sh.full[1][ob], ot, abort, bound);
           fence_proxy_async();
         }
         if (leader) {
@@ -1091,6 +1094,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       for (int32_t i = 0; i <= steps && steps > 0; ++i) {
         if (i < steps) scores(i);
         if (i > 0) outputs(i - 1);
+        if (__any_sync(kAllLanes, *abort != 0)) break;
       }
       if (steps > 0) n += steps;
     }
@@ -1107,6 +1111,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
   }
 
   __syncthreads();
+  const bool gave_up = *abort != 0;
   // ---- a split item: its ranks, which all see the same tiles, join
   Handed last{};
   if (has_split) {
@@ -1124,7 +1129,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     const int first_col = (warp >> 2) * 16, own = lane & 15;
     if (warp < kLoadWarp && (warp & 3) == 0 && lane < 16) {
       joint[first_col + lane] = reference;
-      joint[NH + first_col + lane] = l[0];
+      joint[NH + first_col + lane] = gave_up ? NAN : l[0];  // and so every rank's results
     }
     cluster_sync();
     // Rank r is pipeline r mod kPipes of CTA r / kPipes.
@@ -1161,7 +1166,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       const float2 down = reference == -INFINITY ? make_float2(1.f, 0.f) : exp2_factors(reference - whole_r);
       const float by = down.y * inverse;
       const bool far = __any_sync(kAllLanes, down.x != 1.f);
-      if (rank == 0 && (warp & 3) == 0 && lane < 16 && *abort == 0) {
+      if (rank == 0 && (warp & 3) == 0 && lane < 16) {
         const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, first_col + lane);
         if (col.used) {
           a.lse[static_cast<int64_t>(last.row + col.query) * a.heads + col.head] =
@@ -1206,7 +1211,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     for (int32_t e = tid * 4; e < joins * C::kValueDim; e += kRankThreads * 4) {
       const int32_t c = e / C::kValueDim, d = e - c * C::kValueDim;
       const Column col = find_column<NH>(a, plan, last.count, last.kv, last.block, mine + c);
-      if (!col.used || *abort != 0) continue;
+      if (!col.used) continue;
       float4 y{0.f, 0.f, 0.f, 0.f};
       for (uint32_t r = 0; r < ranks; ++r) {
         const float4 x = *reinterpret_cast<const float4*>(joined + r * share * C::kValueDim + e);
@@ -1224,6 +1229,24 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+  }
+  if (gave_up) {  // no result of this pipeline's items is left as it was before the call
+    uint32_t unit = blockIdx.x * C::kPipes + pipe;
+    bool rest = has_split && !last.split && rank == 0;  // a split item without keys
+    while (unit < plan.whole || rest) {
+      const bool whole = unit < plan.whole;
+      const Work work = find_work(a, plan, whole ? unit : split_unit, 0, 1);
+      unit = whole ? unit + whole_step : unit;
+      rest = rest && whole;
+      for (int c = warp; c < NH; c += C::kPipeWarps) {
+        const Column col = find_column<NH>(a, plan, work.span.count, work.kv, work.block, c);
+        if (!col.used) continue;
+        const int64_t row = work.span.row + col.query;
+        E* out = static_cast<E*>(a.out) + row * a.out_row + static_cast<int64_t>(col.head) * a.out_head;
+        for (int d = lane; d < C::kValueDim; d += 32) out[d] = static_cast<E>(NAN);
+        if (lane == 0) a.lse[row * a.heads + col.head] = NAN;
+      }
+    }
   }
   if (pipe == 0 && warp == kMmaWarp) {
     tc_fence_after();

@@ -69,6 +69,7 @@ struct AttendArgs {
   bool out_wide;  // rows of out start on 16-byte boundaries
   float* lse;  // (rows, heads), contiguous
   int32_t* status;
+  int64_t wait_cycles;  // bound on a wait inside the kernel
   float scale_log2;  // softmax_scale * log2(e)
   int32_t rows, heads;
   int32_t heads_per_kv;

@@ -27,13 +27,13 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// Wait for phase `parity` of `bar`, for at most about two seconds or until
+// Wait for phase `parity` of `bar`, for about `bound` cycles at most or until
 // *abort is set; on giving up, set *abort. Returns whether the phase completed.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, int64_t bound) {
   if (mbar_try(bar, parity)) return true;
   const long long begin = clock64();
   while (!mbar_try(bar, parity)) {
-    if (*abort != 0 || clock64() - begin > 4000000000LL) {
+    if (*abort != 0 || clock64() - begin >= bound) {
       *abort = 1;
       return false;
     }
