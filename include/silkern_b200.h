@@ -431,7 +431,8 @@ int silkern_merge_partials_v1(const void* outs, int64_t outs_rank, int64_t outs_
 
 /*
  * Bound, in cycles of an SM's clock, on each wait of the attention kernels for
- * another warp. 0 to 2^32; 4e9, about two seconds, to begin with. Holds
+ * another warp's part of one tile of 128 keys (waits over several tiles have as
+ * many times the bound). 0 to 2^32; 4e9, about two seconds, to begin with. Holds
  * for launches, and captures into graphs, from then on in the whole process.
  * Returns the bound before; with a value out of range, changes nothing. For
  * debuggers and other slow surroundings, and for tests: with 0 a kernel gives up

@@ -388,6 +388,8 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
   const uint32_t tmem_all = __shfl_sync(kAllLanes, first.tmem, 0);
   const uint32_t tmem = tmem_all + pipe * C::kPipeColumns;
   volatile int* abort = &sh.abort;
+  // A wait's bound is one tile's, but for a wait that lasts over an item's tiles
+  // or over the empty items before the next one.
   const int64_t bound = a.wait_cycles;
   pdl_wait();
   pdl_launch_dependents();
@@ -396,6 +398,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
   const uint32_t ctas = cluster_size();
   const uint32_t rank = cluster_ctarank() * C::kPipes + pipe, ranks = ctas * C::kPipes;
   const uint32_t whole_step = gridDim.x * C::kPipes;
+  const int64_t item_bound = bound * (1 + plan.units / whole_step);
   const uint32_t split_unit = plan.whole + blockIdx.x / ctas;
   const bool has_split = split_unit < plan.units;
   // Softmax state that outlives the loop for a split item.
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     const int group_barrier = kFirstGroup + pipe * C::kGroups + wg;
     uint32_t n = 0, n3 = 0, b = 0, turn = 0;  // tiles so far; modulo 3; stage and its turn
     for (uint32_t seq = 0;; ++seq) {
-      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort, bound);
+      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort, item_bound);
       // Everybody stops or nobody: the groups' barriers count on it.
       if (named_barrier_or(1 + pipe, C::kSoftmax, *abort != 0)) break;
       const Handed h = sh.handed[seq & 1];
@@ -862,6 +865,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     // end here: out 0, lse -inf.
     const int w = warp - kSplitWarp;
     uint32_t unit = blockIdx.x * C::kPipes + pipe, seq = 0;
+    int32_t steps_before = 0;  // tiles of the item before
     bool shared = false;
     while (true) {
       Work work;
@@ -924,7 +928,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
         __syncwarp();
         bring(w * kBatch);
       }
-      if (seq > 0) warp_wait(&sh.queries_read, (seq - 1) & 1, abort, bound);
+      if (seq > 0) warp_wait(&sh.queries_read, (seq - 1) & 1, abort, bound * (steps_before + 1));
       if (seq > 1) warp_wait(&sh.finished[seq & 1], ((seq >> 1) - 1) & 1, abort, bound);
       if (__any_sync(kAllLanes, *abort != 0)) break;  // what was handed on stays
       if (end) {
@@ -993,6 +997,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       }
       fence_proxy_async();
       mbar_arrive(smem_addr(&sh.queries[seq & 1]));
+      steps_before = work.steps;
       ++seq;
       if (split) break;
     }
@@ -1016,7 +1021,7 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
     uint32_t n = 0;                                          // tiles before this item
     bool more = true;
     for (uint32_t seq = 0; more; ++seq) {
-      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort, bound);
+      warp_wait(&sh.queries[seq & 1], (seq >> 1) & 1, abort, item_bound);
       if (__any_sync(kAllLanes, *abort != 0)) break;
       const int32_t steps = __shfl_sync(kAllLanes, sh.handed[seq & 1].steps, 0);
       more = steps >= 0 && __shfl_sync(kAllLanes, sh.handed[seq & 1].split, 0) == 0;

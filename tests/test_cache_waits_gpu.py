@@ -1,4 +1,5 @@
-"""The bound on the waits inside the attention kernels: what a call that gives up leaves."""
+"""The bound on the waits inside the attention kernels: what a call that gives up leaves, and that
+a long item alone does not make it give up."""
 
 from __future__ import annotations
 
@@ -106,3 +107,24 @@ def test_a_window_that_gives_up_leaves_other_rows_alone(shape) -> None:
         got = call()
     assert assert_right_or_nan(got, want) > 0
     assert bool((got[0][50:] == 7).all()) and bool((got[1][50:] == 7).all())
+
+
+def test_an_item_may_last_longer_than_a_wait() -> None:
+    """Half a millisecond for each tile, and items of several milliseconds: the
+    wait for an item's end has its tiles' bound, not one's."""
+    dim, rows = 576, 90
+    cache = make_cache(512, 64, 1, dim, latent=True, seed=4)
+    slots = torch.randint(0, 512 * 64, (1, 400_000), generator=torch.Generator().manual_seed(5), dtype=torch.int32).cuda()
+    slots = slots.expand(rows, -1)
+    q = torch.randn((rows, 16, dim), generator=torch.Generator().manual_seed(6)).to(torch.bfloat16).cuda()
+    out, lse = torch.empty((rows, 16, 512), dtype=torch.bfloat16, device="cuda"), torch.empty((rows, 16), device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    cycles = 1_000_000
+    with wait_bound(cycles):
+        begin.record()
+        silkern.attend_selected(q, slots, *cache, out, lse, softmax_scale=dim**-0.5, status=status)
+        end.record()
+    # at 2 GHz at most, an item that lasts the whole call exceeds the bound four times over
+    assert begin.elapsed_time(end) * 2e6 > 4 * cycles
+    assert status.item() == 0 and bool(torch.isfinite(lse).all())
