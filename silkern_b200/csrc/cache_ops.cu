@@ -333,6 +333,10 @@ struct Place {
   Place(const void* base, int64_t inner) : begin(reinterpret_cast<uintptr_t>(base)), bytes(base == nullptr ? 0 : inner) {}
   Place&& along(int64_t n, int64_t step) && {
     if (n > 1) {
+      if (step < 0) {  // the same places, from the lowest
+        begin += static_cast<uintptr_t>((n - 1) * step);
+        step = -step;
+      }
       int at = dims++;
       for (; at > 0 && stride[at - 1] < step; --at) {
         count[at] = count[at - 1];

@@ -375,3 +375,12 @@ def test_strides_past_the_row_numbers_are_refused(lib) -> None:
         assert window(lib, c, **results) == 9
     latent = cache(latent=True, num_blocks=2, k_token=592, k_block=2**35)
     assert selected(lib, latent, out_row=1024, out_head=512, **results) == 9
+
+
+def test_strides_that_run_backwards_are_followed(lib) -> None:
+    """From C, rows may lie from the last address to the first: an overlap with them is seen there."""
+    assert selected(lib, cache(), rows=4, q_row=-256, out=Q - 2 * 256 * 3) == 6
+    assert selected(lib, cache(), rows=4, out=Q + 2 * 256 * 3, out_row=-256) == 6
+    assert selected(lib, cache(), rows=4, out=Q + 2 * 256 * 7 - 2, out_row=-256) == 6
+    assert selected(lib, cache(), rows=4, slots=IDX, slots_row=-32, lse=IDX - 4 * 32 * 3) == 6
+    assert lib.silkern_merge_partials_v1(Q, 32, 16, 8, IDX, 0, 2, 2, 2, 8, Q + 2 * 72, -16, 8, LSE, None) == 6
