@@ -1,6 +1,4 @@
 // The attention kernel for heads of 64.
-#include <array>
-
 #include "attend_kernel.cuh"
 
 namespace silkern {
@@ -12,37 +10,36 @@ int launch_dim64(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch
 int resident_clusters(int size) {
   using C = Config<kDim64, 16, 2>;
   const auto kernel = attend_kernel<kDim64, 16, 2>;
-  static std::mutex mutex;
-  static std::vector<std::pair<int, std::array<int, kMostCluster + 1>>> known;
+  static DeviceBits granted{0};
+  static std::atomic<int> known[kNotedDevices][kMostCluster + 1];  // one more than the number; 0: not asked yet
   int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || allow_launch(reinterpret_cast<const void*>(kernel), kSharedMemory) != SILKERN_OK) {
+  if (cudaGetDevice(&device) != cudaSuccess) {
     (void)cudaGetLastError();
     return 0;
   }
-  std::lock_guard<std::mutex> lock(mutex);
-  for (const auto& k : known) {
-    if (k.first == device) return k.second[size];
+  if (device < kNotedDevices) {
+    const int told = known[device][size].load(std::memory_order_relaxed);
+    if (told > 0) return told - 1;
   }
-  std::array<int, kMostCluster + 1> room{};
-  for (int n = 1; n <= kMostCluster; ++n) {
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = n;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(n, 1, 1);
-    cfg.blockDim = dim3(C::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = kSharedMemory;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&room[n], kernel, &cfg) != cudaSuccess) {
-      (void)cudaGetLastError();
-      room[n] = 0;
-    }
+  if (allow_launch(reinterpret_cast<const void*>(kernel), kSharedMemory, granted) != SILKERN_OK) return 0;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(size, 1, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kSharedMemory;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int room = 0;
+  if (cudaOccupancyMaxActiveClusters(&room, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    room = 0;
   }
-  known.emplace_back(device, room);
-  return room[size];
+  if (device < kNotedDevices) known[device][size].store(room + 1, std::memory_order_relaxed);
+  return room;
 }
 
 }  // namespace silkern

@@ -1262,7 +1262,8 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
 template <CacheShape SHAPE, int NH, int T>
 int launch_config(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l) {
   using C = Config<SHAPE, NH, T>;
-  const int rc = allow_launch(reinterpret_cast<const void*>(attend_kernel<SHAPE, NH, T>), kSharedMemory);
+  static DeviceBits granted{0};
+  const int rc = allow_launch(reinterpret_cast<const void*>(attend_kernel<SHAPE, NH, T>), kSharedMemory, granted);
   if (rc != SILKERN_OK) return rc;
   return launch_pdl(attend_kernel<SHAPE, NH, T>, l.grid, C::kThreads, kSharedMemory, l.cluster, l.stream, a, plan);
 }

@@ -26,7 +26,8 @@ struct AttendLaunch {
 };
 
 // How many clusters of `size` CTAs of these kernels (which all take a whole SM)
-// the current device holds at once. Asked once for each device; 0 on failure.
+// the current device holds at once. Asked once for each device and size; 0 on
+// failure.
 int resident_clusters(int size);
 
 int launch_dim64(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);

@@ -3,10 +3,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
-#include <mutex>
-#include <utility>
-#include <vector>
 
 #include "silkern_b200.h"
 
@@ -48,25 +46,26 @@ int launch_pdl(void (*fn)(P...), unsigned grid, unsigned threads, size_t smem, u
   return launch_pdl_grid(fn, dim3(grid, 1, 1), threads, smem, cluster, stream, args...);
 }
 
+// Devices that `known` notes of a kernel's launch permissions; others are asked
+// for at each call. Nothing here allocates or throws: C callers come in.
+constexpr int kNotedDevices = 64;
+using DeviceBits = std::atomic<uint64_t>;
+
 // Let `kernel` use `bytes` of dynamic shared memory, all of an SM's shared
 // memory, and clusters of up to 16 CTAs, on the current device. The driver is
-// asked once for each kernel and device.
-inline int allow_launch(const void* kernel, int bytes) {
-  static std::mutex mutex;
-  static std::vector<std::pair<const void*, int>> granted;
+// asked once for each kernel (which has a `granted` of its own) and device.
+inline int allow_launch(const void* kernel, int bytes, DeviceBits& granted) {
   int device = 0;
   cudaError_t err = cudaGetDevice(&device);
   if (err == cudaSuccess) {
-    std::lock_guard<std::mutex> lock(mutex);
-    for (const auto& g : granted) {
-      if (g.first == kernel && g.second == device) return SILKERN_OK;
-    }
+    const uint64_t bit = device < kNotedDevices ? uint64_t{1} << device : 0;
+    if ((granted.load(std::memory_order_acquire) & bit) != 0) return SILKERN_OK;
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err == cudaSuccess) {
       err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     }
     if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (err == cudaSuccess) granted.emplace_back(kernel, device);
+    if (err == cudaSuccess) granted.fetch_or(bit, std::memory_order_release);
   }
   if (err == cudaSuccess) return SILKERN_OK;
   (void)cudaGetLastError();

@@ -926,3 +926,47 @@ def test_keys_and_values_in_layouts_of_their_own(kv_heads, dim, layout, dtype) -
     silkern.append_quantized(*new, *apart, *order)
     torch.cuda.synchronize()
     same_cache(apart, same)
+
+
+def test_first_calls_from_several_threads_at_once() -> None:
+    """A fresh process, whose threads are the first to ask for launch
+    permissions and cluster sizes, each on a stream of its own."""
+    import subprocess
+    import sys
+
+    code = """
+import threading, torch
+import silkern_b200 as silkern
+from tests.attention_cases import make_cache
+torch.cuda.init()
+jobs, start = [], threading.Barrier(6)
+for i, (dim, heads, rows) in enumerate([(64, 8, 1), (128, 64, 1), (576, 16, 3), (64, 8, 200), (128, 8, 90), (576, 128, 40)]):
+    latent = dim == 576
+    cache = make_cache(40, 64, 1, dim, latent=latent, seed=i)
+    q = torch.randn((rows, heads, dim), generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).cuda()
+    slots = torch.randint(0, 2560, (rows, 2000), dtype=torch.int32, generator=torch.Generator().manual_seed(i)).cuda()
+    outs = [torch.empty((rows, heads, 512 if latent else dim), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    jobs.append((q, slots, cache, outs, [torch.empty((rows, heads), device="cuda") for _ in range(2)]))
+torch.cuda.synchronize()
+errors = []
+def run(q, slots, cache, outs, lses):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait()
+            for _ in range(20):
+                silkern.attend_selected(q, slots, *cache, outs[0], lses[0], softmax_scale=0.05)
+            torch.cuda.current_stream().synchronize()
+    except Exception as error:
+        errors.append(error)
+threads = [threading.Thread(target=run, args=job) for job in jobs]
+for t in threads: t.start()
+for t in threads: t.join()
+assert not errors, errors
+for q, slots, cache, outs, lses in jobs:
+    silkern.attend_selected(q, slots, *cache, outs[1], lses[1], softmax_scale=0.05)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(lses[0], lses[1]) and bool(torch.isfinite(lses[0]).all())
+print("threads agree")
+"""
+    proc = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert proc.returncode == 0 and "threads agree" in proc.stdout, proc.stderr[-2000:]

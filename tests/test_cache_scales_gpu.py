@@ -19,6 +19,9 @@ from tests.attention_cases import HALF_STEP, score_error  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
+if not torch.cuda.is_available():
+    pytest.skip("a CUDA device is required", allow_module_level=True)
+
 PAGE = 128  # a tile of the kernel, so that a tile's values have one scale
 
 

@@ -16,6 +16,9 @@ from tests.attention_cases import make_cache  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
+if not torch.cuda.is_available():
+    pytest.skip("a CUDA device is required", allow_module_level=True)
+
 SHAPES = {"d64": (64, 64, False), "d128": (128, 128, False), "latent": (576, 512, True)}
 
 
