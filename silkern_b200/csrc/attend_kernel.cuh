@@ -35,7 +35,7 @@
 // count nothing, goes into u as 2^-100) each warp keeps a Q of its own, the
 // largest s of its keys, and takes a second exponential for the sum; at the
 // item's end O and l come to one reference again. That holds for any scales in
-// [2^-100, 2^100], in any order, and costs the usual ones 0 to 4 % (a flag of
+// [2^-100, 2^100], in any order, and costs the usual ones 0 to 5 % (a flag of
 // the tile, looked at behind the barrier that the maxima need anyway).
 //
 // A CTA is one or two pipelines, each a softmax of one key a thread and 16
@@ -51,11 +51,12 @@
 // workspace, one launch.
 //
 // Measured: a decode step of 128 sequences, 8 heads of 128, window 4096 (1.02
-// GB): 197-209 us, 5.2 TB/s, bound by memory. 256 rows of 512 latent keys, 128
+// GB): 207 us, 4.9 TB/s, bound by memory. 256 rows of 512 latent keys, 128
 // heads: 85 us, 428 TFLOP/s, bound by an item's start and end (four tiles
-// between them). 4001 queries of a prompt, window 1024, heads of 64, fp16: 256
-// us, bound by the softmax's instructions. One row over 131072 tokens: 80 us,
-// 3.3 TB/s on the 80 SMs that clusters for 8 heads reach.
+// between them). 4001 queries of a prompt, window 1024, heads of 64, fp16: 268
+// us, bound by the softmax's instructions. One row over 131072 tokens: 81 us,
+// 3.3 TB/s on the 80 SMs that clusters for 8 heads reach. With value scales
+// outside 2^+-kUsual throughout: 5 (latent) to 37 % (prompt) longer.
 #pragma once
 
 #include <cuda_bf16.h>
