@@ -33,6 +33,7 @@ DEPENDS = SOURCES + [
     os.path.join(CSRC, "fastdiv.cuh"),
     os.path.join(CSRC, "ptx.cuh"),
     os.path.join(CSRC, "host.cuh"),
+    os.path.join(CSRC, "cache_checks.cuh"),
     os.path.join(CSRC, "paged.cuh"),
     os.path.join(CSRC, "tcgen05.cuh"),
     os.path.join(CSRC, "attend_plan.cuh"),
