@@ -56,6 +56,7 @@ extern "C" {
 #define SILKERN_E_HEADS 10       /* heads not a positive multiple of the cache's heads */
 #define SILKERN_E_TYPE 11        /* element type is neither SILKERN_BF16 nor SILKERN_F16 */
 #define SILKERN_E_ATTEND 12      /* window, sinks or softmax scale out of range */
+#define SILKERN_E_ROTARY 13      /* rotary or norm columns, amplitude or epsilon out of range */
 
 #define SILKERN_STATUS_BAD_REQUEST 1
 /* Status bit of the converter entry points (OR-ed into *status): a row split
@@ -428,6 +429,60 @@ int silkern_merge_partials_v1(const void* outs, int64_t outs_rank, int64_t outs_
                               int64_t outs_head, const float* lses, int32_t type, int64_t ranks,
                               int64_t rows, int64_t heads, int64_t dim, void* out, int64_t out_row,
                               int64_t out_head, float* lse, void* stream);
+
+/*
+ * Read the 8-bit cache back: sequence b (of `sequences`) has the rows
+ * [cu_tokens[b], cu_tokens[b + 1]) of keys (tokens, kv_heads, key_dim) and
+ * values (tokens, kv_heads, value_dim; NULL for a latent cache), which become
+ * scale * code of the positions starts[b], starts[b] + 1, ... of the request
+ * req_ids[b], through block_table. Rows of positions that other ranks own, and
+ * rows at and past cu_tokens[sequences], are left as they were. The layouts and
+ * the arguments are those of silkern_append_quantized_v1.
+ */
+int silkern_read_quantized_v1(const silkern_cache_v1* cache, void* keys, int64_t key_token,
+                              int64_t key_head, void* values, int64_t value_token,
+                              int64_t value_head, int32_t type, int64_t tokens,
+                              const int32_t* cu_tokens, const int32_t* starts,
+                              const int32_t* req_ids, int64_t sequences,
+                              const int32_t* block_table, int64_t table_rows,
+                              int64_t table_width, int32_t dcp_size, int32_t dcp_rank,
+                              int32_t dcp_interleave, int32_t* status, void* stream);
+
+/*
+ * One set of heads for silkern_rotate_heads_v1: in and out are (tokens, heads,
+ * dim) with unit column stride and strides in elements; the first norm_columns
+ * columns of each head are normed with `weight` (norm_columns elements; NULL
+ * with none).
+ */
+typedef struct silkern_heads_v1 {
+  const void* in;
+  void* out;
+  const void* weight;
+  int64_t in_token, in_head;
+  int64_t out_token, out_head;
+  int32_t heads;
+  int32_t norm_columns;
+} silkern_heads_v1;
+
+/*
+ * Norm and rotation of queries and keys (k may be NULL), for each token and
+ * head, with n = norm_columns:
+ *   y[i] = x[i] weight[i] / sqrt(mean(x[0:n]^2) + eps) for i < n, else x[i];
+ *   (y[a], y[b]) <- amplitude (y[a] cos - y[b] sin, y[b] cos + y[a] sin) of
+ *   positions[token] * frequencies[i] (radians), for each pair i of `pairs`:
+ *   a, b = start + i, start + pairs + i, or start + 2 i, start + 2 i + 1 where
+ *   `interleaved`;
+ * other columns stay. Sums and products are float32, angles are worked out in
+ * 64 bits, and one rounding to the type ends it. weights_f32: weights are
+ * float32, else of `type`. dim is at most SILKERN_MOST_COLUMNS. An output may be
+ * its own input, element for element.
+ */
+#define SILKERN_MOST_COLUMNS 1024
+int silkern_rotate_heads_v1(const silkern_heads_v1* q, const silkern_heads_v1* k, int32_t type,
+                            int64_t tokens, int32_t dim, const int32_t* positions,
+                            const float* frequencies, int32_t pairs, int32_t rotary_start,
+                            int32_t interleaved, int32_t weights_f32, float amplitude, float eps,
+                            void* stream);
 
 /*
  * Bound, in cycles of an SM's clock, on each wait of the attention kernels for

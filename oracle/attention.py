@@ -67,6 +67,32 @@ def append(keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, 
     return k, v, ks, vs
 
 
+def read(keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table, *,
+         dcp_size=1, dcp_rank=0, dcp_interleave=1):
+    """Float64 copies of (keys, values) with the stored tokens in place."""
+    results = []
+    block_size = k_cache.shape[1]
+    cu, first, req = (t.tolist() for t in (cu_tokens, starts, req_ids))
+    for new, cache, scale in ((keys, k_cache, k_scale), (values, v_cache, v_scale)):
+        if cache is None:
+            results.append(None)
+            continue
+        new = new.double().clone()
+        for b in range(len(first)):
+            if not 0 <= req[b] < block_table.shape[0] or first[b] < 0:
+                continue
+            rows = torch.arange(cu[b], cu[b + 1], device=cache.device)
+            mine, local = owned(rows - cu[b] + first[b], dcp_size, dcp_rank, dcp_interleave)
+            mine &= local // block_size < block_table.shape[1]
+            rows, local = rows[mine], local[mine]
+            block = block_table[req[b]].long()[local // block_size]
+            good = (block >= 0) & (block < cache.shape[0])
+            rows, local, block = rows[good], local[good], block[good]
+            new[rows] = cache[block, local % block_size].float().double() * scale[block].double()[:, :, None]
+        results.append(new)
+    return tuple(results)
+
+
 def attend_row(q, slot, k_cache, v_cache, k_scale, v_scale, softmax_scale):
     """One query row (heads, dim) over its int64 slots: (out, lse, spread, near).
 

@@ -28,6 +28,7 @@ from silkern_b200.attention import (
     attend_selected,
     attend_window,
     merge_partials,
+    read_quantized,
 )
 from silkern_b200.contract import (
     DEFAULT_TILE_SIZE,
@@ -37,6 +38,7 @@ from silkern_b200.contract import (
 )
 from silkern_b200.errors import LocalizationError
 from silkern_b200.kernels import localize_hierarchical, localize_rowwise
+from silkern_b200.rotary import rotary_frequencies, rotate_heads
 from silkern_b200.topk import topk_localize
 from silkern_b200.verify import (
     CellReport,
@@ -69,6 +71,9 @@ __all__ = [
     "localize_reference",
     "localize_rowwise",
     "merge_partials",
+    "read_quantized",
+    "rotary_frequencies",
+    "rotate_heads",
     "topk_localize",
     "replay_gate",
     "workspace_shapes",

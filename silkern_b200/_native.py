@@ -46,6 +46,22 @@ class Cache(ctypes.Structure):
     ]
 
 
+class Heads(ctypes.Structure):
+    """``silkern_heads_v1``: one set of heads to norm and rotate."""
+
+    _fields_ = [
+        ("in_", _ptr),
+        ("out", _ptr),
+        ("weight", _ptr),
+        ("in_token", _i64),
+        ("in_head", _i64),
+        ("out_token", _i64),
+        ("out_head", _i64),
+        ("heads", _i32),
+        ("norm_columns", _i32),
+    ]
+
+
 #: name -> (restype, argtypes) for every symbol the header declares.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "silkern_localize_rowwise_v1": (
@@ -109,6 +125,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "silkern_merge_partials_v1": (
         _i32,
         [_ptr, _i64, _i64, _i64, _ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr],
+    ),
+    "silkern_read_quantized_v1": (
+        _i32,
+        [_ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _i32, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _i64,
+         _i64, _i32, _i32, _i32, _ptr, _ptr],
+    ),
+    "silkern_rotate_heads_v1": (
+        _i32,
+        [_ptr, _ptr, _i32, _i64, _i32, _ptr, _ptr, _i32, _i32, _i32, _i32, _f32, _f32, _ptr],
     ),
     "silkern_attend_wait_bound_v1": (_i64, [_i64]),
     "silkern_status_string_v1": (ctypes.c_char_p, [ctypes.c_int]),

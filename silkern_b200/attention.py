@@ -5,6 +5,8 @@ the operators here keep that cache and attend to it:
 
 ``append_quantized``
     Store new tokens as e4m3 codes, one float32 scale for each page and head.
+``read_quantized``
+    Stored tokens back as 16-bit keys and values.
 ``attend_selected``
     Attention of each query row over its slots, as
     :func:`silkern_b200.localize_rowwise` and :func:`silkern_b200.topk_localize`
@@ -221,6 +223,40 @@ def _check_queries(torch, q, cache, out, lse, softmax_scale):
     return rows, heads, q_row, q_head, out_row, out_head, code
 
 
+def _copy(torch, what, kind, keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table,
+          dcp_size, dcp_rank, dcp_interleave, status) -> None:
+    """Tokens into the cache or out of it: the checks that both share, and the call."""
+    device = _on_device(torch, (keys, k_cache, k_scale, cu_tokens, starts, req_ids, block_table),
+                        (values, v_cache, v_scale), kind)
+    code = _type_code(torch, keys.dtype)
+    _check_ints(torch, (cu_tokens, starts, req_ids, block_table), "cu_tokens, starts, req_ids and block_table")
+    cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
+    if (values is None) != (v_cache is None):
+        raise LocalizationError("values are given exactly when the cache has values")
+    tokens = keys.shape[0] if keys.ndim == 3 else 0
+    wanted = (tokens, cache.kv_heads, cache.key_dim)
+    places = []
+    for new in (keys, values):
+        if new is None:
+            places += (None, 0, 0)
+            continue
+        row, head, column = new.stride() if new.ndim == 3 else (0, 0, 0)
+        if new.dtype is not keys.dtype or new.shape != wanted or tokens < 1 or column != 1:
+            raise LocalizationError(
+                "keys and values must be (tokens, kv_heads, dim) of one type with unit column stride")
+        places += (new.data_ptr(), row, head)
+    sequences = starts.shape[0] if starts.ndim == 1 else 0
+    if sequences < 1 or cu_tokens.shape != (sequences + 1,) or req_ids.shape != (sequences,):
+        raise LocalizationError("starts and req_ids need one element per sequence, cu_tokens one more")
+    _check_table(block_table)
+    _check_owner(cache.block_size, dcp_size, dcp_rank, dcp_interleave)
+    status_ptr = _status_pointer(torch, status, device)
+    table_rows, table_width = block_table.shape
+    _launch(torch, device, what, getattr(_native.load(), f"silkern_{what}_v1"), ctypes.addressof(cache), *places, code,
+            tokens, cu_tokens.data_ptr(), starts.data_ptr(), req_ids.data_ptr(), sequences, block_table.data_ptr(), table_rows, table_width, int(dcp_size),
+            int(dcp_rank), int(dcp_interleave), status_ptr)
+
+
 def append_quantized(
     keys,
     values,
@@ -271,36 +307,51 @@ def append_quantized(
         return _traced_op(torch, "append_quantized")(
             keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table, dcp_size,
             dcp_rank, dcp_interleave, status)
-    device = _on_device(torch, (keys, k_cache, k_scale, cu_tokens, starts, req_ids, block_table),
-                        (values, v_cache, v_scale), "append")
-    code = _type_code(torch, keys.dtype)
-    _check_ints(torch, (cu_tokens, starts, req_ids, block_table), "cu_tokens, starts, req_ids and block_table")
-    cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
-    if (values is None) != (v_cache is None):
-        raise LocalizationError("values are given exactly when the cache has values")
-    tokens = keys.shape[0] if keys.ndim == 3 else 0
-    wanted = (tokens, cache.kv_heads, cache.key_dim)
-    places = []
-    for new in (keys, values):
-        if new is None:
-            places += (None, 0, 0)
-            continue
-        row, head, column = new.stride() if new.ndim == 3 else (0, 0, 0)
-        if new.dtype is not keys.dtype or new.shape != wanted or tokens < 1 or column != 1:
-            raise LocalizationError(
-                "keys and values must be (tokens, kv_heads, dim) of one type with unit column stride")
-        places += (new.data_ptr(), row, head)
-    sequences = starts.shape[0] if starts.ndim == 1 else 0
-    if sequences < 1 or cu_tokens.shape != (sequences + 1,) or req_ids.shape != (sequences,):
-        raise LocalizationError("starts and req_ids need one element per sequence, cu_tokens one more")
-    _check_table(block_table)
-    _check_owner(cache.block_size, dcp_size, dcp_rank, dcp_interleave)
-    status_ptr = _status_pointer(torch, status, device)
-    table_rows, table_width = block_table.shape
-    _launch(torch, device, "append_quantized", _native.load().silkern_append_quantized_v1,
-            ctypes.addressof(cache), *places, code, tokens, cu_tokens.data_ptr(), starts.data_ptr(),
-            req_ids.data_ptr(), sequences, block_table.data_ptr(), table_rows, table_width, int(dcp_size),
-            int(dcp_rank), int(dcp_interleave), status_ptr)
+    _copy(torch, "append_quantized", "append", keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids,
+          block_table, dcp_size, dcp_rank, dcp_interleave, status)
+
+
+def read_quantized(
+    keys,
+    values,
+    k_cache,
+    v_cache,
+    k_scale,
+    v_scale,
+    cu_tokens,
+    starts,
+    req_ids,
+    block_table,
+    *,
+    dcp_size: int = 1,
+    dcp_rank: int = 0,
+    dcp_interleave: int = 1,
+    status=None,
+) -> None:
+    """Read stretches of the 8-bit cache back into ``keys`` and ``values``.
+
+    The reverse of :func:`append_quantized`, with its arguments and layouts: the
+    rows ``cu_tokens[b]:cu_tokens[b + 1]`` of ``keys`` and ``values`` become the
+    stored tokens of request ``req_ids[b]`` from position ``starts[b]`` on, each
+    element its code times its page's and head's scale, rounded to the type of
+    ``keys`` (bfloat16 or float16, which holds magnitudes up to 65504). Rows of
+    positions that other ranks own, and rows at and past ``cu_tokens[-1]``, are
+    left as they were. For prompts whose next pieces meet their context in 16
+    bits, or to hand a context on.
+
+    ``status`` gets 1 for a request id outside the table, 2 for a sequence that
+    starts below 0 or ends past position 2**31 - 2, 8 for a token whose page is
+    outside its table row or the cache; their rows are left as they were.
+    """
+    import torch
+
+    _refuse_gradients(torch, keys, values, k_cache, v_cache, k_scale, v_scale)
+    if _compiling(torch):
+        return _traced_op(torch, "read_quantized")(
+            keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table, dcp_size,
+            dcp_rank, dcp_interleave, status)
+    _copy(torch, "read_quantized", "read", keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids,
+          block_table, dcp_size, dcp_rank, dcp_interleave, status)
 
 
 def attend_selected(

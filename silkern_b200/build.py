@@ -23,6 +23,8 @@ SOURCES = [
     os.path.join(CSRC, "topk_localize.cu"),
     os.path.join(CSRC, "atomic_baseline.cu"),
     os.path.join(CSRC, "cache_ops.cu"),
+    os.path.join(CSRC, "cache_read.cu"),
+    os.path.join(CSRC, "rotate.cu"),
     os.path.join(CSRC, "attend.cu"),
     os.path.join(CSRC, "attend_dim64.cu"),
     os.path.join(CSRC, "attend_dim128.cu"),

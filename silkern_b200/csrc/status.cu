@@ -21,6 +21,7 @@ extern "C" const char* silkern_status_string_v1(int code) {
     case SILKERN_E_HEADS: return "heads must be a positive multiple of the cache's heads";
     case SILKERN_E_TYPE: return "element type must be bfloat16 or float16";
     case SILKERN_E_ATTEND: return "window, sinks or softmax scale out of range";
+    case SILKERN_E_ROTARY: return "rotary columns, norm columns, amplitude or epsilon out of range";
     default: break;
   }
   if (code < 0) return cudaGetErrorString(static_cast<cudaError_t>(-code));

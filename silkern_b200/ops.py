@@ -7,7 +7,8 @@
                                                  mapped, local_positions, tile_counts, tile_offsets,
                                                  block_size, dcp_size, dcp_rank, dcp_interleave,
                                                  compact_valid_to_front, tile_size, num_warps, status)
-    torch.ops.silkern_b200.append_quantized, .attend_selected, .attend_window and .merge_partials,
+    torch.ops.silkern_b200.append_quantized, .read_quantized, .rotate_heads, .attend_selected,
+                           .attend_window and .merge_partials,
                                             with the arguments of the launchers, all positional
 
 Each op declares the buffers the kernel writes as mutated (``out``, ``counts``,
@@ -18,8 +19,8 @@ graph break, where the ctypes call of the eager launchers would break the
 graph. At run time an op does exactly what the eager launcher does: the
 reference's checks, then one C ABI call on the current stream.
 
-The public launchers in :mod:`silkern_b200.kernels` and
-:mod:`silkern_b200.attention` route through these ops
+The public launchers in :mod:`silkern_b200.kernels`,
+:mod:`silkern_b200.attention` and :mod:`silkern_b200.rotary` route through these ops
 while ``torch.compile`` traces them and call the C ABI directly otherwise: a
 trip through the dispatcher costs tens of microseconds of host time per call,
 which an eager caller would pay for nothing.
@@ -47,7 +48,7 @@ def register() -> None:
         return
     import torch
 
-    from silkern_b200 import attention, kernels
+    from silkern_b200 import attention, kernels, rotary
 
     @torch.library.custom_op("silkern_b200::localize_rowwise", mutates_args=("out", "counts", "status"))
     def localize_rowwise(
@@ -136,6 +137,55 @@ def register() -> None:
     @append_quantized.register_fake
     def _(keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table, dcp_size,
           dcp_rank, dcp_interleave, status) -> None:
+        return None
+
+    @torch.library.custom_op("silkern_b200::read_quantized", mutates_args=("keys", "values", "status"))
+    def read_quantized(
+        keys: torch.Tensor,
+        values: Optional[torch.Tensor],
+        k_cache: torch.Tensor,
+        v_cache: Optional[torch.Tensor],
+        k_scale: torch.Tensor,
+        v_scale: Optional[torch.Tensor],
+        cu_tokens: torch.Tensor,
+        starts: torch.Tensor,
+        req_ids: torch.Tensor,
+        block_table: torch.Tensor,
+        dcp_size: int,
+        dcp_rank: int,
+        dcp_interleave: int,
+        status: Optional[torch.Tensor],
+    ) -> None:
+        attention.read_quantized(keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids,
+                                 block_table, dcp_size=dcp_size, dcp_rank=dcp_rank, dcp_interleave=dcp_interleave,
+                                 status=status)
+
+    @read_quantized.register_fake
+    def _(keys, values, k_cache, v_cache, k_scale, v_scale, cu_tokens, starts, req_ids, block_table, dcp_size,
+          dcp_rank, dcp_interleave, status) -> None:
+        return None
+
+    @torch.library.custom_op("silkern_b200::rotate_heads", mutates_args=("q_out", "k_out"))
+    def rotate_heads(
+        q: torch.Tensor,
+        k: Optional[torch.Tensor],
+        positions: torch.Tensor,
+        frequencies: torch.Tensor,
+        q_out: torch.Tensor,
+        k_out: Optional[torch.Tensor],
+        q_weight: Optional[torch.Tensor],
+        k_weight: Optional[torch.Tensor],
+        eps: float,
+        rotary_start: int,
+        interleaved: bool,
+        amplitude: float,
+    ) -> None:
+        rotary.rotate_heads(q, k, positions, frequencies, q_out, k_out, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                            rotary_start=rotary_start, interleaved=interleaved, amplitude=amplitude)
+
+    @rotate_heads.register_fake
+    def _(q, k, positions, frequencies, q_out, k_out, q_weight, k_weight, eps, rotary_start, interleaved,
+          amplitude) -> None:
         return None
 
     @torch.library.custom_op("silkern_b200::attend_selected", mutates_args=("out", "lse", "status"))
