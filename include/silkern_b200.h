@@ -51,7 +51,7 @@ extern "C" {
 #define SILKERN_E_TILE 5         /* unsupported tile_size */
 #define SILKERN_E_ALIAS 6        /* an output overlaps an input, another output or itself */
 #define SILKERN_E_GEOMETRY 7     /* explicit launch geometry rejected */
-#define SILKERN_E_SCRATCH 8      /* batch x tiles exceeds SILKERN_NOALLOC_MAX_TILES */
+#define SILKERN_E_SCRATCH 8      /* batch x tiles exceeds SILKERN_NOALLOC_MAX_TILES, or a workspace is too small */
 #define SILKERN_E_CACHE 9        /* unsupported cache geometry, stride or alignment */
 #define SILKERN_E_HEADS 10       /* heads not a positive multiple of the cache's heads */
 #define SILKERN_E_TYPE 11        /* element type is neither SILKERN_BF16 nor SILKERN_F16 */
@@ -414,6 +414,39 @@ int silkern_attend_window_v1(const silkern_cache_v1* cache, const void* q, int64
                              int64_t window, int64_t sinks, int32_t dcp_size, int32_t dcp_rank,
                              int32_t dcp_interleave, void* out, int64_t out_row, int64_t out_head,
                              float* lse, float softmax_scale, int32_t* status, void* stream);
+
+/*
+ * Attention of sequences in groups that share their first tokens. Group g (of
+ * `groups`) is the sequences [cu_groups[g], cu_groups[g + 1]), whose first
+ * prefixes[g] positions are one and the same tokens: they are read once for all
+ * of the group's queries, through the table row of its first sequence's request,
+ * and the positions from prefixes[g] on through each sequence's own. Sequences
+ * of no group, and of one with prefixes[g] <= 0, read everything through their
+ * own. Else as silkern_attend_window_v1 with window 0: the query at position t
+ * sees the positions [0, t] that this rank owns; rows of q before cu_tokens[0]
+ * and from cu_tokens[sequences] on are not touched in out and lse. The cache has
+ * values (key_dim 64 or 128).
+ *
+ * workspace: silkern_shared_workspace_v1 bytes at least, at a multiple of 16,
+ * whose contents do not matter before or after; calls that may run at the same
+ * time need one each. cu_tokens and cu_groups ascend. Equal calls give equal bits.
+ */
+int silkern_attend_shared_v1(const silkern_cache_v1* cache, const void* q, int64_t q_row,
+                             int64_t q_head, int32_t type, int64_t rows, int32_t heads,
+                             const int32_t* cu_tokens, const int32_t* lengths,
+                             const int32_t* req_ids, int64_t sequences, const int32_t* cu_groups,
+                             const int32_t* prefixes, int64_t groups, const int32_t* block_table,
+                             int64_t table_rows, int64_t table_width, int32_t dcp_size,
+                             int32_t dcp_rank, int32_t dcp_interleave, void* out, int64_t out_row,
+                             int64_t out_head, float* lse, float softmax_scale, void* workspace,
+                             int64_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * Bytes of workspace that silkern_attend_shared_v1 needs for these sizes, or
+ * minus a SILKERN_E_* code where it takes none such. Host only.
+ */
+int64_t silkern_shared_workspace_v1(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim,
+                                    int64_t sequences, int64_t groups);
 
 /*
  * Join the partial results of `ranks` context-parallel ranks:

@@ -158,6 +158,44 @@ def attend_window(q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache,
     return tuple(torch.stack(part) for part in zip(*rows))
 
 
+def attend_shared(q, cu_tokens, lengths, req_ids, cu_groups, prefixes, block_table, k_cache, v_cache, k_scale, v_scale, *,
+                  softmax_scale, dcp_size=1, dcp_rank=0, dcp_interleave=1):
+    """(out, lse, spread, peak) of the rows in [cu_tokens[0], cu_tokens[-1]). ``peak`` (rows, heads,
+    value_dim) is a row's largest product of weight and value scale, times the sum of its codes' magnitudes."""
+    rows = []
+    block_size, heads, kv_heads = k_cache.shape[1], q.shape[1], k_cache.shape[2]
+    cu, length, req, cut, prefix = (t.tolist() for t in (cu_tokens, lengths, req_ids, cu_groups, prefixes))
+    for b in range(len(length)):
+        group = next((g for g in range(len(prefix)) if cut[g] <= b < cut[g + 1]), None)
+        for i in range(cu[b], cu[b + 1]):
+            last = length[b] - (cu[b + 1] - i)
+            position = torch.arange(max(last + 1, 0), device=q.device)
+            slots = []
+            for behind in (False, True):
+                leader = req[b] if group is None or behind else req[cut[group]]
+                inside = position < (0 if group is None else prefix[group])
+                mine, local = owned(position, dcp_size, dcp_rank, dcp_interleave)
+                local = local[mine & (~inside if behind else inside)]
+                if 0 <= leader < block_table.shape[0]:
+                    local = local[local // block_size < block_table.shape[1]]
+                    block = block_table[leader].long()[local // block_size]
+                    good = (block >= 0) & (block < k_cache.shape[0])
+                    slots.append((block * block_size + local % block_size)[good])
+            slot = torch.cat(slots) if slots else torch.empty(0, dtype=torch.int64, device=q.device)
+            out, lse, spread, _ = attend_row(q[i], slot, k_cache, v_cache, k_scale, v_scale, softmax_scale)
+            peak = torch.zeros_like(out)
+            if slot.numel():
+                block, offset = slot // block_size, slot % block_size
+                k = k_cache[block, offset].float().double() * k_scale[block].double()[:, :, None]
+                score = torch.einsum("hgd,nhd->hgn", q[i].double().reshape(kv_heads, heads // kv_heads, -1), k) * softmax_scale
+                scaled = score + v_scale[block].double().T[:, None].log2() * math.log(2.0)
+                most = torch.exp(scaled.amax(-1).reshape(heads) - lse)
+                codes = v_cache[block, offset].float().double().abs().sum(0)
+                peak = most[:, None] * codes.repeat_interleave(heads // kv_heads, 0)
+            rows.append((out, lse, spread, peak))
+    return tuple(torch.stack(part) for part in zip(*rows))
+
+
 def merge(outs, lses):
     lse = torch.logsumexp(lses.double(), dim=0)
     weight = torch.where(lses > -math.inf, torch.exp(lses.double() - lse), 0.0)

@@ -26,9 +26,11 @@ from __future__ import annotations
 from silkern_b200.attention import (
     append_quantized,
     attend_selected,
+    attend_shared,
     attend_window,
     merge_partials,
     read_quantized,
+    shared_workspace_bytes,
 )
 from silkern_b200.contract import (
     DEFAULT_TILE_SIZE,
@@ -64,6 +66,7 @@ __all__ = [
     "ReplayGateReport",
     "append_quantized",
     "attend_selected",
+    "attend_shared",
     "attend_window",
     "conformance",
     "exact_stable_compact_reference",
@@ -74,6 +77,7 @@ __all__ = [
     "read_quantized",
     "rotary_frequencies",
     "rotate_heads",
+    "shared_workspace_bytes",
     "topk_localize",
     "replay_gate",
     "workspace_shapes",

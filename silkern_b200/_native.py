@@ -126,6 +126,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_ptr, _i64, _i64, _i64, _ptr, _i32, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr],
     ),
+    "silkern_attend_shared_v1": (
+        _i32,
+        [_ptr, _ptr, _i64, _i64, _i32, _i64, _i32, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr,
+         _i64, _i64, _i32, _i32, _i32, _ptr, _i64, _i64, _ptr, _f32, _ptr, _i64, _ptr, _ptr],
+    ),
+    "silkern_shared_workspace_v1": (_i64, [_i64, _i32, _i32, _i32, _i64, _i64]),
     "silkern_read_quantized_v1": (
         _i32,
         [_ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _i32, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _i64,

@@ -15,6 +15,9 @@ the operators here keep that cache and attend to it:
     Attention through the block table over a sliding window and a few first
     tokens that stay visible, or over the whole context; one query for each
     sequence or pieces of prompts.
+``attend_shared``
+    Attention of sequences in groups that share their first tokens, which are
+    read once for all of a group.
 ``merge_partials``
     Each rank's output and log-sum-exp over its own tokens, joined.
 
@@ -483,6 +486,103 @@ def attend_window(
             lengths.data_ptr(), req_ids.data_ptr(), sequences, block_table.data_ptr(), table_rows, table_width,
             int(window), int(sinks), int(dcp_size), int(dcp_rank), int(dcp_interleave), out.data_ptr(), out_row,
             out_head, lse.data_ptr(), softmax_scale, status_ptr)
+
+
+def shared_workspace_bytes(rows: int, heads: int, kv_heads: int, dim: int, sequences: int, groups: int) -> int:
+    """Bytes of workspace that :func:`attend_shared` needs for ``q`` of (rows, heads,
+    dim), a cache of ``kv_heads`` heads and as many sequences and groups."""
+    sizes = (rows, heads, kv_heads, dim, sequences, groups)
+    if not all(_is_int(n) and 1 <= n <= _INT32_MAX for n in sizes):
+        raise LocalizationError("sizes must be positive int32 integers")
+    needed = _native.load().silkern_shared_workspace_v1(*(int(n) for n in sizes))
+    if needed < 0:
+        _native.check(-needed, "shared_workspace_bytes")
+    return needed
+
+
+def attend_shared(
+    q,
+    cu_tokens,
+    lengths,
+    req_ids,
+    cu_groups,
+    prefixes,
+    block_table,
+    k_cache,
+    v_cache,
+    k_scale,
+    v_scale,
+    out,
+    lse,
+    workspace,
+    *,
+    softmax_scale: float,
+    dcp_size: int = 1,
+    dcp_rank: int = 0,
+    dcp_interleave: int = 1,
+    status=None,
+) -> None:
+    """Attention over the whole context, for sequences that share their first tokens.
+
+    Sequences are given as to :func:`attend_window`. Group ``g`` is the sequences
+    ``cu_groups[g]:cu_groups[g + 1]`` (int32, one more element than groups), whose
+    first ``prefixes[g]`` positions (int32, one for each group) hold the same
+    tokens. These are read once for all queries of the group, through the block
+    table row of its first sequence; the positions from ``prefixes[g]`` on are
+    read through each sequence's own row, so that pages which hold both sorts
+    need no copy of the shared tokens. A sequence of no group, or of one with no
+    prefix, reads everything through its own row. Each query sees the positions
+    up to its own that this rank owns.
+
+    The cache has values, with heads of 64 or 128 columns. ``workspace`` is a contiguous CUDA tensor of
+    :func:`shared_workspace_bytes` bytes at least, at a multiple of 16; its
+    contents do not matter before or after a call, and calls that may run at the
+    same time (two streams, two graphs) need one each. Layouts, types and
+    results are otherwise those of :func:`attend_selected`, and rows of ``q``
+    outside the sequences are left as they were in ``out`` and ``lse``.
+
+    Keys are shared among the GPU's SMs by the lengths themselves, so that long
+    sequences may stand among short ones.
+
+    ``status`` gets 1 for a request id outside the table (nothing is seen through
+    its row), 2 for a length below the number of queries (those at negative
+    positions see nothing), 8 for a visible token whose page is outside the table
+    row or the cache (left out) and 16 for a wait inside the kernel that ran out,
+    whose results are NaN (it does not occur in a working launch).
+    """
+    import torch
+
+    _refuse_gradients(torch, q, k_cache, v_cache, k_scale, v_scale, out, lse, workspace)
+    if _compiling(torch):
+        return _traced_op(torch, "attend_shared")(
+            q, cu_tokens, lengths, req_ids, cu_groups, prefixes, block_table, k_cache, v_cache, k_scale, v_scale, out,
+            lse, workspace, softmax_scale, dcp_size, dcp_rank, dcp_interleave, status)
+    ints = (cu_tokens, lengths, req_ids, cu_groups, prefixes, block_table)
+    device = _on_device(torch, (q, *ints, k_cache, k_scale, out, lse, workspace), (v_cache, v_scale), "attention")
+    _check_ints(torch, ints, "cu_tokens, lengths, req_ids, cu_groups, prefixes and block_table")
+    cache = _cache(torch, k_cache, v_cache, k_scale, v_scale)
+    if v_cache is None:
+        raise LocalizationError("attend_shared needs a cache with values: latent ones go to attend_window")
+    rows, heads, q_row, q_head, out_row, out_head, code = _check_queries(torch, q, cache, out, lse, softmax_scale)
+    sequences = lengths.shape[0] if lengths.ndim == 1 else 0
+    if sequences < 1 or cu_tokens.shape != (sequences + 1,) or req_ids.shape != (sequences,):
+        raise LocalizationError("lengths and req_ids need one element per sequence, cu_tokens one more")
+    groups = prefixes.shape[0] if prefixes.ndim == 1 else 0
+    if groups < 1 or cu_groups.shape != (groups + 1,):
+        raise LocalizationError("prefixes need one element per group, and at least one, cu_groups one more")
+    _check_table(block_table)
+    _check_owner(cache.block_size, dcp_size, dcp_rank, dcp_interleave)
+    workspace_bytes = workspace.numel() * workspace.element_size()
+    if not workspace.is_contiguous() or workspace.data_ptr() & 15:
+        raise LocalizationError("workspace must be contiguous, at a multiple of 16 bytes")
+    status_ptr = _status_pointer(torch, status, device)
+    table_rows, table_width = block_table.shape
+    _launch(torch, device, "attend_shared", _native.load().silkern_attend_shared_v1,
+            ctypes.addressof(cache), q.data_ptr(), q_row, q_head, code, rows, heads, cu_tokens.data_ptr(),
+            lengths.data_ptr(), req_ids.data_ptr(), sequences, cu_groups.data_ptr(), prefixes.data_ptr(), groups,
+            block_table.data_ptr(), table_rows, table_width, int(dcp_size), int(dcp_rank), int(dcp_interleave),
+            out.data_ptr(), out_row, out_head, lse.data_ptr(), softmax_scale, workspace.data_ptr(), workspace_bytes,
+            status_ptr)
 
 
 def merge_partials(outs, lses, out, lse=None) -> None:

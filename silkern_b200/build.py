@@ -29,6 +29,7 @@ SOURCES = [
     os.path.join(CSRC, "attend_dim64.cu"),
     os.path.join(CSRC, "attend_dim128.cu"),
     os.path.join(CSRC, "attend_latent.cu"),
+    os.path.join(CSRC, "shared.cu"),
     os.path.join(CSRC, "status.cu"),
 ]
 DEPENDS = SOURCES + [

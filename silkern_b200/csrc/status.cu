@@ -16,7 +16,7 @@ extern "C" const char* silkern_status_string_v1(int code) {
     case SILKERN_E_ALIAS: return "an output buffer overlaps an input, another output or itself";
     case SILKERN_E_GEOMETRY: return "explicit launch geometry rejected";
     case SILKERN_E_SCRATCH:
-      return "batch x tiles exceeds the allocation-free entry point's static workspace";
+      return "batch x tiles exceeds the allocation-free entry point's static workspace, or a workspace is too small";
     case SILKERN_E_CACHE: return "unsupported cache geometry, stride or alignment";
     case SILKERN_E_HEADS: return "heads must be a positive multiple of the cache's heads";
     case SILKERN_E_TYPE: return "element type must be bfloat16 or float16";

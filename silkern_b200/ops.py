@@ -8,7 +8,7 @@
                                                  block_size, dcp_size, dcp_rank, dcp_interleave,
                                                  compact_valid_to_front, tile_size, num_warps, status)
     torch.ops.silkern_b200.append_quantized, .read_quantized, .rotate_heads, .attend_selected,
-                           .attend_window and .merge_partials,
+                           .attend_window, .attend_shared and .merge_partials,
                                             with the arguments of the launchers, all positional
 
 Each op declares the buffers the kernel writes as mutated (``out``, ``counts``,
@@ -238,6 +238,37 @@ def register() -> None:
     @attend_window.register_fake
     def _(q, cu_tokens, lengths, req_ids, block_table, k_cache, v_cache, k_scale, v_scale, out, lse, softmax_scale,
           window, sinks, dcp_size, dcp_rank, dcp_interleave, status) -> None:
+        return None
+
+    @torch.library.custom_op("silkern_b200::attend_shared", mutates_args=("out", "lse", "workspace", "status"))
+    def attend_shared(
+        q: torch.Tensor,
+        cu_tokens: torch.Tensor,
+        lengths: torch.Tensor,
+        req_ids: torch.Tensor,
+        cu_groups: torch.Tensor,
+        prefixes: torch.Tensor,
+        block_table: torch.Tensor,
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        k_scale: torch.Tensor,
+        v_scale: torch.Tensor,
+        out: torch.Tensor,
+        lse: torch.Tensor,
+        workspace: torch.Tensor,
+        softmax_scale: float,
+        dcp_size: int,
+        dcp_rank: int,
+        dcp_interleave: int,
+        status: Optional[torch.Tensor],
+    ) -> None:
+        attention.attend_shared(q, cu_tokens, lengths, req_ids, cu_groups, prefixes, block_table, k_cache, v_cache,
+                                k_scale, v_scale, out, lse, workspace, softmax_scale=softmax_scale, dcp_size=dcp_size,
+                                dcp_rank=dcp_rank, dcp_interleave=dcp_interleave, status=status)
+
+    @attend_shared.register_fake
+    def _(q, cu_tokens, lengths, req_ids, cu_groups, prefixes, block_table, k_cache, v_cache, k_scale, v_scale, out,
+          lse, workspace, softmax_scale, dcp_size, dcp_rank, dcp_interleave, status) -> None:
         return None
 
     @torch.library.custom_op("silkern_b200::merge_partials", mutates_args=("out", "lse"))

@@ -64,3 +64,25 @@ def assert_attention(out, lse, want, q, k_cache, k_scale, softmax_scale):
     assert bool((lse[empty] == -float("inf")).all()) and bool((out[empty] == 0).all())
     off = (lse.double() - ref_lse)[~empty].abs()
     assert off.numel() == 0 or float((off - 2.0**-22 * ref_lse[~empty].abs()).max()) <= ds + 2.0**-20
+
+
+def assert_shared(out, lse, want, q, k_cache, k_scale, softmax_scale):
+    """out within half a step of the output's type, plus what the weights' errors make.
+
+    A weight p of a value of scale s enters the product in fp16 as x = 2^6 p s / (P S), with S a scale near those of its
+    run of keys (s within [2^-8, 2^4] of it) and P the largest weight so far or less, by 2^4 at most. Half a step of
+    fp16 is 2^-11 x, or 2^-25 below 2^-14: an error of 2^-31 P S in p s, at most 2^-23 of the largest p s. Where scales
+    are further apart, x = 2^6 p s / (the largest p s so far, or less by 2^4 at most) has the same bound. Scores'
+    errors count twice, in the weight and in the sum; exponentials, float32 sums of a run, and the joining of runs add
+    2^-18."""
+    ref_out, ref_lse, spread, peak = want
+    ds = score_error(q, k_cache, k_scale, softmax_scale)
+    bound = HALF_STEP[out.dtype] * ref_out.abs() + (2.0**-11 + 2.0**-18 + 2 * ds) * spread + 2.0**-22 * peak
+    bound += 2.0**-25 if out.dtype == torch.float16 else 1e-30
+    error = (out.double() - ref_out).abs()
+    bad = ~(error <= bound)
+    assert not bool(bad.any()), f"{int(bad.sum())} outputs off, worst {float((error / bound).nan_to_num(9e9).max()):.3g} bounds"
+    empty = ref_lse == -float("inf")
+    assert bool((lse[empty] == -float("inf")).all()) and bool((out[empty] == 0).all())
+    off = (lse.double() - ref_lse)[~empty].abs()
+    assert off.numel() == 0 or float((off - 2.0**-22 * ref_lse[~empty].abs()).max()) <= ds + 2.0**-19
