@@ -30,6 +30,8 @@ SOURCES = [
     os.path.join(CSRC, "attend_dim128.cu"),
     os.path.join(CSRC, "attend_latent.cu"),
     os.path.join(CSRC, "shared.cu"),
+    os.path.join(CSRC, "shared_dim64.cu"),
+    os.path.join(CSRC, "shared_dim128.cu"),
     os.path.join(CSRC, "status.cu"),
 ]
 DEPENDS = SOURCES + [
@@ -41,6 +43,8 @@ DEPENDS = SOURCES + [
     os.path.join(CSRC, "tcgen05.cuh"),
     os.path.join(CSRC, "attend_plan.cuh"),
     os.path.join(CSRC, "attend_kernel.cuh"),
+    os.path.join(CSRC, "shared_plan.cuh"),
+    os.path.join(CSRC, "shared_kernel.cuh"),
     os.path.join(INCLUDE, "silkern_b200.h"),
 ]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

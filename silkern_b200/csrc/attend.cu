@@ -15,6 +15,10 @@ namespace {
 // About two seconds.
 std::atomic<int64_t> wait_bound{4000000000};
 
+}  // namespace
+
+int64_t attend_wait_bound() { return wait_bound.load(std::memory_order_relaxed); }
+
 int multiprocessors() {
   int device = 0, n = 0;
   if (cudaGetDevice(&device) != cudaSuccess ||
@@ -24,6 +28,8 @@ int multiprocessors() {
   }
   return n;
 }
+
+namespace {
 
 // One tensor's rows of a token and head: the pitch that divides its strides,
 // and the strides in units of it. False where a row's number passes 31 bits.
@@ -48,7 +54,7 @@ bool find_rows(const PagedCache& c, int64_t block, int64_t token, int64_t head, 
 }  // namespace
 
 int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
-  a.wait_cycles = wait_bound.load(std::memory_order_relaxed);
+  a.wait_cycles = attend_wait_bound();
   const bool latent = key_dim == 576, half = type == SILKERN_F16;
   const int32_t group = a.heads_per_kv;
   // Queries that may share a CTA's keys: one for a selected row; for

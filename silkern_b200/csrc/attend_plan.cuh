@@ -30,6 +30,10 @@ struct AttendLaunch {
 // failure.
 int resident_clusters(int size);
 
+// The bound on an attention kernel's waits, and the current device's SMs.
+int64_t attend_wait_bound();
+int multiprocessors();
+
 int launch_dim64(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);
 int launch_dim128(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);
 int launch_latent(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);

@@ -1,122 +1,368 @@
-// Attention of sequences in groups that share their first tokens.
+// Attention of sequences in groups that share their first tokens: the plan, the
+// joining of what the GPU's SMs found, and the entry points.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 
+#include "attend_plan.cuh"
 #include "cache_checks.cuh"
 #include "host.cuh"
 #include "paged.cuh"
 #include "ptx.cuh"
+#include "shared_plan.cuh"
 #include "silkern_b200.h"
-#include "tcgen05.cuh"
 
 namespace silkern {
 
 namespace {
 
-struct SharedArgs {
-  PagedCache cache;
-  const void* q;
-  int64_t q_row, q_head;
-  void* out;
-  int64_t out_row, out_head;
-  float* lse;
-  int32_t* status;
-  float scale;
-  int32_t rows, heads, heads_per_kv;
-  int32_t sequences, groups;
-  const int32_t* cu_tokens;
-  const int32_t* lengths;
-  const int32_t* req_ids;
-  const int32_t* cu_groups;
-  const int32_t* prefixes;
-  const int32_t* table;
-  int64_t table_rows;
-  uint32_t table_width;
-  Ownership own;
+// ---------------------------------------------------------------- the plan
+
+constexpr int kPlanThreads = 1024;
+
+// A segment's tokens, keys and table row.
+struct Segment {
+  int32_t seq, seqs;
+  int32_t token, tokens;
+  int32_t key_first, key_end;  // rank-local
+  int32_t table_row;
 };
 
-// The last i in [0, n) with at(i) <= x, for at ascending from at(0) <= x.
-template <typename F>
-__device__ __forceinline__ int32_t last_at_most(int32_t n, int32_t x, F at) {
-  int32_t low = 0, high = n;
-  while (high - low > 1) {
-    const int32_t mid = low + (high - low) / 2;
-    if (at(mid) <= x) low = mid; else high = mid;
+__device__ __forceinline__ Segment find_segment(const SharedArgs& a, int32_t index) {
+  Segment s{0, 0, 0, 0, 0, 0, 0};
+  if (index < a.groups) {
+    s.seq = a.cut(index);
+    s.seqs = max(a.cut(index + 1) - s.seq, 0);
+    if (s.seqs == 0) return s;
+    s.token = a.cu(s.seq);
+    s.tokens = max(a.cu(s.seq + s.seqs) - s.token, 0);
+    s.key_end = a.limits()[index];
+    s.table_row = load_int(a.req_ids + s.seq);
+  } else {
+    s.seq = index - a.groups;
+    s.seqs = 1;
+    s.token = a.cu(s.seq);
+    s.tokens = max(a.cu(s.seq + 1) - s.token, 0);
+    const int32_t length = load_int(a.lengths + s.seq);
+    if (s.tokens > 0 && length < s.tokens) flag_status(a.status, SILKERN_STATUS_BAD_LENGTH);
+    s.key_end = a.keys_below(length);
+    if (s.seq >= a.cut(0) && s.seq < a.cut(a.groups)) {
+      const int32_t group = last_at_most(a.groups, s.seq, [&](int32_t i) { return a.cut(i); });
+      s.key_first = a.keys_below(load_int(a.prefixes + group));
+    }
+    s.table_row = load_int(a.req_ids + s.seq);
   }
-  return low;
+  if (s.tokens > 0 && s.key_end > s.key_first && (s.table_row < 0 || s.table_row >= a.table_rows)) {
+    flag_status(a.status, SILKERN_STATUS_BAD_REQUEST);
+    s.tokens = 0;
+  }
+  return s;
 }
 
-// A warp for each (query, head), one key at a time: right for every case.
-template <typename T, int DIM>
-__global__ void __launch_bounds__(256) shared_simple_kernel(const __grid_constant__ SharedArgs a) {
-  constexpr int kEach = DIM / 32;
+// Rows [256 block, ...) of a segment: how many, and the keys that they see.
+__device__ __forceinline__ SharedItem item_of(const SharedArgs& a, const Segment& s, bool prefix, int32_t block) {
+  SharedItem it{};
+  it.row = block * kBlockRows;
+  it.rows = min(s.tokens * a.heads_per_kv - it.row, kBlockRows);
+  it.key_begin = s.key_first & ~15;
+  it.key_first = s.key_first;
+  it.key_end = s.key_end;
+  if (!prefix && s.tokens > 1) {  // up to its last query's
+    const int32_t last = static_cast<int32_t>(fastdiv(it.row + it.rows - 1, a.per_kv));
+    const int64_t position = static_cast<int64_t>(load_int(a.lengths + s.seq)) - (s.tokens - last);
+    it.key_end = position < 0 ? 0 : min(it.key_end, a.keys_below(static_cast<int32_t>(position + 1)));
+  }
+  it.tiles = it.key_end > it.key_first
+                 ? static_cast<int32_t>((static_cast<int64_t>(it.key_end) - it.key_begin + kSharedTile - 1) / kSharedTile)
+                 : 0;
+  it.table_row = s.table_row;
+  it.token = s.token;
+  it.seq = s.seq;
+  it.seqs = s.seqs;
+  it.prefix = prefix ? 1 : 0;
+  return it;
+}
+
+// One CTA lays out the items: a thread for each segment, and prefix sums over
+// them. 128 sequences: about 4 us, most of it the chain of dependent loads.
+__global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_constant__ SharedArgs a, int32_t ctas) {
+  __shared__ int64_t sums[3][32];
   pdl_wait();
   pdl_launch_dependents();
-  const int32_t lane = threadIdx.x & 31;
-  const int64_t pair = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (pair >= static_cast<int64_t>(a.rows) * a.heads) return;
+  const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // Prefixes end where the last query of the group sees no further.
+  for (int32_t g = warp; g < a.groups; g += kPlanThreads / 32) {
+    const int32_t first = a.cut(g), last = a.cut(g + 1);
+    int32_t most = 0;
+    for (int32_t s = first + lane; s < last; s += 32) {
+      if (a.cu(s + 1) > a.cu(s)) most = max(most, load_int(a.lengths + s));
+    }
+    most = __reduce_max_sync(kAllLanes, most);
+    if (lane == 0) a.limits()[g] = a.keys_below(min(most, load_int(a.prefixes + g)));
+  }
+  __syncthreads();
+  const int32_t segments = a.groups + a.sequences;
+  int64_t before[3] = {0, 0, 0};  // items, units, rows of second copies
+  for (int32_t base = 0; base < segments; base += kPlanThreads) {
+    const int32_t index = base + threadIdx.x;
+    Segment s{};
+    int32_t blocks = 0;
+    const bool prefix = index < a.groups;
+    int64_t mine[3] = {0, 0, 0};
+    if (index < segments) {
+      s = find_segment(a, index);
+      if (s.tokens > 0 && s.key_end > s.key_first) {
+        blocks = (s.tokens * a.heads_per_kv + kBlockRows - 1) / kBlockRows;
+        mine[0] = blocks;
+        for (int32_t b = 0; b < blocks; ++b) {
+          const SharedItem it = item_of(a, s, prefix, b);
+          mine[1] += units_of(it.tiles);
+          if (it.rows <= kSlotRows) mine[2] += it.rows;
+          if (prefix) {  // the others are alike, but for the last's rows
+            mine[1] += static_cast<int64_t>(units_of(it.tiles)) * (blocks - 1);
+            const int32_t rest = s.tokens * a.heads_per_kv - (blocks - 1) * kBlockRows;
+            mine[2] = rest <= kSlotRows ? rest : 0;
+            break;
+          }
+        }
+      }
+    }
+    int64_t upto[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      int64_t x = mine[k];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(kAllLanes, x, d);
+        if (lane >= d) x += y;
+      }
+      upto[k] = x;
+      if (lane == 31) sums[k][warp] = x;
+    }
+    __syncthreads();
+    int64_t all[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      int64_t x = sums[k][lane];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(kAllLanes, x, d);
+        if (lane >= d) x += y;
+      }
+      all[k] = __shfl_sync(kAllLanes, x, 31);
+      const int64_t warps_before = __shfl_sync(kAllLanes, x, max(warp - 1, 0));
+      upto[k] += before[k] - mine[k] + (warp > 0 ? warps_before : 0);
+    }
+    if (index < segments) {
+      a.first()[index] = blocks > 0 ? static_cast<int32_t>(upto[0]) : -1;
+      for (int32_t b = 0; b < blocks; ++b) {
+        SharedItem it = item_of(a, s, prefix, b);
+        it.begin = upto[1];
+        it.extra = static_cast<int32_t>(upto[2]);
+        upto[1] += units_of(it.tiles);
+        if (it.rows <= kSlotRows) upto[2] += it.rows;
+        *a.item(static_cast<int32_t>(upto[0]) + b) = it;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) before[k] += all[k];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    SharedHeader h;
+    h.units = before[1] * a.cache.kv_heads;
+    h.share = max((h.units + ctas - 1) / ctas, static_cast<int64_t>(kLeastUnits));
+    h.items = static_cast<int32_t>(before[0]);
+    h.failed = 0;
+    *a.header() = h;
+  }
+}
+
+// ---------------------------------------------------------------- joining
+
+// The fragments of one row of an item: the first CTA's, and those of the CTAs
+// that went on with it.
+struct Parts {
+  int64_t first, copy, next;  // partial rows; copy -1: none
+  int64_t stride;             // from a CTA's to the next one's
+  int32_t count;              // of fragments
+  int32_t both;               // 1: the two slots have a copy each
+};
+
+__device__ __forceinline__ Parts find_parts(const SharedArgs& a, int32_t segment, int32_t token, int32_t head, int64_t place) {
+  Parts p{0, -1, 0, kBlockRows, 0, 0};
+  const int32_t first = load_int(a.first() + segment);
+  if (first < 0) return p;
+  const int32_t kv = static_cast<int32_t>(fastdiv(head, a.per_kv));
+  const int32_t seg_token = load_int(&a.item(first)->token);
+  const int32_t row = (token - seg_token) * a.heads_per_kv + (head - kv * a.heads_per_kv);
+  const SharedItem* it = a.item(first + row / kBlockRows);
+  const int32_t tiles = load_int(&it->tiles);
+  if (tiles == 0) return p;
+  const int64_t share = __ldcg(&a.header()->share);
+  const int64_t zero = __ldcg(&it->begin) * a.cache.kv_heads + static_cast<int64_t>(kv) * units_of(tiles) + kStart;
+  const int64_t c0 = zero / share, c1 = (zero + tiles - 1) / share;
+  const int32_t r = row % kBlockRows, rows = load_int(&it->rows);
+  p.count = static_cast<int32_t>(c1 - c0 + 1);
+  p.first = place;
+  p.next = a.at.starts + (c0 + 1) * kBlockRows + r;
+  if (rows <= kSlotRows) {
+    p.both = 1;
+    p.copy = a.at.copies + static_cast<int64_t>(load_int(&it->extra)) * a.cache.kv_heads + static_cast<int64_t>(kv) * rows + r;
+  }
+  return p;
+}
+__device__ __forceinline__ int64_t part_at(const Parts& p, int32_t i) {
+  const int32_t c = p.both ? i >> 1 : i;
+  const bool second = p.both && (i & 1);
+  if (c == 0) return second ? p.copy : p.first;
+  return p.next + (c - 1) * p.stride + (second ? kSlotRows : 0);
+}
+
+// WARPS warps to a (query, head): one where there are many of them, eight where
+// few rows have many fragments. Lanes weigh the fragments, then each warp adds up
+// its share of them in order, and the first the warps'.
+template <typename T, int DIM, int WARPS>
+__global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant__ SharedArgs a) {
+  constexpr int kEach = DIM / 32;  // columns of a lane
+  __shared__ float partial[WARPS == 1 ? 1 : 8][DIM];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t w = WARPS == 1 ? 0 : warp;
+  const int64_t pair = WARPS == 1 ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
+  const int64_t pairs = static_cast<int64_t>(a.rows) * a.heads;
+  if (pair >= pairs) return;
   const int32_t token = static_cast<int32_t>(pair / a.heads), head = static_cast<int32_t>(pair - static_cast<int64_t>(token) * a.heads);
-  if (token < load_int(a.cu_tokens) || token >= load_int(a.cu_tokens + a.sequences)) return;
-  const int32_t seq = last_at_most(a.sequences, token, [&](int32_t i) { return load_int(a.cu_tokens + i); });
-  const int32_t position = load_int(a.lengths + seq) - (load_int(a.cu_tokens + seq + 1) - token);
-  if (lane == 0 && load_int(a.lengths + seq) < load_int(a.cu_tokens + seq + 1) - load_int(a.cu_tokens + seq)) {
-    flag_status(a.status, SILKERN_STATUS_BAD_LENGTH);
+  if (token < a.cu(0) || token >= a.cu(a.sequences)) return;
+  const int32_t seq = warp_last_at_most(a.sequences, token, [&](int32_t i) { return a.cu(i); });
+  Parts part[2];
+  part[0] = Parts{0, -1, 0, 0, 0, 0};
+  if (seq >= a.cut(0) && seq < a.cut(a.groups)) {
+    const int32_t group = warp_last_at_most(a.groups, seq, [&](int32_t i) { return a.cut(i); });
+    part[0] = find_parts(a, group, token, head, pair);
   }
-  int32_t prefix = 0, leader = seq;
-  if (seq >= load_int(a.cu_groups) && seq < load_int(a.cu_groups + a.groups)) {
-    const int32_t group = last_at_most(a.groups, seq, [&](int32_t i) { return load_int(a.cu_groups + i); });
-    leader = load_int(a.cu_groups + group);
-    prefix = max(load_int(a.prefixes + group), 0);
+  part[1] = find_parts(a, a.groups + seq, token, head, pairs + pair);
+  const int32_t n0 = part[0].count << part[0].both, n = n0 + (part[1].count << part[1].both);
+  auto place = [&](int32_t i) { return i < n0 ? part_at(part[0], i) : part_at(part[1], i - n0); };
+  float top = -INFINITY;
+  for (int32_t i = lane; i < n; i += 32) {
+    const float l = __ldcg(a.part_lse() + place(i));
+    top = l != l ? l : top != top ? top : fmaxf(top, l);
   }
-  const uint32_t kv = head / a.heads_per_kv;
-  const T* q = static_cast<const T*>(a.q) + token * a.q_row + head * a.q_head;
-  float x[kEach], y[kEach], top = -INFINITY, total = 0.f;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    x[i] = static_cast<float>(q[lane * kEach + i]);
-    y[i] = 0.f;
+  for (int d = 16; d > 0; d >>= 1) {
+    const float l = __shfl_xor_sync(kAllLanes, top, d);
+    top = l != l ? l : top != top ? top : fmaxf(top, l);
   }
-  const uint32_t seen = position < 0 ? 0u : a.own.owned_before(static_cast<uint32_t>(position) + 1u);
-  const uint32_t cut = a.own.owned_before(static_cast<uint32_t>(prefix));
-  for (uint32_t j = 0; j < seen; ++j) {
-    const int32_t req = load_int(a.req_ids + (j < cut ? leader : seq));
-    if (req < 0 || req >= a.table_rows) {
-      if (lane == 0) flag_status(a.status, SILKERN_STATUS_BAD_REQUEST);
-      continue;
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = 0.f, y[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) y[e] = 0.f;
+  // Each round of 32 fragments: a lane has one's place and weight, and the
+  // warps take turns with them, four on their way at once.
+  for (int32_t i0 = 0; i0 < n; i0 += 32) {
+    const int32_t i = i0 + lane;
+    const int64_t at = i < n ? place(i) : 0;
+    const float weight = i < n ? exp2f(__ldcg(a.part_lse() + at) - base) : 0.f;
+    float sum = weight;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, d);
+    total += sum;
+    const int32_t here = min(32, n - i0);
+    for (int32_t j0 = w; j0 < here; j0 += 4 * WARPS) {
+      float x[4][kEach], by[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int32_t j = j0 + k * WARPS;
+        by[k] = __shfl_sync(kAllLanes, weight, j & 31);
+        const int64_t from = __shfl_sync(kAllLanes, at, j & 31);
+        if (j >= here) by[k] = 0.f;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) x[k][e] = 0.f;
+        if (by[k] != 0.f) {  // a fragment without weight has no outputs
+          const float* p = a.part_out() + from * DIM + lane * kEach;
+          if constexpr (kEach == 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+            x[k][0] = v.x;
+            x[k][1] = v.y;
+            x[k][2] = v.z;
+            x[k][3] = v.w;
+          } else {
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(p));
+            x[k][0] = v.x;
+            x[k][1] = v.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) y[e] = fmaf(by[k], x[k][e], y[e]);
+      }
     }
-    const uint32_t page = fastdiv(j, a.cache.block), offset = j - page * a.cache.block.divisor;
-    const int32_t block = page < a.table_width ? load_int(a.table + req * static_cast<int64_t>(a.table_width) + page) : -1;
-    if (static_cast<uint32_t>(block) >= a.cache.num_blocks) {
-      if (lane == 0) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
-      continue;
-    }
-    auto code = [](uint8_t c) {
-      const uint32_t h = e4m3x2_to_f16x2(c);
-      return __half2float(__low2half(*reinterpret_cast<const __half2*>(&h)));
-    };
-    const uint8_t* k = a.cache.k + block * a.cache.k_block + offset * a.cache.k_token + kv * a.cache.k_head;
-    const uint8_t* v = a.cache.v + block * a.cache.v_block + offset * a.cache.v_token + kv * a.cache.v_head;
-    const int64_t scales = static_cast<int64_t>(block) * a.cache.kv_heads + kv;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) s = fmaf(x[i], code(k[lane * kEach + i]), s);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(kAllLanes, s, d);
-    s *= a.cache.k_scale[scales] * a.scale;
-    const float best = fmaxf(top, s), keep = expf(top - best), weight = expf(s - best);
-    top = best;
-    total = total * keep + weight;
-    const float w = weight * a.cache.v_scale[scales];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) y[i] = y[i] * keep + w * code(v[lane * kEach + i]);
   }
-  T* out = static_cast<T*>(a.out) + token * a.out_row + head * a.out_head;
-  const float inverse = seen == 0 || total == 0.f ? 0.f : 1.f / total;
+  if constexpr (WARPS > 1) {
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) out[lane * kEach + i] = static_cast<T>(y[i] * inverse);
-  if (lane == 0) a.lse[pair] = top + logf(total);
+    for (int e = 0; e < kEach; ++e) partial[warp][lane * kEach + e] = y[e];
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      y[e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) y[e] += partial[i][lane * kEach + e];
+    }
+  }
+  float inverse = total == 0.f ? 0.f : 1.f / total, lse = (top + log2f(total)) * 0.69314718055994531f;
+  if (load_int(&a.header()->failed) != 0) inverse = lse = NAN;
+  T* out = static_cast<T*>(a.out) + token * a.out_row + head * a.out_head + lane * kEach;
+  T rounded[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) rounded[e] = static_cast<T>(y[e] * inverse);
+  if (a.out_wide) {
+    if constexpr (kEach == 4) {
+      *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(rounded);
+    } else {
+      *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(rounded);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) out[e] = rounded[e];
+  }
+  if (lane == 0) a.lse[pair] = lse;
+}
+
+template <typename T, int DIM>
+int launch_join(const SharedArgs& a, cudaStream_t stream) {
+  const int64_t pairs = static_cast<int64_t>(a.rows) * a.heads;
+  // Eight warps to a row while all rows' fit the GPU at once.
+  if (pairs <= 8 * kMostCtas) return launch_pdl(shared_join_kernel<T, DIM, 8>, static_cast<unsigned>(pairs), 256, 0, 1, stream, a);
+  return launch_pdl(shared_join_kernel<T, DIM, 1>, static_cast<unsigned>((pairs + 7) / 8), 256, 0, 1, stream, a);
+}
+
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// The workspace's layout.
+int lay_out(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, int64_t sequences, int64_t groups, SharedLayout* at) {
+  if (rows < 1 || rows > 0x7fffffff || sequences < 1 || sequences > 0x3fffffff || groups < 1 || groups > 0x3fffffff) return SILKERN_E_SHAPE;
+  if (heads < 1 || heads > 65535 || kv_heads < 1 || heads % kv_heads != 0) return SILKERN_E_HEADS;
+  if (dim != 64 && dim != 128) return SILKERN_E_CACHE;
+  if (rows * heads > 0x3fffffff) return SILKERN_E_SHAPE;
+  const int64_t each = rows * (heads / kv_heads), segments = sequences + groups;
+  at->limits = 64;
+  at->first = at->limits + 4 * groups;
+  at->items = round_up(at->first + 4 * segments, 64);
+  at->most_items = 2 * (each / kBlockRows) + segments;
+  at->starts = 2 * rows * heads;
+  at->copies = at->starts + int64_t{kMostCtas} * kBlockRows;
+  const int64_t partial = at->copies + kv_heads * std::min(2 * each, kSlotRows * segments);
+  at->lse = at->items + 64 * at->most_items;
+  at->out = round_up(at->lse + 4 * partial, 64);
+  at->bytes = at->out + 4 * partial * dim;
+  return SILKERN_OK;
 }
 
 }  // namespace
@@ -126,10 +372,9 @@ using namespace silkern;
 
 extern "C" int64_t silkern_shared_workspace_v1(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, int64_t sequences,
                                                int64_t groups) {
-  if (rows < 1 || rows > 0x7fffffff || sequences < 1 || sequences > 0x3fffffff || groups < 1 || groups > 0x3fffffff) return -SILKERN_E_SHAPE;
-  if (heads < 1 || heads > 65535 || kv_heads < 1 || heads % kv_heads != 0) return -SILKERN_E_HEADS;
-  if (dim != 64 && dim != 128) return -SILKERN_E_CACHE;
-  return 16;
+  SharedLayout at{};
+  const int rc = lay_out(rows, heads, kv_heads, dim, sequences, groups, &at);
+  return rc == SILKERN_OK ? at.bytes : -rc;
 }
 
 extern "C" int silkern_attend_shared_v1(const silkern_cache_v1* cache, const void* q, int64_t q_row, int64_t q_head,
@@ -148,15 +393,17 @@ extern "C" int silkern_attend_shared_v1(const silkern_cache_v1* cache, const voi
     return SILKERN_E_NULL;
   }
   if (type != SILKERN_BF16 && type != SILKERN_F16) return SILKERN_E_TYPE;
-  const int64_t needed = silkern_shared_workspace_v1(rows, heads, cache->kv_heads, cache->key_dim, sequences, groups);
-  if (needed < 0) return static_cast<int>(-needed);
+  rc = lay_out(rows, heads, cache->kv_heads, cache->key_dim, sequences, groups, &a.at);
+  if (rc != SILKERN_OK) return rc;
   if (table_rows < 1 || table_width < 1 || table_width > 0x7fffffff) return SILKERN_E_SHAPE;
-  if (workspace_bytes < needed) return SILKERN_E_SCRATCH;
+  if (workspace_bytes < a.at.bytes) return SILKERN_E_SCRATCH;
   if (q_row % 8 != 0 || q_head % 8 != 0 || reinterpret_cast<uintptr_t>(q) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
     return SILKERN_E_CACHE;
   }
-  if (!std::isfinite(softmax_scale * 1.4426950408889634f)) return SILKERN_E_ATTEND;
+  a.scale_log2 = std::fabs(softmax_scale) * 1.4426950408889634f;
+  a.q_sign = softmax_scale < 0.f ? -1.f : 1.f;
+  if (!std::isfinite(a.scale_log2)) return SILKERN_E_ATTEND;
   rc = check_owner(cache->block_size, dcp_size, dcp_rank, dcp_interleave, &a.own);
   if (rc != SILKERN_OK) return rc;
   const Place written[3] = {Place(out, 2 * int64_t{cache->value_dim}).along(rows, 2 * out_row).along(heads, 2 * out_head),
@@ -175,10 +422,14 @@ extern "C" int silkern_attend_shared_v1(const silkern_cache_v1* cache, const voi
   a.out_head = out_head;
   a.lse = lse;
   a.status = status;
-  a.scale = softmax_scale;
   a.rows = static_cast<int32_t>(rows);
   a.heads = heads;
   a.heads_per_kv = heads / cache->kv_heads;
+  a.per_kv = make_fastdiv(static_cast<uint32_t>(a.heads_per_kv));
+  a.out_wide = out_row % 4 == 0 && out_head % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
+  a.work = static_cast<uint8_t*>(workspace);
+  a.wait_cycles = attend_wait_bound();
+  a.runs = cache->block_size % 16 == 0;
   a.sequences = static_cast<int32_t>(sequences);
   a.groups = static_cast<int32_t>(groups);
   a.cu_tokens = cu_tokens;
@@ -189,9 +440,13 @@ extern "C" int silkern_attend_shared_v1(const silkern_cache_v1* cache, const voi
   a.table = block_table;
   a.table_rows = table_rows;
   a.table_width = static_cast<uint32_t>(table_width);
-  const int64_t ctas = (rows * heads + 7) / 8;
-  if (ctas > 0x7fffffff) return SILKERN_E_SHAPE;
-  void (*fn)(SharedArgs) = type == SILKERN_BF16 ? (cache->key_dim == 64 ? shared_simple_kernel<__nv_bfloat16, 64> : shared_simple_kernel<__nv_bfloat16, 128>)
-                                                : (cache->key_dim == 64 ? shared_simple_kernel<__half, 64> : shared_simple_kernel<__half, 128>);
-  return launch_pdl(fn, static_cast<unsigned>(ctas), 256, 0, 1, static_cast<cudaStream_t>(stream), a);
+  const cudaStream_t on = static_cast<cudaStream_t>(stream);
+  const int sms = multiprocessors(), ctas = sms < kMostCtas ? sms : kMostCtas;
+  rc = launch_pdl(shared_plan_kernel, 1, kPlanThreads, 0, 1, on, a, ctas);
+  if (rc != SILKERN_OK) return rc;
+  const bool half = type == SILKERN_F16, narrow = cache->key_dim == 64;
+  rc = narrow ? launch_shared_dim64(a, half, ctas, on) : launch_shared_dim128(a, half, ctas, on);
+  if (rc != SILKERN_OK) return rc;
+  if (narrow) return half ? launch_join<__half, 64>(a, on) : launch_join<__nv_bfloat16, 64>(a, on);
+  return half ? launch_join<__half, 128>(a, on) : launch_join<__nv_bfloat16, 128>(a, on);
 }
