@@ -53,6 +53,23 @@ bool find_rows(const PagedCache& c, int64_t block, int64_t token, int64_t head, 
 
 }  // namespace
 
+int set_rows(PagedCache& c) {
+  Rows k, v;
+  if (!find_rows(c, c.k_block, c.k_token, c.k_head, &k) ||
+      !find_rows(c, c.v_block, c.v_token, c.v_head, &v)) {
+    return SILKERN_E_CACHE;
+  }
+  c.k_block_rows = k.block;
+  c.k_token_rows = k.token;
+  c.k_head_rows = k.head;
+  c.k_pitch = k.pitch;
+  c.v_block_rows = v.block;
+  c.v_token_rows = v.token;
+  c.v_head_rows = v.head;
+  c.v_pitch = v.pitch;
+  return SILKERN_OK;
+}
+
 int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
   a.wait_cycles = attend_wait_bound();
   const bool latent = key_dim == 576, half = type == SILKERN_F16;
@@ -130,20 +147,8 @@ int launch_attend(AttendArgs& a, int key_dim, int type, cudaStream_t stream) {
       plan.whole = static_cast<uint32_t>(pipes > 1 && left <= grid ? units - left : units);
     }
   }
-  Rows k, v;
-  PagedCache& c = a.cache;
-  if (!find_rows(c, c.k_block, c.k_token, c.k_head, &k) ||
-      !find_rows(c, c.v_block, c.v_token, c.v_head, &v)) {
-    return SILKERN_E_CACHE;
-  }
-  c.k_block_rows = k.block;
-  c.k_token_rows = k.token;
-  c.k_head_rows = k.head;
-  c.k_pitch = k.pitch;
-  c.v_block_rows = v.block;
-  c.v_token_rows = v.token;
-  c.v_head_rows = v.head;
-  c.v_pitch = v.pitch;
+  const int rc = set_rows(a.cache);
+  if (rc != SILKERN_OK) return rc;
   AttendLaunch l{columns, half, static_cast<unsigned>(grid), cluster, stream};
   return key_dim == 64 ? launch_dim64(a, plan, l) : key_dim == 128 ? launch_dim128(a, plan, l) : launch_latent(a, plan, l);
 }

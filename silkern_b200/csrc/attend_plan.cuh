@@ -34,6 +34,10 @@ int resident_clusters(int size);
 int64_t attend_wait_bound();
 int multiprocessors();
 
+// A cache's strides in rows of a common pitch; SILKERN_E_CACHE where a row's
+// number passes 31 bits.
+int set_rows(PagedCache& c);
+
 int launch_dim64(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);
 int launch_dim128(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);
 int launch_latent(const AttendArgs& a, const AttendPlan& plan, const AttendLaunch& l);

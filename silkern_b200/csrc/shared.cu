@@ -440,6 +440,8 @@ extern "C" int silkern_attend_shared_v1(const silkern_cache_v1* cache, const voi
   a.table = block_table;
   a.table_rows = table_rows;
   a.table_width = static_cast<uint32_t>(table_width);
+  rc = set_rows(a.cache);
+  if (rc != SILKERN_OK) return rc;
   const cudaStream_t on = static_cast<cudaStream_t>(stream);
   const int sms = multiprocessors(), ctas = sms < kMostCtas ? sms : kMostCtas;
   rc = launch_pdl(shared_plan_kernel, 1, kPlanThreads, 0, 1, on, a, ctas);

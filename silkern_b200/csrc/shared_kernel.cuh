@@ -38,70 +38,35 @@ namespace silkern {
 
 namespace shared {
 
-constexpr int kLoadWarps = 8;
+constexpr int kLoadWarps = 4;
 constexpr int kMmaWarp = 8 + kLoadWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr int kWalkWarp = kMmaWarp + 1;
+constexpr int kFenceWarp = kWalkWarp + 1;        // one for K, one for V
+constexpr int kThreads = (kFenceWarp + 2) * 32;  // 512: up to 128 registers each
+constexpr int kRing = 4;  // fragments known ahead
 constexpr int kStages = 2;  // of K and of V
 constexpr int kNotes = 3;   // a tile's scales live until its V is read
 
-struct Note {
+struct __align__(16) Note {
   float k[kSharedTile];  // what a score is multiplied by
-  float v[kSharedTile];  // value scales; -1: a key that does not count
-  int4 seen[kLoadWarps]; // largest and smallest exponent of value scales, whether a key does not count
+  float v[kSharedTile];  // value scales; -1: a key whose page is not in the cache
+  int4 seen[kLoadWarps]; // largest and smallest exponent of value scales, whether such a key is among them
 };
-
-template <int DIM>
-struct __align__(1024) Memory {
-  uint8_t q[2][kSlotRows * DIM * 2];
-  uint8_t k[kStages][kSharedTile * DIM * 2];
-  uint8_t v[kStages][kSharedTile * DIM * 2];
-  Note note[kNotes];
-  uint64_t k_full[kStages], k_free[kStages], v_full[kStages], v_free[kStages];
-  uint64_t scores[2], weights[2], queries[2], done[2], drained;
-  uint32_t tmem;
-  int32_t abort;
-};
-
-// The piece of 16 bytes `piece` of row `row` of an operand tile: chunks of 64
-// columns, 128 bytes a row, swizzled.
-__device__ __forceinline__ uint32_t tile_place(uint32_t row, uint32_t piece) {
-  return (piece >> 3) * (kSharedTile * 128) + row * 128 + (((piece ^ row) & 7) << 4);
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
-      : "memory");
-}
-// A from TMEM: 128 lanes, two fp16 to a column.
-__device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
 
 // A part of an item and cache head that one CTA takes.
 struct Fragment {
-  SharedItem item;
   int32_t kv;
-  int32_t first, last;  // tiles
-  bool split;           // the slots take turns with the tiles
+  int32_t first, last;  // tiles; the CTA's last fragment is followed by one with last 0
+  int32_t split;        // the slots take turns with the tiles
+  int32_t key_begin, key_first, key_end;
+  int32_t table_row;
+  int32_t token, row, rows;
+  int32_t seq, seqs;
+  int32_t extra, prefix;
 
   // Tiles of a slot.
   __device__ __forceinline__ int32_t steps(int slot) const {
     return split ? (last - first + 1 - slot) >> 1 : last - first;
-  }
-  __device__ __forceinline__ int32_t tile(int slot, int32_t step) const {
-    return first + (split ? 2 * step + slot : step);
   }
 };
 
@@ -146,11 +111,9 @@ struct Walk {
       const int64_t zero = base + static_cast<int64_t>(kv) * cost + kStart;  // of the first tile
       const int64_t last = min(end - zero, static_cast<int64_t>(ahead.tiles));
       const int64_t first = max(at - zero, int64_t{0});
-      f.item = ahead;
-      f.kv = kv;
-      f.first = static_cast<int32_t>(first);
-      f.last = static_cast<int32_t>(last);
-      f.split = ahead.rows <= kSlotRows;
+      f = Fragment{kv, static_cast<int32_t>(first), static_cast<int32_t>(last), ahead.rows <= kSlotRows ? 1 : 0,
+                   ahead.key_begin, ahead.key_first, ahead.key_end, ahead.table_row, ahead.token, ahead.row, ahead.rows,
+                   ahead.seq, ahead.seqs, ahead.extra, ahead.prefix};
       at = min(zero + ahead.tiles, end);
       if (kv + 1 == heads && at == zero + ahead.tiles) {
         ++next_item;
@@ -161,6 +124,204 @@ struct Walk {
     return false;
   }
 };
+
+template <int DIM>
+struct __align__(1024) Memory {
+  uint8_t q[2][kSlotRows * DIM * 2];
+  uint8_t k[kStages][kSharedTile * DIM * 2];
+  uint8_t v[kStages][kSharedTile * DIM * 2];
+  Note note[kNotes];
+  Fragment ring[kRing];
+  // [0]: of K, [1]: of V. Stored by the loading warps; ready for the MMAs; read by them.
+  uint64_t stored[2][kStages], ready[2][kStages], free[2][kStages];
+  uint64_t scores[2], weights[2], queries[2], done[2], drained;
+  uint64_t ring_full[kRing], ring_free[kRing];
+  uint32_t tmem;
+  int32_t abort;
+};
+
+// The piece of 16 bytes `piece` of row `row` of an operand tile: chunks of 64
+// columns, 128 bytes a row, swizzled.
+__device__ __forceinline__ uint32_t tile_place(uint32_t row, uint32_t piece) {
+  return (piece >> 3) * (kSharedTile * 128) + row * 128 + (((piece ^ row) & 7) << 4);
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+// A from TMEM: 128 lanes, two fp16 to a column.
+__device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+using silkern::tmem_st16;
+using silkern::tmem_wait_ld;
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]),
+        "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]),
+        "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(addr));
+}
+// The loaded registers may be used after this.
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                 "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+                 "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                 "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// A tile's scores of one row, as its scales and masks make them. RUNS: keys
+// [16 i, 16 i + 16) share a page; MASKED: of the tile's keys only [low, high)
+// count, and those whose page is in the cache.
+struct Row {
+  const Note* note;
+  float unscale;
+  int32_t low, high;
+};
+// The largest score of the 32 in x, the keys from `at` on.
+template <bool RUNS, bool MASKED>
+__device__ __forceinline__ float largest(const Row& r, int at, const float (&x)[32]) {
+  float best = -INFINITY;
+  if constexpr (RUNS && !MASKED) {
+#pragma unroll
+    for (int c = 0; c < 32; c += 16) {
+      float b0 = x[c], b1 = x[c + 1];
+#pragma unroll
+      for (int i = 2; i < 16; i += 4) {
+        b0 = max3(b0, x[c + i], x[c + i + 1]);
+        if (i + 3 < 16) b1 = max3(b1, x[c + i + 2], x[c + i + 3]);
+      }
+      best = fmaxf(best, fmaxf(b0, b1) * r.note->k[at + c]);
+    }
+  } else {
+    float b[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int j = RUNS ? at + (i & 16) : at + i;
+      float s = x[i] * r.note->k[j];
+      if (MASKED && (at + i < r.low || at + i >= r.high || r.note->v[j] < 0.f)) s = -INFINITY;
+      b[i & 1] = fmaxf(b[i & 1], s);
+    }
+    best = fmaxf(b[0], b[1]);
+  }
+  return best * r.unscale;
+}
+// Weights of the 32 scores in x against `base`: their sum is added to sum0 and
+// sum1, their products with the value scales in `unit`s go out in pairs.
+template <bool RUNS, bool MASKED>
+__device__ __forceinline__ void weigh(const Row& r, int at, const float (&x)[32], float base, float unit, float& sum0,
+                                      float& sum1, uint32_t (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const int j = RUNS ? at + (i & 16) : at + i;
+    const float by0 = r.note->k[j] * r.unscale, vs0 = r.note->v[j] * unit;
+    const float by1 = RUNS ? by0 : r.note->k[j + 1] * r.unscale, vs1 = RUNS ? vs0 : r.note->v[j + 1] * unit;
+    float p0, p1, w0, w1;
+    fma_pair(x[i], x[i + 1], by0, by1, -base, -base, p0, p1);
+    bool out0 = false, out1 = false;
+    if constexpr (MASKED) {
+      out0 = at + i < r.low || at + i >= r.high || vs0 < 0.f;
+      out1 = at + i + 1 < r.low || at + i + 1 >= r.high || vs1 < 0.f;
+    }
+    p0 = out0 ? 0.f : exp2_approx(p0);
+    p1 = out1 ? 0.f : exp2_approx(p1);
+    add_pair(sum0, sum1, p0, p1, sum0, sum1);
+    mul_pair(p0, p1, vs0, vs1, w0, w1);
+    w[i / 2] = pack_f16x2(out0 ? 0.f : w0, out1 ? 0.f : w1);
+  }
+}
+template <bool RUNS, bool MASKED>
+__device__ __forceinline__ float largest_of_tile(const Row& r, uint32_t s_at) {
+  float best = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kSharedTile; c += 32) {
+    float x[32];
+    tmem_ld32(s_at + c, x);
+    tmem_wait_ld(x);
+    best = fmaxf(best, largest<RUNS, MASKED>(r, c, x));
+  }
+  return best;
+}
+template <bool RUNS, bool MASKED>
+__device__ __forceinline__ float weigh_tile(const Row& r, uint32_t s_at, float base, float unit) {
+  float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < kSharedTile; c += 32) {
+    float x[32];
+    uint32_t w[16];
+    tmem_ld32(s_at + c, x);
+    tmem_wait_ld(x);
+    weigh<RUNS, MASKED>(r, c, x, base, unit, sum0, sum1, w);
+    tmem_st16(s_at + c / 2, w);
+  }
+  return sum0 + sum1;
+}
+// Where the value scales of a tile are far from the first's: the largest score
+// times value scale, and the weights against a reference of their own.
+__device__ __forceinline__ float heaviest_of_tile(const Row& r, uint32_t s_at) {
+  float most = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kSharedTile; c += 16) {
+    float x[16];
+    tmem_ld16(s_at + c, x);
+    tmem_wait_ld(x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float vs = r.note->v[c + i];
+      const float u = x[i] * r.note->k[c + i] * r.unscale + log2f(vs);
+      if (c + i >= r.low && c + i < r.high && !(vs < 0.f)) most = fmaxf(most, u);
+    }
+  }
+  return most;
+}
+__device__ __forceinline__ float weigh_heavy_tile(const Row& r, uint32_t s_at, float base, float reference) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < kSharedTile; c += 32) {
+    float x[32];
+    uint32_t w[16];
+    tmem_ld32(s_at + c, x);
+    tmem_wait_ld(x);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float vs = r.note->v[c + i], t = x[i] * r.note->k[c + i] * r.unscale;
+      const bool counts = c + i >= r.low && c + i < r.high && !(vs < 0.f);
+      sum += counts ? exp2_approx(t - base) : 0.f;
+      x[i] = counts ? exp2_approx(t + log2f(vs) - reference + 6.f) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack_f16x2(x[2 * i], x[2 * i + 1]);
+    tmem_st16(s_at + c / 2, w);
+  }
+  return sum;
+}
 
 template <typename T>
 __device__ __forceinline__ float2 widen(uint32_t pair) {
@@ -173,21 +334,24 @@ __device__ __forceinline__ float2 widen(uint32_t pair) {
 
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_constant__ SharedArgs a) {
-  extern __shared__ uint8_t raw_memory[];
-  Memory<DIM>& m = *reinterpret_cast<Memory<DIM>*>((reinterpret_cast<uintptr_t>(raw_memory) + 1023) & ~uintptr_t{1023});
+  extern __shared__ __align__(1024) uint8_t raw_memory[];
+  Memory<DIM>& m = *reinterpret_cast<Memory<DIM>*>(raw_memory);
   const int warp = __shfl_sync(kAllLanes, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_addr(&m.k_full[i]), kLoadWarps);
-      mbar_init(smem_addr(&m.v_full[i]), kLoadWarps);
-      mbar_init(smem_addr(&m.k_free[i]), 1);
-      mbar_init(smem_addr(&m.v_free[i]), 1);
+    for (int i = 0; i < 2 * kStages; ++i) {
+      mbar_init(smem_addr(&m.stored[i / kStages][i % kStages]), kLoadWarps);
+      mbar_init(smem_addr(&m.ready[i / kStages][i % kStages]), 1);
+      mbar_init(smem_addr(&m.free[i / kStages][i % kStages]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_addr(&m.scores[i]), 1);
       mbar_init(smem_addr(&m.weights[i]), 4);
       mbar_init(smem_addr(&m.queries[i]), 4);
       mbar_init(smem_addr(&m.done[i]), 1);
+    }
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(smem_addr(&m.ring_full[i]), 1);
+      mbar_init(smem_addr(&m.ring_free[i]), kWalkWarp + 2);  // every other warp
     }
     mbar_init(smem_addr(&m.drained), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -213,9 +377,13 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     if (lane == 0) mbar_arrive(smem_addr(bar));
   };
 
-  Walk walk;
-  Fragment f;
-  walk.start(a);
+  // The next fragment, behind `seq` others; false when there is none, or a wait ran
+  // out. A warp that has read what it needs of it frees its place.
+  auto next_fragment = [&](uint32_t seq) {
+    return wait(&m.ring_full[seq % kRing], seq / kRing & 1) && m.ring[seq % kRing].last > 0;
+  };
+  auto free_fragment = [&](uint32_t seq) { arrive(&m.ring_free[seq % kRing]); };
+  uint32_t seq = 0;
 
   if (warp < 8) {
     // ==================================================== softmax
@@ -226,15 +394,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     uint32_t tiles_before = 0;  // of the CTA, for the notes' turns
     uint32_t turn = 0, done_turn = 0;
     bool going = true;
-    while (going && walk.next(a, f)) {
-      const SharedItem& it = f.item;
+    for (; going && next_fragment(seq); ++seq) {
+      const Fragment f = m.ring[seq % kRing];
+      free_fragment(seq);
       const int32_t steps = f.steps(slot);
       const int32_t r = f.split ? row_in_slot : slot * kSlotRows + row_in_slot;  // of the block
-      const bool used = r < it.rows;
+      const bool used = r < f.rows;
       const bool warp_used = __any_sync(kAllLanes, used);
-      const int32_t row = it.row + (used ? r : 0);
+      const int32_t row = f.row + (used ? r : 0);
       const int32_t within = static_cast<int32_t>(fastdiv(row, a.per_kv));
-      const int32_t token = it.token + within;
+      const int32_t token = f.token + within;
       const int32_t head = f.kv * a.heads_per_kv + row - within * a.heads_per_kv;
       if (steps > 0) {
         // ---- the row's queries, and how far it sees
@@ -245,8 +414,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           uint4 x[DIM / 8];
 #pragma unroll
           for (int i = 0; i < DIM / 8; ++i) x[i] = __ldcg(q + i);
-          const int32_t seq = it.seqs == 1 ? it.seq : it.seq + last_at_most(it.seqs, token, [&](int32_t i) { return a.cu(it.seq + i); });
-          const int64_t position = static_cast<int64_t>(load_int(a.lengths + seq)) - (a.cu(seq + 1) - token);
+          const int32_t sequence = f.seqs == 1 ? f.seq : f.seq + last_at_most(f.seqs, token, [&](int32_t i) { return a.cu(f.seq + i); });
+          const int64_t position = static_cast<int64_t>(load_int(a.lengths + sequence)) - (a.cu(sequence + 1) - token);
           limit = position < 0 ? 0 : a.keys_below(static_cast<int32_t>(position + 1));
           uint32_t most = 0;  // the largest magnitude, by its bits
 #pragma unroll
@@ -274,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
         int32_t exponent = 0;
         bool known = false, usual = true;
         for (int32_t step = 0; step < steps; ++step) {
-          const int32_t tile = f.tile(slot, step);
+          const int32_t tile = f.first + (f.split ? 2 * step + slot : step);
           const Note& note = m.note[(tiles_before + static_cast<uint32_t>(tile - f.first)) % kNotes];
           if (!wait(&m.scores[slot], turn & 1)) {
             going = false;
@@ -299,45 +468,14 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
               usual = false;
               reference = top + exponent;
             }
-            const int32_t first_key = it.key_begin + tile * kSharedTile;
-            const bool masked = holes != 0 || __any_sync(kAllLanes, used && limit < first_key + kSharedTile);
-            const int32_t seen = limit - first_key;  // keys of the tile that the row may see
+            const int32_t first_key = f.key_begin + tile * kSharedTile;
+            const Row at{&note, unscale, f.key_first - first_key, min(limit, f.key_end) - first_key};
+            const bool masked = holes != 0 || __any_sync(kAllLanes, used && (at.low > 0 || at.high < kSharedTile));
             // ---- the largest score, and the largest weight where values' scales count
-            float best = -INFINITY, heaviest = -INFINITY;
-            if (usual && !masked && a.runs) {
-#pragma unroll 1
-              for (int c = 0; c < 8; c += 2) {
-                float x[16], y[16];
-                tmem_ld16(s_at + c * 16, x);
-                tmem_ld16(s_at + c * 16 + 16, y);
-                tmem_wait_ld(x);
-                tmem_wait_ld(y);
-                float b0 = x[0], b1 = y[0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) {
-                  b0 = fmaxf(b0, x[i]);
-                  b1 = fmaxf(b1, y[i]);
-                }
-                best = fmaxf(best, fmaxf(b0 * note.k[c * 16], b1 * note.k[c * 16 + 16]));
-              }
-              best *= unscale;
-            } else {
-#pragma unroll 1
-              for (int c = 0; c < 8; ++c) {
-                float x[16];
-                tmem_ld16(s_at + c * 16, x);
-                tmem_wait_ld(x);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float vs = note.v[c * 16 + i];
-                  if (!(vs < 0.f) && c * 16 + i < seen) {
-                    const float t = x[i] * note.k[c * 16 + i] * unscale;
-                    best = fmaxf(best, t);
-                    if (!usual) heaviest = fmaxf(heaviest, t + log2f(vs));
-                  }
-                }
-              }
-            }
+            const float best = !masked && a.runs ? largest_of_tile<true, false>(at, s_at)
+                               : a.runs          ? largest_of_tile<true, true>(at, s_at)
+                                                 : largest_of_tile<false, true>(at, s_at);
+            const float heaviest = usual ? -INFINITY : heaviest_of_tile(at, s_at);
             // ---- references move, with the sum and the outputs
             const bool up = best > top + 4.f || (top == -INFINITY && best > top);
             const bool heavier = !usual && (heaviest > reference + 4.f || (reference == -INFINITY && heaviest > reference));
@@ -365,55 +503,14 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
             }
             // ---- the weights
             const float base = top == -INFINITY ? 0.f : top;
-            float sum0 = 0.f, sum1 = 0.f;
-            if (usual && !masked && a.runs) {
+            if (usual) {
               const float unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - exponent) << 23);
-#pragma unroll 2
-              for (int c = 0; c < 8; ++c) {
-                const float by = note.k[c * 16] * unscale, vs = note.v[c * 16] * unit;
-                float x[16];
-                tmem_ld16(s_at + c * 16, x);
-                tmem_wait_ld(x);
-                uint32_t w[8];
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                  float p0, p1, w0, w1;
-                  fma_pair(x[i], x[i + 1], by, by, -base, -base, p0, p1);
-                  p0 = exp2_approx(p0);
-                  p1 = exp2_approx(p1);
-                  add_pair(sum0, sum1, p0, p1, sum0, sum1);
-                  mul_pair(p0, p1, vs, vs, w0, w1);
-                  w[i / 2] = pack_f16x2(w0, w1);
-                }
-                tmem_st8(s_at + c * 8, w);
-              }
+              total += !masked && a.runs ? weigh_tile<true, false>(at, s_at, base, unit)
+                       : a.runs          ? weigh_tile<true, true>(at, s_at, base, unit)
+                                         : weigh_tile<false, true>(at, s_at, base, unit);
             } else {
-              const float unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - exponent) << 23);
-              const float heavy = reference == -INFINITY ? 0.f : reference;
-#pragma unroll 1
-              for (int c = 0; c < 8; ++c) {
-                float x[16];
-                tmem_ld16(s_at + c * 16, x);
-                tmem_wait_ld(x);
-                uint32_t w[8];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float vs = note.v[c * 16 + i];
-                  float p = 0.f, y = 0.f;
-                  if (!(vs < 0.f) && c * 16 + i < seen) {
-                    const float t = x[i] * note.k[c * 16 + i] * unscale;
-                    p = exp2_approx(t - base);
-                    y = usual ? p * vs * unit : exp2_approx(t + log2f(vs) - heavy + 6.f);
-                  }
-                  sum0 += p;
-                  x[i] = y;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = pack_f16x2(x[2 * i], x[2 * i + 1]);
-                tmem_st8(s_at + c * 8, w);
-              }
+              total += weigh_heavy_tile(at, s_at, base, reference == -INFINITY ? 0.f : reference);
             }
-            total += sum0 + sum1;
             tmem_wait_st();
           }
           tc_fence_before();
@@ -432,9 +529,9 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           if (f.first > 0) {
             place = a.at.starts + blockIdx.x * static_cast<int64_t>(kBlockRows) + slot * kSlotRows + row_in_slot;
           } else if (f.split && slot == 1) {
-            place = a.at.copies + static_cast<int64_t>(it.extra) * a.cache.kv_heads + static_cast<int64_t>(f.kv) * it.rows + r;
+            place = a.at.copies + static_cast<int64_t>(f.extra) * a.cache.kv_heads + static_cast<int64_t>(f.kv) * f.rows + r;
           } else {
-            place = it.prefix != 0 ? own_place : pairs + own_place;
+            place = f.prefix != 0 ? own_place : pairs + own_place;
           }
           // 2^(reference - top - 6) / total, in the usual case 2^(E - 6) / total.
           const float lift = usual ? static_cast<float>(exponent) : reference - top;
@@ -458,74 +555,94 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
       } else if (used) {
         // A fragment of one tile, all of it the other slot's.
         const int64_t place = f.first > 0 ? a.at.starts + blockIdx.x * static_cast<int64_t>(kBlockRows) + slot * kSlotRows + row_in_slot
-                                          : a.at.copies + static_cast<int64_t>(it.extra) * a.cache.kv_heads +
-                                                static_cast<int64_t>(f.kv) * it.rows + r;
+                                          : a.at.copies + static_cast<int64_t>(f.extra) * a.cache.kv_heads +
+                                                static_cast<int64_t>(f.kv) * f.rows + r;
         a.part_lse()[place] = -INFINITY;
       }
       tiles_before += f.last - f.first;
     }
   } else if (warp < kMmaWarp) {
     // ==================================================== keys and values
-    // A warp widens 16 of a tile's rows, 16 codes a lane at a time; lanes 0 to 15
-    // know the places of its rows. Codes are on their way a tile ahead.
+    // A warp widens 32 of a tile's rows, 16 codes a lane at a time; each lane
+    // knows the place of one. As soon as a tile's keys are stored the next
+    // one's are on their way, and so the values: half a tile is in flight while
+    // the other half is widened.
     constexpr int kLanes = DIM / 16;        // to a row
     constexpr int kAtOnce = 32 / kLanes;    // rows
-    constexpr int kTurns = 16 / kAtOnce;
+    constexpr int kTurns = 32 / kAtOnce;
     const int w = warp - 8;
-    const int known_row = kAtOnce * w + (lane & (kAtOnce - 1)) + kAtOnce * kLoadWarps * ((lane & 15) / kAtOnce);
-    struct Batch {
-      uint4 k[kTurns], v[kTurns];
-      float by, vs;
-      bool any;
+    const int known_row = kAtOnce * w + (lane & (kAtOnce - 1)) + kAtOnce * kLoadWarps * (lane / kAtOnce);
+    // Eight neighbouring lanes take four pieces of two rows: with the swizzle,
+    // their stores of 16 bytes reach all banks.
+    const int my_row = kLanes == 4 ? lane >> 2 : (lane >> 2 & 1) | (lane >> 4 << 1);
+    const int my_piece = kLanes == 4 ? lane & 3 : (lane & 3) | (lane >> 3 & 1) << 2;
+    constexpr uint32_t kStep = kAtOnce * kLoadWarps * 128;  // from a row of this lane to the next: a multiple of 8 rows
+    const uint32_t to = tile_place(kAtOnce * w + my_row, 2 * my_piece);
+    bool bad = false;
+    // The next tile, and the fragment that it belongs to.
+    int32_t kv = 0, key = 0, key_first = 0, key_end = 0, tiles = 0, entry = 0;
+    const int32_t* table = nullptr;
+    auto advance = [&]() {  // to the next fragment; whether there is one
+      if (!next_fragment(seq)) return false;
+      const Fragment& f = m.ring[seq % kRing];
+      kv = f.kv;
+      key = f.key_begin + f.first * kSharedTile + known_row;  // this lane's
+      key_first = f.key_first;
+      key_end = f.key_end;
+      tiles = f.last - f.first;
+      table = a.table + f.table_row * static_cast<int64_t>(a.table_width);
+      free_fragment(seq);
+      ++seq;
+      return true;
     };
-    Batch batch[2];
-    int32_t tile = 0, entry = 0;
-    bool more = walk.next(a, f), bad = false;
-    if (more) tile = f.first;
-    auto page_of = [&](int32_t key) { return fastdiv(static_cast<uint32_t>(key), a.cache.block); };
-    auto fetch = [&]() {  // the table's entry for this lane's row of the next tile
-      const uint32_t page = min(page_of(f.item.key_begin + tile * kSharedTile + known_row), a.table_width - 1);
-      entry = load_int(a.table + f.item.table_row * static_cast<int64_t>(a.table_width) + page);
+    bool more = advance();
+    // This lane's row of the next tile: its places, and its scales.
+    int32_t k_row = -1, v_row = -1;
+    float by = 0.f, vs = -1.f;
+    bool counts = false;
+    auto fetch = [&]() {  // the table's entry of the next tile
+      entry = load_int(table + min(fastdiv(static_cast<uint32_t>(key), a.cache.block), a.table_width - 1));
     };
-    auto issue = [&](Batch& b) {
-      b.any = more;
-      if (!more) return;
-      const int32_t key = f.item.key_begin + tile * kSharedTile + known_row;
-      const uint32_t page = page_of(key), offset = key - page * a.cache.block.divisor, block = entry;
-      const bool wanted = key >= f.item.key_first && key < f.item.key_end;
-      const bool good = wanted && page < a.table_width && block < a.cache.num_blocks;
-      bad = bad || (wanted && !good);
-      const int64_t k_place = good ? block * a.cache.k_block + offset * a.cache.k_token + f.kv * a.cache.k_head : -1;
-      const int64_t v_place = block * a.cache.v_block + offset * a.cache.v_token + f.kv * a.cache.v_head;
-      b.by = 0.f;
-      b.vs = -1.f;
-      if (good) {
-        const int64_t s = static_cast<int64_t>(block) * a.cache.kv_heads + f.kv;
-        b.by = __ldcg(a.cache.k_scale + s) * a.scale_log2;
-        b.vs = __ldcg(a.cache.v_scale + s);
+    auto locate = [&]() {  // places of the next tile, and the entry of the one behind it
+      const uint32_t page = fastdiv(static_cast<uint32_t>(key), a.cache.block), block = static_cast<uint32_t>(entry);
+      const uint32_t offset = key - page * a.cache.block.divisor;
+      const bool wanted = key >= key_first && key < key_end;
+      const bool held = page < a.table_width && block < a.cache.num_blocks;
+      bad = bad || (wanted && !held);
+      counts = wanted && held;
+      k_row = counts ? static_cast<int32_t>(block * a.cache.k_block_rows + offset * a.cache.k_token_rows + kv * a.cache.k_head_rows) : -1;
+      v_row = counts ? static_cast<int32_t>(block * a.cache.v_block_rows + offset * a.cache.v_token_rows + kv * a.cache.v_head_rows) : -1;
+      by = 0.f;
+      vs = wanted && !held ? -1.f : 0.f;
+      if (held) {
+        const int64_t s = static_cast<int64_t>(block) * a.cache.kv_heads + kv;
+        by = __ldcg(a.cache.k_scale + s);
+        vs = __ldcg(a.cache.v_scale + s);
       }
-      const int piece = lane & (kLanes - 1);
-#pragma unroll
-      for (int i = 0; i < kTurns; ++i) {
-        const int from = lane / kLanes + kAtOnce * i;
-        const int64_t kp = __shfl_sync(kAllLanes, k_place, from), vp = __shfl_sync(kAllLanes, v_place, from);
-        b.k[i] = b.v[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (kp >= 0) {
-          b.k[i] = __ldcg(reinterpret_cast<const uint4*>(a.cache.k + kp) + piece);
-          b.v[i] = __ldcg(reinterpret_cast<const uint4*>(a.cache.v + vp) + piece);
-        }
-      }
-      if (++tile == f.last) {
-        more = walk.next(a, f);
-        if (more) tile = f.first;
-      }
+      key += kSharedTile;
+      if (--tiles == 0) more = advance();
       if (more) fetch();
     };
-    uint32_t turn = 0;
-    auto widen_to = [&](uint32_t to, const uint4 (&codes)[kTurns]) {
+    uint4 codes[2][kTurns];
+    // (All exchanges come before the first load: they would wait for loads.)
+    auto load = [&](uint4 (&c)[kTurns], const uint8_t* base, int64_t pitch, int32_t row) {
+      int32_t r[kTurns];
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) r[i] = __shfl_sync(kAllLanes, row, my_row + kAtOnce * i);
+      asm volatile("" ::: "memory");
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
-        const uint32_t row = kAtOnce * w + lane / kLanes + kAtOnce * kLoadWarps * i, piece = 2 * (lane & (kLanes - 1));
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ge.s32 p, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n"
+            " @p ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n}"
+            : "=&r"(c[i].x), "=&r"(c[i].y), "=&r"(c[i].z), "=&r"(c[i].w)
+            : "l"(base + r[i] * pitch + my_piece * 16), "r"(r[i])
+            : "memory");
+      }
+    };
+    auto widen_to = [&](uint32_t tile_at, const uint4 (&codes)[kTurns]) {
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
         const uint32_t c[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
         uint32_t h[8];
 #pragma unroll
@@ -533,51 +650,45 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           h[2 * k] = e4m3x2_to_f16x2(static_cast<uint16_t>(c[k] & 0xffffu));
           h[2 * k + 1] = e4m3x2_to_f16x2(static_cast<uint16_t>(c[k] >> 16));
         }
-        // The second half of a row goes the other way round, so that eight
-        // lanes reach all banks.
-        if (piece >= 8) {
-          st_shared_v4(to + tile_place(row, piece + 1), h[4], h[5], h[6], h[7]);
-          st_shared_v4(to + tile_place(row, piece), h[0], h[1], h[2], h[3]);
-        } else {
-          st_shared_v4(to + tile_place(row, piece), h[0], h[1], h[2], h[3]);
-          st_shared_v4(to + tile_place(row, piece + 1), h[4], h[5], h[6], h[7]);
-        }
+        st_shared_v4(tile_at + to + i * kStep, h[0], h[1], h[2], h[3]);
+        st_shared_v4(tile_at + (to ^ 16) + i * kStep, h[4], h[5], h[6], h[7]);
       }
     };
-    auto step = [&](Batch& now, Batch& next) {
-      issue(next);
-      if (!now.any) return false;
-      const uint32_t stage = turn % kStages, parity = (turn / kStages & 1) ^ 1;
-      if (!wait(&m.k_free[stage], parity)) return false;
-      widen_to(smem_addr(m.k[stage]), now.k);
-      Note& note = m.note[turn % kNotes];
-      const int32_t e = static_cast<int32_t>(__float_as_uint(now.vs) >> 23 & 0xff);
-      const bool counts = now.vs > 0.f && e != 255;  // neither 0, nor NaN, nor a key that does not count
-      const int32_t most = __reduce_max_sync(kAllLanes, counts ? e - 127 : -1000);
-      const int32_t least = __reduce_min_sync(kAllLanes, counts ? e - 127 : 1000);
-      const bool holes = __any_sync(kAllLanes, now.vs < 0.f);
-      if (lane < 16) {
-        note.k[known_row] = now.by;
-        note.v[known_row] = now.vs;
-      }
-      if (lane == 0) note.seen[w] = make_int4(most, least, holes ? 1 : 0, 0);
-      fence_proxy_async();
-      arrive(&m.k_full[stage]);
-      if (!wait(&m.v_free[stage], parity)) return false;
-      widen_to(smem_addr(m.v[stage]), now.v);
-      fence_proxy_async();
-      arrive(&m.v_full[stage]);
-      ++turn;
-      return true;
-    };
+    uint32_t turn = 0;
     if (more) {
       fetch();
-      issue(batch[0]);
-      while (step(batch[0], batch[1]) && step(batch[1], batch[0])) {
+      locate();
+      load(codes[0], a.cache.k, a.cache.k_pitch, k_row);
+      load(codes[1], a.cache.v, a.cache.v_pitch, v_row);
+      bool ahead = true;
+      while (ahead) {
+        const float tile_by = by * a.scale_log2, tile_vs = vs;
+        const bool tile_counts = counts;
+        ahead = more;
+        if (ahead) locate();
+        const uint32_t stage = turn % kStages, parity = (turn / kStages & 1) ^ 1;
+        if (!wait(&m.free[0][stage], parity)) break;
+        widen_to(smem_addr(m.k[stage]), codes[0]);
+        Note& note = m.note[turn % kNotes];
+        const int32_t e = static_cast<int32_t>(__float_as_uint(tile_vs) >> 23 & 0xff);
+        const bool known = tile_counts && tile_vs > 0.f && e != 255;  // neither 0 nor NaN
+        const int32_t most = __reduce_max_sync(kAllLanes, known ? e - 127 : -1000);
+        const int32_t least = __reduce_min_sync(kAllLanes, known ? e - 127 : 1000);
+        const bool holes = __any_sync(kAllLanes, tile_vs < 0.f);
+        note.k[known_row] = tile_by;
+        note.v[known_row] = tile_vs;
+        if (lane == 0) note.seen[w] = make_int4(most, least, holes ? 1 : 0, 0);
+        arrive(&m.stored[0][stage]);
+        if (ahead) load(codes[0], a.cache.k, a.cache.k_pitch, k_row);
+        if (!wait(&m.free[1][stage], parity)) break;
+        widen_to(smem_addr(m.v[stage]), codes[1]);
+        arrive(&m.stored[1][stage]);
+        if (ahead) load(codes[1], a.cache.v, a.cache.v_pitch, v_row);
+        ++turn;
       }
     }
     if (bad) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
-  } else {
+  } else if (warp == kMmaWarp) {
     // ==================================================== MMAs
     constexpr uint32_t kScoreDesc = mma_descriptor(128, kSharedTile, 0, false, false);
     constexpr uint32_t kOutDesc = mma_descriptor(128, DIM, 0, false, true);
@@ -585,13 +696,15 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     const bool leader = elect_one();
     uint32_t k_turn = 0, v_turn = 0, weights_turn[2] = {0, 0}, queries_turn[2] = {0, 0};
     bool going = true;
-    while (going && walk.next(a, f)) {
-      const int32_t ops = f.split ? f.last - f.first : 2 * (f.last - f.first);
+    for (; going && next_fragment(seq); ++seq) {
+      const bool split = m.ring[seq % kRing].split != 0;
+      const int32_t tiles = m.ring[seq % kRing].last - m.ring[seq % kRing].first, ops = split ? tiles : 2 * tiles;
+      free_fragment(seq);
       for (int32_t n = 0; n <= ops; ++n) {
         if (n < ops) {  // scores
           const int slot = n & 1;
           const uint32_t stage = k_turn % kStages;
-          if ((f.split || slot == 0) && !wait(&m.k_full[stage], k_turn / kStages & 1)) going = false;
+          if ((split || slot == 0) && !wait(&m.ready[0][stage], k_turn / kStages & 1)) going = false;
           if (going && n < 2) going = wait(&m.queries[slot], queries_turn[slot]++ & 1);
           if (!going) break;
           tc_fence_after();
@@ -603,17 +716,17 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
               const uint32_t at = (k / 4 * kChunk + k % 4 * 32) >> 4;
               mma_f16(tmem + kScoresAt + slot * kSharedTile, qd + at, kd + at, kScoreDesc, k > 0);
             }
-            if (f.split || slot == 1) mma_commit(smem_addr(&m.k_free[stage]));
+            if (split || slot == 1) mma_commit(smem_addr(&m.free[0][stage]));
             mma_commit(smem_addr(&m.scores[slot]));
           }
           __syncwarp();
-          if (f.split || slot == 1) ++k_turn;
+          if (split || slot == 1) ++k_turn;
         }
         if (n > 0) {  // outputs of the one before
           const int slot = (n - 1) & 1;
           const uint32_t stage = v_turn % kStages;
           if (!wait(&m.weights[slot], weights_turn[slot]++ & 1)) going = false;
-          if (going && (f.split || slot == 0)) going = wait(&m.v_full[stage], v_turn / kStages & 1);
+          if (going && (split || slot == 0)) going = wait(&m.ready[1][stage], v_turn / kStages & 1);
           if (!going) break;
           tc_fence_after();
           if (leader) {
@@ -623,11 +736,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
               mma_f16_tmem(tmem + slot * DIM, tmem + kScoresAt + slot * kSharedTile + k * 8, vd + (k * 2048 >> 4), kOutDesc,
                            k > 0 || n > 2);
             }
-            if (f.split || slot == 1) mma_commit(smem_addr(&m.v_free[stage]));
+            if (split || slot == 1) mma_commit(smem_addr(&m.free[1][stage]));
             if (n + 1 >= ops) mma_commit(smem_addr(&m.done[slot]));
           }
           __syncwarp();
-          if (f.split || slot == 1) ++v_turn;
+          if (split || slot == 1) ++v_turn;
         }
       }
     }
@@ -639,6 +752,35 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
         }
       }
       __syncwarp();
+    }
+  } else if (warp >= kFenceWarp) {
+    // ==================================================== from stores to operands
+    // The loading warps store through the generic proxy, the tensor core reads
+    // through another. The fence between takes hundreds of cycles, of a loading
+    // warp until its loads are in, of the MMAs' warp while the tensor core waits.
+    const int which = warp - kFenceWarp;
+    uint32_t turn = 0;
+    bool going = true;
+    for (; going && next_fragment(seq); ++seq) {
+      const int32_t tiles = m.ring[seq % kRing].last - m.ring[seq % kRing].first;
+      free_fragment(seq);
+      for (int32_t i = 0; i < tiles && going; ++i, ++turn) {
+        going = wait(&m.stored[which][turn % kStages], turn / kStages & 1);
+        fence_proxy_async();
+        arrive(&m.ready[which][turn % kStages]);
+      }
+    }
+  } else {
+    // ==================================================== the CTA's fragments
+    Walk walk;
+    Fragment f;
+    walk.start(a);
+    for (bool more = true; more; ++seq) {
+      more = walk.next(a, f);
+      if (!more) f.last = 0;
+      if (!wait(&m.ring_free[seq % kRing], (seq / kRing & 1) ^ 1)) break;
+      if (lane == 0) m.ring[seq % kRing] = f;
+      arrive(&m.ring_full[seq % kRing]);
     }
   }
   tc_fence_before();
@@ -654,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
 template <typename T, int DIM>
 int launch(const SharedArgs& a, unsigned grid, cudaStream_t stream) {
   static DeviceBits granted{0};
-  constexpr int bytes = static_cast<int>(sizeof(Memory<DIM>)) + 1024;
+  constexpr int bytes = static_cast<int>(sizeof(Memory<DIM>));
   static_assert(bytes <= 227 * 1024, "shared memory");
   void (*fn)(SharedArgs) = shared_kernel<T, DIM>;
   const int rc = allow_launch(reinterpret_cast<const void*>(fn), bytes, granted);
