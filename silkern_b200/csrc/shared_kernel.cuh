@@ -13,13 +13,13 @@
 // Q goes in as fp16 with a power of two for each row, its largest magnitude in
 // [2^8, 2^9): exact but for columns below 2^-23 of the row's largest. The keys'
 // scales, one for each page, are left to the scores: x = s kscale |softmax_scale|
-// log2(e) 2^-row. Weights p = 2^(x - M) with M at most the largest x so far, and 4
+// log2(e) 2^-row. Weights p = 2^(x - M) with M at most the largest x so far, and 8
 // below it at most, so that O is rescaled seldom. What meets V is w = p vscale
-// 2^(6 - E) in fp16, E the exponent of the first tile's largest value scale: with
-// scales in [2^(E - 8), 2^(E + 4)) w is below 2^15, keeps 11 bits down to 2^-14 and
-// half a step of 2^-25 below, 2^-31 of the largest weight. Tiles with other scales
+// 2^(3 - E) in fp16, E the exponent of the first tile's largest value scale: with
+// scales in [2^(E - 6), 2^(E + 4)) w is below 2^15, keeps 11 bits down to 2^-14 and
+// half a step of 2^-25 below, 2^-28 of the largest weight. Tiles with other scales
 // (and all after them) keep a reference R of their own for w = 2^(x + log2 vscale -
-// R + 6), at a second exponential for each key. Sums, M, R, S and O are float32.
+// R + 3), at a second exponential for each key. Sums, M, R, S and O are float32.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -46,11 +46,17 @@ constexpr int kThreads = (kFenceWarp + 2) * 32;  // 512: up to 128 registers eac
 constexpr int kRing = 4;  // fragments known ahead
 constexpr int kStages = 2;  // of K and of V
 constexpr int kNotes = 3;   // a tile's scales live until its V is read
+// Weights go up to 2^kReach before their reference moves, and meet V times
+// 2^kShift, with value scales in [2^(E - kBelow), 2^(E + kAbove + 1)): below 2^15.
+constexpr int kReach = 8, kShift = 3, kAbove = 3, kBelow = 6;
+static_assert(kReach + kShift + kAbove + 1 <= 15, "fp16 ends at 2^16");
 
 struct __align__(16) Note {
   float k[kSharedTile];  // what a score is multiplied by
   float v[kSharedTile];  // value scales; -1: a key whose page is not in the cache
-  int4 seen[kLoadWarps]; // largest and smallest exponent of value scales, whether such a key is among them
+  // Largest and smallest exponent of value scales, whether such a key is among
+  // them: of each loading warp's keys, and of the tile's.
+  int4 seen[kLoadWarps], all;
 };
 
 // A part of an item and cache head that one CTA takes.
@@ -283,6 +289,33 @@ __device__ __forceinline__ float weigh_tile(const Row& r, uint32_t s_at, float b
   }
   return sum0 + sum1;
 }
+// Both in one pass, against a reference that the tile may turn out to pass: the
+// weights stay in registers (`w`), and `best` says how far the scores went.
+__device__ __forceinline__ float weigh_ahead(const Row& r, uint32_t s_at, float base, float unit, float& best, uint32_t (&w)[64]) {
+  float sum0 = 0.f, sum1 = 0.f;
+  best = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < kSharedTile; c += 32) {
+    float x[32];
+    uint32_t part[16];
+    tmem_ld32(s_at + c, x);
+    tmem_wait_ld(x);
+    best = fmaxf(best, largest<true, false>(r, c, x));
+    weigh<true, false>(r, c, x, base, unit, sum0, sum1, part);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[c / 2 + i] = part[i];
+  }
+  return sum0 + sum1;
+}
+__device__ __forceinline__ void store_weights(uint32_t s_at, const uint32_t (&w)[64]) {
+#pragma unroll
+  for (int c = 0; c < 64; c += 16) {
+    uint32_t part[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part[i] = w[c + i];
+    tmem_st16(s_at + c, part);
+  }
+}
 // Where the value scales of a tile are far from the first's: the largest score
 // times value scale, and the weights against a reference of their own.
 __device__ __forceinline__ float heaviest_of_tile(const Row& r, uint32_t s_at) {
@@ -314,7 +347,7 @@ __device__ __forceinline__ float weigh_heavy_tile(const Row& r, uint32_t s_at, f
       const float vs = r.note->v[c + i], t = x[i] * r.note->k[c + i] * r.unscale;
       const bool counts = c + i >= r.low && c + i < r.high && !(vs < 0.f);
       sum += counts ? exp2_approx(t - base) : 0.f;
-      x[i] = counts ? exp2_approx(t + log2f(vs) - reference + 6.f) : 0.f;
+      x[i] = counts ? exp2_approx(t + log2f(vs) - reference + kShift) : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = pack_f16x2(x[2 * i], x[2 * i + 1]);
@@ -368,9 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   pdl_launch_dependents();
   constexpr uint32_t kScoresAt = 256;  // TMEM columns: outputs of the slots from 0 and DIM on, scores from here
 
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    mbar_wait(smem_addr(bar), parity, abort, bound);
-    return !__any_sync(kAllLanes, *abort != 0);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // a whole warp; false once a wait ran out
+    return __all_sync(kAllLanes, mbar_wait(smem_addr(bar), parity, abort, bound)) != 0;
   };
   auto arrive = [&](uint64_t* bar) {  // once for the warp, behind all of its lanes
     __syncwarp();
@@ -436,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
                          pack_f16x2(b2.x * by, b2.y * by), pack_f16x2(b3.x * by, b3.y * by));
           }
         }
+        const int32_t all_see = __reduce_min_sync(kAllLanes, used ? min(limit, f.key_end) : 0x7fffffff);
         fence_proxy_async();
         arrive(&m.queries[slot]);
 
@@ -452,33 +485,40 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           ++turn;
           tc_fence_after();
           if (warp_used) {
-            int32_t most = -1000, least = 1000, holes = 0;
-#pragma unroll
-            for (int i = 0; i < kLoadWarps; ++i) {
-              const int4 s = note.seen[i];
-              most = max(most, s.x);
-              least = min(least, s.y);
-              holes |= s.z;
-            }
+            const int32_t most = note.all.x, least = note.all.y, holes = note.all.z;
             if (!known && most > -1000) {
               known = true;
               exponent = most;
             }
-            if (usual && most > -1000 && (most > exponent + 3 || least < exponent - 8)) {
+            if (usual && most > -1000 && (most > exponent + kAbove || least < exponent - kBelow)) {
               usual = false;
               reference = top + exponent;
             }
             const int32_t first_key = f.key_begin + tile * kSharedTile;
             const Row at{&note, unscale, f.key_first - first_key, min(limit, f.key_end) - first_key};
-            const bool masked = holes != 0 || __any_sync(kAllLanes, used && (at.low > 0 || at.high < kSharedTile));
+            const bool masked = holes != 0 || at.low > 0 || all_see - first_key < kSharedTile;
+            const float unit = __uint_as_float(static_cast<uint32_t>(127 + kShift - exponent) << 23);
+            // ---- most tiles leave the references where they are
+            bool stays = usual && !masked && a.runs && step > 0;
+            if (stays) {
+              uint32_t w[64];
+              float best;
+              const float sum = weigh_ahead(at, s_at, top, unit, best, w);
+              stays = __all_sync(kAllLanes, best <= top + kReach || best != best);
+              if (stays) {
+                total += sum;
+                store_weights(s_at, w);
+              }
+            }
+            if (!stays) {
             // ---- the largest score, and the largest weight where values' scales count
             const float best = !masked && a.runs ? largest_of_tile<true, false>(at, s_at)
                                : a.runs          ? largest_of_tile<true, true>(at, s_at)
                                                  : largest_of_tile<false, true>(at, s_at);
             const float heaviest = usual ? -INFINITY : heaviest_of_tile(at, s_at);
             // ---- references move, with the sum and the outputs
-            const bool up = best > top + 4.f || (top == -INFINITY && best > top);
-            const bool heavier = !usual && (heaviest > reference + 4.f || (reference == -INFINITY && heaviest > reference));
+            const bool up = best > top + kReach || (top == -INFINITY && best > top);
+            const bool heavier = !usual && (heaviest > reference + kReach || (reference == -INFINITY && heaviest > reference));
             if (__any_sync(kAllLanes, up || heavier)) {
               const float to = up ? best : top;
               const float down = up ? exp2f(top - to) : 1.f;
@@ -504,12 +544,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
             // ---- the weights
             const float base = top == -INFINITY ? 0.f : top;
             if (usual) {
-              const float unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - exponent) << 23);
               total += !masked && a.runs ? weigh_tile<true, false>(at, s_at, base, unit)
                        : a.runs          ? weigh_tile<true, true>(at, s_at, base, unit)
                                          : weigh_tile<false, true>(at, s_at, base, unit);
             } else {
               total += weigh_heavy_tile(at, s_at, base, reference == -INFINITY ? 0.f : reference);
+            }
             }
             tmem_wait_st();
           }
@@ -533,9 +573,9 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           } else {
             place = f.prefix != 0 ? own_place : pairs + own_place;
           }
-          // 2^(reference - top - 6) / total, in the usual case 2^(E - 6) / total.
+          // 2^(reference - top - kShift) / total, in the usual case 2^(E - kShift) / total.
           const float lift = usual ? static_cast<float>(exponent) : reference - top;
-          const float by = total > 0.f || total != total ? exp2f(lift - 6.f) / total : 0.f;
+          const float by = total > 0.f || total != total ? exp2f(lift - kShift) / total : 0.f;
           float4* out = reinterpret_cast<float4*>(a.part_out() + place * DIM);
 #pragma unroll 1
           for (int c = 0; c < DIM; c += 16) {
@@ -693,22 +733,28 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     constexpr uint32_t kScoreDesc = mma_descriptor(128, kSharedTile, 0, false, false);
     constexpr uint32_t kOutDesc = mma_descriptor(128, DIM, 0, false, true);
     constexpr uint32_t kChunk = kSharedTile * 128;  // bytes of 64 columns of a tile
-    const bool leader = elect_one();
-    uint32_t k_turn = 0, v_turn = 0, weights_turn[2] = {0, 0}, queries_turn[2] = {0, 0};
-    bool going = true;
-    for (; going && next_fragment(seq); ++seq) {
-      const bool split = m.ring[seq % kRing].split != 0;
-      const int32_t tiles = m.ring[seq % kRing].last - m.ring[seq % kRing].first, ops = split ? tiles : 2 * tiles;
-      free_fragment(seq);
-      for (int32_t n = 0; n <= ops; ++n) {
-        if (n < ops) {  // scores
-          const int slot = n & 1;
-          const uint32_t stage = k_turn % kStages;
-          if ((split || slot == 0) && !wait(&m.ready[0][stage], k_turn / kStages & 1)) going = false;
-          if (going && n < 2) going = wait(&m.queries[slot], queries_turn[slot]++ & 1);
-          if (!going) break;
-          tc_fence_after();
-          if (leader) {
+    // One lane does it all. Between two tiles of a slot lie its weights' arrival,
+    // PV, and the next QK: what else there is to wait for is waited for before.
+    if (elect_one()) {
+      auto lone_wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(smem_addr(bar), parity, abort, bound); };
+      uint32_t k_turn = 0, v_turn = 0, weights_turn[2] = {0, 0}, queries_turn[2] = {0, 0};
+      bool going = true;
+      for (; going; ++seq) {
+        going = lone_wait(&m.ring_full[seq % kRing], seq / kRing & 1);
+        const Fragment& f = m.ring[seq % kRing];
+        if (!going || f.last == 0) break;
+        const bool split = f.split != 0;
+        const int32_t tiles = f.last - f.first, ops = split ? tiles : 2 * tiles;
+        mbar_arrive(smem_addr(&m.ring_free[seq % kRing]));
+        bool k_seen = false;
+        for (int32_t n = 0; n <= ops; ++n) {
+          if (n < ops) {  // scores
+            const int slot = n & 1;
+            const uint32_t stage = k_turn % kStages;
+            if ((split || slot == 0) && !k_seen) going = lone_wait(&m.ready[0][stage], k_turn / kStages & 1);
+            if (going && n < 2) going = lone_wait(&m.queries[slot], queries_turn[slot]++ & 1);
+            if (!going) break;
+            tc_fence_after();
             const uint64_t qd = smem_descriptor(smem_addr(m.q[slot]), 16, 1024, kSwizzle128);
             const uint64_t kd = smem_descriptor(smem_addr(m.k[stage]), 16, 1024, kSwizzle128);
 #pragma unroll
@@ -716,43 +762,42 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
               const uint32_t at = (k / 4 * kChunk + k % 4 * 32) >> 4;
               mma_f16(tmem + kScoresAt + slot * kSharedTile, qd + at, kd + at, kScoreDesc, k > 0);
             }
-            if (split || slot == 1) mma_commit(smem_addr(&m.free[0][stage]));
             mma_commit(smem_addr(&m.scores[slot]));
+            if (split || slot == 1) {
+              mma_commit(smem_addr(&m.free[0][stage]));
+              ++k_turn;
+            }
           }
-          __syncwarp();
-          if (split || slot == 1) ++k_turn;
-        }
-        if (n > 0) {  // outputs of the one before
-          const int slot = (n - 1) & 1;
-          const uint32_t stage = v_turn % kStages;
-          if (!wait(&m.weights[slot], weights_turn[slot]++ & 1)) going = false;
-          if (going && (split || slot == 0)) going = wait(&m.ready[1][stage], v_turn / kStages & 1);
-          if (!going) break;
-          tc_fence_after();
-          if (leader) {
+          if (n > 0) {  // outputs of the one before
+            const int slot = (n - 1) & 1;
+            const uint32_t stage = v_turn % kStages;
+            if (split || slot == 0) going = lone_wait(&m.ready[1][stage], v_turn / kStages & 1);
+            k_seen = n + 1 < ops && (split || slot == 0) && mbar_try(smem_addr(&m.ready[0][k_turn % kStages]), k_turn / kStages & 1);
+            if (going) going = lone_wait(&m.weights[slot], weights_turn[slot]++ & 1);
+            if (!going) break;
+            tc_fence_after();
             const uint64_t vd = smem_descriptor(smem_addr(m.v[stage]), kChunk, 1024, kSwizzle128);
 #pragma unroll
             for (int k = 0; k < kSharedTile / 16; ++k) {
               mma_f16_tmem(tmem + slot * DIM, tmem + kScoresAt + slot * kSharedTile + k * 8, vd + (k * 2048 >> 4), kOutDesc,
                            k > 0 || n > 2);
             }
-            if (split || slot == 1) mma_commit(smem_addr(&m.free[1][stage]));
+            if (split || slot == 1) {
+              mma_commit(smem_addr(&m.free[1][stage]));
+              ++v_turn;
+            }
             if (n + 1 >= ops) mma_commit(smem_addr(&m.done[slot]));
           }
-          __syncwarp();
-          if (split || slot == 1) ++v_turn;
         }
       }
-    }
-    if (!going) {  // gave up: let what was issued finish before the memory goes
-      if (leader) {
+      if (!going) {  // gave up: let what was issued finish before the memory goes
         mma_commit(smem_addr(&m.drained));
         const long long begin = clock64();
         while (!mbar_try(smem_addr(&m.drained), 0) && clock64() - begin < 4000000000LL) {
         }
       }
-      __syncwarp();
     }
+    __syncwarp();
   } else if (warp >= kFenceWarp) {
     // ==================================================== from stores to operands
     // The loading warps store through the generic proxy, the tensor core reads
@@ -766,6 +811,15 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
       free_fragment(seq);
       for (int32_t i = 0; i < tiles && going; ++i, ++turn) {
         going = wait(&m.stored[which][turn % kStages], turn / kStages & 1);
+        if (which == 0 && lane == 0) {
+          Note& note = m.note[turn % kNotes];
+          int4 all = note.seen[0];
+#pragma unroll
+          for (int k = 1; k < kLoadWarps; ++k) {
+            all = make_int4(max(all.x, note.seen[k].x), min(all.y, note.seen[k].y), all.z | note.seen[k].z, 0);
+          }
+          note.all = all;
+        }
         fence_proxy_async();
         arrive(&m.ready[which][turn % kStages]);
       }
