@@ -39,13 +39,14 @@ namespace silkern {
 namespace shared {
 
 constexpr int kLoadWarps = 4;
-constexpr int kMmaWarp = 8 + kLoadWarps;
-constexpr int kWalkWarp = kMmaWarp + 1;
-constexpr int kFenceWarp = kWalkWarp + 1;        // one for K, one for V
-constexpr int kThreads = (kFenceWarp + 2) * 32;  // 512: up to 128 registers each
-constexpr int kRing = 4;  // fragments known ahead
+constexpr int kMmaWarp = 8 + kLoadWarps;  // one for each slot
+constexpr int kFenceWarp = kMmaWarp + 2;
+constexpr int kWalkWarp = kFenceWarp + 1;
+constexpr int kThreads = (kWalkWarp + 1) * 32;  // 512: up to 128 registers each
+constexpr int kRing = 8;  // fragments known ahead
 constexpr int kStages = 2;  // of K and of V
-constexpr int kNotes = 3;   // a tile's scales live until its V is read
+constexpr int kHalf = kSharedTile / 2;  // keys whose scores are there at once
+constexpr int kNotes = 4;   // a tile's scales live until its V is read, three tiles of K later
 // Weights go up to 2^kReach before their reference moves, and meet V times
 // 2^kShift, with value scales in [2^(E - kBelow), 2^(E + kAbove + 1)): below 2^15.
 constexpr int kReach = 8, kShift = 3, kAbove = 3, kBelow = 6;
@@ -69,10 +70,15 @@ struct Fragment {
   int32_t token, row, rows;
   int32_t seq, seqs;
   int32_t extra, prefix;
+  int32_t one_half;     // the last tile has keys in its first half only
 
-  // Tiles of a slot.
+  // Tiles of a slot, and half tiles.
   __device__ __forceinline__ int32_t steps(int slot) const {
     return split ? (last - first + 1 - slot) >> 1 : last - first;
+  }
+  __device__ __forceinline__ int32_t halves(int slot) const {
+    const bool has_last = !split || ((last - first - 1) & 1) == slot;
+    return 2 * steps(slot) - (has_last ? one_half : 0);
   }
 };
 
@@ -119,7 +125,8 @@ struct Walk {
       const int64_t first = max(at - zero, int64_t{0});
       f = Fragment{kv, static_cast<int32_t>(first), static_cast<int32_t>(last), ahead.rows <= kSlotRows ? 1 : 0,
                    ahead.key_begin, ahead.key_first, ahead.key_end, ahead.table_row, ahead.token, ahead.row, ahead.rows,
-                   ahead.seq, ahead.seqs, ahead.extra, ahead.prefix};
+                   ahead.seq, ahead.seqs, ahead.extra, ahead.prefix,
+                   ahead.key_end - ahead.key_begin - (static_cast<int32_t>(last) - 1) * kSharedTile <= kHalf ? 1 : 0};
       at = min(zero + ahead.tiles, end);
       if (kv + 1 == heads && at == zero + ahead.tiles) {
         ++next_item;
@@ -140,7 +147,8 @@ struct __align__(1024) Memory {
   Fragment ring[kRing];
   // [0]: of K, [1]: of V. Stored by the loading warps; ready for the MMAs; read by them.
   uint64_t stored[2][kStages], ready[2][kStages], free[2][kStages];
-  uint64_t scores[2], weights[2], queries[2], done[2], drained;
+  uint64_t scores[2][2], weights[2][2], done[2][2];  // of a slot and half
+  uint64_t queries[2], drained[2];
   uint64_t ring_full[kRing], ring_free[kRing];
   uint32_t tmem;
   int32_t abort;
@@ -203,11 +211,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// A tile's scores of one row, as its scales and masks make them. RUNS: keys
-// [16 i, 16 i + 16) share a page; MASKED: of the tile's keys only [low, high)
+// Half a tile's scores of one row, as its scales and masks make them. RUNS: keys
+// [16 i, 16 i + 16) share a page; MASKED: of the half's keys only [low, high)
 // count, and those whose page is in the cache.
 struct Row {
-  const Note* note;
+  const float* k;  // of the half's keys
+  const float* v;
   float unscale;
   int32_t low, high;
 };
@@ -224,15 +233,15 @@ __device__ __forceinline__ float largest(const Row& r, int at, const float (&x)[
         b0 = max3(b0, x[c + i], x[c + i + 1]);
         if (i + 3 < 16) b1 = max3(b1, x[c + i + 2], x[c + i + 3]);
       }
-      best = fmaxf(best, fmaxf(b0, b1) * r.note->k[at + c]);
+      best = fmaxf(best, fmaxf(b0, b1) * r.k[at + c]);
     }
   } else {
     float b[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const int j = RUNS ? at + (i & 16) : at + i;
-      float s = x[i] * r.note->k[j];
-      if (MASKED && (at + i < r.low || at + i >= r.high || r.note->v[j] < 0.f)) s = -INFINITY;
+      float s = x[i] * r.k[j];
+      if (MASKED && (at + i < r.low || at + i >= r.high || r.v[j] < 0.f)) s = -INFINITY;
       b[i & 1] = fmaxf(b[i & 1], s);
     }
     best = fmaxf(b[0], b[1]);
@@ -247,8 +256,8 @@ __device__ __forceinline__ void weigh(const Row& r, int at, const float (&x)[32]
 #pragma unroll
   for (int i = 0; i < 32; i += 2) {
     const int j = RUNS ? at + (i & 16) : at + i;
-    const float by0 = r.note->k[j] * r.unscale, vs0 = r.note->v[j] * unit;
-    const float by1 = RUNS ? by0 : r.note->k[j + 1] * r.unscale, vs1 = RUNS ? vs0 : r.note->v[j + 1] * unit;
+    const float by0 = r.k[j] * r.unscale, vs0 = r.v[j] * unit;
+    const float by1 = RUNS ? by0 : r.k[j + 1] * r.unscale, vs1 = RUNS ? vs0 : r.v[j + 1] * unit;
     float p0, p1, w0, w1;
     fma_pair(x[i], x[i + 1], by0, by1, -base, -base, p0, p1);
     bool out0 = false, out1 = false;
@@ -264,10 +273,10 @@ __device__ __forceinline__ void weigh(const Row& r, int at, const float (&x)[32]
   }
 }
 template <bool RUNS, bool MASKED>
-__device__ __forceinline__ float largest_of_tile(const Row& r, uint32_t s_at) {
+__device__ __forceinline__ float largest_of_half(const Row& r, uint32_t s_at) {
   float best = -INFINITY;
 #pragma unroll 1
-  for (int c = 0; c < kSharedTile; c += 32) {
+  for (int c = 0; c < kHalf; c += 32) {
     float x[32];
     tmem_ld32(s_at + c, x);
     tmem_wait_ld(x);
@@ -276,10 +285,10 @@ __device__ __forceinline__ float largest_of_tile(const Row& r, uint32_t s_at) {
   return best;
 }
 template <bool RUNS, bool MASKED>
-__device__ __forceinline__ float weigh_tile(const Row& r, uint32_t s_at, float base, float unit) {
+__device__ __forceinline__ float weigh_half(const Row& r, uint32_t s_at, float base, float unit) {
   float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < kSharedTile; c += 32) {
+  for (int c = 0; c < kHalf; c += 32) {
     float x[32];
     uint32_t w[16];
     tmem_ld32(s_at + c, x);
@@ -291,11 +300,11 @@ __device__ __forceinline__ float weigh_tile(const Row& r, uint32_t s_at, float b
 }
 // Both in one pass, against a reference that the tile may turn out to pass: the
 // weights stay in registers (`w`), and `best` says how far the scores went.
-__device__ __forceinline__ float weigh_ahead(const Row& r, uint32_t s_at, float base, float unit, float& best, uint32_t (&w)[64]) {
+__device__ __forceinline__ float weigh_ahead(const Row& r, uint32_t s_at, float base, float unit, float& best, uint32_t (&w)[kHalf / 2]) {
   float sum0 = 0.f, sum1 = 0.f;
   best = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < kSharedTile; c += 32) {
+  for (int c = 0; c < kHalf; c += 32) {
     float x[32];
     uint32_t part[16];
     tmem_ld32(s_at + c, x);
@@ -307,9 +316,9 @@ __device__ __forceinline__ float weigh_ahead(const Row& r, uint32_t s_at, float 
   }
   return sum0 + sum1;
 }
-__device__ __forceinline__ void store_weights(uint32_t s_at, const uint32_t (&w)[64]) {
+__device__ __forceinline__ void store_weights(uint32_t s_at, const uint32_t (&w)[kHalf / 2]) {
 #pragma unroll
-  for (int c = 0; c < 64; c += 16) {
+  for (int c = 0; c < kHalf / 2; c += 16) {
     uint32_t part[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) part[i] = w[c + i];
@@ -318,33 +327,33 @@ __device__ __forceinline__ void store_weights(uint32_t s_at, const uint32_t (&w)
 }
 // Where the value scales of a tile are far from the first's: the largest score
 // times value scale, and the weights against a reference of their own.
-__device__ __forceinline__ float heaviest_of_tile(const Row& r, uint32_t s_at) {
+__device__ __forceinline__ float heaviest_of_half(const Row& r, uint32_t s_at) {
   float most = -INFINITY;
 #pragma unroll 1
-  for (int c = 0; c < kSharedTile; c += 16) {
+  for (int c = 0; c < kHalf; c += 16) {
     float x[16];
     tmem_ld16(s_at + c, x);
     tmem_wait_ld(x);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float vs = r.note->v[c + i];
-      const float u = x[i] * r.note->k[c + i] * r.unscale + log2f(vs);
+      const float vs = r.v[c + i];
+      const float u = x[i] * r.k[c + i] * r.unscale + log2f(vs);
       if (c + i >= r.low && c + i < r.high && !(vs < 0.f)) most = fmaxf(most, u);
     }
   }
   return most;
 }
-__device__ __forceinline__ float weigh_heavy_tile(const Row& r, uint32_t s_at, float base, float reference) {
+__device__ __forceinline__ float weigh_heavy_half(const Row& r, uint32_t s_at, float base, float reference) {
   float sum = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < kSharedTile; c += 32) {
+  for (int c = 0; c < kHalf; c += 32) {
     float x[32];
     uint32_t w[16];
     tmem_ld32(s_at + c, x);
     tmem_wait_ld(x);
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const float vs = r.note->v[c + i], t = x[i] * r.note->k[c + i] * r.unscale;
+      const float vs = r.v[c + i], t = x[i] * r.k[c + i] * r.unscale;
       const bool counts = c + i >= r.low && c + i < r.high && !(vs < 0.f);
       sum += counts ? exp2_approx(t - base) : 0.f;
       x[i] = counts ? exp2_approx(t + log2f(vs) - reference + kShift) : 0.f;
@@ -374,19 +383,22 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     for (int i = 0; i < 2 * kStages; ++i) {
       mbar_init(smem_addr(&m.stored[i / kStages][i % kStages]), kLoadWarps);
       mbar_init(smem_addr(&m.ready[i / kStages][i % kStages]), 1);
-      mbar_init(smem_addr(&m.free[i / kStages][i % kStages]), 1);
+      mbar_init(smem_addr(&m.free[i / kStages][i % kStages]), 2);  // both slots' MMAs
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&m.scores[i]), 1);
-      mbar_init(smem_addr(&m.weights[i]), 4);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(smem_addr(&m.scores[i][h]), 1);
+        mbar_init(smem_addr(&m.weights[i][h]), 4);
+        mbar_init(smem_addr(&m.done[i][h]), 1);
+      }
       mbar_init(smem_addr(&m.queries[i]), 4);
-      mbar_init(smem_addr(&m.done[i]), 1);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(smem_addr(&m.ring_full[i]), 1);
-      mbar_init(smem_addr(&m.ring_free[i]), kWalkWarp + 2);  // every other warp
+      mbar_init(smem_addr(&m.ring_free[i]), kWalkWarp);  // every other warp
     }
-    mbar_init(smem_addr(&m.drained), 1);
+    mbar_init(smem_addr(&m.drained[0]), 1);
+    mbar_init(smem_addr(&m.drained[1]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     m.abort = 0;
   }
@@ -421,15 +433,14 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     // ==================================================== softmax
     const int slot = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lanes of this warp
-    const uint32_t s_at = tmem + lanes + kScoresAt + slot * kSharedTile, o_at = tmem + lanes + slot * DIM;
+    const uint32_t scores_at = tmem + lanes + kScoresAt + slot * kSharedTile, o_at = tmem + lanes + slot * DIM;
     const int row_in_slot = threadIdx.x & 127;
     uint32_t tiles_before = 0;  // of the CTA, for the notes' turns
-    uint32_t turn = 0, done_turn = 0;
+    uint32_t parity = 0;  // bit h: of half h's scores
     bool going = true;
     for (; going && next_fragment(seq); ++seq) {
-      const Fragment f = m.ring[seq % kRing];
-      free_fragment(seq);
-      const int32_t steps = f.steps(slot);
+      const Fragment& f = m.ring[seq % kRing];
+      const int32_t halves = f.halves(slot);
       const int32_t r = f.split ? row_in_slot : slot * kSlotRows + row_in_slot;  // of the block
       const bool used = r < f.rows;
       const bool warp_used = __any_sync(kAllLanes, used);
@@ -437,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
       const int32_t within = static_cast<int32_t>(fastdiv(row, a.per_kv));
       const int32_t token = f.token + within;
       const int32_t head = f.kv * a.heads_per_kv + row - within * a.heads_per_kv;
-      if (steps > 0) {
+      if (halves > 0) {
         // ---- the row's queries, and how far it sees
         float unscale = 0.f;
         int32_t limit = 0;
@@ -474,34 +485,41 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
 
         float top = -INFINITY, total = 0.f, reference = -INFINITY;
         int32_t exponent = 0;
-        bool known = false, usual = true;
-        for (int32_t step = 0; step < steps; ++step) {
-          const int32_t tile = f.first + (f.split ? 2 * step + slot : step);
-          const Note& note = m.note[(tiles_before + static_cast<uint32_t>(tile - f.first)) % kNotes];
-          if (!wait(&m.scores[slot], turn & 1)) {
+        bool known = false, usual = true, plain = false;
+        const int32_t stride = f.split ? 2 : 1, first_tile = f.split ? slot : 0;  // of the fragment's tiles
+        const int32_t key_first = f.key_first, seen = min(limit, f.key_end);
+        int32_t first_key = f.key_begin + (f.first + first_tile) * kSharedTile;  // of the half
+        const Note* note = nullptr;
+        for (int32_t step = 0; step < halves; ++step) {
+          const int half = step & 1;
+          const uint32_t s_at = scores_at + half * kHalf;
+          if (!wait(&m.scores[slot][half], parity >> half & 1)) {
             going = false;
             break;
           }
-          ++turn;
+          parity ^= 1u << half;
           tc_fence_after();
           if (warp_used) {
-            const int32_t most = note.all.x, least = note.all.y, holes = note.all.z;
-            if (!known && most > -1000) {
-              known = true;
-              exponent = most;
+            if (half == 0) {
+              note = &m.note[(tiles_before + first_tile + (step >> 1) * stride) % kNotes];
+              const int4 all = note->all;
+              if (!known && all.x > -1000) {
+                known = true;
+                exponent = all.x;
+              }
+              if (usual && all.x > -1000 && (all.x > exponent + kAbove || all.y < exponent - kBelow)) {
+                usual = false;
+                reference = top + exponent;
+              }
+              // Nothing of the tile is hidden from any of the warp's rows.
+              plain = usual && a.runs && all.z == 0 && key_first <= first_key && all_see - first_key >= kSharedTile;
             }
-            if (usual && most > -1000 && (most > exponent + kAbove || least < exponent - kBelow)) {
-              usual = false;
-              reference = top + exponent;
-            }
-            const int32_t first_key = f.key_begin + tile * kSharedTile;
-            const Row at{&note, unscale, f.key_first - first_key, min(limit, f.key_end) - first_key};
-            const bool masked = holes != 0 || at.low > 0 || all_see - first_key < kSharedTile;
+            const Row at{note->k + half * kHalf, note->v + half * kHalf, unscale, key_first - first_key, seen - first_key};
             const float unit = __uint_as_float(static_cast<uint32_t>(127 + kShift - exponent) << 23);
             // ---- most tiles leave the references where they are
-            bool stays = usual && !masked && a.runs && step > 0;
+            bool stays = plain && step > 0;
             if (stays) {
-              uint32_t w[64];
+              uint32_t w[kHalf / 2];
               float best;
               const float sum = weigh_ahead(at, s_at, top, unit, best, w);
               stays = __all_sync(kAllLanes, best <= top + kReach || best != best);
@@ -512,10 +530,10 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
             }
             if (!stays) {
             // ---- the largest score, and the largest weight where values' scales count
-            const float best = !masked && a.runs ? largest_of_tile<true, false>(at, s_at)
-                               : a.runs          ? largest_of_tile<true, true>(at, s_at)
-                                                 : largest_of_tile<false, true>(at, s_at);
-            const float heaviest = usual ? -INFINITY : heaviest_of_tile(at, s_at);
+            const float best = plain    ? largest_of_half<true, false>(at, s_at)
+                               : a.runs ? largest_of_half<true, true>(at, s_at)
+                                        : largest_of_half<false, true>(at, s_at);
+            const float heaviest = usual ? -INFINITY : heaviest_of_half(at, s_at);
             // ---- references move, with the sum and the outputs
             const bool up = best > top + kReach || (top == -INFINITY && best > top);
             const bool heavier = !usual && (heaviest > reference + kReach || (reference == -INFINITY && heaviest > reference));
@@ -530,6 +548,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
                 if (heavier) reference = heaviest;
               }
               if (step > 0) {
+                // The half before may still be added up.
+                if (!wait(&m.done[slot][half ^ 1], (parity >> (half ^ 1) & 1) ^ 1)) {
+                  going = false;
+                  break;
+                }
+                tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < DIM; c += 16) {
                   float o[16];
@@ -544,23 +568,22 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
             // ---- the weights
             const float base = top == -INFINITY ? 0.f : top;
             if (usual) {
-              total += !masked && a.runs ? weigh_tile<true, false>(at, s_at, base, unit)
-                       : a.runs          ? weigh_tile<true, true>(at, s_at, base, unit)
-                                         : weigh_tile<false, true>(at, s_at, base, unit);
+              total += plain    ? weigh_half<true, false>(at, s_at, base, unit)
+                       : a.runs ? weigh_half<true, true>(at, s_at, base, unit)
+                                : weigh_half<false, true>(at, s_at, base, unit);
             } else {
-              total += weigh_heavy_tile(at, s_at, base, reference == -INFINITY ? 0.f : reference);
+              total += weigh_heavy_half(at, s_at, base, reference == -INFINITY ? 0.f : reference);
             }
             }
             tmem_wait_st();
           }
           tc_fence_before();
-          arrive(&m.weights[slot]);
+          arrive(&m.weights[slot][half]);
+          first_key += half == 0 ? kHalf : stride * kSharedTile - kHalf;
         }
-        if (!going || !wait(&m.done[slot], done_turn & 1)) {
-          going = false;
-          break;
-        }
-        ++done_turn;
+        // (That the turns before the last are over follows from the last scores.)
+        if (going) going = wait(&m.done[slot][(halves - 1) & 1], (parity >> ((halves - 1) & 1) & 1) ^ 1);
+        if (!going) break;
         tc_fence_after();
         // ---- the fragment's outputs
         if (warp_used) {
@@ -600,6 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
         a.part_lse()[place] = -INFINITY;
       }
       tiles_before += f.last - f.first;
+      free_fragment(seq);
     }
   } else if (warp < kMmaWarp) {
     // ==================================================== keys and values
@@ -694,20 +718,33 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
         st_shared_v4(tile_at + (to ^ 16) + i * kStep, h[4], h[5], h[6], h[7]);
       }
     };
-    uint32_t turn = 0;
+    // Keys are stored a tile ahead of the values: the slots take turns with the
+    // tiles, and one's next scores must not wait for the other's weights.
     if (more) {
       fetch();
       locate();
       load(codes[0], a.cache.k, a.cache.k_pitch, k_row);
       load(codes[1], a.cache.v, a.cache.v_pitch, v_row);
-      bool ahead = true;
-      while (ahead) {
+      auto store_values = [&](uint32_t turn) {
+        const uint32_t stage = turn % kStages;
+        if (!wait(&m.free[1][stage], (turn / kStages & 1) ^ 1)) return false;
+        widen_to(smem_addr(m.v[stage]), codes[1]);
+        arrive(&m.stored[1][stage]);
+        return true;
+      };
+      bool going = true;
+      uint32_t turn = 0;
+      for (bool ahead = true; ahead && going; ++turn) {
         const float tile_by = by * a.scale_log2, tile_vs = vs;
         const bool tile_counts = counts;
+        const int32_t tile_v_row = v_row;
         ahead = more;
         if (ahead) locate();
-        const uint32_t stage = turn % kStages, parity = (turn / kStages & 1) ^ 1;
-        if (!wait(&m.free[0][stage], parity)) break;
+        const uint32_t stage = turn % kStages;
+        if (!wait(&m.free[0][stage], (turn / kStages & 1) ^ 1)) {
+          going = false;
+          break;
+        }
         widen_to(smem_addr(m.k[stage]), codes[0]);
         Note& note = m.note[turn % kNotes];
         const int32_t e = static_cast<int32_t>(__float_as_uint(tile_vs) >> 23 & 0xff);
@@ -720,110 +757,138 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
         if (lane == 0) note.seen[w] = make_int4(most, least, holes ? 1 : 0, 0);
         arrive(&m.stored[0][stage]);
         if (ahead) load(codes[0], a.cache.k, a.cache.k_pitch, k_row);
-        if (!wait(&m.free[1][stage], parity)) break;
-        widen_to(smem_addr(m.v[stage]), codes[1]);
-        arrive(&m.stored[1][stage]);
-        if (ahead) load(codes[1], a.cache.v, a.cache.v_pitch, v_row);
-        ++turn;
+        if (turn > 0) {
+          going = store_values(turn - 1);
+          if (going) load(codes[1], a.cache.v, a.cache.v_pitch, tile_v_row);
+        }
       }
+      if (going) store_values(turn - 1);
     }
     if (bad) flag_status(a.status, SILKERN_STATUS_BAD_SLOT);
-  } else if (warp == kMmaWarp) {
+  } else if (warp < kFenceWarp) {
     // ==================================================== MMAs
-    constexpr uint32_t kScoreDesc = mma_descriptor(128, kSharedTile, 0, false, false);
+    // A warp for each slot. All of it walks, so that descriptors stay in uniform
+    // registers; one lane issues. Each passes every tile, its own or not, so that
+    // their places fill in turn.
+    constexpr uint32_t kScoreDesc = mma_descriptor(128, kHalf, 0, false, false);
     constexpr uint32_t kOutDesc = mma_descriptor(128, DIM, 0, false, true);
     constexpr uint32_t kChunk = kSharedTile * 128;  // bytes of 64 columns of a tile
-    // One lane does it all. Between two tiles of a slot lie its weights' arrival,
-    // PV, and the next QK: what else there is to wait for is waited for before.
-    if (elect_one()) {
-      auto lone_wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(smem_addr(bar), parity, abort, bound); };
-      uint32_t k_turn = 0, v_turn = 0, weights_turn[2] = {0, 0}, queries_turn[2] = {0, 0};
-      bool going = true;
-      for (; going; ++seq) {
-        going = lone_wait(&m.ring_full[seq % kRing], seq / kRing & 1);
-        const Fragment& f = m.ring[seq % kRing];
-        if (!going || f.last == 0) break;
-        const bool split = f.split != 0;
-        const int32_t tiles = f.last - f.first, ops = split ? tiles : 2 * tiles;
-        mbar_arrive(smem_addr(&m.ring_free[seq % kRing]));
-        bool k_seen = false;
-        for (int32_t n = 0; n <= ops; ++n) {
-          if (n < ops) {  // scores
-            const int slot = n & 1;
-            const uint32_t stage = k_turn % kStages;
-            if ((split || slot == 0) && !k_seen) going = lone_wait(&m.ready[0][stage], k_turn / kStages & 1);
-            if (going && n < 2) going = lone_wait(&m.queries[slot], queries_turn[slot]++ & 1);
-            if (!going) break;
+    constexpr uint32_t kTileStep = kSharedTile * DIM * 2 >> 4, kHalfStep = kHalf * 128 >> 4;  // in units of 16 bytes
+    const int slot = warp - kMmaWarp;
+    const bool leader = elect_one();
+    const uint64_t q_desc = smem_descriptor(smem_addr(m.q[slot]), 16, 1024, kSwizzle128);
+    const uint64_t k_desc = smem_descriptor(smem_addr(m.k[0]), 16, 1024, kSwizzle128);
+    const uint64_t v_desc = smem_descriptor(smem_addr(m.v[0]), kChunk, 1024, kSwizzle128);
+    const uint32_t scores_at = tmem + kScoresAt + slot * kSharedTile, o_at = tmem + slot * DIM;
+    uint32_t tiles_before = 0, k_next = 0, v_next = 0;  // tiles of the CTA: before the fragment, not waited for yet
+    uint32_t queries_parity = 0, weights_parity = 0;    // (a bit for each half)
+    bool going = true;
+    // Up to `tile`, of K (0) or V (1): the others' tiles are passed, and it is there.
+    auto reach = [&](int which, uint32_t& next, uint32_t tile) {
+      for (; next <= tile; ++next) {
+        if (!wait(&m.ready[which][next % kStages], next / kStages & 1)) return false;
+        if (next < tile) arrive(&m.free[which][next % kStages]);
+      }
+      return true;
+    };
+    for (; going && next_fragment(seq); ++seq) {
+      const Fragment& f = m.ring[seq % kRing];
+      const int32_t tiles = f.last - f.first, halves = f.halves(slot);
+      const uint32_t own = tiles_before + (f.split != 0 ? slot : 0), stride = f.split != 0 ? 2 : 1;
+      free_fragment(seq);
+      // Scores run two halves ahead of the outputs, so that the softmax finds the
+      // next ones when it is through with a half.
+      for (int32_t i = -2; i < halves; ++i) {
+        const uint32_t half = i & 1, s_at = scores_at + half * kHalf;
+        if (i >= 0) {  // outputs
+          const uint32_t tile = own + (i >> 1) * stride, stage = tile % kStages;
+          if (half == 0 && !(going = reach(1, v_next, tile))) break;
+          if (!(going = wait(&m.weights[slot][half], weights_parity >> half & 1))) break;
+          weights_parity ^= 1u << half;
+          tc_fence_after();
+          const uint64_t vd = v_desc + stage * kTileStep + half * kHalfStep;
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < kHalf / 16; ++k) {
+              mma_f16_tmem(o_at, s_at + k * 8, vd + (k * 2048 >> 4), kOutDesc, k > 0 || i > 0);
+            }
+            mma_commit(smem_addr(&m.done[slot][half]));
+            if (half == 1 || i + 1 == halves) mma_commit(smem_addr(&m.free[1][stage]));
+          }
+          __syncwarp();
+        }
+        if (i + 2 < halves) {  // scores
+          const uint32_t tile = own + ((i + 2) >> 1) * stride, stage = tile % kStages;
+          if (half == 0 && !(going = reach(0, k_next, tile))) break;
+          if (i == -2) {
+            if (!(going = wait(&m.queries[slot], queries_parity))) break;
+            queries_parity ^= 1;
             tc_fence_after();
-            const uint64_t qd = smem_descriptor(smem_addr(m.q[slot]), 16, 1024, kSwizzle128);
-            const uint64_t kd = smem_descriptor(smem_addr(m.k[stage]), 16, 1024, kSwizzle128);
+          }
+          const uint64_t kd = k_desc + stage * kTileStep + half * kHalfStep;
+          if (leader) {
 #pragma unroll
             for (int k = 0; k < DIM / 16; ++k) {
               const uint32_t at = (k / 4 * kChunk + k % 4 * 32) >> 4;
-              mma_f16(tmem + kScoresAt + slot * kSharedTile, qd + at, kd + at, kScoreDesc, k > 0);
+              mma_f16(s_at, q_desc + at, kd + at, kScoreDesc, k > 0);
             }
-            mma_commit(smem_addr(&m.scores[slot]));
-            if (split || slot == 1) {
-              mma_commit(smem_addr(&m.free[0][stage]));
-              ++k_turn;
-            }
+            mma_commit(smem_addr(&m.scores[slot][half]));
+            if (half == 1 || i + 3 == halves) mma_commit(smem_addr(&m.free[0][stage]));
           }
-          if (n > 0) {  // outputs of the one before
-            const int slot = (n - 1) & 1;
-            const uint32_t stage = v_turn % kStages;
-            if (split || slot == 0) going = lone_wait(&m.ready[1][stage], v_turn / kStages & 1);
-            k_seen = n + 1 < ops && (split || slot == 0) && mbar_try(smem_addr(&m.ready[0][k_turn % kStages]), k_turn / kStages & 1);
-            if (going) going = lone_wait(&m.weights[slot], weights_turn[slot]++ & 1);
-            if (!going) break;
-            tc_fence_after();
-            const uint64_t vd = smem_descriptor(smem_addr(m.v[stage]), kChunk, 1024, kSwizzle128);
-#pragma unroll
-            for (int k = 0; k < kSharedTile / 16; ++k) {
-              mma_f16_tmem(tmem + slot * DIM, tmem + kScoresAt + slot * kSharedTile + k * 8, vd + (k * 2048 >> 4), kOutDesc,
-                           k > 0 || n > 2);
-            }
-            if (split || slot == 1) {
-              mma_commit(smem_addr(&m.free[1][stage]));
-              ++v_turn;
-            }
-            if (n + 1 >= ops) mma_commit(smem_addr(&m.done[slot]));
-          }
+          __syncwarp();
         }
       }
-      if (!going) {  // gave up: let what was issued finish before the memory goes
-        mma_commit(smem_addr(&m.drained));
-        const long long begin = clock64();
-        while (!mbar_try(smem_addr(&m.drained), 0) && clock64() - begin < 4000000000LL) {
-        }
+      tiles_before += tiles;
+      // The other slot's last tile.
+      if (going && k_next < tiles_before) {
+        going = reach(0, k_next, tiles_before - 1);
+        if (going) arrive(&m.free[0][(tiles_before - 1) % kStages]);
+      }
+      if (going && v_next < tiles_before) {
+        going = reach(1, v_next, tiles_before - 1);
+        if (going) arrive(&m.free[1][(tiles_before - 1) % kStages]);
       }
     }
-    __syncwarp();
-  } else if (warp >= kFenceWarp) {
+    if (!going) {  // gave up: let what was issued finish before the memory goes
+      if (leader) {
+        mma_commit(smem_addr(&m.drained[slot]));
+        const long long begin = clock64();
+        while (!mbar_try(smem_addr(&m.drained[slot]), 0) && clock64() - begin < 4000000000LL) {
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp == kFenceWarp) {
     // ==================================================== from stores to operands
     // The loading warps store through the generic proxy, the tensor core reads
     // through another. The fence between takes hundreds of cycles, of a loading
-    // warp until its loads are in, of the MMAs' warp while the tensor core waits.
-    const int which = warp - kFenceWarp;
+    // warp until its loads are in, of an MMAs' warp while the tensor core waits.
     uint32_t turn = 0;
     bool going = true;
+    auto pass = [&](int which, uint32_t tile) {
+      const uint32_t stage = tile % kStages;
+      if (!wait(&m.stored[which][stage], tile / kStages & 1)) return false;
+      if (which == 0 && lane == 0) {
+        Note& note = m.note[tile % kNotes];
+        int4 all = note.seen[0];
+#pragma unroll
+        for (int k = 1; k < kLoadWarps; ++k) {
+          all = make_int4(max(all.x, note.seen[k].x), min(all.y, note.seen[k].y), all.z | note.seen[k].z, 0);
+        }
+        note.all = all;
+      }
+      fence_proxy_async();
+      arrive(&m.ready[which][stage]);
+      return true;
+    };
     for (; going && next_fragment(seq); ++seq) {
       const int32_t tiles = m.ring[seq % kRing].last - m.ring[seq % kRing].first;
       free_fragment(seq);
       for (int32_t i = 0; i < tiles && going; ++i, ++turn) {
-        going = wait(&m.stored[which][turn % kStages], turn / kStages & 1);
-        if (which == 0 && lane == 0) {
-          Note& note = m.note[turn % kNotes];
-          int4 all = note.seen[0];
-#pragma unroll
-          for (int k = 1; k < kLoadWarps; ++k) {
-            all = make_int4(max(all.x, note.seen[k].x), min(all.y, note.seen[k].y), all.z | note.seen[k].z, 0);
-          }
-          note.all = all;
-        }
-        fence_proxy_async();
-        arrive(&m.ready[which][turn % kStages]);
+        going = pass(0, turn) && (turn == 0 || pass(1, turn - 1));
       }
     }
+    if (going && turn > 0) pass(1, turn - 1);
   } else {
     // ==================================================== the CTA's fragments
     Walk walk;
