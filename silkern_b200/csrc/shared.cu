@@ -117,15 +117,14 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
         blocks = (s.tokens * a.heads_per_kv + kBlockRows - 1) / kBlockRows;
         mine[0] = blocks;
         for (int32_t b = 0; b < blocks; ++b) {
-          const SharedItem it = item_of(a, s, prefix, b);
-          mine[1] += units_of(it.tiles);
-          if (it.rows <= kSlotRows) mine[2] += it.rows;
-          if (prefix) {  // the others are alike, but for the last's rows
-            mine[1] += static_cast<int64_t>(units_of(it.tiles)) * (blocks - 1);
-            const int32_t rest = s.tokens * a.heads_per_kv - (blocks - 1) * kBlockRows;
-            mine[2] = rest <= kSlotRows ? rest : 0;
-            break;
+          // (A prefix's blocks are alike, but for the last's rows.)
+          if (prefix && b == 1) {
+            mine[1] *= blocks - 1;
+            b = blocks - 1;
           }
+          const SharedItem it = item_of(a, s, prefix, b);
+          mine[1] += units_of(it.tiles, it.rows);
+          if (it.rows <= kSlotRows) mine[2] += it.rows;
         }
       }
     }
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
         SharedItem it = item_of(a, s, prefix, b);
         it.begin = upto[1];
         it.extra = static_cast<int32_t>(upto[2]);
-        upto[1] += units_of(it.tiles);
+        upto[1] += units_of(it.tiles, it.rows);
         if (it.rows <= kSlotRows) upto[2] += it.rows;
         *a.item(static_cast<int32_t>(upto[0]) + b) = it;
       }
@@ -201,10 +200,10 @@ __device__ __forceinline__ Parts find_parts(const SharedArgs& a, int32_t segment
   const SharedItem* it = a.item(first + row / kBlockRows);
   const int32_t tiles = load_int(&it->tiles);
   if (tiles == 0) return p;
-  const int64_t share = __ldcg(&a.header()->share);
-  const int64_t zero = __ldcg(&it->begin) * a.cache.kv_heads + static_cast<int64_t>(kv) * units_of(tiles) + kStart;
-  const int64_t c0 = zero / share, c1 = (zero + tiles - 1) / share;
   const int32_t r = row % kBlockRows, rows = load_int(&it->rows);
+  const int64_t share = __ldcg(&a.header()->share);
+  const int64_t zero = __ldcg(&it->begin) * a.cache.kv_heads + kv * units_of(tiles, rows) + units_of_start(rows);
+  const int64_t c0 = zero / share, c1 = (zero + static_cast<int64_t>(tiles - 1) * units_of_tile(rows)) / share;
   p.count = static_cast<int32_t>(c1 - c0 + 1);
   p.first = place;
   p.next = a.at.starts + (c0 + 1) * kBlockRows + r;

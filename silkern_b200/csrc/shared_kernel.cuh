@@ -65,6 +65,7 @@ struct Fragment {
   int32_t kv;
   int32_t first, last;  // tiles; the CTA's last fragment is followed by one with last 0
   int32_t split;        // the slots take turns with the tiles
+  int32_t lead;         // the slot that the first tile is then for
   int32_t key_begin, key_first, key_end;
   int32_t table_row;
   int32_t token, row, rows;
@@ -72,13 +73,13 @@ struct Fragment {
   int32_t extra, prefix;
   int32_t one_half;     // the last tile has keys in its first half only
 
-  // Tiles of a slot, and half tiles.
-  __device__ __forceinline__ int32_t steps(int slot) const {
-    return split ? (last - first + 1 - slot) >> 1 : last - first;
-  }
+  // A slot's first tile, from the fragment's first on, and its half tiles.
+  __device__ __forceinline__ int32_t own(int slot) const { return split ? slot ^ lead : 0; }
+  __device__ __forceinline__ int32_t stride() const { return split ? 2 : 1; }
   __device__ __forceinline__ int32_t halves(int slot) const {
-    const bool has_last = !split || ((last - first - 1) & 1) == slot;
-    return 2 * steps(slot) - (has_last ? one_half : 0);
+    const int32_t tiles = last - first, mine = split ? (tiles - own(slot) + 1) >> 1 : tiles;
+    const bool has_last = !split || ((tiles - 1) & 1) == own(slot);
+    return 2 * mine - (has_last ? one_half : 0);
   }
 };
 
@@ -86,6 +87,7 @@ struct Fragment {
 struct Walk {
   int64_t at, end;
   int32_t next_item, items;
+  uint32_t tiles_before;
   SharedItem ahead;
 
   __device__ __forceinline__ void load_ahead(const SharedArgs& a) {
@@ -102,6 +104,7 @@ struct Walk {
     at = share * blockIdx.x;
     end = min(at + share, units);
     next_item = 0;
+    tiles_before = 0;
     if (at >= end) return;
     const int64_t heads = a.cache.kv_heads;
     next_item = warp_last_at_most(items, at, [&](int32_t i) { return __ldcg(&a.item(i)->begin) * heads; });
@@ -111,28 +114,31 @@ struct Walk {
   __device__ __forceinline__ bool next(const SharedArgs& a, Fragment& f) {
     const int64_t heads = a.cache.kv_heads;
     while (at < end) {
-      const int32_t cost = units_of(ahead.tiles);
-      const int64_t base = ahead.begin * heads;
-      const int64_t inside = at - base;
+      const int64_t cost = units_of(ahead.tiles, ahead.rows), base = ahead.begin * heads, inside = at - base;
       if (cost == 0 || inside >= cost * heads) {
         if (++next_item >= items) break;
         load_ahead(a);
         continue;
       }
-      const int32_t kv = static_cast<int32_t>(inside / cost);
-      const int64_t zero = base + static_cast<int64_t>(kv) * cost + kStart;  // of the first tile
-      const int64_t last = min(end - zero, static_cast<int64_t>(ahead.tiles));
-      const int64_t first = max(at - zero, int64_t{0});
-      f = Fragment{kv, static_cast<int32_t>(first), static_cast<int32_t>(last), ahead.rows <= kSlotRows ? 1 : 0,
+      const int32_t each = units_of_tile(ahead.rows), kv = static_cast<int32_t>(inside / cost);
+      const int64_t zero = base + kv * cost + units_of_start(ahead.rows);  // of the first tile
+      auto tiles_before_unit = [&](int64_t unit) {
+        return static_cast<int32_t>(unit <= zero ? 0 : min((unit - zero + each - 1) / each, static_cast<int64_t>(ahead.tiles)));
+      };
+      const int32_t first = tiles_before_unit(at), last = tiles_before_unit(end);
+      f = Fragment{kv, first, last, ahead.rows <= kSlotRows ? 1 : 0, static_cast<int32_t>(tiles_before & 1),
                    ahead.key_begin, ahead.key_first, ahead.key_end, ahead.table_row, ahead.token, ahead.row, ahead.rows,
                    ahead.seq, ahead.seqs, ahead.extra, ahead.prefix,
-                   ahead.key_end - ahead.key_begin - (static_cast<int32_t>(last) - 1) * kSharedTile <= kHalf ? 1 : 0};
-      at = min(zero + ahead.tiles, end);
-      if (kv + 1 == heads && at == zero + ahead.tiles) {
+                   ahead.key_end - ahead.key_begin - (last - 1) * kSharedTile <= kHalf ? 1 : 0};
+      at = min(base + (kv + 1) * cost, end);
+      if (kv + 1 == heads && at == base + heads * cost) {
         ++next_item;
         load_ahead(a);
       }
-      if (last > first) return true;
+      if (last > first) {
+        tiles_before += last - first;
+        return true;
+      }
     }
     return false;
   }
@@ -175,6 +181,11 @@ __device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b,
       "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 using silkern::tmem_st16;
 using silkern::tmem_wait_ld;
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
@@ -211,109 +222,54 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// Half a tile's scores of one row, as its scales and masks make them. RUNS: keys
-// [16 i, 16 i + 16) share a page; MASKED: of the half's keys only [low, high)
-// count, and those whose page is in the cache.
+// Half a tile's scores of one row, as its scales and masks make them: keys [low,
+// high) count, and of them those whose page is in the cache.
 struct Row {
   const float* k;  // of the half's keys
   const float* v;
   float unscale;
   int32_t low, high;
 };
-// The largest score of the 32 in x, the keys from `at` on.
-template <bool RUNS, bool MASKED>
-__device__ __forceinline__ float largest(const Row& r, int at, const float (&x)[32]) {
-  float best = -INFINITY;
-  if constexpr (RUNS && !MASKED) {
+
+// The usual half: nothing of it is hidden from the row, and each 16 keys share a
+// page and its scales. Weights against `base`, which a score may turn out to pass
+// (`best` says how far they went): their sum, and in `w` their products with the
+// value scales in `unit`s.
+__device__ __forceinline__ float weigh_plain(const Row& r, uint32_t s_at, float base, float unit, float& best,
+                                             uint32_t (&w)[kHalf / 2]) {
+  float sum0 = 0.f, sum1 = 0.f, most = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < 32; c += 16) {
-      float b0 = x[c], b1 = x[c + 1];
+  for (int c = 0; c < kHalf; c += 32) {
+    float x[32];
+    tmem_ld32(s_at + c, x);
+    tmem_wait_ld(x);
+    float k[2], by[2], vs[2];
 #pragma unroll
-      for (int i = 2; i < 16; i += 4) {
-        b0 = max3(b0, x[c + i], x[c + i + 1]);
-        if (i + 3 < 16) b1 = max3(b1, x[c + i + 2], x[c + i + 3]);
+    for (int run = 0; run < 2; ++run) {
+      k[run] = r.k[c + 16 * run];
+      by[run] = k[run] * r.unscale;
+      vs[run] = r.v[c + 16 * run] * unit;
+      float b0 = x[16 * run], b1 = x[16 * run + 1];
+#pragma unroll
+      for (int i = 16 * run + 2; i < 16 * run + 16; i += 4) {
+        b0 = max3(b0, x[i], x[i + 1]);
+        if (i + 3 < 16 * run + 16) b1 = max3(b1, x[i + 2], x[i + 3]);
       }
-      best = fmaxf(best, fmaxf(b0, b1) * r.k[at + c]);
+      most = fmaxf(most, fmaxf(b0, b1) * k[run]);
     }
-  } else {
-    float b[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int j = RUNS ? at + (i & 16) : at + i;
-      float s = x[i] * r.k[j];
-      if (MASKED && (at + i < r.low || at + i >= r.high || r.v[j] < 0.f)) s = -INFINITY;
-      b[i & 1] = fmaxf(b[i & 1], s);
+    for (int i = 0; i < 32; i += 2) {
+      const int run = i / 16;
+      float p0, p1, w0, w1;
+      fma_pair(x[i], x[i + 1], by[run], by[run], -base, -base, p0, p1);
+      p0 = exp2_approx(p0);
+      p1 = exp2_approx(p1);
+      add_pair(sum0, sum1, p0, p1, sum0, sum1);
+      mul_pair(p0, p1, vs[run], vs[run], w0, w1);
+      w[(c + i) / 2] = pack_f16x2(w0, w1);
     }
-    best = fmaxf(b[0], b[1]);
   }
-  return best * r.unscale;
-}
-// Weights of the 32 scores in x against `base`: their sum is added to sum0 and
-// sum1, their products with the value scales in `unit`s go out in pairs.
-template <bool RUNS, bool MASKED>
-__device__ __forceinline__ void weigh(const Row& r, int at, const float (&x)[32], float base, float unit, float& sum0,
-                                      float& sum1, uint32_t (&w)[16]) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 2) {
-    const int j = RUNS ? at + (i & 16) : at + i;
-    const float by0 = r.k[j] * r.unscale, vs0 = r.v[j] * unit;
-    const float by1 = RUNS ? by0 : r.k[j + 1] * r.unscale, vs1 = RUNS ? vs0 : r.v[j + 1] * unit;
-    float p0, p1, w0, w1;
-    fma_pair(x[i], x[i + 1], by0, by1, -base, -base, p0, p1);
-    bool out0 = false, out1 = false;
-    if constexpr (MASKED) {
-      out0 = at + i < r.low || at + i >= r.high || vs0 < 0.f;
-      out1 = at + i + 1 < r.low || at + i + 1 >= r.high || vs1 < 0.f;
-    }
-    p0 = out0 ? 0.f : exp2_approx(p0);
-    p1 = out1 ? 0.f : exp2_approx(p1);
-    add_pair(sum0, sum1, p0, p1, sum0, sum1);
-    mul_pair(p0, p1, vs0, vs1, w0, w1);
-    w[i / 2] = pack_f16x2(out0 ? 0.f : w0, out1 ? 0.f : w1);
-  }
-}
-template <bool RUNS, bool MASKED>
-__device__ __forceinline__ float largest_of_half(const Row& r, uint32_t s_at) {
-  float best = -INFINITY;
-#pragma unroll 1
-  for (int c = 0; c < kHalf; c += 32) {
-    float x[32];
-    tmem_ld32(s_at + c, x);
-    tmem_wait_ld(x);
-    best = fmaxf(best, largest<RUNS, MASKED>(r, c, x));
-  }
-  return best;
-}
-template <bool RUNS, bool MASKED>
-__device__ __forceinline__ float weigh_half(const Row& r, uint32_t s_at, float base, float unit) {
-  float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll 1
-  for (int c = 0; c < kHalf; c += 32) {
-    float x[32];
-    uint32_t w[16];
-    tmem_ld32(s_at + c, x);
-    tmem_wait_ld(x);
-    weigh<RUNS, MASKED>(r, c, x, base, unit, sum0, sum1, w);
-    tmem_st16(s_at + c / 2, w);
-  }
-  return sum0 + sum1;
-}
-// Both in one pass, against a reference that the tile may turn out to pass: the
-// weights stay in registers (`w`), and `best` says how far the scores went.
-__device__ __forceinline__ float weigh_ahead(const Row& r, uint32_t s_at, float base, float unit, float& best, uint32_t (&w)[kHalf / 2]) {
-  float sum0 = 0.f, sum1 = 0.f;
-  best = -INFINITY;
-#pragma unroll
-  for (int c = 0; c < kHalf; c += 32) {
-    float x[32];
-    uint32_t part[16];
-    tmem_ld32(s_at + c, x);
-    tmem_wait_ld(x);
-    best = fmaxf(best, largest<true, false>(r, c, x));
-    weigh<true, false>(r, c, x, base, unit, sum0, sum1, part);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[c / 2 + i] = part[i];
-  }
+  best = most * r.unscale;
   return sum0 + sum1;
 }
 __device__ __forceinline__ void store_weights(uint32_t s_at, const uint32_t (&w)[kHalf / 2]) {
@@ -325,10 +281,17 @@ __device__ __forceinline__ void store_weights(uint32_t s_at, const uint32_t (&w)
     tmem_st16(s_at + c, part);
   }
 }
-// Where the value scales of a tile are far from the first's: the largest score
-// times value scale, and the weights against a reference of their own.
-__device__ __forceinline__ float heaviest_of_half(const Row& r, uint32_t s_at) {
-  float most = -INFINITY;
+// Any half, in two passes and little code (what runs seldom is fetched from far):
+// first the largest score, and where value scales are far from the first tile's
+// the largest of scores with log2 of their values' scales; then the weights.
+__device__ __forceinline__ float score_of(const Row& r, int i, float x, float& vs) {
+  vs = r.v[i];
+  const float t = x * r.k[i] * r.unscale;
+  return i >= r.low && i < r.high && !(vs < 0.f) ? t : -INFINITY;
+}
+__device__ __forceinline__ float largest_of_half(const Row& r, uint32_t s_at, bool usual, float& heaviest) {
+  float best = -INFINITY;
+  heaviest = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < kHalf; c += 16) {
     float x[16];
@@ -336,31 +299,34 @@ __device__ __forceinline__ float heaviest_of_half(const Row& r, uint32_t s_at) {
     tmem_wait_ld(x);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float vs = r.v[c + i];
-      const float u = x[i] * r.k[c + i] * r.unscale + log2f(vs);
-      if (c + i >= r.low && c + i < r.high && !(vs < 0.f)) most = fmaxf(most, u);
+      float vs;
+      const float t = score_of(r, c + i, x[i], vs);
+      best = fmaxf(best, t);
+      if (!usual) heaviest = fmaxf(heaviest, t + __log2f(vs));
     }
   }
-  return most;
+  return best;
 }
-__device__ __forceinline__ float weigh_heavy_half(const Row& r, uint32_t s_at, float base, float reference) {
+__device__ __forceinline__ float weigh_half(const Row& r, uint32_t s_at, float base, float unit, bool usual, float reference) {
   float sum = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < kHalf; c += 32) {
-    float x[32];
-    uint32_t w[16];
-    tmem_ld32(s_at + c, x);
+  for (int c = 0; c < kHalf; c += 16) {
+    float x[16];
+    uint32_t w[8];
+    tmem_ld16(s_at + c, x);
     tmem_wait_ld(x);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float vs = r.v[c + i], t = x[i] * r.k[c + i] * r.unscale;
-      const bool counts = c + i >= r.low && c + i < r.high && !(vs < 0.f);
-      sum += counts ? exp2_approx(t - base) : 0.f;
-      x[i] = counts ? exp2_approx(t + log2f(vs) - reference + kShift) : 0.f;
+    for (int i = 0; i < 16; ++i) {
+      float vs;
+      const float t = score_of(r, c + i, x[i], vs);
+      const float p = exp2_approx(t - base);
+      sum += p;
+      x[i] = usual ? p * (vs * unit) : exp2_approx(t + __log2f(vs) - reference + kShift);
+      if (t == -INFINITY) x[i] = 0.f;  // whatever its value's scale is
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack_f16x2(x[2 * i], x[2 * i + 1]);
-    tmem_st16(s_at + c / 2, w);
+    for (int i = 0; i < 8; ++i) w[i] = pack_f16x2(x[2 * i], x[2 * i + 1]);
+    tmem_st8(s_at + c / 2, w);
   }
   return sum;
 }
@@ -441,15 +407,23 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     for (; going && next_fragment(seq); ++seq) {
       const Fragment& f = m.ring[seq % kRing];
       const int32_t halves = f.halves(slot);
-      const int32_t r = f.split ? row_in_slot : slot * kSlotRows + row_in_slot;  // of the block
+      const int32_t r = f.split ? row_in_slot : slot * kSlotRows + row_in_slot;  // this lane's, of the block
       const bool used = r < f.rows;
       const bool warp_used = __any_sync(kAllLanes, used);
-      const int32_t row = f.row + (used ? r : 0);
-      const int32_t within = static_cast<int32_t>(fastdiv(row, a.per_kv));
-      const int32_t token = f.token + within;
-      const int32_t head = f.kv * a.heads_per_kv + row - within * a.heads_per_kv;
+      const int32_t row = f.row + (used ? r : 0), within = static_cast<int32_t>(fastdiv(row, a.per_kv));
+      const int32_t token = f.token + within, head = f.kv * a.heads_per_kv + row - within * a.heads_per_kv;
+      // Where its part of the result goes.
+      int64_t place = static_cast<int64_t>(token) * a.heads + head;
+      if (f.first > 0) {
+        place = a.at.starts + blockIdx.x * static_cast<int64_t>(kBlockRows) + slot * kSlotRows + row_in_slot;
+      } else if (f.split && slot == 1) {
+        place = a.at.copies + static_cast<int64_t>(f.extra) * a.cache.kv_heads + static_cast<int64_t>(f.kv) * f.rows + r;
+      } else if (f.prefix == 0) {
+        place += static_cast<int64_t>(a.rows) * a.heads;
+      }
+      float result = -INFINITY, by_end = 0.f;  // log-sum-exp, factor of the outputs
       if (halves > 0) {
-        // ---- the row's queries, and how far it sees
+        // ---- the row's queries, in fp16, and how far it sees
         float unscale = 0.f;
         int32_t limit = 0;
         if (warp_used) {
@@ -467,8 +441,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
                                            __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
           }
           most = max(most & 0xffffu, most >> 16);
-          const float largest = widen<T>(most).x;
-          const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -100), 127);
+          const float most_value = widen<T>(most).x;
+          const int e = min(max(static_cast<int>(__float_as_uint(most_value) >> 23) - 127, -100), 127);
           unscale = __uint_as_float(static_cast<uint32_t>(e - 8 + 127) << 23);
           const float by = __uint_as_float(static_cast<uint32_t>(8 - e + 127) << 23) * a.q_sign;
           const uint32_t to = smem_addr(m.q[slot]);
@@ -480,13 +454,12 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           }
         }
         const int32_t all_see = __reduce_min_sync(kAllLanes, used ? min(limit, f.key_end) : 0x7fffffff);
-        fence_proxy_async();
         arrive(&m.queries[slot]);
 
         float top = -INFINITY, total = 0.f, reference = -INFINITY;
         int32_t exponent = 0;
-        bool known = false, usual = true, plain = false;
-        const int32_t stride = f.split ? 2 : 1, first_tile = f.split ? slot : 0;  // of the fragment's tiles
+        bool known = false, usual = true, pages = false;
+        const int32_t stride = f.stride(), first_tile = f.own(slot);
         const int32_t key_first = f.key_first, seen = min(limit, f.key_end);
         int32_t first_key = f.key_begin + (f.first + first_tile) * kSharedTile;  // of the half
         const Note* note = nullptr;
@@ -511,69 +484,59 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
                 usual = false;
                 reference = top + exponent;
               }
-              // Nothing of the tile is hidden from any of the warp's rows.
-              plain = usual && a.runs && all.z == 0 && key_first <= first_key && all_see - first_key >= kSharedTile;
+              pages = usual && a.runs && all.z == 0;
             }
+            // Nothing of the half is hidden from any of the warp's rows.
+            const bool plain = pages && key_first <= first_key && all_see - first_key >= kHalf;
             const Row at{note->k + half * kHalf, note->v + half * kHalf, unscale, key_first - first_key, seen - first_key};
             const float unit = __uint_as_float(static_cast<uint32_t>(127 + kShift - exponent) << 23);
-            // ---- most tiles leave the references where they are
-            bool stays = plain && step > 0;
-            if (stays) {
-              uint32_t w[kHalf / 2];
-              float best;
-              const float sum = weigh_ahead(at, s_at, top, unit, best, w);
-              stays = __all_sync(kAllLanes, best <= top + kReach || best != best);
-              if (stays) {
-                total += sum;
-                store_weights(s_at, w);
+            uint32_t w[kHalf / 2];
+            float sum = 0.f;
+            for (bool again = true; again;) {
+              float best, heaviest = -INFINITY;
+              if (plain) {
+                sum = weigh_plain(at, s_at, top == -INFINITY ? 0.f : top, unit, best, w);
+              } else {
+                best = largest_of_half(at, s_at, usual, heaviest);
               }
-            }
-            if (!stays) {
-            // ---- the largest score, and the largest weight where values' scales count
-            const float best = plain    ? largest_of_half<true, false>(at, s_at)
-                               : a.runs ? largest_of_half<true, true>(at, s_at)
-                                        : largest_of_half<false, true>(at, s_at);
-            const float heaviest = usual ? -INFINITY : heaviest_of_half(at, s_at);
-            // ---- references move, with the sum and the outputs
-            const bool up = best > top + kReach || (top == -INFINITY && best > top);
-            const bool heavier = !usual && (heaviest > reference + kReach || (reference == -INFINITY && heaviest > reference));
-            if (__any_sync(kAllLanes, up || heavier)) {
-              const float to = up ? best : top;
-              const float down = up ? exp2f(top - to) : 1.f;
-              total *= down;
-              top = to;
-              float by = down;
-              if (!usual) {
-                by = heavier ? exp2f(reference - heaviest) : 1.f;
-                if (heavier) reference = heaviest;
-              }
-              if (step > 0) {
-                // The half before may still be added up.
-                if (!wait(&m.done[slot][half ^ 1], (parity >> (half ^ 1) & 1) ^ 1)) {
-                  going = false;
-                  break;
+              // References seldom move; then the sum and the outputs do, and a plain
+              // half is weighed once more.
+              const bool up = best > top + kReach, heavier = heaviest > reference + kReach;
+              const bool moves = __any_sync(kAllLanes, up || heavier);
+              if (moves) {
+                float by = 1.f;
+                if (up) {
+                  by = exp2f(top - best);
+                  total *= by;
+                  top = best;
                 }
-                tc_fence_after();
+                if (!usual) {
+                  by = heavier ? exp2f(reference - heaviest) : 1.f;
+                  if (heavier) reference = heaviest;
+                }
+                if (step > 0) {
+                  // The half before may still be added up.
+                  if (!(going = wait(&m.done[slot][half ^ 1], (parity >> (half ^ 1) & 1) ^ 1))) break;
+                  tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < DIM; c += 16) {
-                  float o[16];
-                  tmem_ld16(o_at + c, o);
-                  tmem_wait_ld(o);
+                  for (int c = 0; c < DIM; c += 16) {
+                    float o[16];
+                    tmem_ld16(o_at + c, o);
+                    tmem_wait_ld(o);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) o[i] *= by;
-                  tmem_st16(o_at + c, o);
+                    for (int i = 0; i < 16; ++i) o[i] *= by;
+                    tmem_st16(o_at + c, o);
+                  }
                 }
               }
+              again = plain && moves;
             }
-            // ---- the weights
-            const float base = top == -INFINITY ? 0.f : top;
-            if (usual) {
-              total += plain    ? weigh_half<true, false>(at, s_at, base, unit)
-                       : a.runs ? weigh_half<true, true>(at, s_at, base, unit)
-                                : weigh_half<false, true>(at, s_at, base, unit);
+            if (!going) break;
+            if (plain) {
+              total += sum;
+              store_weights(s_at, w);
             } else {
-              total += weigh_heavy_half(at, s_at, base, reference == -INFINITY ? 0.f : reference);
-            }
+              total += weigh_half(at, s_at, top == -INFINITY ? 0.f : top, unit, usual, reference == -INFINITY ? 0.f : reference);
             }
             tmem_wait_st();
           }
@@ -581,46 +544,34 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           arrive(&m.weights[slot][half]);
           first_key += half == 0 ? kHalf : stride * kSharedTile - kHalf;
         }
-        // (That the turns before the last are over follows from the last scores.)
-        if (going) going = wait(&m.done[slot][(halves - 1) & 1], (parity >> ((halves - 1) & 1) & 1) ^ 1);
         if (!going) break;
+        // 2^(reference - top - kShift) / total, in the usual case 2^(E - kShift) / total.
+        const float lift = usual ? static_cast<float>(exponent) : reference - top;
+        by_end = total > 0.f || total != total ? exp2f(lift - kShift) / total : 0.f;
+        result = total == 0.f ? -INFINITY : top + log2f(total);
+      }
+      if (used) a.part_lse()[place] = result;
+      if (halves > 0) {
+        // (That the turns before the last are over follows from the last scores.)
+        const int half = (halves - 1) & 1;
+        if (!wait(&m.done[slot][half], (parity >> half & 1) ^ 1)) break;
         tc_fence_after();
-        // ---- the fragment's outputs
         if (warp_used) {
-          const int64_t pairs = static_cast<int64_t>(a.rows) * a.heads, own_place = static_cast<int64_t>(token) * a.heads + head;
-          int64_t place;
-          if (f.first > 0) {
-            place = a.at.starts + blockIdx.x * static_cast<int64_t>(kBlockRows) + slot * kSlotRows + row_in_slot;
-          } else if (f.split && slot == 1) {
-            place = a.at.copies + static_cast<int64_t>(f.extra) * a.cache.kv_heads + static_cast<int64_t>(f.kv) * f.rows + r;
-          } else {
-            place = f.prefix != 0 ? own_place : pairs + own_place;
-          }
-          // 2^(reference - top - kShift) / total, in the usual case 2^(E - kShift) / total.
-          const float lift = usual ? static_cast<float>(exponent) : reference - top;
-          const float by = total > 0.f || total != total ? exp2f(lift - kShift) / total : 0.f;
           float4* out = reinterpret_cast<float4*>(a.part_out() + place * DIM);
 #pragma unroll 1
-          for (int c = 0; c < DIM; c += 16) {
-            float o[16];
-            tmem_ld16(o_at + c, o);
+          for (int c = 0; c < DIM; c += 32) {
+            float o[32];
+            tmem_ld32(o_at + c, o);
             tmem_wait_ld(o);
             if (used) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                out[c / 4 + i] = make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
+              for (int i = 0; i < 8; ++i) {
+                out[c / 4 + i] = make_float4(o[4 * i] * by_end, o[4 * i + 1] * by_end, o[4 * i + 2] * by_end, o[4 * i + 3] * by_end);
               }
             }
           }
-          if (used) a.part_lse()[place] = total == 0.f ? -INFINITY : top + log2f(total);
         }
         tc_fence_before();
-      } else if (used) {
-        // A fragment of one tile, all of it the other slot's.
-        const int64_t place = f.first > 0 ? a.at.starts + blockIdx.x * static_cast<int64_t>(kBlockRows) + slot * kSlotRows + row_in_slot
-                                          : a.at.copies + static_cast<int64_t>(f.extra) * a.cache.kv_heads +
-                                                static_cast<int64_t>(f.kv) * f.rows + r;
-        a.part_lse()[place] = -INFINITY;
       }
       tiles_before += f.last - f.first;
       free_fragment(seq);
@@ -794,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     for (; going && next_fragment(seq); ++seq) {
       const Fragment& f = m.ring[seq % kRing];
       const int32_t tiles = f.last - f.first, halves = f.halves(slot);
-      const uint32_t own = tiles_before + (f.split != 0 ? slot : 0), stride = f.split != 0 ? 2 : 1;
+      const uint32_t own = tiles_before + f.own(slot), stride = f.stride();
       free_fragment(seq);
       // Scores run two halves ahead of the outputs, so that the softmax finds the
       // next ones when it is through with a half.
@@ -823,6 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
           if (i == -2) {
             if (!(going = wait(&m.queries[slot], queries_parity))) break;
             queries_parity ^= 1;
+            fence_proxy_async();  // (the softmax would wait for its stores to global memory)
             tc_fence_after();
           }
           const uint64_t kd = k_desc + stage * kTileStep + half * kHalfStep;

@@ -5,11 +5,12 @@
 // sequence's own tokens with its own. Its rows are its (query, head) pairs of
 // one cache head, token by token, in blocks of 256; an item is one block of rows
 // over the segment's keys, for every cache head. Items' tiles of 128 keys, item
-// by item and head by head, are one line of units (with kStart more for each
-// item and head, for what its start and end cost), which the grid's CTAs cut
-// into equal parts, by the lengths that stand on the device. A CTA's share of an
-// item and head is a fragment, whose outputs and log-sum-exps go to the
-// workspace; a second kernel joins each row's.
+// by item and head by head, are one line of units of time (with some more for
+// each item and head, for its start and end), which the grid's CTAs cut into
+// equal parts, by the lengths that stand on the device. A tile is the CTA's in
+// whose part its first unit lies. A CTA's share of an item and head is a
+// fragment, whose outputs and log-sum-exps go to the workspace; a second kernel
+// joins each row's.
 #pragma once
 
 #include "paged.cuh"
@@ -19,8 +20,7 @@ namespace silkern {
 constexpr int kSharedTile = 128;   // keys
 constexpr int kSlotRows = 128;     // rows of a softmax warpgroup
 constexpr int kBlockRows = 2 * kSlotRows;
-constexpr int kStart = 3;          // units for an item's start and end
-constexpr int kLeastUnits = 4;     // of a CTA
+constexpr int kLeastUnits = 16;    // of a CTA: a tile of every sort at least
 constexpr int kMostCtas = 148;     // one to an SM
 
 struct SharedHeader {
@@ -102,7 +102,14 @@ struct SharedArgs {
   }
 };
 
-__device__ __forceinline__ int32_t units_of(int32_t tiles) { return tiles > 0 ? tiles + kStart : 0; }
+// Units of a tile, and of an item's start and end, by its rows: about 700 cycles
+// each, as measured. Up to 128 rows the slots take turns with the tiles, and one's
+// start hides behind the other's tiles.
+__device__ __forceinline__ int32_t units_of_tile(int32_t rows) { return rows <= kSlotRows ? 4 : 5; }
+__device__ __forceinline__ int32_t units_of_start(int32_t rows) { return rows <= kSlotRows ? 8 : 24; }
+__device__ __forceinline__ int64_t units_of(int32_t tiles, int32_t rows) {
+  return tiles > 0 ? units_of_start(rows) + static_cast<int64_t>(tiles) * units_of_tile(rows) : 0;
+}
 
 // The last i in [0, n) with at(i) <= x, for at that ascends from at(0) <= x.
 template <typename F>
