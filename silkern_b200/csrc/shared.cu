@@ -185,39 +185,32 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
 // that went on with it.
 struct Parts {
   int64_t first, copy, next;  // partial rows; copy -1: none
-  int64_t stride;             // from a CTA's to the next one's
   int32_t count;              // of fragments
   int32_t both;               // 1: the two slots have a copy each
 };
 
-__device__ __forceinline__ Parts find_parts(const SharedArgs& a, int32_t segment, int32_t token, int32_t head, int64_t place) {
-  Parts p{0, -1, 0, kBlockRows, 0, 0};
-  const int32_t first = load_int(a.first() + segment);
-  if (first < 0) return p;
-  const int32_t kv = static_cast<int32_t>(fastdiv(head, a.per_kv));
-  const int32_t seg_token = load_int(&a.item(first)->token);
-  const int32_t row = (token - seg_token) * a.heads_per_kv + (head - kv * a.heads_per_kv);
-  const SharedItem* it = a.item(first + row / kBlockRows);
-  const int32_t tiles = load_int(&it->tiles);
-  if (tiles == 0) return p;
-  const int32_t r = row % kBlockRows, rows = load_int(&it->rows);
-  const int64_t share = __ldcg(&a.header()->share);
-  const int64_t zero = __ldcg(&it->begin) * a.cache.kv_heads + kv * units_of(tiles, rows) + units_of_start(rows);
+// `first`: the segment's first item, `row` the row's number in the segment.
+__device__ __forceinline__ Parts find_parts(const SharedArgs& a, int32_t first, int32_t row, int32_t kv, int64_t share, int64_t place) {
+  const SharedItem* it = a.item(max(first, 0) + row / kBlockRows);
+  // (Loads that wait for one another cost more than some too many.)
+  const int32_t tiles = load_int(&it->tiles), rows = load_int(&it->rows), extra = load_int(&it->extra);
+  const int64_t begin = __ldcg(&it->begin);
+  const int32_t r = row % kBlockRows;
+  const int64_t zero = begin * a.cache.kv_heads + kv * units_of(tiles, rows) + units_of_start(rows);
   const int64_t c0 = zero / share, c1 = (zero + static_cast<int64_t>(tiles - 1) * units_of_tile(rows)) / share;
-  p.count = static_cast<int32_t>(c1 - c0 + 1);
-  p.first = place;
-  p.next = a.at.starts + (c0 + 1) * kBlockRows + r;
+  Parts p{place, -1, a.at.starts + (c0 + 1) * kBlockRows + r, static_cast<int32_t>(c1 - c0 + 1), 0};
   if (rows <= kSlotRows) {
     p.both = 1;
-    p.copy = a.at.copies + static_cast<int64_t>(load_int(&it->extra)) * a.cache.kv_heads + static_cast<int64_t>(kv) * rows + r;
+    p.copy = a.at.copies + static_cast<int64_t>(extra) * a.cache.kv_heads + static_cast<int64_t>(kv) * rows + r;
   }
+  if (first < 0 || tiles <= 0) p.count = 0;
   return p;
 }
 __device__ __forceinline__ int64_t part_at(const Parts& p, int32_t i) {
   const int32_t c = p.both ? i >> 1 : i;
   const bool second = p.both && (i & 1);
   if (c == 0) return second ? p.copy : p.first;
-  return p.next + (c - 1) * p.stride + (second ? kSlotRows : 0);
+  return p.next + (c - 1) * int64_t{kBlockRows} + (second ? kSlotRows : 0);
 }
 
 // WARPS warps to a (query, head): one where there are many of them, eight where
@@ -236,14 +229,17 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant_
   if (pair >= pairs) return;
   const int32_t token = static_cast<int32_t>(pair / a.heads), head = static_cast<int32_t>(pair - static_cast<int64_t>(token) * a.heads);
   if (token < a.cu(0) || token >= a.cu(a.sequences)) return;
+  const int64_t share = __ldcg(&a.header()->share);
+  const int32_t failed = load_int(&a.header()->failed);
+  const int32_t cut_first = a.cut(0), cut_last = a.cut(a.groups);
   const int32_t seq = warp_last_at_most(a.sequences, token, [&](int32_t i) { return a.cu(i); });
-  Parts part[2];
-  part[0] = Parts{0, -1, 0, 0, 0, 0};
-  if (seq >= a.cut(0) && seq < a.cut(a.groups)) {
-    const int32_t group = warp_last_at_most(a.groups, seq, [&](int32_t i) { return a.cut(i); });
-    part[0] = find_parts(a, group, token, head, pair);
-  }
-  part[1] = find_parts(a, a.groups + seq, token, head, pairs + pair);
+  const bool grouped = seq >= cut_first && seq < cut_last;
+  const int32_t group = grouped ? warp_last_at_most(a.groups, seq, [&](int32_t i) { return a.cut(i); }) : 0;
+  const int32_t own_first = load_int(a.first() + a.groups + seq), own_token = a.cu(seq);
+  const int32_t group_first = grouped ? load_int(a.first() + group) : -1, group_token = grouped ? a.cu(a.cut(group)) : token;
+  const int32_t kv = static_cast<int32_t>(fastdiv(head, a.per_kv)), in_kv = head - kv * a.heads_per_kv;
+  const Parts part[2] = {find_parts(a, group_first, (token - group_token) * a.heads_per_kv + in_kv, kv, share, pair),
+                         find_parts(a, own_first, (token - own_token) * a.heads_per_kv + in_kv, kv, share, pairs + pair)};
   const int32_t n0 = part[0].count << part[0].both, n = n0 + (part[1].count << part[1].both);
   auto place = [&](int32_t i) { return i < n0 ? part_at(part[0], i) : part_at(part[1], i - n0); };
   float top = -INFINITY;
@@ -316,7 +312,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant_
     }
   }
   float inverse = total == 0.f ? 0.f : 1.f / total, lse = (top + log2f(total)) * 0.69314718055994531f;
-  if (load_int(&a.header()->failed) != 0) inverse = lse = NAN;
+  if (failed != 0) inverse = lse = NAN;
   T* out = static_cast<T*>(a.out) + token * a.out_row + head * a.out_head + lane * kEach;
   T rounded[kEach];
 #pragma unroll
