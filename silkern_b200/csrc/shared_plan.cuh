@@ -102,11 +102,11 @@ struct SharedArgs {
   }
 };
 
-// Units of a tile, and of an item's start and end, by its rows: about 700 cycles
+// Units of a tile, and of an item's start and end, by its rows: about 530 cycles
 // each, as measured. Up to 128 rows the slots take turns with the tiles, and one's
 // start hides behind the other's tiles.
-__device__ __forceinline__ int32_t units_of_tile(int32_t rows) { return rows <= kSlotRows ? 4 : 5; }
-__device__ __forceinline__ int32_t units_of_start(int32_t rows) { return rows <= kSlotRows ? 8 : 24; }
+__device__ __forceinline__ int32_t units_of_tile(int32_t rows) { return rows <= kSlotRows ? 6 : 8; }
+__device__ __forceinline__ int32_t units_of_start(int32_t rows) { return rows <= kSlotRows ? 19 : 46; }
 __device__ __forceinline__ int64_t units_of(int32_t tiles, int32_t rows) {
   return tiles > 0 ? units_of_start(rows) + static_cast<int64_t>(tiles) * units_of_tile(rows) : 0;
 }
