@@ -15,7 +15,7 @@ namespace silkern {
 
 namespace {
 
-constexpr int kRotateThreads = 256;
+constexpr int kRotateThreads = 256;  // at most
 constexpr int kMostColumns = SILKERN_MOST_COLUMNS;
 
 struct HeadSet {
@@ -32,7 +32,9 @@ struct RotateArgs {
   const float* frequencies;
   int32_t tokens, dim, pairs, start;  // pairs: of rotary columns, the first in column `start`
   int32_t all_heads;                  // of both sets
-  int32_t group, slots;               // lanes to a head; pieces of 8 columns that pair up
+  int32_t normed[2];                  // the heads [normed[0], normed[1]) of them have a norm
+  int32_t group;                      // lanes to a normed head
+  FastDiv slots;                      // by a head's slots of two pieces of 8 columns
   int32_t heads_a_cta;
   bool interleaved, weights_f32;
   float amplitude, eps;
@@ -85,10 +87,10 @@ __device__ __forceinline__ float2 turn(int32_t position, float frequency, float 
   return make_float2(c * amplitude, s * amplitude);
 }
 
-// The place in a head's columns of a thread's two pieces of 8. The first
-// pairs / 8 slots of a head rotate in halves: the piece and the one that it is
-// paired with. Other slots hold pieces half the slots apart, in the order that
-// leaves those out; -1: none.
+// The place in a head's columns of a slot's two pieces of 8. The first pairs / 8
+// slots of a head rotate in halves: the piece and the one that it is paired with.
+// Other slots hold pieces half the slots apart, in the order that leaves those
+// out; -1: none.
 struct Pieces {
   int32_t a, b;
   bool rotates;  // a with b
@@ -96,7 +98,7 @@ struct Pieces {
 __device__ __forceinline__ Pieces pieces_of(const RotateArgs& g, int32_t slot) {
   const int32_t total = g.dim >> 3;
   if (g.interleaved) {
-    const int32_t b = slot + g.slots;
+    const int32_t b = slot + static_cast<int32_t>(g.slots.divisor);
     return {slot * 8, b < total ? b * 8 : -1, false};
   }
   const int32_t turned = g.pairs >> 3, first = g.start >> 3;
@@ -106,126 +108,176 @@ __device__ __forceinline__ Pieces pieces_of(const RotateArgs& g, int32_t slot) {
   return {place(plain), plain + half < rest ? place(plain + half) : -1, false};
 }
 
-// One CTA for a token and up to heads_a_cta of its heads, `group` lanes to a
-// head, N slots of two pieces of 8 columns to a lane. The token's cos and sin
-// are worked out once, for all of the CTA's heads, and the weights widened,
-// while the first heads are on their way. Every element is read and written
-// once.
+struct Tables {
+  float cos[kMostColumns / 2], sin[kMostColumns / 2];
+  float weight[2][kMostColumns];
+};
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void rotate_slot(const RotateArgs& g, const Tables& t, int32_t slot, const Pieces& at, float (&a)[8],
+                                            float (&b)[8]) {
+  if (at.rotates) {
+    float c[8], s[8];
+    load8(t.cos + slot * 8, c);
+    load8(t.sin + slot * 8, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = a[i], y = b[i];
+      a[i] = x * c[i] - y * s[i];
+      b[i] = y * c[i] + x * s[i];
+    }
+  } else if (g.interleaved) {
+    auto turn = [&](int32_t column, float (&x)[8]) {
+      const int32_t pair = (column - g.start) >> 1;
+      if (column < g.start || pair >= g.pairs) return;
+      const float4 c = *reinterpret_cast<const float4*>(t.cos + pair), s = *reinterpret_cast<const float4*>(t.sin + pair);
+      const float cs[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x0 = x[2 * i], x1 = x[2 * i + 1];
+        x[2 * i] = x0 * cs[i] - x1 * ss[i];
+        x[2 * i + 1] = x1 * cs[i] + x0 * ss[i];
+      }
+    };
+    turn(at.a, a);
+    if (at.b >= 0) turn(at.b, b);
+  }
+}
+
+// One CTA for a token and up to heads_a_cta of its heads. The token's cos and sin
+// are worked out once, for all of the CTA's heads, and the weights widened. Heads
+// with a norm take `group` lanes each and N slots a lane; the slots of the others
+// are dealt out one by one, four a thread on their way at once. Every element is
+// read and written once, 16 bytes at a time.
 template <typename T, int N>
 __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_constant__ RotateArgs g) {
-  __shared__ __align__(16) float table[2][kMostColumns / 2];  // cos, sin
-  __shared__ __align__(16) float weights[2][kMostColumns];
+  __shared__ __align__(16) Tables tables;
   pdl_wait();
   pdl_launch_dependents();
-  const int32_t token = blockIdx.x;
-  const int32_t lane = threadIdx.x % g.group, team = threadIdx.x / g.group, teams = kRotateThreads / g.group;
+  const int32_t token = blockIdx.x, threads = blockDim.x;
   const int32_t first = blockIdx.y * g.heads_a_cta, last = min(first + g.heads_a_cta, g.all_heads);
-  auto set_of = [&](int32_t head) -> const HeadSet& { return g.set[head < g.set[0].heads ? 0 : 1]; };
+  const int32_t q_heads = g.set[0].heads;
+  auto source = [&](int32_t head) {
+    const HeadSet& s = g.set[head < q_heads ? 0 : 1];
+    return static_cast<const T*>(s.in) + token * s.in_token + (head < q_heads ? head : head - q_heads) * s.in_head;
+  };
+  auto target = [&](int32_t head) {
+    const HeadSet& s = g.set[head < q_heads ? 0 : 1];
+    return static_cast<T*>(s.out) + token * s.out_token + (head < q_heads ? head : head - q_heads) * s.out_head;
+  };
+  const int32_t normed_first = max(first, g.normed[0]), normed_last = min(last, g.normed[1]);
+  const int32_t lane = threadIdx.x % g.group, team = threadIdx.x / g.group, teams = threads / g.group;
+  Pieces at[N];
   uint4 raw[N][2];
   auto fetch = [&](int32_t head) {
-    const HeadSet& s = set_of(head);
-    const int32_t h = head < g.set[0].heads ? head : head - g.set[0].heads;
-    const T* p = static_cast<const T*>(s.in) + token * s.in_token + h * s.in_head;
+    const T* p = source(head);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int32_t slot = lane + n * g.group;
       raw[n][0] = raw[n][1] = make_uint4(0u, 0u, 0u, 0u);
-      if (slot < g.slots) {
-        const Pieces at = pieces_of(g, slot);
-        raw[n][0] = load_wide(p + at.a);
-        if (at.b >= 0) raw[n][1] = load_wide(p + at.b);
-      }
+      if (at[n].a >= 0) raw[n][0] = load_wide(p + at[n].a);
+      if (at[n].b >= 0) raw[n][1] = load_wide(p + at[n].b);
     }
   };
-  int32_t head = first + team;
-  if (head < last) fetch(head);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int32_t slot = lane + n * g.group;
+    at[n] = slot < static_cast<int32_t>(g.slots.divisor) ? pieces_of(g, slot) : Pieces{-1, -1, false};
+  }
+  int32_t head = normed_first + team;
+  if (head < normed_last) fetch(head);
   const int32_t position = g.positions[token];
-  for (int32_t i = threadIdx.x; i < g.pairs; i += kRotateThreads) {
+  for (int32_t i = threadIdx.x; i < g.pairs; i += threads) {
     const float2 t = turn(position, g.frequencies[i], g.amplitude);
-    table[0][i] = t.x;
-    table[1][i] = t.y;
+    tables.cos[i] = t.x;
+    tables.sin[i] = t.y;
   }
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    if (k == 0 ? first >= g.set[0].heads : last <= g.set[0].heads) continue;
-    for (int32_t i = threadIdx.x; i < g.set[k].norm; i += kRotateThreads) {
-      weights[k][i] = g.weights_f32 ? static_cast<const float*>(g.set[k].weight)[i]
-                                    : static_cast<float>(static_cast<const T*>(g.set[k].weight)[i]);
+    if (k == 0 ? first >= q_heads : last <= q_heads) continue;
+    for (int32_t i = threadIdx.x; i < g.set[k].norm; i += threads) {
+      tables.weight[k][i] = g.weights_f32 ? static_cast<const float*>(g.set[k].weight)[i]
+                                          : static_cast<float>(static_cast<const T*>(g.set[k].weight)[i]);
     }
   }
   __syncthreads();
-  // Lanes of a head share a warp; a warp's heads run out together or not, so
-  // that every lane takes part in the exchanges.
-  for (int32_t base = first; base < last; base += teams, head += teams) {
-    const bool live = head < last;
-    const HeadSet& s = set_of(live ? head : first);
-    const int k = &s == &g.set[0] ? 0 : 1;
-    if (base > first && live) fetch(head);
-    float x[N][2][8];
+  // Lanes of a head share a warp; all of a warp goes as often round, so that every
+  // lane takes part in the exchanges.
+  for (int32_t base = normed_first; base < normed_last; base += teams, head += teams) {
+    const bool live = head < normed_last;
+    const int k = live && head >= q_heads ? 1 : 0;
+    const int32_t norm = g.set[k].norm;
+    float x[N][2][8], sum = 0.f;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      unpack8<T>(raw[n][0], x[n][0]);
-      unpack8<T>(raw[n][1], x[n][1]);
-    }
-    if (g.set[0].norm | g.set[1].norm) {
-      float sum = 0.f;
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int32_t slot = lane + n * g.group;
-        if (slot >= g.slots) continue;
-        const Pieces at = pieces_of(g, slot);
+      for (int e = 0; e < 2; ++e) {
+        unpack8<T>(raw[n][e], x[n][e]);
+        const int32_t column = e == 0 ? at[n].a : at[n].b;
+        if (column >= 0 && column < norm) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (at.a + i < s.norm) sum = fmaf(x[n][0][i], x[n][0][i], sum);
-          if (at.b >= 0 && at.b + i < s.norm) sum = fmaf(x[n][1][i], x[n][1][i], sum);
-        }
-      }
-      for (int d = g.group >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, d);
-      const float r = s.norm > 0 ? rsqrtf(sum / static_cast<float>(s.norm) + g.eps) : 1.f;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int32_t slot = lane + n * g.group;
-        if (slot >= g.slots) continue;
-        const Pieces at = pieces_of(g, slot);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (at.a + i < s.norm) x[n][0][i] *= r * weights[k][at.a + i];
-          if (at.b >= 0 && at.b + i < s.norm) x[n][1][i] *= r * weights[k][at.b + i];
+          for (int i = 0; i < 8; ++i) sum = fmaf(x[n][e][i], x[n][e][i], sum);
         }
       }
     }
+    if (head + teams < normed_last) fetch(head + teams);
+    for (int d = g.group >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, d);
     if (!live) continue;
-    const int32_t h = head < g.set[0].heads ? head : head - g.set[0].heads;
-    T* out = static_cast<T*>(s.out) + token * s.out_token + h * s.out_head;
+    const float r = rsqrtf(sum / static_cast<float>(norm) + g.eps);
+    T* out = target(head);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int32_t slot = lane + n * g.group;
-      if (slot >= g.slots) continue;
-      const Pieces at = pieces_of(g, slot);
-      if (at.rotates) {
+      if (at[n].a < 0) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float c = table[0][slot * 8 + i], z = table[1][slot * 8 + i];
-          const float a = x[n][0][i], b = x[n][1][i];
-          x[n][0][i] = a * c - b * z;
-          x[n][1][i] = b * c + a * z;
-        }
-      } else if (g.interleaved) {
+      for (int e = 0; e < 2; ++e) {
+        const int32_t column = e == 0 ? at[n].a : at[n].b;
+        if (column >= 0 && column < norm) {
+          float w[8];
+          load8(tables.weight[k] + column, w);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int32_t at_pair = ((e == 0 ? at.a : at.b) - g.start) >> 1;
-          if ((e == 1 && at.b < 0) || at_pair < 0 || at_pair >= g.pairs) continue;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float c = table[0][at_pair + i], z = table[1][at_pair + i];
-            const float a = x[n][e][2 * i], b = x[n][e][2 * i + 1];
-            x[n][e][2 * i] = a * c - b * z;
-            x[n][e][2 * i + 1] = b * c + a * z;
-          }
+          for (int i = 0; i < 8; ++i) x[n][e][i] *= r * w[i];
         }
       }
-      *reinterpret_cast<uint4*>(out + at.a) = pack8<T>(x[n][0]);
-      if (at.b >= 0) *reinterpret_cast<uint4*>(out + at.b) = pack8<T>(x[n][1]);
+      rotate_slot(g, tables, lane + n * g.group, at[n], x[n][0], x[n][1]);
+      *reinterpret_cast<uint4*>(out + at[n].a) = pack8<T>(x[n][0]);
+      if (at[n].b >= 0) *reinterpret_cast<uint4*>(out + at[n].b) = pack8<T>(x[n][1]);
+    }
+  }
+  // Heads without a norm: those below normed_first and from normed_last on.
+  const int32_t below = min(last, g.normed[0]) - first, slots = g.slots.divisor;
+  const int32_t before = max(below, 0), behind_first = max(first, g.normed[1]), plain = before + max(last - behind_first, 0);
+  constexpr int kAtOnce = 4;
+  for (int32_t i0 = threadIdx.x; i0 < plain * slots; i0 += kAtOnce * threads) {
+    uint4 ahead[kAtOnce][2];
+    Pieces piece[kAtOnce];
+    int32_t of[kAtOnce], slot[kAtOnce];
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      const int32_t i = i0 + n * threads;
+      ahead[n][0] = ahead[n][1] = make_uint4(0u, 0u, 0u, 0u);
+      piece[n] = Pieces{-1, -1, false};
+      of[n] = slot[n] = 0;
+      if (i < plain * slots) {
+        const int32_t h = static_cast<int32_t>(fastdiv(i, g.slots));
+        slot[n] = i - h * slots;
+        of[n] = h < before ? first + h : behind_first + h - before;
+        piece[n] = pieces_of(g, slot[n]);
+        const T* p = source(of[n]);
+        ahead[n][0] = load_wide(p + piece[n].a);
+        if (piece[n].b >= 0) ahead[n][1] = load_wide(p + piece[n].b);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      if (piece[n].a < 0) continue;
+      float a[8], b[8];
+      unpack8<T>(ahead[n][0], a);
+      unpack8<T>(ahead[n][1], b);
+      rotate_slot(g, tables, slot[n], piece[n], a, b);
+      T* out = target(of[n]);
+      *reinterpret_cast<uint4*>(out + piece[n].a) = pack8<T>(a);
+      if (piece[n].b >= 0) *reinterpret_cast<uint4*>(out + piece[n].b) = pack8<T>(b);
     }
   }
 }
@@ -285,13 +337,7 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_narrow_kernel(const __g
 
 template <typename T>
 void (*rotate_for(int each))(RotateArgs) {
-  switch (each) {
-    case 1: return rotate_kernel<T, 1>;
-    case 2: return rotate_kernel<T, 2>;
-    case 3: return rotate_kernel<T, 3>;
-    case 4: return rotate_kernel<T, 4>;
-    default: return rotate_kernel<T, 5>;
-  }
+  return each == 1 ? rotate_kernel<T, 1> : each == 2 ? rotate_kernel<T, 2> : rotate_kernel<T, 3>;
 }
 
 Place place_of_heads(const void* base, int32_t dim, int64_t tokens, int64_t token, int32_t heads, int64_t head) {
@@ -322,8 +368,12 @@ extern "C" int silkern_rotate_heads_v1(const silkern_heads_v1* q, const silkern_
     if (s.norm_columns < 0 || s.norm_columns > dim) return SILKERN_E_ROTARY;
     if (s.norm_columns > 0 && s.weight == nullptr) return SILKERN_E_NULL;
     g.set[i] = HeadSet{s.in, s.out, s.weight, s.in_token, s.in_head, s.out_token, s.out_head, s.heads, s.norm_columns};
+    if (s.norm_columns > 0) {
+      if (g.normed[1] == 0) g.normed[0] = g.all_heads;
+      g.normed[1] = g.all_heads + s.heads;
+    }
     g.all_heads += s.heads;
-    wide = wide && (s.in_token | s.in_head | s.out_token | s.out_head) % 8 == 0 &&
+    wide = wide && s.norm_columns % 8 == 0 && (s.in_token | s.in_head | s.out_token | s.out_head) % 8 == 0 &&
            (reinterpret_cast<uintptr_t>(s.in) | reinterpret_cast<uintptr_t>(s.out)) % 16 == 0;
   }
   // An output is its own input, element for element, or lies apart from every
@@ -354,31 +404,49 @@ extern "C" int silkern_rotate_heads_v1(const silkern_heads_v1* q, const silkern_
   g.weights_f32 = weights_f32 != 0;
   g.amplitude = amplitude;
   g.eps = eps;
-  int each = 0, teams = kRotateThreads / 32;
+  int each = 1, threads = kRotateThreads;
+  int64_t in_turn = kRotateThreads / 32;  // heads of a CTA at once
+  g.group = 32;
   if (wide) {
-    const int total = dim / 8, turned = g.interleaved ? 0 : pairs / 8;
-    g.slots = turned + (total - 2 * turned + 1) / 2;
-    // Lanes to a head: of the powers of two with at most five slots to a lane,
-    // the one with the fewest slots left empty, and the most lanes among equals.
+    const int total = dim / 8, turned = g.interleaved ? 0 : pairs / 8, slots = turned + (total - 2 * turned + 1) / 2;
+    g.slots = make_fastdiv(static_cast<uint32_t>(slots));
+    // Lanes to a normed head: of the powers of two with at most three slots to a
+    // lane, the one with the fewest slots left empty, and the most lanes among
+    // equals.
     int least = 0;
     for (int group = 32; group >= 1; group >>= 1) {
-      const int n = (g.slots + group - 1) / group;
-      if (n <= 5 && (each == 0 || n * group < least)) {
+      const int n = (slots + group - 1) / group;
+      if (n <= 3 && (least == 0 || n * group < least)) {
         each = n;
         g.group = group;
         least = n * group;
       }
     }
-    teams = kRotateThreads / g.group;
+    in_turn = kRotateThreads / g.group;
   }
   // A token's heads in one CTA, unless few tokens leave SMs without work.
   int64_t parts = 1;
-  while (parts * teams < g.all_heads && parts * tokens < 2 * 148) ++parts;
+  while (parts * in_turn < g.all_heads && parts * tokens < 2 * 148) ++parts;
   g.heads_a_cta = static_cast<int32_t>((g.all_heads + parts - 1) / parts);
   parts = (g.all_heads + g.heads_a_cta - 1) / g.heads_a_cta;
+  const int32_t normed = g.normed[1] - g.normed[0];
+  if (wide && normed > 0) {
+    // As many threads as leave the fewest without a head in the last round (72
+    // heads of 8 lanes: 192 threads, three rounds).
+    const int64_t heads = normed < g.heads_a_cta ? normed : g.heads_a_cta;
+    int64_t best = 0;
+    for (int candidate = kRotateThreads; candidate >= 128; candidate -= 32) {
+      const int64_t teams = candidate / g.group, rounds = (heads + teams - 1) / teams;
+      const int64_t filled = heads * 1000 / (rounds * teams);
+      if (filled > best) {
+        best = filled;
+        threads = candidate;
+      }
+    }
+  }
   void (*fn)(RotateArgs) = type == SILKERN_BF16
                                ? (wide ? rotate_for<__nv_bfloat16>(each) : rotate_narrow_kernel<__nv_bfloat16>)
                                : (wide ? rotate_for<__half>(each) : rotate_narrow_kernel<__half>);
-  return launch_pdl_grid(fn, dim3(static_cast<unsigned>(tokens), static_cast<unsigned>(parts), 1), kRotateThreads, 0, 1,
+  return launch_pdl_grid(fn, dim3(static_cast<unsigned>(tokens), static_cast<unsigned>(parts), 1), threads, 0, 1,
                          static_cast<cudaStream_t>(stream), g);
 }
