@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -35,7 +36,8 @@ struct RotateArgs {
   int32_t normed[2];                  // the heads [normed[0], normed[1]) of them have a norm
   int32_t group;                      // lanes to a normed head
   FastDiv slots;                      // by a head's slots of two pieces of 8 columns
-  int32_t heads_a_cta;
+  int32_t heads_a_cta, tokens_a_cta;  // all heads where there are several tokens
+  FastDiv by_normed, by_plain;        // then: by a token's normed heads, by its other heads' slots
   bool interleaved, weights_f32;
   float amplitude, eps;
 };
@@ -116,12 +118,12 @@ __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
   const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
-__device__ __forceinline__ void rotate_slot(const RotateArgs& g, const Tables& t, int32_t slot, const Pieces& at, float (&a)[8],
+__device__ __forceinline__ void rotate_slot(const RotateArgs& g, const Tables& t, int32_t row, int32_t slot, const Pieces& at, float (&a)[8],
                                             float (&b)[8]) {
   if (at.rotates) {
     float c[8], s[8];
-    load8(t.cos + slot * 8, c);
-    load8(t.sin + slot * 8, s);
+    load8(t.cos + row + slot * 8, c);
+    load8(t.sin + row + slot * 8, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = a[i], y = b[i];
@@ -132,7 +134,7 @@ __device__ __forceinline__ void rotate_slot(const RotateArgs& g, const Tables& t
     auto turn = [&](int32_t column, float (&x)[8]) {
       const int32_t pair = (column - g.start) >> 1;
       if (column < g.start || pair >= g.pairs) return;
-      const float4 c = *reinterpret_cast<const float4*>(t.cos + pair), s = *reinterpret_cast<const float4*>(t.sin + pair);
+      const float4 c = *reinterpret_cast<const float4*>(t.cos + row + pair), s = *reinterpret_cast<const float4*>(t.sin + row + pair);
       const float cs[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -146,33 +148,39 @@ __device__ __forceinline__ void rotate_slot(const RotateArgs& g, const Tables& t
   }
 }
 
-// One CTA for a token and up to heads_a_cta of its heads. The token's cos and sin
-// are worked out once, for all of the CTA's heads, and the weights widened. Heads
+// One CTA for a token and up to heads_a_cta of its heads, or for all heads of a few
+// tokens. The tokens' cos and sin are worked out once, for all of the CTA's heads,
+// and the weights widened. Heads
 // with a norm take `group` lanes each and N slots a lane; the slots of the others
-// are dealt out one by one, four a thread on their way at once. Every element is
+// are dealt out one by one, two a thread on their way at once. Every element is
 // read and written once, 16 bytes at a time.
 template <typename T, int N>
-__global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_constant__ RotateArgs g) {
+__global__ void __launch_bounds__(kRotateThreads, 4) rotate_kernel(const __grid_constant__ RotateArgs g) {
   __shared__ __align__(16) Tables tables;
   pdl_wait();
   pdl_launch_dependents();
-  const int32_t token = blockIdx.x, threads = blockDim.x;
+  const int32_t token0 = blockIdx.x * g.tokens_a_cta, threads = blockDim.x;
+  const int32_t tokens = min(g.tokens_a_cta, g.tokens - token0);
   const int32_t first = blockIdx.y * g.heads_a_cta, last = min(first + g.heads_a_cta, g.all_heads);
   const int32_t q_heads = g.set[0].heads;
-  auto source = [&](int32_t head) {
+  auto source = [&](int32_t token, int32_t head) {
     const HeadSet& s = g.set[head < q_heads ? 0 : 1];
-    return static_cast<const T*>(s.in) + token * s.in_token + (head < q_heads ? head : head - q_heads) * s.in_head;
+    return static_cast<const T*>(s.in) + (token0 + token) * s.in_token + (head < q_heads ? head : head - q_heads) * s.in_head;
   };
-  auto target = [&](int32_t head) {
+  auto target = [&](int32_t token, int32_t head) {
     const HeadSet& s = g.set[head < q_heads ? 0 : 1];
-    return static_cast<T*>(s.out) + token * s.out_token + (head < q_heads ? head : head - q_heads) * s.out_head;
+    return static_cast<T*>(s.out) + (token0 + token) * s.out_token + (head < q_heads ? head : head - q_heads) * s.out_head;
   };
   const int32_t normed_first = max(first, g.normed[0]), normed_last = min(last, g.normed[1]);
   const int32_t lane = threadIdx.x % g.group, team = threadIdx.x / g.group, teams = threads / g.group;
   Pieces at[N];
   uint4 raw[N][2];
-  auto fetch = [&](int32_t head) {
-    const T* p = source(head);
+  // Units: a token and one of its normed heads.
+  const int32_t normed = max(normed_last - normed_first, 0), units = tokens * normed;
+  auto token_of = [&](int32_t unit) { return tokens > 1 ? static_cast<int32_t>(fastdiv(unit, g.by_normed)) : 0; };
+  auto fetch = [&](int32_t unit) {
+    const int32_t token = token_of(unit);
+    const T* p = source(token, normed_first + unit - token * normed);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       raw[n][0] = raw[n][1] = make_uint4(0u, 0u, 0u, 0u);
@@ -185,11 +193,39 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
     const int32_t slot = lane + n * g.group;
     at[n] = slot < static_cast<int32_t>(g.slots.divisor) ? pieces_of(g, slot) : Pieces{-1, -1, false};
   }
-  int32_t head = normed_first + team;
-  if (head < normed_last) fetch(head);
-  const int32_t position = g.positions[token];
-  for (int32_t i = threadIdx.x; i < g.pairs; i += threads) {
-    const float2 t = turn(position, g.frequencies[i], g.amplitude);
+  int32_t unit = team;
+  if (unit < units) fetch(unit);
+  // Heads without a norm: those below normed_first and from normed_last on.
+  const int32_t below = min(last, g.normed[0]) - first, slots = g.slots.divisor;
+  const int32_t before = max(below, 0), behind_first = max(first, g.normed[1]), plain = before + max(last - behind_first, 0);
+  const int32_t each = plain * slots, all = tokens * each;
+  constexpr int kAtOnce = 2;
+  struct Dealt {
+    int32_t token, head, slot;  // slot -1: none
+  };
+  uint4 ahead[kAtOnce][2];
+  Dealt dealt[kAtOnce];
+  auto deal = [&](int32_t i0) {
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      const int32_t i = i0 + n * threads;
+      ahead[n][0] = ahead[n][1] = make_uint4(0u, 0u, 0u, 0u);
+      dealt[n] = Dealt{0, 0, -1};
+      if (i < all) {
+        const int32_t token = tokens > 1 ? static_cast<int32_t>(fastdiv(i, g.by_plain)) : 0;
+        const int32_t j = i - token * each, h = static_cast<int32_t>(fastdiv(j, g.slots));
+        dealt[n] = Dealt{token, h < before ? first + h : behind_first + h - before, j - h * slots};
+        const Pieces piece = pieces_of(g, dealt[n].slot);
+        const T* p = source(token, dealt[n].head);
+        ahead[n][0] = load_wide(p + piece.a);
+        if (piece.b >= 0) ahead[n][1] = load_wide(p + piece.b);
+      }
+    }
+  };
+  if (units == 0) deal(threadIdx.x);
+  for (int32_t i = threadIdx.x; i < g.pairs * tokens; i += threads) {
+    const int32_t token = i / g.pairs;
+    const float2 t = turn(g.positions[token0 + token], g.frequencies[i - token * g.pairs], g.amplitude);
     tables.cos[i] = t.x;
     tables.sin[i] = t.y;
   }
@@ -204,8 +240,9 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
   __syncthreads();
   // Lanes of a head share a warp; all of a warp goes as often round, so that every
   // lane takes part in the exchanges.
-  for (int32_t base = normed_first; base < normed_last; base += teams, head += teams) {
-    const bool live = head < normed_last;
+  for (int32_t base = 0; base < units; base += teams, unit += teams) {
+    const bool live = unit < units;
+    const int32_t token = live ? token_of(unit) : 0, head = normed_first + unit - token * normed;
     const int k = live && head >= q_heads ? 1 : 0;
     const int32_t norm = g.set[k].norm;
     float x[N][2][8], sum = 0.f;
@@ -221,11 +258,11 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
         }
       }
     }
-    if (head + teams < normed_last) fetch(head + teams);
+    if (unit + teams < units) fetch(unit + teams);
     for (int d = g.group >> 1; d > 0; d >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, d);
     if (!live) continue;
     const float r = rsqrtf(sum / static_cast<float>(norm) + g.eps);
-    T* out = target(head);
+    T* out = target(token, head);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       if (at[n].a < 0) continue;
@@ -239,46 +276,27 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
           for (int i = 0; i < 8; ++i) x[n][e][i] *= r * w[i];
         }
       }
-      rotate_slot(g, tables, lane + n * g.group, at[n], x[n][0], x[n][1]);
+      rotate_slot(g, tables, token * g.pairs, lane + n * g.group, at[n], x[n][0], x[n][1]);
       *reinterpret_cast<uint4*>(out + at[n].a) = pack8<T>(x[n][0]);
       if (at[n].b >= 0) *reinterpret_cast<uint4*>(out + at[n].b) = pack8<T>(x[n][1]);
     }
   }
-  // Heads without a norm: those below normed_first and from normed_last on.
-  const int32_t below = min(last, g.normed[0]) - first, slots = g.slots.divisor;
-  const int32_t before = max(below, 0), behind_first = max(first, g.normed[1]), plain = before + max(last - behind_first, 0);
-  constexpr int kAtOnce = 4;
-  for (int32_t i0 = threadIdx.x; i0 < plain * slots; i0 += kAtOnce * threads) {
-    uint4 ahead[kAtOnce][2];
-    Pieces piece[kAtOnce];
-    int32_t of[kAtOnce], slot[kAtOnce];
+  if (units > 0) deal(threadIdx.x);
+  for (int32_t i0 = threadIdx.x; i0 < all; i0 += kAtOnce * threads) {
 #pragma unroll
     for (int n = 0; n < kAtOnce; ++n) {
-      const int32_t i = i0 + n * threads;
-      ahead[n][0] = ahead[n][1] = make_uint4(0u, 0u, 0u, 0u);
-      piece[n] = Pieces{-1, -1, false};
-      of[n] = slot[n] = 0;
-      if (i < plain * slots) {
-        const int32_t h = static_cast<int32_t>(fastdiv(i, g.slots));
-        slot[n] = i - h * slots;
-        of[n] = h < before ? first + h : behind_first + h - before;
-        piece[n] = pieces_of(g, slot[n]);
-        const T* p = source(of[n]);
-        ahead[n][0] = load_wide(p + piece[n].a);
-        if (piece[n].b >= 0) ahead[n][1] = load_wide(p + piece[n].b);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < kAtOnce; ++n) {
-      if (piece[n].a < 0) continue;
+      const Dealt& d = dealt[n];
+      if (d.slot < 0) continue;
+      const Pieces piece = pieces_of(g, d.slot);
       float a[8], b[8];
       unpack8<T>(ahead[n][0], a);
       unpack8<T>(ahead[n][1], b);
-      rotate_slot(g, tables, slot[n], piece[n], a, b);
-      T* out = target(of[n]);
-      *reinterpret_cast<uint4*>(out + piece[n].a) = pack8<T>(a);
-      if (piece[n].b >= 0) *reinterpret_cast<uint4*>(out + piece[n].b) = pack8<T>(b);
+      rotate_slot(g, tables, d.token * g.pairs, d.slot, piece, a, b);
+      T* out = target(d.token, d.head);
+      *reinterpret_cast<uint4*>(out + piece.a) = pack8<T>(a);
+      if (piece.b >= 0) *reinterpret_cast<uint4*>(out + piece.b) = pack8<T>(b);
     }
+    deal(i0 + kAtOnce * threads);
   }
 }
 
@@ -337,7 +355,7 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_narrow_kernel(const __g
 
 template <typename T>
 void (*rotate_for(int each))(RotateArgs) {
-  return each == 1 ? rotate_kernel<T, 1> : each == 2 ? rotate_kernel<T, 2> : rotate_kernel<T, 3>;
+  return each == 1 ? rotate_kernel<T, 1> : rotate_kernel<T, 2>;
 }
 
 Place place_of_heads(const void* base, int32_t dim, int64_t tokens, int64_t token, int32_t heads, int64_t head) {
@@ -410,13 +428,14 @@ extern "C" int silkern_rotate_heads_v1(const silkern_heads_v1* q, const silkern_
   if (wide) {
     const int total = dim / 8, turned = g.interleaved ? 0 : pairs / 8, slots = turned + (total - 2 * turned + 1) / 2;
     g.slots = make_fastdiv(static_cast<uint32_t>(slots));
-    // Lanes to a normed head: of the powers of two with at most three slots to a
-    // lane, the one with the fewest slots left empty, and the most lanes among
-    // equals.
+    // Lanes to a normed head: of the powers of two with at most two slots to a lane
+    // (three take registers that the others' occupancy needs: 76 us for 65 on 1001
+    // tokens of 129 latent heads), the one with the fewest slots left empty, and the
+    // most lanes among equals.
     int least = 0;
     for (int group = 32; group >= 1; group >>= 1) {
       const int n = (slots + group - 1) / group;
-      if (n <= 3 && (least == 0 || n * group < least)) {
+      if (n <= 2 && (least == 0 || n * group < least)) {
         each = n;
         g.group = group;
         least = n * group;
@@ -424,16 +443,28 @@ extern "C" int silkern_rotate_heads_v1(const silkern_heads_v1* q, const silkern_
     }
     in_turn = kRotateThreads / g.group;
   }
-  // A token's heads in one CTA, unless few tokens leave SMs without work.
-  int64_t parts = 1;
+  // A token's heads in one CTA of at most 48 KB, unless few tokens leave SMs
+  // without work.
+  int64_t parts = (2 * int64_t{dim} * g.all_heads + 49151) / 49152;
   while (parts * in_turn < g.all_heads && parts * tokens < 2 * 148) ++parts;
   g.heads_a_cta = static_cast<int32_t>((g.all_heads + parts - 1) / parts);
   parts = (g.all_heads + g.heads_a_cta - 1) / g.heads_a_cta;
   const int32_t normed = g.normed[1] - g.normed[0];
+  g.tokens_a_cta = 1;
+  if (wide && parts == 1) {
+    // Several tokens while a CTA has less than 48 KB of them, there is room for their
+    // cos and sin, and six CTAs for each SM.
+    const int64_t bytes = 2 * int64_t{dim} * g.all_heads;
+    const int64_t most = std::min({(49152 + bytes - 1) / bytes, int64_t{kMostColumns / 2 / pairs}, tokens / (6 * 148)});
+    g.tokens_a_cta = static_cast<int32_t>(std::max(most, int64_t{1}));
+    g.by_normed = make_fastdiv(static_cast<uint32_t>(normed > 0 ? normed : 1));
+    const int64_t plain = (g.all_heads - normed) * static_cast<int64_t>(g.slots.divisor);
+    g.by_plain = make_fastdiv(static_cast<uint32_t>(plain > 0 ? plain : 1));
+  }
   if (wide && normed > 0) {
     // As many threads as leave the fewest without a head in the last round (72
     // heads of 8 lanes: 192 threads, three rounds).
-    const int64_t heads = normed < g.heads_a_cta ? normed : g.heads_a_cta;
+    const int64_t heads = int64_t{normed < g.heads_a_cta ? normed : g.heads_a_cta} * g.tokens_a_cta;
     int64_t best = 0;
     for (int candidate = kRotateThreads; candidate >= 128; candidate -= 32) {
       const int64_t teams = candidate / g.group, rounds = (heads + teams - 1) / teams;
@@ -447,6 +478,6 @@ extern "C" int silkern_rotate_heads_v1(const silkern_heads_v1* q, const silkern_
   void (*fn)(RotateArgs) = type == SILKERN_BF16
                                ? (wide ? rotate_for<__nv_bfloat16>(each) : rotate_narrow_kernel<__nv_bfloat16>)
                                : (wide ? rotate_for<__half>(each) : rotate_narrow_kernel<__half>);
-  return launch_pdl_grid(fn, dim3(static_cast<unsigned>(tokens), static_cast<unsigned>(parts), 1), threads, 0, 1,
+  return launch_pdl_grid(fn, dim3(static_cast<unsigned>((tokens + g.tokens_a_cta - 1) / g.tokens_a_cta), static_cast<unsigned>(parts), 1), threads, 0, 1,
                          static_cast<cudaStream_t>(stream), g);
 }
