@@ -186,6 +186,18 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) 
                "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, float (&v)[8]) {  // and waits
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\ntcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+      : "r"(addr)
+      : "memory");
+}
 using silkern::tmem_st16;
 using silkern::tmem_wait_ld;
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
@@ -231,12 +243,62 @@ struct Row {
   int32_t low, high;
 };
 
+// All of these are short loops: an SM's warps run seven programs here, and straight
+// code of some hundred instructions waits for its own fetching (64 keys unrolled
+// took 1250 cycles, a masked half 15000).
+//
 // The usual half: nothing of it is hidden from the row, and each 16 keys share a
-// page and its scales. Weights against `base`, which a score may turn out to pass
-// (`best` says how far they went): their sum, and in `w` their products with the
-// value scales in `unit`s.
-__device__ __forceinline__ float weigh_plain(const Row& r, uint32_t s_at, float base, float unit, float& best,
-                                             uint32_t (&w)[kHalf / 2]) {
+// page and its scales.
+__device__ __forceinline__ float largest_plain(const Row& r, uint32_t s_at) {
+  float most = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kHalf; c += 32) {
+    float x[32];
+    tmem_ld32(s_at + c, x);
+    const float k0 = r.k[c], k1 = r.k[c + 16];
+    tmem_wait_ld(x);
+    float b[4] = {x[0], x[1], x[16], x[17]};
+#pragma unroll
+    for (int i = 2; i < 14; i += 4) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        b[2 * j] = max3(b[2 * j], x[16 * j + i], x[16 * j + i + 1]);
+        b[2 * j + 1] = max3(b[2 * j + 1], x[16 * j + i + 2], x[16 * j + i + 3]);
+      }
+    }
+    most = max3(most, max3(b[0], b[1], fmaxf(x[14], x[15])) * k0, max3(b[2], b[3], fmaxf(x[30], x[31])) * k1);
+  }
+  return most * r.unscale;
+}
+// The weights against `base`: their sum is returned, their products with the value
+// scales in `unit`s take the scores' place.
+__device__ __forceinline__ float weigh_plain(const Row& r, uint32_t s_at, float base, float unit) {
+  float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < kHalf; c += 16) {
+    float x[16];
+    uint32_t w[8];
+    tmem_ld16(s_at + c, x);
+    const float by = r.k[c] * r.unscale, vs = r.v[c] * unit;
+    tmem_wait_ld(x);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      float p0, p1, w0, w1;
+      fma_pair(x[i], x[i + 1], by, by, -base, -base, p0, p1);
+      p0 = exp2_approx(p0);
+      p1 = exp2_approx(p1);
+      add_pair(sum0, sum1, p0, p1, sum0, sum1);
+      mul_pair(p0, p1, vs, vs, w0, w1);
+      w[i / 2] = pack_f16x2(w0, w1);
+    }
+    tmem_st8(s_at + c / 2, w);
+  }
+  return sum0 + sum1;
+}
+// Both at once, against a reference that a score may turn out to pass (`best` says
+// how far they went), so that the weights stay in registers: straight code, but
+// the one that nearly every half takes.
+__device__ __forceinline__ float weigh_ahead(const Row& r, uint32_t s_at, float base, float unit, float& best, uint32_t (&w)[2][16]) {
   float sum0 = 0.f, sum1 = 0.f, most = -INFINITY;
 #pragma unroll
   for (int c = 0; c < kHalf; c += 32) {
@@ -266,23 +328,13 @@ __device__ __forceinline__ float weigh_plain(const Row& r, uint32_t s_at, float 
       p1 = exp2_approx(p1);
       add_pair(sum0, sum1, p0, p1, sum0, sum1);
       mul_pair(p0, p1, vs[run], vs[run], w0, w1);
-      w[(c + i) / 2] = pack_f16x2(w0, w1);
+      w[c / 32][i / 2] = pack_f16x2(w0, w1);
     }
   }
   best = most * r.unscale;
   return sum0 + sum1;
 }
-__device__ __forceinline__ void store_weights(uint32_t s_at, const uint32_t (&w)[kHalf / 2]) {
-#pragma unroll
-  for (int c = 0; c < kHalf / 2; c += 16) {
-    uint32_t part[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) part[i] = w[c + i];
-    tmem_st16(s_at + c, part);
-  }
-}
-// Any half, in two passes and little code (what runs seldom is fetched from far):
-// first the largest score, and where value scales are far from the first tile's
+// Any half: the largest score, and where value scales are far from the first tile's
 // the largest of scores with log2 of their values' scales; then the weights.
 __device__ __forceinline__ float score_of(const Row& r, int i, float x, float& vs) {
   vs = r.v[i];
@@ -293,12 +345,11 @@ __device__ __forceinline__ float largest_of_half(const Row& r, uint32_t s_at, bo
   float best = -INFINITY;
   heaviest = -INFINITY;
 #pragma unroll 1
-  for (int c = 0; c < kHalf; c += 16) {
-    float x[16];
-    tmem_ld16(s_at + c, x);
-    tmem_wait_ld(x);
+  for (int c = 0; c < kHalf; c += 8) {
+    float x[8];
+    tmem_ld8(s_at + c, x);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       float vs;
       const float t = score_of(r, c + i, x[i], vs);
       best = fmaxf(best, t);
@@ -310,13 +361,12 @@ __device__ __forceinline__ float largest_of_half(const Row& r, uint32_t s_at, bo
 __device__ __forceinline__ float weigh_half(const Row& r, uint32_t s_at, float base, float unit, bool usual, float reference) {
   float sum = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < kHalf; c += 16) {
-    float x[16];
-    uint32_t w[8];
-    tmem_ld16(s_at + c, x);
-    tmem_wait_ld(x);
+  for (int c = 0; c < kHalf; c += 8) {
+    float x[8];
+    uint32_t w[4];
+    tmem_ld8(s_at + c, x);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       float vs;
       const float t = score_of(r, c + i, x[i], vs);
       const float p = exp2_approx(t - base);
@@ -325,8 +375,8 @@ __device__ __forceinline__ float weigh_half(const Row& r, uint32_t s_at, float b
       if (t == -INFINITY) x[i] = 0.f;  // whatever its value's scale is
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = pack_f16x2(x[2 * i], x[2 * i + 1]);
-    tmem_st8(s_at + c / 2, w);
+    for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(x[2 * i], x[2 * i + 1]);
+    tmem_st4(s_at + c / 2, w);
   }
   return sum;
 }
@@ -490,53 +540,53 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
             const bool plain = pages && key_first <= first_key && all_see - first_key >= kHalf;
             const Row at{note->k + half * kHalf, note->v + half * kHalf, unscale, key_first - first_key, seen - first_key};
             const float unit = __uint_as_float(static_cast<uint32_t>(127 + kShift - exponent) << 23);
-            uint32_t w[kHalf / 2];
-            float sum = 0.f;
-            for (bool again = true; again;) {
-              float best, heaviest = -INFINITY;
-              if (plain) {
-                sum = weigh_plain(at, s_at, top == -INFINITY ? 0.f : top, unit, best, w);
-              } else {
-                best = largest_of_half(at, s_at, usual, heaviest);
+            // ---- most halves leave the references where they are
+            bool stays = plain && step > 0;
+            if (stays) {
+              uint32_t w[2][16];
+              float best;
+              const float sum = weigh_ahead(at, s_at, top == -INFINITY ? 0.f : top, unit, best, w);
+              stays = __all_sync(kAllLanes, !(best > top + kReach));
+              if (stays) {
+                total += sum;
+                tmem_st16(s_at, w[0]);
+                tmem_st16(s_at + 16, w[1]);
               }
-              // References seldom move; then the sum and the outputs do, and a plain
-              // half is weighed once more.
-              const bool up = best > top + kReach, heavier = heaviest > reference + kReach;
-              const bool moves = __any_sync(kAllLanes, up || heavier);
-              if (moves) {
-                float by = 1.f;
-                if (up) {
-                  by = exp2f(top - best);
-                  total *= by;
-                  top = best;
-                }
-                if (!usual) {
-                  by = heavier ? exp2f(reference - heaviest) : 1.f;
-                  if (heavier) reference = heaviest;
-                }
-                if (step > 0) {
-                  // The half before may still be added up.
-                  if (!(going = wait(&m.done[slot][half ^ 1], (parity >> (half ^ 1) & 1) ^ 1))) break;
-                  tc_fence_after();
-#pragma unroll 1
-                  for (int c = 0; c < DIM; c += 16) {
-                    float o[16];
-                    tmem_ld16(o_at + c, o);
-                    tmem_wait_ld(o);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] *= by;
-                    tmem_st16(o_at + c, o);
-                  }
-                }
-              }
-              again = plain && moves;
             }
-            if (!going) break;
-            if (plain) {
-              total += sum;
-              store_weights(s_at, w);
-            } else {
-              total += weigh_half(at, s_at, top == -INFINITY ? 0.f : top, unit, usual, reference == -INFINITY ? 0.f : reference);
+            if (!stays) {
+            float heaviest = -INFINITY;
+            const float best = plain ? largest_plain(at, s_at) : largest_of_half(at, s_at, usual, heaviest);
+            // References seldom move; then the sum and the outputs do.
+            const bool up = best > top + kReach, heavier = heaviest > reference + kReach;
+            if (__any_sync(kAllLanes, up || heavier)) {
+              float by = 1.f;
+              if (up) {
+                by = exp2f(top - best);
+                total *= by;
+                top = best;
+              }
+              if (!usual) {
+                by = heavier ? exp2f(reference - heaviest) : 1.f;
+                if (heavier) reference = heaviest;
+              }
+              if (step > 0) {
+                // The half before may still be added up.
+                if (!(going = wait(&m.done[slot][half ^ 1], (parity >> (half ^ 1) & 1) ^ 1))) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < DIM; c += 16) {
+                  float o[16];
+                  tmem_ld16(o_at + c, o);
+                  tmem_wait_ld(o);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[i] *= by;
+                  tmem_st16(o_at + c, o);
+                }
+              }
+            }
+            const float base = top == -INFINITY ? 0.f : top;
+            total += plain ? weigh_plain(at, s_at, base, unit)
+                           : weigh_half(at, s_at, base, unit, usual, reference == -INFINITY ? 0.f : reference);
             }
             tmem_wait_st();
           }
