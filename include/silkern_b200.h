@@ -429,7 +429,10 @@ int silkern_attend_window_v1(const silkern_cache_v1* cache, const void* q, int64
  *
  * workspace: silkern_shared_workspace_v1 bytes at least, at a multiple of 16,
  * whose contents do not matter before or after; calls that may run at the same
- * time need one each. cu_tokens and cu_groups ascend. Equal calls give equal bits.
+ * time need one each. cu_tokens and cu_groups ascend: where they do not, nothing
+ * is seen (out 0, lse -inf) and SILKERN_STATUS_BAD_LENGTH is set. A wait inside
+ * the kernel that runs out makes all of the call's rows NaN. Equal calls give
+ * equal bits. Fastest with block_size a multiple of 16.
  */
 int silkern_attend_shared_v1(const silkern_cache_v1* cache, const void* q, int64_t q_row,
                              int64_t q_head, int32_t type, int64_t rows, int32_t heads,

@@ -542,13 +542,16 @@ def attend_shared(
     outside the sequences are left as they were in ``out`` and ``lse``.
 
     Keys are shared among the GPU's SMs by the lengths themselves, so that long
-    sequences may stand among short ones.
+    sequences may stand among short ones. Pages of a multiple of 16 tokens are
+    the fast ones.
 
     ``status`` gets 1 for a request id outside the table (nothing is seen through
     its row), 2 for a length below the number of queries (those at negative
     positions see nothing), 8 for a visible token whose page is outside the table
     row or the cache (left out) and 16 for a wait inside the kernel that ran out,
-    whose results are NaN (it does not occur in a working launch).
+    with NaN in all of the call's rows (it does not occur in a working launch).
+    ``cu_tokens`` and ``cu_groups`` ascend; where they do not, nothing is seen
+    (outputs 0, ``lse`` -inf) and 2 is set.
     """
     import torch
 

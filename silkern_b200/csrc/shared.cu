@@ -102,7 +102,13 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     most = __reduce_max_sync(kAllLanes, most);
     if (lane == 0) a.limits()[g] = a.keys_below(min(most, load_int(a.prefixes + g)));
   }
-  __syncthreads();
+  // Sequences and groups that descend could have more items than the workspace
+  // holds: such a call has none.
+  bool descends = false;
+  for (int32_t i = threadIdx.x; i < a.sequences; i += kPlanThreads) descends = descends || a.cu(i + 1) < a.cu(i);
+  for (int32_t i = threadIdx.x; i < a.groups; i += kPlanThreads) descends = descends || a.cut(i + 1) < a.cut(i);
+  descends = __syncthreads_or(descends);
+  if (descends && threadIdx.x == 0) flag_status(a.status, SILKERN_STATUS_BAD_LENGTH);
   const int32_t segments = a.groups + a.sequences;
   int64_t before[3] = {0, 0, 0};  // items, units, rows of second copies
   for (int32_t base = 0; base < segments; base += kPlanThreads) {
@@ -111,7 +117,7 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     int32_t blocks = 0;
     const bool prefix = index < a.groups;
     int64_t mine[3] = {0, 0, 0};
-    if (index < segments) {
+    if (index < segments && !descends) {
       s = find_segment(a, index);
       if (s.tokens > 0 && s.key_end > s.key_first) {
         blocks = (s.tokens * a.heads_per_kv + kBlockRows - 1) / kBlockRows;
@@ -191,6 +197,7 @@ struct Parts {
 
 // `first`: the segment's first item, `row` the row's number in the segment.
 __device__ __forceinline__ Parts find_parts(const SharedArgs& a, int32_t first, int32_t row, int32_t kv, int64_t share, int64_t place) {
+  row = max(row, 0);  // (below it in a call whose groups descend)
   const SharedItem* it = a.item(max(first, 0) + row / kBlockRows);
   // (Loads that wait for one another cost more than some too many.)
   const int32_t tiles = load_int(&it->tiles), rows = load_int(&it->rows), extra = load_int(&it->extra);

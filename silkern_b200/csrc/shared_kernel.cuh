@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     mbar_init(smem_addr(&m.drained[0]), 1);
     mbar_init(smem_addr(&m.drained[1]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    m.abort = 0;
+    m.abort = a.wait_cycles == 0 ? 1 : 0;
   }
   if (warp == kMmaWarp) tmem_alloc(smem_addr(&m.tmem), 512);
   tc_fence_before();
@@ -429,8 +429,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
   pdl_launch_dependents();
   constexpr uint32_t kScoresAt = 256;  // TMEM columns: outputs of the slots from 0 and DIM on, scores from here
 
-  auto wait = [&](uint64_t* bar, uint32_t parity) {  // a whole warp; false once a wait ran out
-    return __all_sync(kAllLanes, mbar_wait(smem_addr(bar), parity, abort, bound)) != 0;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int32_t tiles = 1) {  // a whole warp; false once a wait ran out
+    return __all_sync(kAllLanes, mbar_wait(smem_addr(bar), parity, abort, bound * tiles)) != 0;
   };
   auto arrive = [&](uint64_t* bar) {  // once for the warp, behind all of its lanes
     __syncwarp();
@@ -554,39 +554,39 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
               }
             }
             if (!stays) {
-            float heaviest = -INFINITY;
-            const float best = plain ? largest_plain(at, s_at) : largest_of_half(at, s_at, usual, heaviest);
-            // References seldom move; then the sum and the outputs do.
-            const bool up = best > top + kReach, heavier = heaviest > reference + kReach;
-            if (__any_sync(kAllLanes, up || heavier)) {
-              float by = 1.f;
-              if (up) {
-                by = exp2f(top - best);
-                total *= by;
-                top = best;
-              }
-              if (!usual) {
-                by = heavier ? exp2f(reference - heaviest) : 1.f;
-                if (heavier) reference = heaviest;
-              }
-              if (step > 0) {
-                // The half before may still be added up.
-                if (!(going = wait(&m.done[slot][half ^ 1], (parity >> (half ^ 1) & 1) ^ 1))) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int c = 0; c < DIM; c += 16) {
-                  float o[16];
-                  tmem_ld16(o_at + c, o);
-                  tmem_wait_ld(o);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) o[i] *= by;
-                  tmem_st16(o_at + c, o);
+              float heaviest = -INFINITY;
+              const float best = plain ? largest_plain(at, s_at) : largest_of_half(at, s_at, usual, heaviest);
+              // References seldom move; then the sum and the outputs do.
+              const bool up = best > top + kReach, heavier = heaviest > reference + kReach;
+              if (__any_sync(kAllLanes, up || heavier)) {
+                float by = 1.f;
+                if (up) {
+                  by = exp2f(top - best);
+                  total *= by;
+                  top = best;
+                }
+                if (!usual) {
+                  by = heavier ? exp2f(reference - heaviest) : 1.f;
+                  if (heavier) reference = heaviest;
+                }
+                if (step > 0) {
+                  // The half before may still be added up.
+                  if (!(going = wait(&m.done[slot][half ^ 1], (parity >> (half ^ 1) & 1) ^ 1))) break;
+                  tc_fence_after();
+  #pragma unroll 1
+                  for (int c = 0; c < DIM; c += 16) {
+                    float o[16];
+                    tmem_ld16(o_at + c, o);
+                    tmem_wait_ld(o);
+  #pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] *= by;
+                    tmem_st16(o_at + c, o);
+                  }
                 }
               }
-            }
-            const float base = top == -INFINITY ? 0.f : top;
-            total += plain ? weigh_plain(at, s_at, base, unit)
-                           : weigh_half(at, s_at, base, unit, usual, reference == -INFINITY ? 0.f : reference);
+              const float base = top == -INFINITY ? 0.f : top;
+              total += plain ? weigh_plain(at, s_at, base, unit)
+                             : weigh_half(at, s_at, base, unit, usual, reference == -INFINITY ? 0.f : reference);
             }
             tmem_wait_st();
           }
@@ -899,8 +899,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
     for (bool more = true; more; ++seq) {
       more = walk.next(a, f);
       if (!more) f.last = 0;
-      if (!wait(&m.ring_free[seq % kRing], (seq / kRing & 1) ^ 1)) break;
-      if (lane == 0) m.ring[seq % kRing] = f;
+      // (The place's last fragment may have only begun.)
+      Fragment& to = m.ring[seq % kRing];
+      if (!wait(&m.ring_free[seq % kRing], (seq / kRing & 1) ^ 1, seq < kRing ? 1 : 2 + to.last - to.first)) break;
+      __syncwarp();
+      if (lane == 0) to = f;
       arrive(&m.ring_full[seq % kRing]);
     }
   }

@@ -69,12 +69,12 @@ def assert_attention(out, lse, want, q, k_cache, k_scale, softmax_scale):
 def assert_shared(out, lse, want, q, k_cache, k_scale, softmax_scale):
     """out within half a step of the output's type, plus what the weights' errors make.
 
-    A weight p of a value of scale s enters the product in fp16 as x = 2^6 p s / (P S), with S a scale near those of its
-    run of keys (s within [2^-8, 2^4] of it) and P the largest weight so far or less, by 2^4 at most. Half a step of
-    fp16 is 2^-11 x, or 2^-25 below 2^-14: an error of 2^-31 P S in p s, at most 2^-23 of the largest p s. Where scales
-    are further apart, x = 2^6 p s / (the largest p s so far, or less by 2^4 at most) has the same bound. Scores'
-    errors count twice, in the weight and in the sum; exponentials, float32 sums of a run, and the joining of runs add
-    2^-18."""
+    A weight p of a value of scale s enters the product in fp16 as x = 2^3 p s / (P S), with S the power of two below the
+    largest scale of the row's first tile (s within [2^-6, 2^4) S) and P the largest weight so far or less, by 2^8 at
+    most: below 2^15. Half a step of fp16 is 2^-11 x, or 2^-25 below 2^-14: an error of 2^-28 P S in p s, at most 2^-22
+    of the largest p s, which is 2^-6 P S at least. Where scales are further apart, x = 2^3 p s / (the largest p s so
+    far, or less by 2^8 at most) has the same bound. Scores' errors count twice, in the weight and in the sum;
+    exponentials, float32 sums of a run, and the joining of runs add 2^-18."""
     ref_out, ref_lse, spread, peak = want
     ds = score_error(q, k_cache, k_scale, softmax_scale)
     bound = HALF_STEP[out.dtype] * ref_out.abs() + (2.0**-11 + 2.0**-18 + 2 * ds) * spread + 2.0**-22 * peak

@@ -292,6 +292,31 @@ def test_equal_calls_give_equal_bits_and_agree_with_the_window() -> None:
     assert float((lse - other_lse).abs().max()) < 2.0**-15
 
 
+@pytest.mark.parametrize("kv_heads,group,dim", [(4, 8, 128), (1, 24, 64), (2, 4, 128)])
+def test_ctas_with_items_of_both_sorts(kv_heads, group, dim) -> None:
+    """Enough keys for whole runs of tiles in each CTA, behind prefixes of more and of less than 128 rows, so that CTAs go
+    from items whose slots take turns to items whose slots go together and back."""
+    sizes = [1, 90, 3, 40, 2, 130, 1]
+    prefixes = [3000, 2500, 700, 1111, 4000, 900, 64]
+    own = [1 + 331 * i % 1500 for i in range(sum(sizes) + 5)]
+    Batch(sizes, prefixes, own, [1] * len(own), heads=kv_heads * group, kv_heads=kv_heads, dim=dim, block=64, seed=30, alone=5).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_negative_scale(dtype) -> None:
+    b = Batch([3], [300], [30, 1, 150], [1, 2, 1], dtype=dtype, seed=31)
+    b.scale = -0.1
+    b.check()
+
+
+def test_equal_requests_and_equal_pages() -> None:
+    """Several sequences of one request, and a page that stands twice in a row."""
+    b = Batch([3], [200], [30, 40, 50], [1, 1, 1], seed=32)
+    b.req[1] = b.req[0]
+    b.table[int(b.req[0]), 3] = b.table[int(b.req[0]), 2]
+    b.check()
+
+
 def test_graphs_streams_two_at_once_and_compiled_callers() -> None:
     b = Batch([3], [1000], [30, 40, 150], [1, 1, 2], heads=16, kv_heads=2, seed=19)
     c = Batch([2], [500], [10, 20], [1, 1], heads=16, kv_heads=2, seed=20)
