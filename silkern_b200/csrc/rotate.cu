@@ -150,10 +150,13 @@ __device__ __forceinline__ void rotate_slot(const RotateArgs& g, const Tables& t
 
 // One CTA for a token and up to heads_a_cta of its heads, or for all heads of a few
 // tokens. The tokens' cos and sin are worked out once, for all of the CTA's heads,
-// and the weights widened. Heads
-// with a norm take `group` lanes each and N slots a lane; the slots of the others
-// are dealt out one by one, two a thread on their way at once. Every element is
-// read and written once, 16 bytes at a time.
+// and the weights widened. Heads with a norm take `group` lanes each and N slots a
+// lane; the slots of the others are dealt out one by one, two a thread on their way
+// at once. Every element is read and written once, 16 bytes at a time. Bound by
+// memory and, with norms, by instruction issue: 8192 tokens of 72 normed heads of
+// 128 columns (302 MB) 60 us, 5.0 TB/s; 1001 tokens of 129 heads of 576, 64 of them
+// rotary (298 MB), 57 us, 5.2 TB/s. Four CTAs to an SM (64 registers): with
+// three (80) or five (48, spilled) 64 us each.
 template <typename T, int N>
 __global__ void __launch_bounds__(kRotateThreads, 4) rotate_kernel(const __grid_constant__ RotateArgs g) {
   __shared__ __align__(16) Tables tables;
