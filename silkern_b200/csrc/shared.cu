@@ -28,31 +28,53 @@ struct Segment {
   int32_t token, tokens;
   int32_t key_first, key_end;  // rank-local
   int32_t table_row;
+  int32_t length;  // of a sequence
 };
 
-__device__ __forceinline__ Segment find_segment(const SharedArgs& a, int32_t index) {
-  Segment s{0, 0, 0, 0, 0, 0, 0};
+// Groups' first sequences, prefixes, the longest length of each, and their first
+// items, in shared memory as far as there is room; else where the call has them,
+// and in the workspace.
+constexpr int kHeldGroups = 1024;
+struct Groups {
+  int32_t cut[kHeldGroups + 1], prefix[kHeldGroups], longest[kHeldGroups], first[kHeldGroups];
+};
+__device__ __forceinline__ int32_t cut_of(const SharedArgs& a, const Groups& m, int32_t g) {
+  return a.groups <= kHeldGroups ? m.cut[g] : a.cut(g);
+}
+__device__ __forceinline__ int32_t prefix_of(const SharedArgs& a, const Groups& m, int32_t g) {
+  return a.groups <= kHeldGroups ? m.prefix[g] : load_int(a.prefixes + g);
+}
+__device__ __forceinline__ int32_t group_of(const SharedArgs& a, const Groups& m, int32_t seq) {  // -1: none
+  if (seq < cut_of(a, m, 0) || seq >= cut_of(a, m, a.groups)) return -1;
+  return last_at_most(a.groups, seq, [&](int32_t i) { return cut_of(a, m, i); });
+}
+
+// What a thread loads for its segment, before the groups are known.
+struct Known {
+  int32_t token, end, length, table_row;
+};
+__device__ __forceinline__ Known know_sequence(const SharedArgs& a, int32_t seq) {
+  return {a.cu(seq), a.cu(seq + 1), load_int(a.lengths + seq), load_int(a.req_ids + seq)};
+}
+
+__device__ __forceinline__ Segment find_segment(const SharedArgs& a, const Groups& m, int32_t index, const Known& known) {
+  Segment s{};
+  s.token = known.token;
+  s.tokens = max(known.end - known.token, 0);
+  s.table_row = known.table_row;
   if (index < a.groups) {
-    s.seq = a.cut(index);
-    s.seqs = max(a.cut(index + 1) - s.seq, 0);
-    if (s.seqs == 0) return s;
-    s.token = a.cu(s.seq);
-    s.tokens = max(a.cu(s.seq + s.seqs) - s.token, 0);
-    s.key_end = a.limits()[index];
-    s.table_row = load_int(a.req_ids + s.seq);
+    s.seq = cut_of(a, m, index);
+    s.seqs = cut_of(a, m, index + 1) - s.seq;
+    const int32_t longest = a.groups <= kHeldGroups ? m.longest[index] : a.limits()[index];
+    s.key_end = a.keys_below(min(longest, prefix_of(a, m, index)));
   } else {
     s.seq = index - a.groups;
     s.seqs = 1;
-    s.token = a.cu(s.seq);
-    s.tokens = max(a.cu(s.seq + 1) - s.token, 0);
-    const int32_t length = load_int(a.lengths + s.seq);
-    if (s.tokens > 0 && length < s.tokens) flag_status(a.status, SILKERN_STATUS_BAD_LENGTH);
-    s.key_end = a.keys_below(length);
-    if (s.seq >= a.cut(0) && s.seq < a.cut(a.groups)) {
-      const int32_t group = last_at_most(a.groups, s.seq, [&](int32_t i) { return a.cut(i); });
-      s.key_first = a.keys_below(load_int(a.prefixes + group));
-    }
-    s.table_row = load_int(a.req_ids + s.seq);
+    s.length = known.length;
+    if (s.tokens > 0 && s.length < s.tokens) flag_status(a.status, SILKERN_STATUS_BAD_LENGTH);
+    s.key_end = a.keys_below(s.length);
+    const int32_t group = group_of(a, m, s.seq);
+    if (group >= 0) s.key_first = a.keys_below(prefix_of(a, m, group));
   }
   if (s.tokens > 0 && s.key_end > s.key_first && (s.table_row < 0 || s.table_row >= a.table_rows)) {
     flag_status(a.status, SILKERN_STATUS_BAD_REQUEST);
@@ -71,7 +93,7 @@ __device__ __forceinline__ SharedItem item_of(const SharedArgs& a, const Segment
   it.key_end = s.key_end;
   if (!prefix && s.tokens > 1) {  // up to its last query's
     const int32_t last = static_cast<int32_t>(fastdiv(it.row + it.rows - 1, a.per_kv));
-    const int64_t position = static_cast<int64_t>(load_int(a.lengths + s.seq)) - (s.tokens - last);
+    const int64_t position = static_cast<int64_t>(s.length) - (s.tokens - last);
     it.key_end = position < 0 ? 0 : min(it.key_end, a.keys_below(static_cast<int32_t>(position + 1)));
   }
   it.tiles = it.key_end > it.key_first
@@ -86,30 +108,64 @@ __device__ __forceinline__ SharedItem item_of(const SharedArgs& a, const Segment
 }
 
 // One CTA lays out the items: a thread for each segment, and prefix sums over
-// them. 128 sequences: about 4 us, most of it the chain of dependent loads.
+// them. Fewer dependent loads than launches cost: 4.7 us alone in a graph for 4
+// sequences, 6.2 for 256 in 5 groups.
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_constant__ SharedArgs a, int32_t ctas) {
   __shared__ int64_t sums[3][32];
+  __shared__ Groups groups;
   pdl_wait();
   pdl_launch_dependents();
   const int32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // Prefixes end where the last query of the group sees no further.
-  for (int32_t g = warp; g < a.groups; g += kPlanThreads / 32) {
-    const int32_t first = a.cut(g), last = a.cut(g + 1);
-    int32_t most = 0;
-    for (int32_t s = first + lane; s < last; s += 32) {
-      if (a.cu(s + 1) > a.cu(s)) most = max(most, load_int(a.lengths + s));
-    }
-    most = __reduce_max_sync(kAllLanes, most);
-    if (lane == 0) a.limits()[g] = a.keys_below(min(most, load_int(a.prefixes + g)));
+  const int32_t segments = a.groups + a.sequences;
+  const bool held = a.groups <= kHeldGroups;
+  // All loads that wait for none, and whether sequences or groups descend: such a
+  // call could have more items than the workspace holds, and has none.
+  const int32_t my_seq = static_cast<int32_t>(threadIdx.x) - a.groups;
+  Known known{};
+  if (my_seq >= 0 && my_seq < a.sequences) known = know_sequence(a, my_seq);
+  bool descends = known.end < known.token;
+  for (int32_t i = kPlanThreads - a.groups + static_cast<int32_t>(threadIdx.x); i < a.sequences; i += kPlanThreads) {
+    descends = descends || (i >= 0 && a.cu(i + 1) < a.cu(i));
   }
-  // Sequences and groups that descend could have more items than the workspace
-  // holds: such a call has none.
-  bool descends = false;
-  for (int32_t i = threadIdx.x; i < a.sequences; i += kPlanThreads) descends = descends || a.cu(i + 1) < a.cu(i);
-  for (int32_t i = threadIdx.x; i < a.groups; i += kPlanThreads) descends = descends || a.cut(i + 1) < a.cut(i);
+  for (int32_t g = threadIdx.x; g < a.groups; g += kPlanThreads) {
+    const int32_t first = a.cut(g), last = a.cut(g + 1);
+    descends = descends || last < first;
+    if (held) {
+      groups.cut[g] = first;
+      if (g + 1 == a.groups) groups.cut[g + 1] = last;
+      groups.prefix[g] = load_int(a.prefixes + g);
+      groups.longest[g] = 0;
+    }
+  }
   descends = __syncthreads_or(descends);
   if (descends && threadIdx.x == 0) flag_status(a.status, SILKERN_STATUS_BAD_LENGTH);
-  const int32_t segments = a.groups + a.sequences;
+  // Prefixes end where the last query of the group sees no further.
+  if (descends) {
+  } else if (held) {
+    const int32_t index = threadIdx.x;
+    if (index < a.groups) {
+      const int32_t first = groups.cut[index], last = groups.cut[index + 1];
+      if (last > first) known = {a.cu(first), a.cu(last), 0, load_int(a.req_ids + first)};
+    }
+    for (int32_t base = 0; base < segments; base += kPlanThreads) {
+      const int32_t seq = base + index - a.groups;
+      if (seq < 0 || seq >= a.sequences) continue;
+      const Known k = base == 0 ? known : know_sequence(a, seq);
+      const int32_t group = k.end > k.token ? group_of(a, groups, seq) : -1;
+      if (group >= 0) atomicMax(&groups.longest[group], k.length);
+    }
+  } else {
+    for (int32_t g = warp; g < a.groups; g += kPlanThreads / 32) {
+      const int32_t first = a.cut(g), last = a.cut(g + 1);
+      int32_t most = 0;
+      for (int32_t s = first + lane; s < last; s += 32) {
+        if (a.cu(s + 1) > a.cu(s)) most = max(most, load_int(a.lengths + s));
+      }
+      most = __reduce_max_sync(kAllLanes, most);
+      if (lane == 0) a.limits()[g] = most;
+    }
+  }
+  __syncthreads();
   int64_t before[3] = {0, 0, 0};  // items, units, rows of second copies
   for (int32_t base = 0; base < segments; base += kPlanThreads) {
     const int32_t index = base + threadIdx.x;
@@ -118,7 +174,16 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     const bool prefix = index < a.groups;
     int64_t mine[3] = {0, 0, 0};
     if (index < segments && !descends) {
-      s = find_segment(a, index);
+      if (base > 0 || !held) {
+        if (index >= a.groups) {
+          known = know_sequence(a, index - a.groups);
+        } else {
+          const int32_t first = a.cut(index), last = a.cut(index + 1);
+          known = Known{};
+          if (last > first) known = {a.cu(first), a.cu(last), 0, load_int(a.req_ids + first)};
+        }
+      }
+      s = find_segment(a, groups, index, known);
       if (s.tokens > 0 && s.key_end > s.key_first) {
         blocks = (s.tokens * a.heads_per_kv + kBlockRows - 1) / kBlockRows;
         mine[0] = blocks;
@@ -160,16 +225,28 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       const int64_t warps_before = __shfl_sync(kAllLanes, x, max(warp - 1, 0));
       upto[k] += before[k] - mine[k] + (warp > 0 ? warps_before : 0);
     }
-    if (index < segments) {
-      a.first()[index] = blocks > 0 ? static_cast<int32_t>(upto[0]) : -1;
-      for (int32_t b = 0; b < blocks; ++b) {
-        SharedItem it = item_of(a, s, prefix, b);
-        it.begin = upto[1];
-        it.extra = static_cast<int32_t>(upto[2]);
-        upto[1] += units_of(it.tiles, it.rows);
-        if (it.rows <= kSlotRows) upto[2] += it.rows;
-        *a.item(static_cast<int32_t>(upto[0]) + b) = it;
+    const int32_t first_item = blocks > 0 ? static_cast<int32_t>(upto[0]) : -1;
+    if (prefix) {
+      a.first()[index] = first_item;
+      if (held) groups.first[index] = first_item;
+    }
+    for (int32_t b = 0; b < blocks; ++b) {
+      SharedItem it = item_of(a, s, prefix, b);
+      it.begin = upto[1];
+      it.extra = static_cast<int32_t>(upto[2]);
+      upto[1] += units_of(it.tiles, it.rows);
+      if (it.rows <= kSlotRows) upto[2] += it.rows;
+      *a.item(static_cast<int32_t>(upto[0]) + b) = it;
+    }
+    __syncthreads();
+    if (index >= a.groups && index < segments) {  // what joining has to know
+      const int32_t seq = index - a.groups, group = descends ? -1 : group_of(a, groups, seq);
+      int4 record = make_int4(first_item, known.token, -1, known.token);
+      if (group >= 0) {
+        record.z = held ? groups.first[group] : a.first()[group];
+        record.w = a.cu(cut_of(a, groups, group));
       }
+      a.records()[seq] = record;
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) before[k] += all[k];
@@ -220,9 +297,17 @@ __device__ __forceinline__ int64_t part_at(const Parts& p, int32_t i) {
   return p.next + (c - 1) * int64_t{kBlockRows} + (second ? kSlotRows : 0);
 }
 
+__device__ __forceinline__ Parts parts_of_lane(const Parts& p, int32_t lane) {
+  return {__shfl_sync(kAllLanes, p.first, lane), __shfl_sync(kAllLanes, p.copy, lane), __shfl_sync(kAllLanes, p.next, lane),
+          __shfl_sync(kAllLanes, p.count, lane), __shfl_sync(kAllLanes, p.both, lane)};
+}
+
 // WARPS warps to a (query, head): one where there are many of them, eight where
-// few rows have many fragments. Lanes weigh the fragments, then each warp adds up
-// its share of them in order, and the first the warps'.
+// few rows have many fragments (a call with 64 of 37: 104 us for 113; with 512, 119
+// for 125; with 1024, 139.3 for 138.4). A lane looks the group's
+// fragments up, its neighbour the sequence's own; lanes weigh the fragments, then
+// each warp adds up its share of them in order, and the first the warps'. Bound by
+// the chain of loads: several heads to a warp were slower.
 template <typename T, int DIM, int WARPS>
 __global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant__ SharedArgs a) {
   constexpr int kEach = DIM / 32;  // columns of a lane
@@ -238,19 +323,20 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant_
   if (token < a.cu(0) || token >= a.cu(a.sequences)) return;
   const int64_t share = __ldcg(&a.header()->share);
   const int32_t failed = load_int(&a.header()->failed);
-  const int32_t cut_first = a.cut(0), cut_last = a.cut(a.groups);
   const int32_t seq = warp_last_at_most(a.sequences, token, [&](int32_t i) { return a.cu(i); });
-  const bool grouped = seq >= cut_first && seq < cut_last;
-  const int32_t group = grouped ? warp_last_at_most(a.groups, seq, [&](int32_t i) { return a.cut(i); }) : 0;
-  const int32_t own_first = load_int(a.first() + a.groups + seq), own_token = a.cu(seq);
-  const int32_t group_first = grouped ? load_int(a.first() + group) : -1, group_token = grouped ? a.cu(a.cut(group)) : token;
+  const int4 record = __ldcg(a.records() + seq);  // the sequence's first item and token, its group's
   const int32_t kv = static_cast<int32_t>(fastdiv(head, a.per_kv)), in_kv = head - kv * a.heads_per_kv;
-  const Parts part[2] = {find_parts(a, group_first, (token - group_token) * a.heads_per_kv + in_kv, kv, share, pair),
-                         find_parts(a, own_first, (token - own_token) * a.heads_per_kv + in_kv, kv, share, pairs + pair)};
+  const bool own = lane & 1;
+  const Parts mine = find_parts(a, own ? record.x : record.z, (token - (own ? record.y : record.w)) * a.heads_per_kv + in_kv, kv, share,
+                                own ? pairs + pair : pair);
+  const Parts part[2] = {parts_of_lane(mine, 0), parts_of_lane(mine, 1)};
   const int32_t n0 = part[0].count << part[0].both, n = n0 + (part[1].count << part[1].both);
   auto place = [&](int32_t i) { return i < n0 ? part_at(part[0], i) : part_at(part[1], i - n0); };
-  float top = -INFINITY;
-  for (int32_t i = lane; i < n; i += 32) {
+  // This lane's of the first 32 fragments.
+  const int64_t first_at = lane < n ? place(lane) : 0;
+  const float first_lse = lane < n ? __ldcg(a.part_lse() + first_at) : -INFINITY;
+  float top = first_lse;
+  for (int32_t i = lane + 32; i < n; i += 32) {
     const float l = __ldcg(a.part_lse() + place(i));
     top = l != l ? l : top != top ? top : fmaxf(top, l);
   }
@@ -266,22 +352,21 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant_
   // Each round of 32 fragments: a lane has one's place and weight, and the
   // warps take turns with them, four on their way at once.
   for (int32_t i0 = 0; i0 < n; i0 += 32) {
-    const int32_t i = i0 + lane;
-    const int64_t at = i < n ? place(i) : 0;
-    const float weight = i < n ? exp2f(__ldcg(a.part_lse() + at) - base) : 0.f;
+    const int64_t at = i0 == 0 ? first_at : i0 + lane < n ? place(i0 + lane) : 0;
+    const float weight = i0 + lane >= n ? 0.f : exp2f((i0 == 0 ? first_lse : __ldcg(a.part_lse() + at)) - base);
     float sum = weight;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, d);
     total += sum;
-    const int32_t here = min(32, n - i0);
-    for (int32_t j0 = w; j0 < here; j0 += 4 * WARPS) {
+    const int32_t left = min(32, n - i0);
+    for (int32_t j0 = w; j0 < left; j0 += 4 * WARPS) {
       float x[4][kEach], by[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int32_t j = j0 + k * WARPS;
         by[k] = __shfl_sync(kAllLanes, weight, j & 31);
         const int64_t from = __shfl_sync(kAllLanes, at, j & 31);
-        if (j >= here) by[k] = 0.f;
+        if (j >= left) by[k] = 0.f;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) x[k][e] = 0.f;
         if (by[k] != 0.f) {  // a fragment without weight has no outputs
@@ -340,8 +425,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant_
 template <typename T, int DIM>
 int launch_join(const SharedArgs& a, cudaStream_t stream) {
   const int64_t pairs = static_cast<int64_t>(a.rows) * a.heads;
-  // Eight warps to a row while all rows' fit the GPU at once.
-  if (pairs <= 8 * kMostCtas) return launch_pdl(shared_join_kernel<T, DIM, 8>, static_cast<unsigned>(pairs), 256, 0, 1, stream, a);
+  if (pairs <= 4 * kMostCtas) return launch_pdl(shared_join_kernel<T, DIM, 8>, static_cast<unsigned>(pairs), 256, 0, 1, stream, a);
   return launch_pdl(shared_join_kernel<T, DIM, 1>, static_cast<unsigned>((pairs + 7) / 8), 256, 0, 1, stream, a);
 }
 
@@ -356,7 +440,8 @@ int lay_out(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, int64_t 
   const int64_t each = rows * (heads / kv_heads), segments = sequences + groups;
   at->limits = 64;
   at->first = at->limits + 4 * groups;
-  at->items = round_up(at->first + 4 * segments, 64);
+  at->records = round_up(at->first + 4 * groups, 64);
+  at->items = round_up(at->records + 16 * sequences, 64);
   at->most_items = 2 * (each / kBlockRows) + segments;
   at->starts = 2 * rows * heads;
   at->copies = at->starts + int64_t{kMostCtas} * kBlockRows;

@@ -48,8 +48,9 @@ static_assert(sizeof(SharedItem) == 64, "read in four parts");
 
 // Where things lie in the workspace, in bytes from its start.
 struct SharedLayout {
-  int64_t limits;    // (groups,): a prefix's keys that any query sees
-  int64_t first;     // (groups + sequences,): a segment's first item; -1: none
+  int64_t limits;    // (groups,): the longest length, where they are too many for the plan's shared memory
+  int64_t first;     // (groups,): a prefix's first item; -1: none
+  int64_t records;   // (sequences,): its first item (-1: none) and token, its group's first item and token
   int64_t items;
   int64_t most_items;
   int64_t lse;       // of the partial rows, base 2
@@ -90,6 +91,7 @@ struct SharedArgs {
   __device__ __forceinline__ SharedHeader* header() const { return reinterpret_cast<SharedHeader*>(work); }
   __device__ __forceinline__ SharedItem* item(int32_t i) const { return reinterpret_cast<SharedItem*>(work + at.items) + i; }
   __device__ __forceinline__ int32_t* first() const { return reinterpret_cast<int32_t*>(work + at.first); }
+  __device__ __forceinline__ int4* records() const { return reinterpret_cast<int4*>(work + at.records); }
   __device__ __forceinline__ int32_t* limits() const { return reinterpret_cast<int32_t*>(work + at.limits); }
   __device__ __forceinline__ float* part_lse() const { return reinterpret_cast<float*>(work + at.lse); }
   __device__ __forceinline__ float* part_out() const { return reinterpret_cast<float*>(work + at.out); }

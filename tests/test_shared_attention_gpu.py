@@ -302,6 +302,14 @@ def test_ctas_with_items_of_both_sorts(kv_heads, group, dim) -> None:
     Batch(sizes, prefixes, own, [1] * len(own), heads=kv_heads * group, kv_heads=kv_heads, dim=dim, block=64, seed=30, alone=5).check()
 
 
+@pytest.mark.parametrize("groups,alone", [(3, 1500), (1024, 3), (1025, 3), (1400, 700)])
+def test_more_sequences_and_groups_than_a_plan_holds_at_once(groups, alone) -> None:
+    sizes = [i % 2 for i in range(groups - 1)] + [2]
+    prefixes = [i % 23 for i in range(groups)]
+    own = [1 + i % 7 for i in range(sum(sizes) + alone)]
+    Batch(sizes, prefixes, own, [(i + 1) % 3 and 1 for i in range(len(own))], heads=2, kv_heads=1, dim=64, seed=33, alone=alone).check()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_a_negative_scale(dtype) -> None:
     b = Batch([3], [300], [30, 1, 150], [1, 2, 1], dtype=dtype, seed=31)
