@@ -20,6 +20,14 @@
 // half a step of 2^-25 below, 2^-28 of the largest weight. Tiles with other scales
 // (and all after them) keep a reference R of their own for w = 2^(x + log2 vscale -
 // R + 3), at a second exponential for each key. Sums, M, R, S and O are float32.
+//
+// A tile takes 3000 cycles with up to 128 rows, 3700 with up to 256; of these the
+// tensor core 1300 and 2600, the exponentials 1024 and 2048. The first is bound by
+// the latency of the codes' loads (a lane has registers for one tile of K and one
+// of V on their way), the second by the chain of a half's scores, weights and
+// outputs beside the other slot's. 128 sequences of 64 heads of 128 behind 32768
+// shared tokens, with 20 to 1000 of their own: 238 us with plan and joining, 588
+// TFLOP/s; 16 behind 131072: 137 us, 2.0 TB/s.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -104,7 +104,7 @@ struct SharedArgs {
   }
 };
 
-// Units of a tile, and of an item's start and end, by its rows: about 530 cycles
+// Units of a tile, and of an item's start and end, by its rows: about 500 cycles
 // each, as measured. Up to 128 rows the slots take turns with the tiles, and one's
 // start hides behind the other's tiles.
 __device__ __forceinline__ int32_t units_of_tile(int32_t rows) { return rows <= kSlotRows ? 6 : 8; }

@@ -311,9 +311,10 @@ def test_more_sequences_and_groups_than_a_plan_holds_at_once(groups, alone) -> N
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_a_negative_scale(dtype) -> None:
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_scales_that_are_not_positive(dtype, scale) -> None:
     b = Batch([3], [300], [30, 1, 150], [1, 2, 1], dtype=dtype, seed=31)
-    b.scale = -0.1
+    b.scale = scale
     b.check()
 
 
