@@ -859,15 +859,16 @@ __global__ void __launch_bounds__(kThreads, 1) shared_kernel(const __grid_consta
         if (going) arrive(&m.free[1][(tiles_before - 1) % kStages]);
       }
     }
-    if (!going) {  // gave up: let what was issued finish before the memory goes
-      if (leader) {
-        mma_commit(smem_addr(&m.drained[slot]));
-        const long long begin = clock64();
-        while (!mbar_try(smem_addr(&m.drained[slot]), 0) && clock64() - begin < 4000000000LL) {
-        }
+    // However the walk ended, what this lane issued finishes before the memory and
+    // the TMEM go: where another warp gave up, nothing else waits for it. (Elsewhere
+    // the softmax waits as long.)
+    if (leader) {
+      mma_commit(smem_addr(&m.drained[slot]));
+      const long long begin = clock64();
+      while (!mbar_try(smem_addr(&m.drained[slot]), 0) && clock64() - begin < 4000000000LL) {
       }
-      __syncwarp();
     }
+    __syncwarp();
   } else if (warp == kFenceWarp) {
     // ==================================================== from stores to operands
     // The loading warps store through the generic proxy, the tensor core reads

@@ -126,3 +126,25 @@ def test_arrays_that_descend_are_flagged_and_nothing_is_seen(cu, groups) -> None
     call.cu, call.cu_groups = ints(1, 2, 12, 13, 37), ints(0, 2, 4)
     again = call()
     assert torch.equal(again[0], good[0]) and torch.equal(again[1], good[1])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (64, 1, 128), (48, 1, 64)])
+def test_waits_that_run_out_in_the_middle(heads, kv_heads, dim) -> None:
+    """Bounds from a fraction of a tile's time to that of many tiles: warps give up at every point of the work, beside
+    others that are through with theirs or still issue. A call is right, or NaN throughout with its status bit; the next
+    one is right."""
+    call = Call(heads, kv_heads, dim, torch.bfloat16)
+    want = call(status=call.status)
+    assert int(call.status) == 0 and bool(want[1].isfinite().all())
+    for bound in [int(100 * 1.5**i) for i in range(16)]:
+        call.status.zero_()
+        with wait_bound(bound):
+            out, lse = call(status=call.status)
+        gone = int(call.status) != 0
+        assert int(call.status) in (0, STATUS_WAIT_TIMEOUT)
+        if gone:
+            assert bool(out[1:37].isnan().all()) and bool(lse[1:37].isnan().all())
+        else:
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        again = call()
+        assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
