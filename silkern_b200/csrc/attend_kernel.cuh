@@ -1104,20 +1104,21 @@ __global__ void __launch_bounds__(Config<SHAPE, NH, T>::kThreads, 1)
       }
       if (steps > 0) n += steps;
     }
-    if (__any_sync(kAllLanes, *abort != 0)) {  // gave up: let what was issued finish before the memory goes
-      if (leader) {
-        mma_commit(smem_addr(&sh.drained));
-        const long long begin = clock64();
-        while (!mbar_try(smem_addr(&sh.drained), 0) && clock64() - begin < 4000000000LL) {
-        }
-        flag_status(a.status, SILKERN_STATUS_WAIT_TIMEOUT);
+    // However the walk ended, what this lane issued finishes before the memory and
+    // the TMEM go: another warp may still give up, and then nothing else waits for it.
+    // (Elsewhere the softmax waits as long.)
+    if (leader) {
+      mma_commit(smem_addr(&sh.drained));
+      const long long begin = clock64();
+      while (!mbar_try(smem_addr(&sh.drained), 0) && clock64() - begin < 4000000000LL) {
       }
-      __syncwarp();
     }
+    __syncwarp();
   }
 
   __syncthreads();
   const bool gave_up = *abort != 0;
+  if (gave_up && warp == kMmaWarp && lane == 0) flag_status(a.status, SILKERN_STATUS_WAIT_TIMEOUT);
   // ---- a split item: its ranks, which all see the same tiles, join
   Handed last{};
   if (has_split) {

@@ -131,3 +131,35 @@ def test_an_item_may_last_longer_than_a_wait() -> None:
     # at 2 GHz at most, an item that lasts the whole call exceeds the bound four times over
     assert begin.elapsed_time(end) * 2e6 > 4 * cycles
     assert status.item() == 0 and bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("rows", [1, 9, 80, 200])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_waits_that_run_out_in_the_middle(shape, rows) -> None:
+    """Bounds from a fraction of a tile's time to that of many tiles: warps give up at every point of the work, the
+    last wait for an item's end among them. What is NaN comes with its status bit, and the next call is right."""
+    dim, value_dim, latent = SHAPES[shape]
+    cache = make_cache(64, 64, 1, dim, latent=latent, seed=7)
+    g = torch.Generator().manual_seed(rows)
+    slots = torch.randint(0, 4096, (rows, 3000), generator=g, dtype=torch.int32).cuda()
+    counts = torch.randint(1, 3001, (rows,), generator=g, dtype=torch.int32).cuda()
+    q = torch.randn((rows, 16, dim), generator=g).to(torch.bfloat16).cuda()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def call(**more):
+        out = torch.full((rows, 16, value_dim), 7.0, dtype=torch.bfloat16, device="cuda")
+        lse = torch.full((rows, 16), 7.0, device="cuda")
+        silkern.attend_selected(q, slots, *cache, out, lse, softmax_scale=dim**-0.5, counts=counts, **more)
+        return out, lse
+
+    want = call(status=status)
+    assert status.item() == 0 and not bool(want[1].isnan().any())
+    for bound in [0] + [int(100 * 1.6**i) for i in range(13)]:
+        status.zero_()
+        with wait_bound(bound):
+            got = call(status=status)
+        odd = assert_right_or_nan(got, want)
+        # (A pipeline without an item may give up its wait for one.)
+        assert status.item() in ((STATUS_WAIT_TIMEOUT,) if odd else (0, STATUS_WAIT_TIMEOUT))
+        again = call()
+        assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
