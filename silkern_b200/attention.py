@@ -196,7 +196,8 @@ def _check_owner(block_size, dcp_size, dcp_rank, dcp_interleave) -> None:
 def _check_scale(softmax_scale) -> None:
     try:
         finite = math.isfinite(softmax_scale)
-    except (TypeError, ValueError, RuntimeError) as error:  # RuntimeError: a tensor of several elements
+    except (TypeError, ValueError, RuntimeError, OverflowError) as error:
+        # RuntimeError: a tensor of several elements; OverflowError: an integer that no float holds
         raise LocalizationError("softmax_scale must be a finite number") from error
     if not finite:
         raise LocalizationError("softmax_scale must be finite")

@@ -384,3 +384,11 @@ def test_strides_that_run_backwards_are_followed(lib) -> None:
     assert selected(lib, cache(), rows=4, out=Q + 2 * 256 * 7 - 2, out_row=-256) == 6
     assert selected(lib, cache(), rows=4, slots=IDX, slots_row=-32, lse=IDX - 4 * 32 * 3) == 6
     assert lib.silkern_merge_partials_v1(Q, 32, 16, 8, IDX, 0, 2, 2, 2, 8, Q + 2 * 72, -16, 8, LSE, None) == 6
+
+
+@pytest.mark.parametrize("scale", [10**400, -(10**400), 1j, None, "1", [0.1], torch.ones(2)])
+def test_a_scale_that_is_no_number_of_ours_is_refused(scale) -> None:
+    from silkern_b200 import attention
+
+    with pytest.raises(silkern.LocalizationError, match="softmax_scale must be"):
+        attention._check_scale(scale)
