@@ -53,25 +53,40 @@ def rotary_frequencies(
 
     if not _is_int(columns) or columns < 2 or columns % 2:
         raise LocalizationError("rotary columns must be a positive even integer")
-    if not (math.isfinite(base) and base > 0 and math.isfinite(factor) and factor >= 1):
-        raise LocalizationError("base must be positive, factor at least 1, and both finite")
+    base, factor = float(_number(base, "base")), float(_number(factor, "factor"))
+    if base <= 0 or factor < 1:
+        raise LocalizationError("base must be positive and factor at least 1")
     if method not in ("none", "positions", "base", "parts"):
         raise LocalizationError('method must be "none", "positions", "base" or "parts"')
     amplitude = 1.0
     if method == "base" and columns > 2:
-        base = base * factor ** (columns / (columns - 2))
+        try:
+            base = base * factor ** (columns / (columns - 2))
+        except OverflowError:
+            base = math.inf
+        if base == math.inf:
+            raise LocalizationError("factor is too large for this base")
     step = torch.arange(0, columns, 2, dtype=torch.float64) / columns
     frequencies = base**-step
     if method == "positions":
         frequencies = frequencies / factor
     elif method == "parts":
-        if not _is_int(original_length) or original_length < 1 or not 0 <= slow < fast:
-            raise LocalizationError('"parts" needs a positive original_length and 0 <= slow < fast')
+        if not _is_int(original_length) or not 1 <= original_length <= 2**31 - 1:
+            raise LocalizationError('"parts" needs an original_length, a positive int32 integer')
+        try:
+            ordered = 0 <= slow < fast
+        except (TypeError, ValueError, RuntimeError) as error:
+            raise LocalizationError("slow and fast must be numbers") from error
+        if not ordered:
+            raise LocalizationError('"parts" needs 0 <= slow < fast')
         turns = original_length * frequencies / (2 * math.pi)
         keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
         frequencies = frequencies * (keep + (1 - keep) / factor)
         amplitude = 0.1 * math.log(factor) + 1.0
-    return frequencies.to(torch.float32).to(device), amplitude
+    frequencies = frequencies.to(torch.float32)
+    if not bool(frequencies.isfinite().all()):
+        raise LocalizationError("these frequencies pass float32's range")
+    return frequencies.to(device), amplitude
 
 
 def _number(value, name: str) -> float:

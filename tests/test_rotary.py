@@ -170,3 +170,17 @@ def test_read_launcher_refuses_what_append_refuses() -> None:
     a["keys"].requires_grad_()
     with pytest.raises(silkern.LocalizationError, match="gradient"):
         silkern.read_quantized(**a)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(base="x"), dict(base=None), dict(base=1j), dict(base=10**400), dict(base=torch.tensor([1e4, 2.0])), dict(factor="2"),
+    dict(factor=None), dict(factor=10**400), dict(base=1e300, factor=1e300, method="base"),
+    dict(base=1e300, factor=1e12, method="base"), dict(base=1e-300),
+    dict(method="parts", original_length=4096, slow=None), dict(method="parts", original_length=4096, slow="a"),
+    dict(method="parts", original_length=4096, fast=None), dict(method="parts", original_length=4096, fast=math.nan),
+    dict(method="parts", original_length=10**400),
+    dict(method="parts", original_length=4096.0), dict(method=["parts"]), dict(method=None)])
+def test_frequencies_of_no_numbers_are_refused(bad) -> None:
+    """With a LocalizationError, and so are those that float32 does not hold."""
+    with pytest.raises(silkern.LocalizationError):
+        silkern.rotary_frequencies(**{"columns": 64, "factor": 2.0, **bad})
