@@ -434,6 +434,7 @@ int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 // The workspace's layout.
 int lay_out(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, int64_t sequences, int64_t groups, SharedLayout* at) {
   if (rows < 1 || rows > 0x7fffffff || sequences < 1 || sequences > 0x3fffffff || groups < 1 || groups > 0x3fffffff) return SILKERN_E_SHAPE;
+  if (sequences + groups > 0x7fffffff - kPlanThreads) return SILKERN_E_SHAPE;  // the plan's rounds end below 2^31
   if (heads < 1 || heads > 65535 || kv_heads < 1 || heads % kv_heads != 0) return SILKERN_E_HEADS;
   if (dim != 64 && dim != 128) return SILKERN_E_CACHE;
   if (rows * heads > 0x3fffffff) return SILKERN_E_SHAPE;

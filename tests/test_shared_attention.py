@@ -108,3 +108,15 @@ def test_the_oracle_with_copied_tables_is_the_window_oracle(prefix) -> None:
     got = oracle.attend_shared(q, cu, lengths, req, ints(0, 3), ints(prefix), table, *cache, softmax_scale=0.1)
     want = oracle.attend_window(q, cu, lengths, req, table, *cache, softmax_scale=0.1)
     assert torch.allclose(got[0], want[0], atol=1e-12) and torch.allclose(got[1], want[1], atol=1e-12)
+
+
+def test_more_segments_than_the_plan_counts_are_refused(lib) -> None:
+    """A group and a sequence are a segment each; the plan walks them in rounds of 1024 with 32-bit numbers, the round's
+    end included."""
+    most = 2**30 - 1
+    assert lib.silkern_shared_workspace_v1(1, 8, 1, 128, most, most) == -2
+    assert lib.silkern_shared_workspace_v1(1, 8, 1, 128, most, 1) > 0
+    assert lib.silkern_shared_workspace_v1(1, 8, 1, 128, 1, most) > 0
+    assert shared(lib, cache(), seqs=most, groups=most, bytes=2**60) == 2
+    with pytest.raises(silkern.LocalizationError):
+        silkern.shared_workspace_bytes(1, 8, 1, 128, most, most)
