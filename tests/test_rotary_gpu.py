@@ -189,3 +189,38 @@ def test_graphs_streams_and_compiled_callers() -> None:
     a, b = q.clone(), k.clone()
     torch.compile(inplace, fullgraph=True)(a, b, p)
     assert torch.equal(a, want_q) and torch.equal(b, want_k)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,norm", [(1, None, 576), (1, None, 512), (2, 1, 512), (1, None, 0)])
+def test_several_tokens_a_cta_and_two_slots_a_lane(interleaved, heads, kv_heads, norm) -> None:
+    """Few heads of 576 columns, of thousands of tokens: the keys of a long latent prompt alone."""
+    tokens = 4003  # four to a CTA, three in the last
+    q = randn(tokens, heads, 576, dtype=torch.bfloat16, seed=1)
+    k = None if kv_heads is None else randn(tokens, kv_heads, 576, dtype=torch.bfloat16, seed=2)
+    frequencies, _ = silkern.rotary_frequencies(64, device="cuda")
+    weight = 1 + randn(norm, dtype=torch.float32, seed=3) / 4 if norm else None
+    p = positions_of(tokens, 4)
+    check(q, k, p, frequencies, q_weight=weight, rotary_start=512, interleaved=interleaved)
+    if k is not None:
+        check(q, k, p, frequencies, k_weight=weight, rotary_start=512, interleaved=interleaved)
+    check(q, k, p, frequencies, q_weight=weight, rotary_start=512, interleaved=interleaved, inplace=True)
+
+
+def test_views_of_one_projection_in_place_under_compile() -> None:
+    """q and k as slices of one buffer, written in place by a compiled caller that goes on with both."""
+    tokens, heads, kv_heads, dim = 37, 8, 2, 128
+    x = randn(tokens, heads + 2 * kv_heads, dim, dtype=torch.bfloat16, seed=1)
+    frequencies, _ = silkern.rotary_frequencies(dim, device="cuda")
+    weight = torch.ones(dim, device="cuda")
+    p = positions_of(tokens, 3)
+
+    def step(x):
+        q, k = x[:, :heads], x[:, heads : heads + kv_heads]
+        silkern.rotate_heads(q, k, p, frequencies, q, k, q_weight=weight, k_weight=weight)
+        return q * 2, k + 1, x[:, heads + kv_heads :].clone()
+
+    want_x = x.clone()
+    want = step(want_x)
+    got = torch.compile(step, fullgraph=True)(x)
+    assert torch.equal(x, want_x) and all(torch.equal(a, b) for a, b in zip(got, want))

@@ -436,3 +436,24 @@ def test_a_step_from_projections_to_outputs() -> None:
     keys, values = torch.zeros((prefix, kv_heads, dim), dtype=torch.bfloat16, device="cuda"), torch.zeros((prefix, kv_heads, dim), dtype=torch.bfloat16, device="cuda")
     silkern.read_quantized(keys, values, *cache, *scales, ints(0, prefix), ints(0), ints(0), table)
     assert bool((keys != 0).any(-1).all()) and bool((values != 0).any(-1).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 64), (10, 2, 128)])
+def test_prompts_of_many_blocks_behind_a_prefix(dtype, heads, kv_heads, dim) -> None:
+    """Own segments of dozens of blocks, each over keys up to its last query's, beside short ones and behind a prefix."""
+    each = [1500, 1, 700, 333]
+    Batch([3], [777], [n + 20 * (n % 2) for n in each], each, heads=heads, kv_heads=kv_heads, dim=dim, block=64, dtype=dtype, seed=40,
+          alone=1).check()
+
+
+def test_value_scales_farther_apart_than_the_first_tiles_reach() -> None:
+    """Pages of the prefix whose value scales rise, or fall, by more than 2^4 and 2^6 in steps: the second reference
+    takes over in the middle, and the small ones' share of the outputs is theirs."""
+    for falling in (False, True):
+        b = Batch([2], [900], [200, 300], [1, 1], heads=8, kv_heads=2, seed=41)
+        pages = b.table[int(b.req[0])].long()
+        step = torch.arange(pages.numel(), device="cuda") // 8 * 3 - 10
+        assert int(step[:57].max() - step[0]) > 10  # 57 pages of 16 hold the prefix; a tile is 8 of them
+        b.cache[3][pages] = torch.ldexp(torch.ones(pages.numel(), device="cuda"), step.flip(0) if falling else step)[:, None]
+        b.check()
