@@ -109,7 +109,10 @@ __device__ __forceinline__ SharedItem item_of(const SharedArgs& a, const Segment
 
 // One CTA lays out the items: a thread for each segment, and prefix sums over
 // them. Fewer dependent loads than launches cost: 4.7 us alone in a graph for 4
-// sequences, 6.2 for 256 in 5 groups.
+// sequences, 6.2 for 256 in 5 groups. A thread goes through its segment's blocks of
+// 256 rows one by one, which no decode step notices: prompts do, by 0.13 us for each
+// block of the longest segment (4 times 2048 queries of 8 heads behind a prefix,
+// 256 blocks: 43 us by itself and cold, where 4 sequences take 9, of a call of 3.5 ms).
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_constant__ SharedArgs a, int32_t ctas) {
   __shared__ int64_t sums[3][32];
   __shared__ Groups groups;
@@ -431,7 +434,8 @@ int launch_join(const SharedArgs& a, cudaStream_t stream) {
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// The workspace's layout.
+// The workspace's layout. Every (row, head) has a partial result of its group's
+// prefix and one of its own tokens, whether it sees both or not.
 int lay_out(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, int64_t sequences, int64_t groups, SharedLayout* at) {
   if (rows < 1 || rows > 0x7fffffff || sequences < 1 || sequences > 0x3fffffff || groups < 1 || groups > 0x3fffffff) return SILKERN_E_SHAPE;
   if (sequences + groups > 0x7fffffff - kPlanThreads) return SILKERN_E_SHAPE;  // the plan's rounds end below 2^31

@@ -19,7 +19,14 @@
 // scales in [2^(E - 6), 2^(E + 4)) w is below 2^15, keeps 11 bits down to 2^-14 and
 // half a step of 2^-25 below, 2^-28 of the largest weight. Tiles with other scales
 // (and all after them) keep a reference R of their own for w = 2^(x + log2 vscale -
-// R + 3), at a second exponential for each key. Sums, M, R, S and O are float32.
+// R + 3), at a second exponential for each key and without the common case's
+// straight code: 128 sequences of 64 heads behind 16384 tokens take 598 us instead of 190 where
+// some CTAs meet such a tile early. Sums, M, R, S and O are float32.
+//
+// That w is one fp16 number is the price of one multiply-add for each key, where
+// e4m3 and e5m2 parts would take two or three: 2^-11 of w at most where it is above
+// 2^-14. Outputs' errors against 64 bits (relative, root mean square): bfloat16
+// 1.675e-3 where float32 weights have 1.663e-3; float16 2.8e-4 and 3.0e-4 for 2.1e-4.
 //
 // A tile takes 3000 cycles with up to 128 rows, 3700 with up to 256; of these the
 // tensor core 1300 and 2600, the exponentials 1024 and 2048. The first is bound by

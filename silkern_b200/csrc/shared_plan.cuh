@@ -105,8 +105,9 @@ struct SharedArgs {
 };
 
 // Units of a tile, and of an item's start and end, by its rows: about 500 cycles
-// each, as measured. Up to 128 rows the slots take turns with the tiles, and one's
-// start hides behind the other's tiles.
+// each, as measured with 128 columns; those of 64 are cut by the same ones. Up to
+// 128 rows the slots take turns with the tiles, and one's start hides behind the
+// other's tiles.
 __device__ __forceinline__ int32_t units_of_tile(int32_t rows) { return rows <= kSlotRows ? 6 : 8; }
 __device__ __forceinline__ int32_t units_of_start(int32_t rows) { return rows <= kSlotRows ? 19 : 46; }
 __device__ __forceinline__ int64_t units_of(int32_t tiles, int32_t rows) {

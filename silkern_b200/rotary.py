@@ -44,10 +44,13 @@ def rotary_frequencies(
     enlarges the base until the lowest frequency is divided by ``factor`` and the
     highest stays; ``"parts"`` divides those that turn fewer than ``slow`` times
     within ``original_length`` positions, keeps those that turn more than ``fast``
-    times, and goes linearly from one to the other in between, with an
-    amplitude of ``0.1 ln(factor) + 1`` ("YaRN: Efficient Context Window Extension
-    of Large Language Models", sections 3.1 to 3.4). Returns (float32 tensor of
-    ``columns // 2``, float).
+    times, and goes linearly in the number of turns from one to the other in between,
+    with an amplitude of ``0.1 ln(factor) + 1`` ("YaRN: Efficient Context Window
+    Extension of Large Language Models", sections 3.1 to 3.4). Programs that go
+    linearly in the column's number between the two bounds get other
+    frequencies in between: make those of a model that was trained so by its own
+    rule, and pass them to :func:`rotate_heads`, which takes any. Returns
+    (float32 tensor of ``columns // 2``, float).
     """
     import torch
 
