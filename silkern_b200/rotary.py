@@ -69,6 +69,11 @@ def rotary_frequencies(
             base = math.inf
         if base == math.inf:
             raise LocalizationError("factor is too large for this base")
+    # The largest is the first, which is 1, or the last. (On the host: the tensors may be
+    # of any default device, or traced.)
+    last = (columns - 2) / columns * -math.log(base) - (math.log(factor) if method == "positions" else 0.0)
+    if last > math.log(torch.finfo(torch.float32).max):
+        raise LocalizationError("base is too small: its frequencies pass float32's range")
     step = torch.arange(0, columns, 2, dtype=torch.float64) / columns
     frequencies = base**-step
     if method == "positions":
@@ -86,10 +91,7 @@ def rotary_frequencies(
         keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
         frequencies = frequencies * (keep + (1 - keep) / factor)
         amplitude = 0.1 * math.log(factor) + 1.0
-    frequencies = frequencies.to(torch.float32)
-    if not bool(frequencies.isfinite().all()):
-        raise LocalizationError("these frequencies pass float32's range")
-    return frequencies.to(device), amplitude
+    return frequencies.to(torch.float32).to(device), amplitude
 
 
 def _number(value, name: str) -> float:

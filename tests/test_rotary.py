@@ -184,3 +184,20 @@ def test_frequencies_of_no_numbers_are_refused(bad) -> None:
     """With a LocalizationError, and so are those that float32 does not hold."""
     with pytest.raises(silkern.LocalizationError):
         silkern.rotary_frequencies(**{"columns": 64, "factor": 2.0, **bad})
+
+
+def test_frequencies_in_traced_callers_and_on_other_default_devices() -> None:
+    """Nothing in the making of frequencies looks at a tensor's contents."""
+    want, _ = silkern.rotary_frequencies(64, factor=4.0, method="parts", original_length=4096)
+
+    @torch.compile(fullgraph=True, backend="eager")
+    def scaled(x):
+        f, amplitude = silkern.rotary_frequencies(64, factor=4.0, method="parts", original_length=4096)
+        return x * f * amplitude
+
+    assert torch.allclose(scaled(torch.ones(32)), want * (0.1 * math.log(4.0) + 1))
+    with torch.device("meta"):
+        f, _ = silkern.rotary_frequencies(64)
+    assert f.device.type == "meta" and f.shape == (32,)
+    for base in (1e-37, 1e-30):  # large, and within float32
+        assert bool(silkern.rotary_frequencies(64, base=base)[0].isfinite().all())
